@@ -597,6 +597,54 @@ int pkm_kernel_timing_begin(void);
 int pkm_kernel_timing_read(const char* kernel, float* ms_out, int64_t cap, int64_t* count_out);
 int pkm_kernel_timing_end(void);
 
+/* ---------------------------------------------------------------------------
+ * Attention beside the memories.
+ *
+ * A [batch, heads, tokens, dim] tensor of 16-bit numbers: device pointer and
+ * strides in elements; the numbers of one token and head are contiguous. Data
+ * are 16-byte aligned, strides >= 0, multiples of 8, the token stride below 2^22.
+ */
+typedef struct {
+  void* data;
+  int64_t batch, head, token;
+} pkm_heads_t;
+
+/*
+ * Causal attention through a sliding window, with first tokens that stay
+ * visible (sinks), over a padded batch:
+ *   out[b, h, p] = sum_j softmax_j(scale <q[b, h, p], k[b, g, j]>) v[b, g, j],  g = h / (q_heads / kv_heads)
+ * over the keys j with starts[b] <= j <= p < ends[b] and
+ * (p - j < window or j - starts[b] < sinks). Rows that see no key, those
+ * outside [starts, ends) among them, are written as 0, and what q, k and v hold
+ * there is not used.
+ * starts, ends: int32 [batch] on the device, clamped to [0, tokens]; NULL: 0, tokens.
+ * window 0: no window. dim 64 or 128, bf16 or f16, scale > 0.
+ * Logits, softmax and sums are float32; the weights are rounded to the tensors'
+ * type (relative to their row's largest so far) for the product with v.
+ * lse (float32 [batch, q_heads, tokens], may be NULL): log2 of the rows' sums of
+ * exponentials, +inf for rows that see nothing; what the backward reads.
+ */
+int pkm_window_attn_fwd(const pkm_heads_t* q, const pkm_heads_t* k, const pkm_heads_t* v,
+                        const int32_t* starts, const int32_t* ends, int64_t batch, int64_t q_heads,
+                        int64_t kv_heads, int64_t tokens, int64_t dim, int dtype, int64_t window,
+                        int64_t sinks, float scale, const pkm_heads_t* out, float* lse, void* stream);
+
+/* Workspace bytes pkm_window_attn_bwd needs. */
+size_t pkm_window_attn_bwd_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
+                                          int64_t dim, int64_t window, int64_t sinks);
+
+/*
+ * Gradients of pkm_window_attn_fwd, from its inputs, its out and lse, and
+ * grad_out: dq as q, dk and dv as k and v (summed over the query heads that share
+ * a key head), 0 outside [starts, ends). Deterministic. Workspace: 16-byte aligned.
+ */
+int pkm_window_attn_bwd(const pkm_heads_t* q, const pkm_heads_t* k, const pkm_heads_t* v,
+                        const pkm_heads_t* out, const float* lse, const pkm_heads_t* grad_out,
+                        const int32_t* starts, const int32_t* ends, int64_t batch, int64_t q_heads,
+                        int64_t kv_heads, int64_t tokens, int64_t dim, int dtype, int64_t window,
+                        int64_t sinks, float scale, const pkm_heads_t* dq, const pkm_heads_t* dk,
+                        const pkm_heads_t* dv, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
