@@ -645,6 +645,57 @@ int pkm_window_attn_bwd(const pkm_heads_t* q, const pkm_heads_t* k, const pkm_he
                         int64_t sinks, float scale, const pkm_heads_t* dq, const pkm_heads_t* dk,
                         const pkm_heads_t* dv, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * A paged cache of keys and values in 4 bits. A head vector of dim (64 or 128)
+ * numbers is held in groups of 32: the minimum m, the step s = (max - min) / 15,
+ * both in the cache's type (bf16 or f16), and codes c = round((x - m) / s), ties to
+ * even, in [0, 15] (0 where s is 0); the number read back is m + s c.
+ *   codes:  [2 (K, V), pages, kv_heads, page, dim / 2] bytes. Number d = w + 16 i
+ *           (w < 16) of a vector lies in its word w: dim 128: 32-bit words, bits
+ *           4 (i / 2 + 4 (i % 2)); dim 64: 16-bit words, bits 4 i.
+ *   params: [2 (K, V), pages, kv_heads, 2 (s, m), dim / 32, page] of the cache's type
+ * page: tokens of a page, a multiple of 16 up to 4096. Position t of sequence b lies
+ * in page table[b * width + t / page] (int32, on the device), slot t % page. Positions
+ * outside the table and entries that are no page are left out: not written, read
+ * as zeros, not visible.
+ */
+
+/*
+ * Quantises k and v [batch, kv_heads, tokens, dim] into the cache: token t < counts[b]
+ * of sequence b becomes position starts[b] + t. Two tokens of one call that fall on
+ * one slot leave either of them there.
+ */
+int pkm_kv4_append(void* codes, void* params, int64_t pages, int64_t kv_heads, int64_t page, int64_t dim,
+                   int dtype, const pkm_heads_t* k, const pkm_heads_t* v, const int32_t* table,
+                   int64_t width, const int32_t* starts, const int32_t* counts, int64_t batch,
+                   int64_t tokens, void* stream);
+
+/* Reads positions starts[b] + t, t < counts[b], back into k and v [batch, kv_heads, tokens, dim]; zeros for t >= counts[b]. */
+int pkm_kv4_read(const void* codes, const void* params, int64_t pages, int64_t kv_heads, int64_t page,
+                 int64_t dim, int dtype, const int32_t* table, int64_t width, const int32_t* starts,
+                 const int32_t* counts, int64_t batch, int64_t tokens, const pkm_heads_t* k,
+                 const pkm_heads_t* v, void* stream);
+
+/* Workspace bytes pkm_kv4_attend needs (0: none). */
+size_t pkm_kv4_attend_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t queries,
+                                     int64_t dim, int64_t width, int64_t page, int64_t window, int64_t sinks);
+
+/*
+ * Attention of the last `queries` positions of each sequence over its cache: query i of
+ * sequence b, with lengths[b] tokens (int32 on the device, clamped to [0, width * page]),
+ * stands at position p = lengths[b] - queries + i and sees the positions j <= p with
+ * p - j < window or j < sinks (window 0: no window). q, out: [batch, q_heads, queries,
+ * dim] in the cache's type; rows that see nothing (p < 0 among them) are written as 0.
+ * Logits, softmax and sums are float32. The weights are rounded to bf16 (f16 caches:
+ * to twice its digits) with the values' steps in them, and to the cache's type for
+ * the minima. Sums run in a fixed order (deterministic).
+ */
+int pkm_kv4_attend(const void* codes, const void* params, int64_t pages, int64_t kv_heads, int64_t page,
+                   int64_t dim, int dtype, const pkm_heads_t* q, const int32_t* table, int64_t width,
+                   const int32_t* lengths, int64_t batch, int64_t q_heads, int64_t queries, int64_t window,
+                   int64_t sinks, float scale, const pkm_heads_t* out, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

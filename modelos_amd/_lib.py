@@ -276,6 +276,32 @@ SIGNATURES.update({
             c_void_p, c_size_t, c_void_p,  # workspace, bytes, stream
         ],
     ),
+    "pkm_kv4_append": (
+        c_int,
+        [
+            c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int,  # codes, params, pages, heads, page, dim, dtype
+            _HEADS, _HEADS, c_void_p, c_int64, c_void_p, c_void_p,  # k, v, table, width, starts, counts
+            c_int64, c_int64, c_void_p,  # batch, tokens, stream
+        ],
+    ),
+    "pkm_kv4_read": (
+        c_int,
+        [
+            c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int,  # codes, params, pages, heads, page, dim, dtype
+            c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,  # table, width, starts, counts, batch, tokens
+            _HEADS, _HEADS, c_void_p,  # k, v, stream
+        ],
+    ),
+    "pkm_kv4_attend_workspace_size": (c_size_t, [c_int64] * 9),
+    "pkm_kv4_attend": (
+        c_int,
+        [
+            c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int,  # codes, params, pages, heads, page, dim, dtype
+            _HEADS, c_void_p, c_int64, c_void_p,  # q, table, width, lengths
+            c_int64, c_int64, c_int64, c_int64, c_int64, c_float,  # batch, q_heads, queries, window, sinks, scale
+            _HEADS, c_void_p, c_size_t, c_void_p,  # out, workspace, bytes, stream
+        ],
+    ),
 })
 
 # pkm_score_t
