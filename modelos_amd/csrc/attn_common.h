@@ -119,30 +119,45 @@ __device__ __forceinline__ frag_t frag_global(const void* row, int s, int lane) 
   return row ? *(const frag_t*)((const uint8_t*)row + (2 * s + (lane >> 5)) * 16) : z;
 }
 
-// A tile's rows between global memory, registers and LDS, by 256 threads. Rows from `last` on are zeros.
+// 64 lanes' 16 bytes each from a buffer at the lanes' offsets to LDS at `to` (uniform) and on, side by side. In asm,
+// so that the compiler does not wait for it at the next transposing read of another tile; there is no register
+// for it to lose, and tile_wait() before the barrier is the wait. The s_nop: m0 is read one state after its write.
+__device__ __forceinline__ void load_lds16(u32x4_t rsrc, lds_u8* to, uint32_t offset) {
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"((uint32_t)(uintptr_t)to), "v"(offset), "s"(rsrc)
+               : "memory");
+}
+
+// A tile's rows from global memory straight to LDS (no registers in between), by 256 threads. A wave's load
+// writes 64 chunks of 16 bytes side by side; the permutation is in the addresses that the lanes read. Rows from
+// `last` (>= 1) on repeat row last - 1: what lies outside a sequence is never read. The loads are complete after
+// tile_wait().
 template <int D, int ROWS>
 struct TileLoad {
-  static constexpr int CH = D / 8, N = ROWS * CH / 256;
-  frag_t r[N];
-  // base: row 0; stride in bytes (128 rows of it fit in 31 bits)
-  __device__ __forceinline__ void load(const uint8_t* base, uint32_t stride, int last, int tid) {
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), (short)0, 0x7fffffff, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = tid + 256 * i, row = at / CH, c = at % CH;
-      const uint32_t off = row < last ? (uint32_t)row * stride + c * 16 : 0x80000000u;
-      r[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0);
-    }
+  static constexpr int CH = D / 8, PER = 64 / CH, N = ROWS / PER / 4;  // rows and loads of a wave
+  int row, chunk;  // the lane's first row and its bytes within a row
+  __device__ __forceinline__ TileLoad(int tid) {
+    const int wave = tid >> 6, lane = tid & 63;
+    row = wave * PER + lane / CH;
+    // rows of one lane are 4 PER apart, a multiple of 16: one permutation
+    chunk = tile_offset<D>(row, lane % CH) - row * (D * 2);
   }
-  __device__ __forceinline__ void store(lds_u8* tile, int tid) const {
+  // base: row 0 of the tile; stride in bytes (128 rows of it fit in 31 bits)
+  __device__ __forceinline__ void load(lds_u8* tile, const uint8_t* base, uint32_t stride, int last, int tid) const {
+    const u32x4_t rs = {(uint32_t)(uintptr_t)base, (uint32_t)((uintptr_t)base >> 32), 0x7fffffffu, 0x00020000u};
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = tid + 256 * i, row = at / CH, c = at % CH;
-      *(lds_u32x4*)(tile + tile_offset<D>(row, c)) = r[i];
-    }
+    for (int i = 0; i < N; ++i)
+      load_lds16(rs, tile + (wave + 4 * i) * 1024, (uint32_t)min(row + 4 * PER * i, last - 1) * stride + chunk);
   }
 };
+static_assert(TileLoad<128, 64>::PER * 4 % 16 == 0 && TileLoad<64, 64>::PER * 4 % 16 == 0, "one permutation a lane");
+
+// Waits for the wave's loads to LDS.
+__device__ __forceinline__ void tile_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), which the compiler's own counting sees
+  asm volatile("" ::: "memory");
+}
 
 // A [batch, heads, tokens, dim] tensor in a kernel's arguments, strides in elements (pkm_heads_t of the C ABI).
 struct Heads {

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
   const uint8_t* kbase = a.k.at(qb.b, qb.kv, seq.start);
   const uint8_t* vbase = a.v.at(qb.b, qb.kv, seq.start);
   const uint32_t kstride = (uint32_t)(2 * a.k.token), vstride = (uint32_t)(2 * a.v.token);
-  TileLoad<D, kTile> kt, vt;
+  const TileLoad<D, kTile> tl(tid);
 
   f32x16_t o[DT] = {};
   float m = -INFINITY, sum = 0.f;
@@ -117,11 +117,10 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
 
   if (tiles.count > 0) {
     const int t0 = tiles.tile(0) * kTile;
-    kt.load(kbase + (int64_t)t0 * kstride, kstride, seq.n - t0, tid);
-    vt.load(vbase + (int64_t)t0 * vstride, vstride, seq.n - t0, tid);
-    kt.store(lds, tid);
-    vt.store(lds + TB, tid);
+    tl.load(lds, kbase + (int64_t)t0 * kstride, kstride, seq.n - t0, tid);
+    tl.load(lds + TB, vbase + (int64_t)t0 * vstride, vstride, seq.n - t0, tid);
   }
+  tile_wait();
   __syncthreads();
   for (int it = 0; it < tiles.count; ++it) {
     const int j0 = tiles.tile(it) * kTile;
@@ -129,8 +128,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
     const lds_u8* vtile = ktile + TB;
     if (it + 1 < tiles.count) {
       const int t1 = tiles.tile(it + 1) * kTile;
-      kt.load(kbase + (int64_t)t1 * kstride, kstride, seq.n - t1, tid);
-      vt.load(vbase + (int64_t)t1 * vstride, vstride, seq.n - t1, tid);
+      lds_u8* next = lds + ((it + 1) & 1) * 2 * TB;
+      tl.load(next, kbase + (int64_t)t1 * kstride, kstride, seq.n - t1, tid);
+      tl.load(next + TB, vbase + (int64_t)t1 * vstride, vstride, seq.n - t1, tid);
     }
     if (p0 <= p1 && any_visible(p0, p1, j0, j0 + kTile - 1, W, S)) {
       f32x16_t s[2] = {};
@@ -177,11 +177,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[t] = mfma32<T>(frag_cols<D>(vtile, 16 * i, t, lane), pf[i], o[t]);
     }
-    if (it + 1 < tiles.count) {
-      lds_u8* next = lds + ((it + 1) & 1) * 2 * TB;
-      kt.store(next, tid);
-      vt.store(next + TB, tid);
-    }
+    tile_wait();
     __syncthreads();
   }
 
@@ -200,28 +196,13 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
 }
 
 // ---------------------------------------------------------------------------
-// Backward, delta: D / 8 lanes a row.
-// ---------------------------------------------------------------------------
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void window_delta_kernel(const AttnArgs a) {
-  constexpr int L = D / 8;
-  const int64_t at = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
-  if (at >= (int64_t)a.batch * a.q_heads * a.tokens) return;
-  const int row = (int)(at % a.tokens);
-  const int64_t bh = at / a.tokens;
-  const int b = (int)(bh / a.q_heads), head = (int)(bh % a.q_heads);
-  const Span seq = sequence(a, b);
-  float d = 0.f;
-  if (row >= seq.start && row < seq.start + seq.n) {
-    const int at16 = (threadIdx.x % L) * 16;
-    d = vec_dot<T>(ld16(a.o.at(b, head, row) + at16), ld16(a.dO.at(b, head, row) + at16), 0.f);
-  }
-  d = group_sum<L>(d);
-  if (threadIdx.x % L == 0) a.delta[at] = d;
-}
-
-// ---------------------------------------------------------------------------
 // Backward, dQ: as the forward, dS^T = P^T (V dO^T - delta), dQ^T = K^T dS^T.
+//
+// delta comes from the rounded output. What that puts into a row's dS adds up to
+// sum_j dS_j (which is 0), so the sum corrects the delta that dK reads. dS enters its
+// product as two 16-bit numbers, itself rounded and the rest: keys have a common part,
+// which the exact dS, whose sum is 0, cancels and the roundings of one would not (relative error
+// of dQ 2.7e-3 with one, 2.0e-3 with two in bf16, where the result's own rounding is 1.7e-3).
 // ---------------------------------------------------------------------------
 template <typename T, int D>
 __device__ void window_dq_block(const AttnArgs& a, int id, uint8_t* smem) {
@@ -247,22 +228,27 @@ __device__ void window_dq_block(const AttnArgs& a, int id, uint8_t* smem) {
     g[s] = frag_global<D>(grow, s, lane);
   }
   const int64_t at = ((int64_t)qb.b * a.q_heads + qb.head) * a.tokens + row;
-  const float lse = live ? a.lse[at] : INFINITY, delta = live ? a.delta[at] : 0.f;
+  const float lse = live ? a.lse[at] : INFINITY;
+  float delta = 0.f, sum = 0.f;
+  const uint8_t* orow = live ? a.o.at(qb.b, qb.head, row) : nullptr;
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    delta = vec_dot<T>(__builtin_bit_cast(uint4, frag_global<D>(orow, s, lane)), __builtin_bit_cast(uint4, g[s]), delta);
+  delta += swap_halves(delta);
 
   const uint8_t* kbase = a.k.at(qb.b, qb.kv, seq.start);
   const uint8_t* vbase = a.v.at(qb.b, qb.kv, seq.start);
   const uint32_t kstride = (uint32_t)(2 * a.k.token), vstride = (uint32_t)(2 * a.v.token);
-  TileLoad<D, kTile> kt, vt;
+  const TileLoad<D, kTile> tl(tid);
   f32x16_t dq[DT] = {};
   const float c = a.scale * 1.44269504f;
 
   if (tiles.count > 0) {
     const int t0 = tiles.tile(0) * kTile;
-    kt.load(kbase + (int64_t)t0 * kstride, kstride, seq.n - t0, tid);
-    vt.load(vbase + (int64_t)t0 * vstride, vstride, seq.n - t0, tid);
-    kt.store(lds, tid);
-    vt.store(lds + TB, tid);
+    tl.load(lds, kbase + (int64_t)t0 * kstride, kstride, seq.n - t0, tid);
+    tl.load(lds + TB, vbase + (int64_t)t0 * vstride, vstride, seq.n - t0, tid);
   }
+  tile_wait();
   __syncthreads();
   for (int it = 0; it < tiles.count; ++it) {
     const int j0 = tiles.tile(it) * kTile;
@@ -270,8 +256,9 @@ __device__ void window_dq_block(const AttnArgs& a, int id, uint8_t* smem) {
     const lds_u8* vtile = ktile + TB;
     if (it + 1 < tiles.count) {
       const int t1 = tiles.tile(it + 1) * kTile;
-      kt.load(kbase + (int64_t)t1 * kstride, kstride, seq.n - t1, tid);
-      vt.load(vbase + (int64_t)t1 * vstride, vstride, seq.n - t1, tid);
+      lds_u8* next = lds + ((it + 1) & 1) * 2 * TB;
+      tl.load(next, kbase + (int64_t)t1 * kstride, kstride, seq.n - t1, tid);
+      tl.load(next + TB, vbase + (int64_t)t1 * vstride, vstride, seq.n - t1, tid);
     }
     if (p0 <= p1) {
 #pragma unroll
@@ -283,30 +270,40 @@ __device__ void window_dq_block(const AttnArgs& a, int id, uint8_t* smem) {
         for (int i = 0; i < KS; ++i) s = mfma32<T>(frag_rows<D>(ktile, 32 * kb, i, lane), q[i], s);
 #pragma unroll
         for (int i = 0; i < KS; ++i) dp = mfma32<T>(frag_rows<D>(vtile, 32 * kb, i, lane), g[i], dp);
-        const bool all = all_visible(p0, p1, ja, ja + 31, W, S);
+        if (!all_visible(p0, p1, ja, ja + 31, W, S)) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[i] = visible(p, ja + 8 * (i >> 2) + 4 * h + (i & 3), W, S) ? s[i] : -INFINITY;
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float w = exp2_raw(__builtin_fmaf(s[i], c, -lse)) * (dp[i] - delta);
-          s[i] = all || visible(p, ja + 8 * (i >> 2) + 4 * h + (i & 3), W, S) ? w : 0.f;
+          s[i] = exp2_raw(__builtin_fmaf(s[i], c, -lse)) * (dp[i] - delta);
+          sum += s[i];
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          frag_t f;
+          frag_t f, r;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[e] = pack2<T>(s[8 * i + 2 * e], s[8 * i + 2 * e + 1]);
+          for (int e = 0; e < 4; ++e) {
+            const float x = s[8 * i + 2 * e], y = s[8 * i + 2 * e + 1];
+            f[e] = pack2<T>(x, y);
+            r[e] = pack2<T>(x - unpack1<T>(f[e] & 0xffffu), y - unpack1<T>(f[e] >> 16));
+          }
 #pragma unroll
-          for (int t = 0; t < DT; ++t) dq[t] = mfma32<T>(frag_cols<D>(ktile, 32 * kb + 16 * i, t, lane), f, dq[t]);
+          for (int t = 0; t < DT; ++t) {
+            const frag_t kt = frag_cols<D>(ktile, 32 * kb + 16 * i, t, lane);
+            dq[t] = mfma32<T>(kt, f, dq[t]);
+            dq[t] = mfma32<T>(kt, r, dq[t]);
+          }
         }
       }
     }
-    if (it + 1 < tiles.count) {
-      lds_u8* next = lds + ((it + 1) & 1) * 2 * TB;
-      kt.store(next, tid);
-      vt.store(next + TB, tid);
-    }
+    tile_wait();
     __syncthreads();
   }
+  sum += swap_halves(sum);
   if (row >= a.tokens) return;
+  if (live && h == 0) a.delta[at] = delta + sum;
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -358,13 +355,14 @@ __device__ void window_dkv_block(const AttnArgs& a, int id, uint8_t* smem) {
     k[s] = frag_global<D>(krow, s, lane);
     v[s] = frag_global<D>(vrow, s, lane);
   }
-  TileLoad<D, kTile> qt, gt;
+  const TileLoad<D, kTile> tl(tid);
   const uint32_t qstride = (uint32_t)(2 * a.q.token), gstride = (uint32_t)(2 * a.dO.token);
   float aux = 0.f;  // threads 0 .. 63 carry a tile's lse, 64 .. 127 its delta
   const auto load = [&](int i) {
     const int head = kv * G + i / count, t0 = (tile0 + i % count) * kTile;
-    qt.load(a.q.at(b, head, seq.start + t0), qstride, n - t0, tid);
-    gt.load(a.dO.at(b, head, seq.start + t0), gstride, n - t0, tid);
+    lds_u8* buf = lds + (i & 1) * BUF;
+    tl.load(buf, a.q.at(b, head, seq.start + t0), qstride, n - t0, tid);
+    tl.load(buf + TB, a.dO.at(b, head, seq.start + t0), gstride, n - t0, tid);
     if (tid < 2 * kTile) {
       const int r = tid & (kTile - 1);
       const float* from = tid < kTile ? a.lse : a.delta;
@@ -374,8 +372,6 @@ __device__ void window_dkv_block(const AttnArgs& a, int id, uint8_t* smem) {
   };
   const auto store = [&](int i) {
     lds_u8* buf = lds + (i & 1) * BUF;
-    qt.store(buf, tid);
-    gt.store(buf + TB, tid);
     if (tid < 2 * kTile) *(__attribute__((address_space(3))) float*)(buf + 2 * TB + 4 * tid) = aux;
   };
 
@@ -385,6 +381,7 @@ __device__ void window_dkv_block(const AttnArgs& a, int id, uint8_t* smem) {
     load(0);
     store(0);
   }
+  tile_wait();
   __syncthreads();
   for (int it = 0; it < total; ++it) {
     const int p0 = (tile0 + it % count) * kTile;
@@ -402,7 +399,11 @@ __device__ void window_dkv_block(const AttnArgs& a, int id, uint8_t* smem) {
         for (int i = 0; i < KS; ++i) s = mfma32<T>(frag_rows<D>(qtile, 32 * qb, i, lane), k[i], s);
 #pragma unroll
         for (int i = 0; i < KS; ++i) dp = mfma32<T>(frag_rows<D>(gtile, 32 * qb, i, lane), v[i], dp);
-        const bool all = all_visible(pa, pa + 31, k0, k1, W, S);
+        if (!all_visible(pa, pa + 31, k0, k1, W, S)) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[i] = visible(pa + 8 * (i >> 2) + 4 * h + (i & 3), key, W, S) ? s[i] : -INFINITY;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const f32x4_t lse = *(const lds_f32x4*)(stats + 4 * (32 * qb + 8 * e + 4 * h));
@@ -410,11 +411,8 @@ __device__ void window_dkv_block(const AttnArgs& a, int id, uint8_t* smem) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int i = 4 * e + r;
-            const float w = all || visible(pa + 8 * e + 4 * h + r, key, W, S)
-                                ? exp2_raw(__builtin_fmaf(s[i], c, -lse[r]))
-                                : 0.f;
-            s[i] = w;
-            dp[i] = w * (dp[i] - delta[r]);
+            s[i] = exp2_raw(__builtin_fmaf(s[i], c, -lse[r]));
+            dp[i] = s[i] * (dp[i] - delta[r]);
           }
         }
 #pragma unroll
@@ -433,6 +431,7 @@ __device__ void window_dkv_block(const AttnArgs& a, int id, uint8_t* smem) {
       }
     }
     if (it + 1 < total) store(it + 1);
+    tile_wait();
     __syncthreads();
   }
   if (row >= a.tokens) return;
@@ -502,11 +501,8 @@ void launch_fwd(const AttnArgs& a, hipStream_t st) {
 
 template <typename T, int D>
 void launch_bwd(const AttnArgs& a, hipStream_t st) {
-  const int64_t rows = (int64_t)a.batch * a.q_heads * a.tokens;
-  constexpr int per = kThreads / (D / 8);
-  window_delta_kernel<T, D><<<(unsigned)((rows + per - 1) / per), kThreads, 0, st>>>(a);
+  window_dq_kernel<T, D><<<query_blocks(a), kThreads, 0, st>>>(a);  // and delta
   window_dkv_kernel<T, D><<<(unsigned)(a.batch * a.kv_heads * ((a.tokens + 127) / 128)), kThreads, 0, st>>>(a);
-  window_dq_kernel<T, D><<<query_blocks(a), kThreads, 0, st>>>(a);
 }
 
 }  // namespace
