@@ -23,6 +23,9 @@ struct AttnArgs {
   int batch, q_heads, kv_heads, tokens;
   int window, sinks;  // window in [1, tokens] (tokens: no window), sinks in [0, tokens]
   int pack;           // query heads of one key head that share a workgroup: 1, 2 or 4
+  // the backward of the sinks from queries past their windows, when it has workgroups of its own
+  float* far;  // [pairs, 32-sink blocks, far_chunks, 2 (dK, dV), 32, dim]
+  int far_chunks, far_units, dim;  // chunks (0: none), steps of 32 queries in a chunk
   float scale;
 };
 
@@ -58,6 +61,23 @@ struct KeyTiles {
     count = sink + last - lo;
   }
   __device__ __forceinline__ int tile(int i) const { return i < sink ? i : i + near; }
+};
+
+// The steps of 32 queries past the window of the sinks [32 block, 32 block + 32) of a sequence of n tokens, head after head.
+struct FarPlan {
+  int tile0, tiles, units, used;  // first tile, tiles of a head, steps, chunks that hold any
+  int64_t slot;
+  __device__ __forceinline__ FarPlan(const AttnArgs& a, int pair, int block, int n) {
+    const int p0 = 32 * block + a.window;
+    tile0 = p0 / 32;
+    tiles = p0 < n ? (n - 1) / 32 + 1 - tile0 : 0;
+    units = tiles * (a.q_heads / a.kv_heads);
+    used = (units + a.far_units - 1) / a.far_units;
+    slot = ((int64_t)pair * ((a.sinks + 31) / 32) + block) * a.far_chunks;
+  }
+  __device__ __forceinline__ float* part(const AttnArgs& a, int chunk) const {
+    return a.far + (slot + chunk) * (2 * 32 * a.dim);
+  }
 };
 
 // A workgroup's share of the queries: 4 waves of 32 rows each, `pack` heads of one key head beside each other.
@@ -205,12 +225,13 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
 // of dQ 2.7e-3 with one, 2.0e-3 with two in bf16, where the result's own rounding is 1.7e-3).
 // ---------------------------------------------------------------------------
 template <typename T, int D>
-__device__ void window_dq_block(const AttnArgs& a, int id, uint8_t* smem) {
+__global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a) {
   constexpr int KS = D / 16, DT = D / 32, TB = kTile * D * 2;
+  __shared__ __align__(16) uint8_t smem[2 * 2 * TB];
   lds_u8* const lds = (lds_u8*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l = lane & 31, h = lane >> 5;
-  const QueryBlock qb(a, id, wave);
+  const QueryBlock qb(a, blockIdx.x, wave);
   const Span seq = sequence(a, qb.b);
   const int W = a.window, S = a.sinks;
   const int row = qb.row + l;
@@ -311,28 +332,77 @@ __device__ void window_dq_block(const AttnArgs& a, int id, uint8_t* smem) {
   store_row<T, D>(a.dq.at(qb.b, qb.head, row), dq, a.scale, lane);
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a) {
-  __shared__ __align__(16) uint8_t smem[2 * 2 * kTile * D * 2];
-  window_dq_block<T, D>(a, blockIdx.x, smem);
+// ---------------------------------------------------------------------------
+// Backward, dK and dV: 4 waves of 32 keys each; the tiles hold 32 queries and
+// their dO, of every query head of the key head in turn (a shared head's
+// gradient is summed in registers, in a fixed order). The keys stay in LDS and the
+// values in registers: with both in registers a wave needs more than the 256
+// that let two waves share a SIMD.
+// ---------------------------------------------------------------------------
+constexpr int kQueries = 32;
+template <int D>
+struct DkvLds {
+  static constexpr int TB = kQueries * D * 2, BUF = 2 * TB + 2 * kQueries * 4, KEYS = 128 * D * 2;
+  static constexpr int BYTES = KEYS + 2 * BUF;
+};
+
+// One step: 32 queries at [buf, their dO behind them, then lse and delta], the wave's 32 keys in LDS, their values v.
+// masked(i): the row i of the lane's column is not visible; all: none is masked.
+template <typename T, int D, typename F>
+__device__ __forceinline__ void dkv_step(const lds_u8* buf, const lds_u8* keys, const frag_t (&v)[D / 16], float c,
+                                         bool all, F masked, f32x16_t (&dk)[D / 32], f32x16_t (&dv)[D / 32], int lane) {
+  constexpr int KS = D / 16, DT = D / 32, TB = DkvLds<D>::TB;
+  const int h = lane >> 5;
+  const lds_u8* const gtile = buf + TB;
+  const lds_u8* const stats = gtile + TB;
+  f32x16_t s = {}, dp = {};
+#pragma unroll
+  for (int i = 0; i < KS; ++i) s = mfma32<T>(frag_rows<D>(buf, 0, i, lane), frag_rows<D>(keys, 0, i, lane), s);
+#pragma unroll
+  for (int i = 0; i < KS; ++i) dp = mfma32<T>(frag_rows<D>(gtile, 0, i, lane), v[i], dp);
+  if (!all) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = masked(8 * (i >> 2) + 4 * h + (i & 3)) ? -INFINITY : s[i];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const f32x4_t lse = *(const lds_f32x4*)(stats + 4 * (8 * e + 4 * h));
+    const f32x4_t delta = *(const lds_f32x4*)(stats + 4 * (kQueries + 8 * e + 4 * h));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 4 * e + r;
+      s[i] = exp2_raw(__builtin_fmaf(s[i], c, -lse[r]));
+      dp[i] = s[i] * (dp[i] - delta[r]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    frag_t pf, sf;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      pf[e] = pack2<T>(s[8 * i + 2 * e], s[8 * i + 2 * e + 1]);
+      sf[e] = pack2<T>(dp[8 * i + 2 * e], dp[8 * i + 2 * e + 1]);
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) dv[t] = mfma32<T>(frag_cols<D>(gtile, 16 * i, t, lane), pf, dv[t]);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) dk[t] = mfma32<T>(frag_cols<D>(buf, 16 * i, t, lane), sf, dk[t]);
+  }
 }
 
-// ---------------------------------------------------------------------------
-// Backward, dK and dV: 4 waves of 32 keys each; the tiles hold 64 queries and
-// their dO, of every query head of the key head in turn (a shared head's
-// gradient is summed in registers, in a fixed order).
-// ---------------------------------------------------------------------------
 template <typename T, int D>
-__device__ void window_dkv_block(const AttnArgs& a, int id, uint8_t* smem) {
-  constexpr int KS = D / 16, DT = D / 32, TB = kTile * D * 2, BUF = 2 * TB + 2 * kTile * 4;
-  lds_u8* const lds = (lds_u8*)smem;
+__global__ __launch_bounds__(kThreads, 2) void window_dkv_kernel(const AttnArgs a) {
+  constexpr int KS = D / 16, DT = D / 32, TB = DkvLds<D>::TB, BUF = DkvLds<D>::BUF;
+  __shared__ __align__(16) uint8_t smem[DkvLds<D>::BYTES];
+  lds_u8* const keys = (lds_u8*)smem;
+  lds_u8* const lds = keys + DkvLds<D>::KEYS;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l = lane & 31, h = lane >> 5;
-  const int pairs = a.batch * a.kv_heads, pair = id % pairs;
+  const int pairs = a.batch * a.kv_heads, pair = blockIdx.x % pairs;
   const int b = pair / a.kv_heads, kv = pair % a.kv_heads, G = a.q_heads / a.kv_heads;
-  const int first = id / pairs * 128;  // the key block's rows; the first ones are read by most queries
+  const int first = blockIdx.x / pairs * 128;  // the key block's rows; the first ones are read by most queries
   const Span seq = sequence(a, b);
-  const int W = a.window, S = a.sinks, n = seq.n;
+  const int W = a.window, S = a.far_chunks ? 0 : a.sinks, n = seq.n;
   const int row = first + 32 * wave + l;
   const int key = row - seq.start;
   const bool live = row < a.tokens && key >= 0 && key < n;
@@ -342,99 +412,71 @@ __device__ void window_dkv_block(const AttnArgs& a, int id, uint8_t* smem) {
   int tile0 = 0, count = 0;
   if (b0 <= b1) {
     const int last = b0 < S ? n - 1 : min(n - 1, b1 + W - 1);
-    tile0 = b0 / kTile;
-    count = last / kTile + 1 - tile0;
+    tile0 = b0 / kQueries;
+    count = last / kQueries + 1 - tile0;
   }
   const int total = count * G;
 
-  frag_t k[KS], v[KS];
-  const uint8_t* krow = live ? a.k.at(b, kv, row) : nullptr;
+  frag_t v[KS];
   const uint8_t* vrow = live ? a.v.at(b, kv, row) : nullptr;
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    k[s] = frag_global<D>(krow, s, lane);
-    v[s] = frag_global<D>(vrow, s, lane);
-  }
-  const TileLoad<D, kTile> tl(tid);
+  for (int s = 0; s < KS; ++s) v[s] = frag_global<D>(vrow, s, lane);
+  const TileLoad<D, kQueries> tl(tid);
+  float stat = 0.f;
   const uint32_t qstride = (uint32_t)(2 * a.q.token), gstride = (uint32_t)(2 * a.dO.token);
-  float aux = 0.f;  // threads 0 .. 63 carry a tile's lse, 64 .. 127 its delta
   const auto load = [&](int i) {
-    const int head = kv * G + i / count, t0 = (tile0 + i % count) * kTile;
+    const int head = kv * G + i / count, t0 = (tile0 + i % count) * kQueries;
     lds_u8* buf = lds + (i & 1) * BUF;
     tl.load(buf, a.q.at(b, head, seq.start + t0), qstride, n - t0, tid);
     tl.load(buf + TB, a.dO.at(b, head, seq.start + t0), gstride, n - t0, tid);
-    if (tid < 2 * kTile) {
-      const int r = tid & (kTile - 1);
-      const float* from = tid < kTile ? a.lse : a.delta;
-      aux = t0 + r < n ? from[((int64_t)b * a.q_heads + head) * a.tokens + seq.start + t0 + r]
-                       : (tid < kTile ? INFINITY : 0.f);
+    if (wave == 0) {  // lanes 0 .. 31 bring the tile's lse, the others its delta
+      const float* from = h ? a.delta : a.lse;
+      stat = t0 + l < n ? from[((int64_t)b * a.q_heads + head) * a.tokens + seq.start + t0 + l] : (h ? 0.f : INFINITY);
     }
   };
   const auto store = [&](int i) {
-    lds_u8* buf = lds + (i & 1) * BUF;
-    if (tid < 2 * kTile) *(__attribute__((address_space(3))) float*)(buf + 2 * TB + 4 * tid) = aux;
+    if (wave == 0) *(__attribute__((address_space(3))) float*)(lds + (i & 1) * BUF + 2 * TB + 4 * lane) = stat;
   };
 
   f32x16_t dk[DT] = {}, dv[DT] = {};
   const float c = a.scale * 1.44269504f;
   if (total > 0) {
+    // rows of the block before the sequence's start or past its end repeat its ends: their columns are dropped
+    const TileLoad<D, 128> kl(tid);
+    kl.load(keys, a.k.at(b, kv, first), (uint32_t)(2 * a.k.token), seq.start + n - first, tid);
     load(0);
     store(0);
   }
   tile_wait();
   __syncthreads();
   for (int it = 0; it < total; ++it) {
-    const int p0 = (tile0 + it % count) * kTile;
-    const lds_u8* qtile = lds + (it & 1) * BUF;
-    const lds_u8* gtile = qtile + TB;
-    const lds_u8* stats = gtile + TB;
+    const int pa = (tile0 + it % count) * kQueries;
     if (it + 1 < total) load(it + 1);
-    if (k0 <= k1) {
-#pragma unroll
-      for (int qb = 0; qb < 2; ++qb) {
-        const int pa = p0 + 32 * qb;
-        if (!any_visible(pa, pa + 31, k0, k1, W, S)) continue;
-        f32x16_t s = {}, dp = {};
-#pragma unroll
-        for (int i = 0; i < KS; ++i) s = mfma32<T>(frag_rows<D>(qtile, 32 * qb, i, lane), k[i], s);
-#pragma unroll
-        for (int i = 0; i < KS; ++i) dp = mfma32<T>(frag_rows<D>(gtile, 32 * qb, i, lane), v[i], dp);
-        if (!all_visible(pa, pa + 31, k0, k1, W, S)) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            s[i] = visible(pa + 8 * (i >> 2) + 4 * h + (i & 3), key, W, S) ? s[i] : -INFINITY;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f32x4_t lse = *(const lds_f32x4*)(stats + 4 * (32 * qb + 8 * e + 4 * h));
-          const f32x4_t delta = *(const lds_f32x4*)(stats + 4 * (kTile + 32 * qb + 8 * e + 4 * h));
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = 4 * e + r;
-            s[i] = exp2_raw(__builtin_fmaf(s[i], c, -lse[r]));
-            dp[i] = s[i] * (dp[i] - delta[r]);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          frag_t pf, sf;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            pf[e] = pack2<T>(s[8 * i + 2 * e], s[8 * i + 2 * e + 1]);
-            sf[e] = pack2<T>(dp[8 * i + 2 * e], dp[8 * i + 2 * e + 1]);
-          }
-#pragma unroll
-          for (int t = 0; t < DT; ++t) dv[t] = mfma32<T>(frag_cols<D>(gtile, 32 * qb + 16 * i, t, lane), pf, dv[t]);
-#pragma unroll
-          for (int t = 0; t < DT; ++t) dk[t] = mfma32<T>(frag_cols<D>(qtile, 32 * qb + 16 * i, t, lane), sf, dk[t]);
-        }
-      }
+    if (k0 <= k1 && any_visible(pa, pa + kQueries - 1, k0, k1, W, S)) {
+      dkv_step<T, D>(lds + (it & 1) * BUF, keys + 32 * wave * (D * 2), v, c,
+                     all_visible(pa, pa + kQueries - 1, k0, k1, W, S),
+                     [&](int i) { return !visible(pa + i, key, W, S); }, dk, dv, lane);
     }
     if (it + 1 < total) store(it + 1);
     tile_wait();
     __syncthreads();
   }
   if (row >= a.tokens) return;
+  if (a.far_chunks && live && key < a.sinks) {  // the far queries' part, in their order
+    const FarPlan far(a, pair, key / 32, n);
+    for (int i = 0; i < far.used; ++i) {
+      const float* from = far.part(a, i) + (int64_t)(key % 32) * D + 4 * h;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            dk[t][4 * e + r] += from[32 * t + 8 * e + r];
+            dv[t][4 * e + r] += from[32 * D + 32 * t + 8 * e + r];
+          }
+    }
+  }
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -446,10 +488,93 @@ __device__ void window_dkv_block(const AttnArgs& a, int id, uint8_t* smem) {
   store_row<T, D>(a.dv.at(b, kv, row), dv, 1.f, lane);
 }
 
+// The sinks' gradients from the queries past their windows: few keys, most queries. A workgroup takes 32 sinks and
+// a chunk of those queries' steps, four at a time, one a wave; its sums go to the workspace in float32 for
+// window_dkv_kernel. Left in the first key block's workgroup, these steps were the kernel's longest path: 585 us
+// against 335 without sinks at 4096 tokens, window 1024.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 1) void window_dkv_kernel(const AttnArgs a) {
-  __shared__ __align__(16) uint8_t smem[2 * (2 * kTile * D * 2 + 2 * kTile * 4)];
-  window_dkv_block<T, D>(a, blockIdx.x, smem);
+__global__ __launch_bounds__(kThreads, 2) void window_far_kernel(const AttnArgs a) {
+  constexpr int KS = D / 16, DT = D / 32, TB = DkvLds<D>::TB, BUF = DkvLds<D>::BUF, KEYS = 32 * D * 2;
+  __shared__ __align__(16) uint8_t smem[KEYS + 4 * BUF];
+  lds_u8* const keys = (lds_u8*)smem;
+  lds_u8* const lds = keys + KEYS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l = lane & 31, h = lane >> 5;
+  const int pairs = a.batch * a.kv_heads, pair = blockIdx.x % pairs;
+  const int chunk = blockIdx.x / pairs % a.far_chunks, block = blockIdx.x / pairs / a.far_chunks;
+  const int b = pair / a.kv_heads, kv = pair % a.kv_heads, G = a.q_heads / a.kv_heads;
+  const Span seq = sequence(a, b);
+  const int W = a.window, n = seq.n, S = min(a.sinks, n);
+  const FarPlan far(a, pair, block, n);
+  if (chunk >= far.used) return;
+  const int key = 32 * block + l;
+
+  frag_t v[KS];
+  const uint8_t* vrow = key < S ? a.v.at(b, kv, seq.start + key) : nullptr;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) v[s] = frag_global<D>(vrow, s, lane);
+  const TileLoad<D, 32> tl(tid);
+  tl.load(keys, a.k.at(b, kv, seq.start + 32 * block), (uint32_t)(2 * a.k.token), S - 32 * block, tid);
+  f32x16_t dk[DT] = {}, dv[DT] = {};
+  const float c = a.scale * 1.44269504f;
+  const int end = min((chunk + 1) * a.far_units, far.units);
+  for (int u0 = chunk * a.far_units; u0 < end; u0 += 4) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int u = min(u0 + w, end - 1), head = kv * G + u / far.tiles, t0 = (far.tile0 + u % far.tiles) * kQueries;
+      lds_u8* buf = lds + w * BUF;
+      tl.load(buf, a.q.at(b, head, seq.start + t0), (uint32_t)(2 * a.q.token), n - t0, tid);
+      tl.load(buf + TB, a.dO.at(b, head, seq.start + t0), (uint32_t)(2 * a.dO.token), n - t0, tid);
+    }
+    const int u = min(u0 + wave, end - 1), head = kv * G + u / far.tiles, t0 = (far.tile0 + u % far.tiles) * kQueries;
+    const float* from = h ? a.delta : a.lse;
+    const float stat =
+        t0 + l < n ? from[((int64_t)b * a.q_heads + head) * a.tokens + seq.start + t0 + l] : (h ? 0.f : INFINITY);
+    *(__attribute__((address_space(3))) float*)(lds + wave * BUF + 2 * TB + 4 * lane) = stat;
+    tile_wait();
+    __syncthreads();
+    if (u0 + wave < end) {
+      dkv_step<T, D>(lds + wave * BUF, keys, v, c, t0 - (32 * block + 31) >= W && 32 * block + 31 < S,
+                     [&](int i) { return t0 + i - key < W || key >= S; }, dk, dv, lane);
+    }
+    __syncthreads();
+  }
+  // the waves' sums: 2 and 3 go to 0 and 1, then 1 to 0
+  float* const sums = (float*)smem;
+  static_assert(4 * 32 * D * 4 <= KEYS + 4 * BUF, "two waves' sums fit");
+#pragma unroll
+  for (int half = 2; half >= 1; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          sums[(((wave - half) * 2 * DT + t) * 16 + i) * 64 + lane] = dk[t][i];
+          sums[(((wave - half) * 2 * DT + DT + t) * 16 + i) * 64 + lane] = dv[t][i];
+        }
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          dk[t][i] += sums[((wave * 2 * DT + t) * 16 + i) * 64 + lane];
+          dv[t][i] += sums[((wave * 2 * DT + DT + t) * 16 + i) * 64 + lane];
+        }
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+  float* to = far.part(a, chunk) + (int64_t)l * D + 4 * h;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      *(f32x4_t*)(to + 32 * t + 8 * e) = (f32x4_t){dk[t][4 * e], dk[t][4 * e + 1], dk[t][4 * e + 2], dk[t][4 * e + 3]};
+      *(f32x4_t*)(to + 32 * D + 32 * t + 8 * e) =
+          (f32x4_t){dv[t][4 * e], dv[t][4 * e + 1], dv[t][4 * e + 2], dv[t][4 * e + 3]};
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -484,6 +609,7 @@ int fill_args(const char* what, AttnArgs* a, int64_t batch, int64_t q_heads, int
   a->window = (int)(window == 0 || window > tokens ? tokens : window);
   a->sinks = (int)(sinks > tokens ? tokens : sinks);
   a->scale = scale;
+  a->dim = (int)dim;
   const int64_t share = q_heads / kv_heads;
   a->pack = share % 4 == 0 ? 4 : share % 2 == 0 ? 2 : 1;
   return PKM_OK;
@@ -494,6 +620,27 @@ unsigned query_blocks(const AttnArgs& a) {
   return (unsigned)(a.batch * (a.q_heads / a.pack) * ((a.tokens + rows - 1) / rows));
 }
 
+// Whether the sinks' far queries get workgroups of their own, and how many: they do where a first key block would
+// otherwise take more than twice the steps of the others. 512 workgroups in all, of 16 steps at least.
+void plan_far(AttnArgs* a) {
+  a->far_chunks = 0;
+  if (a->sinks == 0 || a->tokens <= 2 * ((int64_t)a->window + 128)) return;
+  const int64_t units = (int64_t)((a->tokens - a->window + 31) / 32 + 1) * (a->q_heads / a->kv_heads);
+  const int64_t blocks = (int64_t)a->batch * a->kv_heads * ((a->sinks + 31) / 32);
+  const int64_t chunks = blocks >= 512 ? 1 : 512 / blocks;
+  int64_t each = (units + chunks - 1) / chunks;
+  each = each < 16 ? 16 : (each + 3) / 4 * 4;
+  a->far_units = (int)each;
+  a->far_chunks = (int)((units + each - 1) / each);
+}
+
+int64_t delta_bytes(const AttnArgs& a) {
+  return ((int64_t)a.batch * a.q_heads * a.tokens * (int64_t)sizeof(float) + 15) / 16 * 16;
+}
+int64_t far_bytes(const AttnArgs& a) {
+  return (int64_t)a.batch * a.kv_heads * ((a.sinks + 31) / 32) * a.far_chunks * 2 * 32 * a.dim * (int64_t)sizeof(float);
+}
+
 template <typename T, int D>
 void launch_fwd(const AttnArgs& a, hipStream_t st) {
   window_fwd_kernel<T, D><<<query_blocks(a), kThreads, 0, st>>>(a);
@@ -502,6 +649,10 @@ void launch_fwd(const AttnArgs& a, hipStream_t st) {
 template <typename T, int D>
 void launch_bwd(const AttnArgs& a, hipStream_t st) {
   window_dq_kernel<T, D><<<query_blocks(a), kThreads, 0, st>>>(a);  // and delta
+  if (a.far_chunks) {
+    const unsigned grid = (unsigned)(a.batch * a.kv_heads * ((a.sinks + 31) / 32) * a.far_chunks);
+    window_far_kernel<T, D><<<grid, kThreads, 0, st>>>(a);
+  }
   window_dkv_kernel<T, D><<<(unsigned)(a.batch * a.kv_heads * ((a.tokens + 127) / 128)), kThreads, 0, st>>>(a);
 }
 
@@ -535,8 +686,13 @@ extern "C" int pkm_window_attn_fwd(const pkm_heads_t* q, const pkm_heads_t* k, c
 
 extern "C" size_t pkm_window_attn_bwd_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
                                                      int64_t dim, int64_t window, int64_t sinks) {
-  (void)kv_heads, (void)dim, (void)window, (void)sinks;
-  return batch <= 0 || q_heads <= 0 || tokens <= 0 ? 0 : (size_t)(batch * q_heads * tokens) * sizeof(float);
+  AttnArgs a = {};
+  if (batch <= 0 || tokens <= 0 ||
+      fill_args("pkm_window_attn_bwd_workspace_size", &a, batch, q_heads, kv_heads, tokens, dim, PKM_DTYPE_BF16, window,
+                sinks, 1.f) != PKM_OK)
+    return 0;
+  plan_far(&a);
+  return (size_t)(delta_bytes(a) + far_bytes(a));
 }
 
 extern "C" int pkm_window_attn_bwd(const pkm_heads_t* q, const pkm_heads_t* k, const pkm_heads_t* v,
@@ -555,11 +711,14 @@ extern "C" int pkm_window_attn_bwd(const pkm_heads_t* q, const pkm_heads_t* k, c
       (rc = check_heads(what, "dq", dq)) || (rc = check_heads(what, "dk", dk)) || (rc = check_heads(what, "dv", dv)))
     return rc;
   PKM_REQUIRE(lse != nullptr, PKM_ERR_INVALID_ARGUMENT, "%s: lse is NULL", what);
-  PKM_REQUIRE(workspace != nullptr && workspace_bytes >= pkm_window_attn_bwd_workspace_size(batch, q_heads, kv_heads, tokens, dim, window, sinks),
-              PKM_ERR_WORKSPACE, "%s: workspace too small", what);
+  plan_far(&a);
+  PKM_REQUIRE(workspace != nullptr && workspace_bytes >= (size_t)(delta_bytes(a) + far_bytes(a)), PKM_ERR_WORKSPACE,
+              "%s: workspace too small", what);
+  PKM_REQUIRE(((uintptr_t)workspace & 15) == 0, PKM_ERR_INVALID_ARGUMENT, "%s: workspace is not 16-byte aligned", what);
   a.q = heads(q), a.k = heads(k), a.v = heads(v), a.o = heads(out), a.dO = heads(grad_out);
   a.dq = heads(dq), a.dk = heads(dk), a.dv = heads(dv);
   a.starts = starts, a.ends = ends, a.lse = const_cast<float*>(lse), a.delta = (float*)workspace;
+  a.far = (float*)((uint8_t*)workspace + delta_bytes(a));
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == PKM_DTYPE_BF16) {
     dim == 128 ? launch_bwd<bf16_t, 128>(a, st) : launch_bwd<bf16_t, 64>(a, st);

@@ -75,6 +75,19 @@ def test_padding_is_not_used(device, dtype, D, window, sinks):
         assert (g[6] == 0).all() and (g[1, :, :37] == 0).all() and (g[2, :, 64:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype,D", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("window,sinks", [(30, 40), (64, 3), (1, 1)])
+def test_sinks_of_padded_long_sequences(device, dtype, D, window, sinks):
+    """Sinks whose far queries have workgroups of their own, in sequences that start and end anywhere."""
+    starts, ends = [0, 101, 0, 250, 500], [600, 600, 333, 290, 600]
+    q, k, v, do = _inputs(len(starts), 600, 4, 2, D, dtype, seed=17)
+    for b in range(len(starts)):
+        for x in (q, k, v, do):
+            x[b, :, : starts[b]] = NAN
+            x[b, :, ends[b] :] = NAN
+    _check(device, q, k, v, do, window, sinks, starts, ends)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
 def test_strides(device, dtype):
     """Heads inside a fused projection, contiguous, expanded, unaligned and sliced: the same numbers every time."""
