@@ -93,21 +93,31 @@ __device__ __forceinline__ int tile_offset(int row, int chunk) {
   return row * (D * 2) + ((chunk ^ f) << 4);
 }
 
-// A operand whose rows are the tile's rows row0 .. row0 + 31, k step s of 16 numbers.
+// Where a lane's operands lie in a tile: the first k step's (rows_at) and the first 32 columns' (cols_at). The others
+// are an xor away, as the permutation is one: tiles start at multiples of 256 bytes.
 template <int D>
-__device__ __forceinline__ frag_t frag_rows(const lds_u8* tile, int row0, int s, int lane) {
-  return *(const lds_u32x4*)(tile + row0 * (D * 2) + tile_offset<D>(lane & 31, 2 * s + (lane >> 5)));
+__device__ __forceinline__ uint32_t rows_at(int lane) {
+  return tile_offset<D>(lane & 31, lane >> 5);
+}
+template <int D>
+__device__ __forceinline__ uint32_t cols_at(int lane) {
+  const int l = lane & 15, h = lane >> 5, g = (lane >> 4) & 1;
+  return tile_offset<D>(4 * h + (l >> 2), 2 * g + ((l & 3) >> 1)) + (l & 1) * 8;
+}
+
+// A operand whose rows are the tile's rows row0 .. row0 + 31, k step s of 16 numbers. at: the tile + rows_at.
+template <int D>
+__device__ __forceinline__ frag_t frag_rows(uint32_t at, int row0, int s) {
+  return *(const lds_u32x4*)(uintptr_t)((at ^ (uint32_t)(s << 5)) + row0 * (D * 2));
 }
 
 // A operand whose rows are the tile's columns 32 t .. 32 t + 31 and whose k are the tile's rows
-// row0 + 8 (j / 4) + 4 h + j % 4 (the order of a C tile used as B operand).
+// row0 + 8 (j / 4) + 4 h + j % 4 (the order of a C tile used as B operand). at: the tile + cols_at.
 template <int D>
-__device__ __forceinline__ frag_t frag_cols(const lds_u8* tile, int row0, int t, int lane) {
-  const int l = lane & 15, h = lane >> 5, g = (lane >> 4) & 1;
-  const int row = 4 * h + (l >> 2), chunk = 4 * t + 2 * g + ((l & 3) >> 1);
-  const lds_u8* base = tile + row0 * (D * 2) + (l & 1) * 8;
-  const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + tile_offset<D>(row, chunk)));
-  const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + tile_offset<D>(row + 8, chunk)));
+__device__ __forceinline__ frag_t frag_cols(uint32_t at, int row0, int t) {
+  const uint32_t p = (at ^ (uint32_t)(t << 6)) + row0 * (D * 2), q = (at ^ (uint32_t)((t << 6) | 32)) + (row0 + 8) * (D * 2);
+  const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)p);
+  const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)q);
   const u32x2_t x = __builtin_bit_cast(u32x2_t, a), y = __builtin_bit_cast(u32x2_t, b);
   return (frag_t){x[0], x[1], y[0], y[1]};
 }
@@ -127,18 +137,19 @@ __device__ __forceinline__ void load_lds16(u32x4_t rsrc, lds_u8* to, uint32_t of
                : "memory");
 }
 
-// A tile's rows from global memory straight to LDS (no registers in between), by 256 threads. A wave's load
+// A tile's rows from global memory straight to LDS (no registers in between), by WAVES waves. A wave's load
 // writes 64 chunks of 16 bytes side by side; the permutation is in the addresses that the lanes read. Rows from
 // `last` (>= 1) on repeat row last - 1: what lies outside a sequence is never read. The loads are complete after
 // tile_wait().
-template <int D, int ROWS>
+template <int D, int ROWS, int WAVES = 4>
 struct TileLoad {
-  static constexpr int CH = D / 8, PER = 64 / CH, N = ROWS / PER / 4;  // rows and loads of a wave
+  static constexpr int CH = D / 8, PER = 64 / CH, N = ROWS / PER / WAVES;  // rows of a load, loads of a wave
+  static_assert(PER * WAVES % 16 == 0 && N * PER * WAVES == ROWS, "one permutation a lane");
   int row, chunk;  // the lane's first row and its bytes within a row
   __device__ __forceinline__ TileLoad(int tid) {
     const int wave = tid >> 6, lane = tid & 63;
     row = wave * PER + lane / CH;
-    // rows of one lane are 4 PER apart, a multiple of 16: one permutation
+    // rows of one lane are WAVES PER apart, a multiple of 16: one permutation
     chunk = tile_offset<D>(row, lane % CH) - row * (D * 2);
   }
   // base: row 0 of the tile; stride in bytes (128 rows of it fit in 31 bits)
@@ -147,17 +158,30 @@ struct TileLoad {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      load_lds16(rs, tile + (wave + 4 * i) * 1024, (uint32_t)min(row + 4 * PER * i, last - 1) * stride + chunk);
+      load_lds16(rs, tile + (wave + WAVES * i) * 1024,
+                 (uint32_t)min(row + WAVES * PER * i, last - 1) * stride + chunk);
   }
 };
-static_assert(TileLoad<128, 64>::PER * 4 % 16 == 0 && TileLoad<64, 64>::PER * 4 % 16 == 0, "one permutation a lane");
+// 64 lanes' float each, as load_lds16.
+__device__ __forceinline__ void load_lds4(u32x4_t rsrc, lds_u8* to, uint32_t offset) {
+  asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"{m0}"((uint32_t)(uintptr_t)to), "v"(offset), "s"(rsrc)
+               : "memory");
+}
 
-// Waits for the wave's loads to LDS.
+// Waits for the wave's loads to LDS but the last N.
+template <int N = 0>
 __device__ __forceinline__ void tile_wait() {
+  static_assert(N < 16, "the low four bits of the count");
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), which the compiler's own counting sees
+  __builtin_amdgcn_s_waitcnt(0x0f70 | N);  // vmcnt(N), which the compiler's own counting sees
   asm volatile("" ::: "memory");
 }
+
+// A point that the compiler moves no LDS read and no matrix instruction across: the loops below issue the reads of
+// a later product in front of each product, and its scheduler would pull them back behind it.
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x0406); }
+
+__device__ __forceinline__ uint32_t lds_address(const lds_u8* p) { return (uint32_t)(uintptr_t)p; }
 
 // A [batch, heads, tokens, dim] tensor in a kernel's arguments, strides in elements (pkm_heads_t of the C ABI).
 struct Heads {

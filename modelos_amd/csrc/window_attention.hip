@@ -107,7 +107,7 @@ struct QueryBlock {
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs a) {
   constexpr int KS = D / 16, DT = D / 32, TB = kTile * D * 2;
-  __shared__ __align__(16) uint8_t smem[2 * 2 * TB];
+  __shared__ __align__(256) uint8_t smem[2 * 2 * TB];
   lds_u8* const lds = (lds_u8*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l = lane & 31, h = lane >> 5;
@@ -144,8 +144,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
   __syncthreads();
   for (int it = 0; it < tiles.count; ++it) {
     const int j0 = tiles.tile(it) * kTile;
-    const lds_u8* ktile = lds + (it & 1) * 2 * TB;
-    const lds_u8* vtile = ktile + TB;
+    const uint32_t tile = lds_address(lds) + (it & 1) * 2 * TB;
+    const uint32_t krows = tile + rows_at<D>(lane), vcols = tile + TB + cols_at<D>(lane);
     if (it + 1 < tiles.count) {
       const int t1 = tiles.tile(it + 1) * kTile;
       lds_u8* next = lds + ((it + 1) & 1) * 2 * TB;
@@ -154,10 +154,26 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
     }
     if (p0 <= p1 && any_visible(p0, p1, j0, j0 + kTile - 1, W, S)) {
       f32x16_t s[2] = {};
+      frag_t f0[3], f1[3];
+      const auto rows = [&](int i) {
+        f0[i % 3] = frag_rows<D>(krows, 0, i);
+        f1[i % 3] = frag_rows<D>(krows, 32, i);
+      };
+      rows(0);
+      rows(1);
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < KS; ++i) s[kb] = mfma32<T>(frag_rows<D>(ktile, 32 * kb, i, lane), q[i], s[kb]);
+      for (int i = 0; i < KS; ++i) {
+        if (i + 2 < KS) rows(i + 2);
+        keep_order();
+        s[0] = mfma32<T>(f0[i % 3], q[i], s[0]);
+        s[1] = mfma32<T>(f1[i % 3], q[i], s[1]);
+        keep_order();
+      }
+      frag_t fv[4];
+      const auto cols = [&](int i) { fv[i % 4] = frag_cols<D>(vcols, 16 * (i / DT), i % DT); };
+      cols(0);
+      cols(1);
+      cols(2);
       if (!all_visible(p0, p1, j0, j0 + kTile - 1, W, S)) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -193,9 +209,12 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
         for (int i = 0; i < 8; ++i) pf[2 * kb + i / 4][i % 4] = pack2<T>(s[kb][2 * i], s[kb][2 * i + 1]);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[t] = mfma32<T>(frag_cols<D>(vtile, 16 * i, t, lane), pf[i], o[t]);
+      for (int i = 0; i < 4 * DT; ++i) {
+        if (i + 3 < 4 * DT) cols(i + 3);
+        keep_order();
+        o[i % DT] = mfma32<T>(fv[i % 4], pf[i / DT], o[i % DT]);
+        keep_order();
+      }
     }
     tile_wait();
     __syncthreads();
@@ -227,7 +246,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a) {
   constexpr int KS = D / 16, DT = D / 32, TB = kTile * D * 2;
-  __shared__ __align__(16) uint8_t smem[2 * 2 * TB];
+  __shared__ __align__(256) uint8_t smem[2 * 2 * TB];
   lds_u8* const lds = (lds_u8*)smem;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l = lane & 31, h = lane >> 5;
@@ -273,8 +292,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
   __syncthreads();
   for (int it = 0; it < tiles.count; ++it) {
     const int j0 = tiles.tile(it) * kTile;
-    const lds_u8* ktile = lds + (it & 1) * 2 * TB;
-    const lds_u8* vtile = ktile + TB;
+    const uint32_t tile = lds_address(lds) + (it & 1) * 2 * TB;
+    const uint32_t krows = tile + rows_at<D>(lane), vrows = krows + TB, kcols = tile + cols_at<D>(lane);
     if (it + 1 < tiles.count) {
       const int t1 = tiles.tile(it + 1) * kTile;
       lds_u8* next = lds + ((it + 1) & 1) * 2 * TB;
@@ -287,10 +306,24 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
         const int ja = j0 + 32 * kb;
         if (!any_visible(p0, p1, ja, ja + 31, W, S)) continue;
         f32x16_t s = {}, dp = {};
+        frag_t fk[3], fv[3];
+        const auto rows = [&](int i) {
+          fk[i % 3] = frag_rows<D>(krows, 32 * kb, i);
+          fv[i % 3] = frag_rows<D>(vrows, 32 * kb, i);
+        };
+        rows(0);
+        rows(1);
 #pragma unroll
-        for (int i = 0; i < KS; ++i) s = mfma32<T>(frag_rows<D>(ktile, 32 * kb, i, lane), q[i], s);
-#pragma unroll
-        for (int i = 0; i < KS; ++i) dp = mfma32<T>(frag_rows<D>(vtile, 32 * kb, i, lane), g[i], dp);
+        for (int i = 0; i < KS; ++i) {
+          if (i + 2 < KS) rows(i + 2);
+          keep_order();
+          s = mfma32<T>(fk[i % 3], q[i], s);
+          dp = mfma32<T>(fv[i % 3], g[i], dp);
+          keep_order();
+        }
+        const auto cols = [&](int i) { fk[i % 3] = frag_cols<D>(kcols, 32 * kb + 16 * (i / DT), i % DT); };
+        cols(0);
+        cols(1);
         if (!all_visible(p0, p1, ja, ja + 31, W, S)) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -301,21 +334,22 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
           s[i] = exp2_raw(__builtin_fmaf(s[i], c, -lse)) * (dp[i] - delta);
           sum += s[i];
         }
+        frag_t f[2], r[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          frag_t f, r;
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = s[8 * i + 2 * e], y = s[8 * i + 2 * e + 1];
-            f[e] = pack2<T>(x, y);
-            r[e] = pack2<T>(x - unpack1<T>(f[e] & 0xffffu), y - unpack1<T>(f[e] >> 16));
+            f[i][e] = pack2<T>(x, y);
+            r[i][e] = pack2<T>(x - unpack1<T>(f[i][e] & 0xffffu), y - unpack1<T>(f[i][e] >> 16));
           }
 #pragma unroll
-          for (int t = 0; t < DT; ++t) {
-            const frag_t kt = frag_cols<D>(ktile, 32 * kb + 16 * i, t, lane);
-            dq[t] = mfma32<T>(kt, f, dq[t]);
-            dq[t] = mfma32<T>(kt, r, dq[t]);
-          }
+        for (int i = 0; i < 2 * DT; ++i) {
+          if (i + 2 < 2 * DT) cols(i + 2);
+          keep_order();
+          dq[i % DT] = mfma32<T>(fk[i % 3], f[i / DT], dq[i % DT]);
+          dq[i % DT] = mfma32<T>(fk[i % 3], r[i / DT], dq[i % DT]);
+          keep_order();
         }
       }
     }
@@ -333,41 +367,62 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
 }
 
 // ---------------------------------------------------------------------------
-// Backward, dK and dV: 4 waves of 32 keys each; the tiles hold 32 queries and
+// Backward, dK and dV: 128 keys a workgroup; the tiles hold 64 queries and
 // their dO, of every query head of the key head in turn (a shared head's
-// gradient is summed in registers, in a fixed order). The keys stay in LDS and the
+// gradient is summed in registers, in a fixed order). Of the 8 waves, 4 take 32
+// keys each with the tiles' first 32 queries, 4 the same with the second. The keys stay in LDS and the
 // values in registers: with both in registers a wave needs more than the 256
-// that let two waves share a SIMD.
+// that let two waves share a SIMD. Three stages of tiles, two of them on their way.
 // ---------------------------------------------------------------------------
 constexpr int kQueries = 32;
 template <int D>
 struct DkvLds {
-  static constexpr int TB = kQueries * D * 2, BUF = 2 * TB + 2 * kQueries * 4, KEYS = 128 * D * 2;
-  static constexpr int BYTES = KEYS + 2 * BUF;
+  static constexpr int TB = kQueries * D * 2, BUF = 2 * TB + 2 * kQueries * 4;  // a step's
 };
 
-// One step: 32 queries at [buf, their dO behind them, then lse and delta], the wave's 32 keys in LDS, their values v.
+// One step: 32 queries, their dO, lse and delta, and the wave's 32 keys in LDS, their values v.
 // masked(i): the row i of the lane's column is not visible; all: none is masked.
 template <typename T, int D, typename F>
-__device__ __forceinline__ void dkv_step(const lds_u8* buf, const lds_u8* keys, const frag_t (&v)[D / 16], float c,
+__device__ __forceinline__ void dkv_step(const lds_u8* qtile, const lds_u8* gtile, const lds_u8* lses,
+                                         const lds_u8* deltas, const lds_u8* keys, const frag_t (&v)[D / 16], float c,
                                          bool all, F masked, f32x16_t (&dk)[D / 32], f32x16_t (&dv)[D / 32], int lane) {
-  constexpr int KS = D / 16, DT = D / 32, TB = DkvLds<D>::TB;
+  constexpr int KS = D / 16, DT = D / 32;
+  asm volatile("" : "+v"(lane));  // the addresses below are worked out anew in each step: kept over the loop, they spill
   const int h = lane >> 5;
-  const lds_u8* const gtile = buf + TB;
-  const lds_u8* const stats = gtile + TB;
+  const uint32_t at = rows_at<D>(lane), qrows = lds_address(qtile) + at, grows = lds_address(gtile) + at;
+  const uint32_t krows = lds_address(keys) + at;
   f32x16_t s = {}, dp = {};
+  frag_t fq[3], fk[3], fg[3];
+  const auto rows = [&](int i) {
+    fq[i % 3] = frag_rows<D>(qrows, 0, i);
+    fk[i % 3] = frag_rows<D>(krows, 0, i);
+    fg[i % 3] = frag_rows<D>(grows, 0, i);
+  };
+  rows(0);
+  rows(1);
 #pragma unroll
-  for (int i = 0; i < KS; ++i) s = mfma32<T>(frag_rows<D>(buf, 0, i, lane), frag_rows<D>(keys, 0, i, lane), s);
-#pragma unroll
-  for (int i = 0; i < KS; ++i) dp = mfma32<T>(frag_rows<D>(gtile, 0, i, lane), v[i], dp);
+  for (int i = 0; i < KS; ++i) {
+    if (i + 2 < KS) rows(i + 2);
+    keep_order();
+    s = mfma32<T>(fq[i % 3], fk[i % 3], s);
+    dp = mfma32<T>(fg[i % 3], v[i], dp);
+    keep_order();
+  }
+  const uint32_t qcols = lds_address(qtile) + cols_at<D>(lane), gcols = lds_address(gtile) + cols_at<D>(lane);
+  const auto cols = [&](int i) {
+    fg[i % 3] = frag_cols<D>(gcols, 16 * (i / DT), i % DT);
+    fq[i % 3] = frag_cols<D>(qcols, 16 * (i / DT), i % DT);
+  };
+  cols(0);
+  cols(1);
   if (!all) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = masked(8 * (i >> 2) + 4 * h + (i & 3)) ? -INFINITY : s[i];
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const f32x4_t lse = *(const lds_f32x4*)(stats + 4 * (8 * e + 4 * h));
-    const f32x4_t delta = *(const lds_f32x4*)(stats + 4 * (kQueries + 8 * e + 4 * h));
+    const f32x4_t lse = *(const lds_f32x4*)(lses + 4 * (8 * e + 4 * h));
+    const f32x4_t delta = *(const lds_f32x4*)(deltas + 4 * (8 * e + 4 * h));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 4 * e + r;
@@ -375,45 +430,49 @@ __device__ __forceinline__ void dkv_step(const lds_u8* buf, const lds_u8* keys, 
       dp[i] = s[i] * (dp[i] - delta[r]);
     }
   }
+  frag_t pf[2], sf[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    frag_t pf, sf;
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      pf[e] = pack2<T>(s[8 * i + 2 * e], s[8 * i + 2 * e + 1]);
-      sf[e] = pack2<T>(dp[8 * i + 2 * e], dp[8 * i + 2 * e + 1]);
+      pf[i][e] = pack2<T>(s[8 * i + 2 * e], s[8 * i + 2 * e + 1]);
+      sf[i][e] = pack2<T>(dp[8 * i + 2 * e], dp[8 * i + 2 * e + 1]);
     }
 #pragma unroll
-    for (int t = 0; t < DT; ++t) dv[t] = mfma32<T>(frag_cols<D>(gtile, 16 * i, t, lane), pf, dv[t]);
-#pragma unroll
-    for (int t = 0; t < DT; ++t) dk[t] = mfma32<T>(frag_cols<D>(buf, 16 * i, t, lane), sf, dk[t]);
+  for (int i = 0; i < 2 * DT; ++i) {
+    if (i + 2 < 2 * DT) cols(i + 2);
+    keep_order();
+    dv[i % DT] = mfma32<T>(fg[i % 3], pf[i / DT], dv[i % DT]);
+    dk[i % DT] = mfma32<T>(fq[i % 3], sf[i / DT], dk[i % DT]);
+    keep_order();
   }
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void window_dkv_kernel(const AttnArgs a) {
-  constexpr int KS = D / 16, DT = D / 32, TB = DkvLds<D>::TB, BUF = DkvLds<D>::BUF;
-  __shared__ __align__(16) uint8_t smem[DkvLds<D>::BYTES];
+__global__ __launch_bounds__(512, 2) void window_dkv_kernel(const AttnArgs a) {
+  constexpr int KS = D / 16, DT = D / 32, TB = kTile * D * 2, KEYS = 128 * D * 2;
+  constexpr int STAGE = 2 * TB + 8 * 256, LOADS = 2 * TileLoad<D, kTile, 8>::N + 1;  // a wave's loads of a stage
+  __shared__ __align__(256) uint8_t smem[KEYS + 3 * STAGE];
   lds_u8* const keys = (lds_u8*)smem;
-  lds_u8* const lds = keys + DkvLds<D>::KEYS;
+  lds_u8* const lds = keys + KEYS;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l = lane & 31, h = lane >> 5;
+  const int l = lane & 31, h = lane >> 5, kw = wave & 3, qw = wave >> 2;
   const int pairs = a.batch * a.kv_heads, pair = blockIdx.x % pairs;
   const int b = pair / a.kv_heads, kv = pair % a.kv_heads, G = a.q_heads / a.kv_heads;
   const int first = blockIdx.x / pairs * 128;  // the key block's rows; the first ones are read by most queries
   const Span seq = sequence(a, b);
   const int W = a.window, S = a.far_chunks ? 0 : a.sinks, n = seq.n;
-  const int row = first + 32 * wave + l;
+  const int row = first + 32 * kw + l;
   const int key = row - seq.start;
   const bool live = row < a.tokens && key >= 0 && key < n;
-  const int k0 = max(first + 32 * wave - seq.start, 0), k1 = min(first + 32 * wave + 31 - seq.start, n - 1);
+  const int k0 = max(first + 32 * kw - seq.start, 0), k1 = min(first + 32 * kw + 31 - seq.start, n - 1);
   // the queries that see the block: from its first key to the window's end of its last, or all of them
   const int b0 = max(first - seq.start, 0), b1 = min(first + 127 - seq.start, n - 1);
   int tile0 = 0, count = 0;
   if (b0 <= b1) {
     const int last = b0 < S ? n - 1 : min(n - 1, b1 + W - 1);
-    tile0 = b0 / kQueries;
-    count = last / kQueries + 1 - tile0;
+    tile0 = b0 / kTile;
+    count = last / kTile + 1 - tile0;
   }
   const int total = count * G;
 
@@ -421,47 +480,71 @@ __global__ __launch_bounds__(kThreads, 2) void window_dkv_kernel(const AttnArgs 
   const uint8_t* vrow = live ? a.v.at(b, kv, row) : nullptr;
 #pragma unroll
   for (int s = 0; s < KS; ++s) v[s] = frag_global<D>(vrow, s, lane);
-  const TileLoad<D, kQueries> tl(tid);
-  float stat = 0.f;
+  const TileLoad<D, kTile, 8> tl(tid);
   const uint32_t qstride = (uint32_t)(2 * a.q.token), gstride = (uint32_t)(2 * a.dO.token);
   const auto load = [&](int i) {
-    const int head = kv * G + i / count, t0 = (tile0 + i % count) * kQueries;
-    lds_u8* buf = lds + (i & 1) * BUF;
+    const int head = kv * G + i / count, t0 = (tile0 + i % count) * kTile;
+    lds_u8* buf = lds + i % 3 * STAGE;
     tl.load(buf, a.q.at(b, head, seq.start + t0), qstride, n - t0, tid);
     tl.load(buf + TB, a.dO.at(b, head, seq.start + t0), gstride, n - t0, tid);
-    if (wave == 0) {  // lanes 0 .. 31 bring the tile's lse, the others its delta
-      const float* from = h ? a.delta : a.lse;
-      stat = t0 + l < n ? from[((int64_t)b * a.q_heads + head) * a.tokens + seq.start + t0 + l] : (h ? 0.f : INFINITY);
-    }
-  };
-  const auto store = [&](int i) {
-    if (wave == 0) *(__attribute__((address_space(3))) float*)(lds + (i & 1) * BUF + 2 * TB + 4 * lane) = stat;
+    // 64 rows' lse by wave 0, delta by wave 1; the other waves load lse too, to where nobody reads it, so that
+    // every wave has as many loads in flight
+    const float* from = (wave == 1 ? a.delta : a.lse) + ((int64_t)b * a.q_heads + head) * a.tokens + seq.start + t0;
+    const u32x4_t rs = {(uint32_t)(uintptr_t)from, (uint32_t)((uintptr_t)from >> 32), 0x7fffffffu, 0x00020000u};
+    load_lds4(rs, buf + 2 * TB + 256 * wave, 4 * (uint32_t)min(lane, n - t0 - 1));
   };
 
   f32x16_t dk[DT] = {}, dv[DT] = {};
   const float c = a.scale * 1.44269504f;
   if (total > 0) {
     // rows of the block before the sequence's start or past its end repeat its ends: their columns are dropped
-    const TileLoad<D, 128> kl(tid);
+    const TileLoad<D, 128, 8> kl(tid);
     kl.load(keys, a.k.at(b, kv, first), (uint32_t)(2 * a.k.token), seq.start + n - first, tid);
     load(0);
-    store(0);
+    if (total > 1) load(1);
   }
-  tile_wait();
-  __syncthreads();
+  tile_wait();  // and for v: the compiler does not know of the loads to LDS and would wait for them at its use
   for (int it = 0; it < total; ++it) {
-    const int pa = (tile0 + it % count) * kQueries;
-    if (it + 1 < total) load(it + 1);
-    if (k0 <= k1 && any_visible(pa, pa + kQueries - 1, k0, k1, W, S)) {
-      dkv_step<T, D>(lds + (it & 1) * BUF, keys + 32 * wave * (D * 2), v, c,
-                     all_visible(pa, pa + kQueries - 1, k0, k1, W, S),
-                     [&](int i) { return !visible(pa + i, key, W, S); }, dk, dv, lane);
+    // stage it has come, of every wave's loads; stage it - 1 is read no more
+    if (it + 1 < total) {
+      tile_wait<LOADS>();
+    } else {
+      tile_wait();
     }
-    if (it + 1 < total) store(it + 1);
-    tile_wait();
-    __syncthreads();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (it + 2 < total) load(it + 2);
+    const int pa = (tile0 + it % count) * kTile + kQueries * qw;
+    if (k0 <= k1 && any_visible(pa, pa + kQueries - 1, k0, k1, W, S)) {
+      const lds_u8* buf = lds + it % 3 * STAGE;
+      dkv_step<T, D>(buf + TB / 2 * qw, buf + TB + TB / 2 * qw, buf + 2 * TB + 128 * qw, buf + 2 * TB + 256 + 128 * qw,
+                     keys + 32 * kw * (D * 2), v, c,
+                     pa + kQueries <= n && all_visible(pa, pa + kQueries - 1, k0, k1, W, S),
+                     [&](int i) { return !(pa + i < n && visible(pa + i, key, W, S)); }, dk, dv, lane);
+    }
   }
-  if (row >= a.tokens) return;
+  // the two query halves' sums
+  __syncthreads();
+  static_assert(4 * 2 * 32 * D * 4 <= KEYS + 3 * STAGE, "four waves' sums fit");
+  float* const sums = (float*)smem + kw * (2 * 32 * D) + lane;
+  if (qw == 1) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        sums[(t * 16 + i) * 64] = dk[t][i];
+        sums[((DT + t) * 16 + i) * 64] = dv[t][i];
+      }
+  }
+  __syncthreads();
+  if (qw == 1 || row >= a.tokens) return;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      dk[t][i] += sums[(t * 16 + i) * 64];
+      dv[t][i] += sums[((DT + t) * 16 + i) * 64];
+    }
   if (a.far_chunks && live && key < a.sinks) {  // the far queries' part, in their order
     const FarPlan far(a, pair, key / 32, n);
     for (int i = 0; i < far.used; ++i) {
@@ -495,7 +578,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_dkv_kernel(const AttnArgs 
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_far_kernel(const AttnArgs a) {
   constexpr int KS = D / 16, DT = D / 32, TB = DkvLds<D>::TB, BUF = DkvLds<D>::BUF, KEYS = 32 * D * 2;
-  __shared__ __align__(16) uint8_t smem[KEYS + 4 * BUF];
+  __shared__ __align__(256) uint8_t smem[KEYS + 4 * BUF];
   lds_u8* const keys = (lds_u8*)smem;
   lds_u8* const lds = keys + KEYS;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -534,7 +617,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_far_kernel(const AttnArgs 
     tile_wait();
     __syncthreads();
     if (u0 + wave < end) {
-      dkv_step<T, D>(lds + wave * BUF, keys, v, c, t0 - (32 * block + 31) >= W && 32 * block + 31 < S,
+      const lds_u8* buf = lds + wave * BUF;
+      dkv_step<T, D>(buf, buf + TB, buf + 2 * TB, buf + 2 * TB + 4 * kQueries, keys, v, c, t0 - (32 * block + 31) >= W && 32 * block + 31 < S,
                      [&](int i) { return t0 + i - key < W || key >= S; }, dk, dv, lane);
     }
     __syncthreads();
@@ -653,7 +737,7 @@ void launch_bwd(const AttnArgs& a, hipStream_t st) {
     const unsigned grid = (unsigned)(a.batch * a.kv_heads * ((a.sinks + 31) / 32) * a.far_chunks);
     window_far_kernel<T, D><<<grid, kThreads, 0, st>>>(a);
   }
-  window_dkv_kernel<T, D><<<(unsigned)(a.batch * a.kv_heads * ((a.tokens + 127) / 128)), kThreads, 0, st>>>(a);
+  window_dkv_kernel<T, D><<<(unsigned)(a.batch * a.kv_heads * ((a.tokens + 127) / 128)), 512, 0, st>>>(a);
 }
 
 }  // namespace
