@@ -191,6 +191,7 @@ struct AttendArgs {
   int batch, q_heads, queries;
   int window, sinks;  // window 0: none
   int per, splits;    // tiles of a workgroup; workgroups of a row block
+  int shift;          // log2 of the page, -1 if it is no power of two
   float scale;
 };
 
@@ -208,14 +209,19 @@ struct CacheTiles {
   __device__ __forceinline__ int tile(int i) const { return i < sink ? i : i + near; }
 };
 
-// Codes at bits 4 k of both halves of x as numbers 16 + c of type T.
-template <typename T>
+// Codes at bits 4 k of both halves of x as f16 numbers c 2^-24 (k even) or c 2^-20 (k odd): subnormal numbers,
+// whose fraction they are. The matrix instructions take them exactly, so there is no conversion and no offset to
+// take off again.
 __device__ __forceinline__ uint32_t code_pair(uint32_t x, int k) {
-  constexpr bool bf = __is_same(T, bf16_t);
-  constexpr int at = bf ? 3 : 6;  // the lowest bit of a unit in 16 .. 32
-  const int s = 4 * k - at;
-  const uint32_t y = s >= 0 ? x >> s : x << -s;
-  return (y & (bf ? 0x00780078u : 0x03c003c0u)) | (bf ? 0x41804180u : 0x4c004c00u);
+  return (k & 2 ? x >> 8 : x) & (k & 1 ? 0x00f000f0u : 0x000f000fu);
+}
+constexpr float kEven = 16777216.f, kOdd = 1048576.f;  // 2^24, 2^20
+
+// x to a packed pair of T (f) and what is left of it (r)
+template <typename T>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t* f, uint32_t* r) {
+  *f = pack2<T>(x, y);
+  *r = pack2<T>(x - unpack1<T>(*f & 0xffffu), y - unpack1<T>(*f >> 16));
 }
 
 // One tile as it is loaded.
@@ -226,10 +232,21 @@ struct RawTile {
   u32x2_t p[2];           // 4 tokens of one row of params, K and V
 };
 
+// S = q K^T over codes: with q K = sum_g s_g (q c)_g + m_g (sum q)_g the codes go into the matrix instructions as they
+// are, and the steps and minima touch 16 x 16 results instead of 16 x D numbers. O = P V the same way round: the weights
+// take the values' steps, sum_t (p_t s_tg) c_t + sum_t p_t m_tg. A wave takes tiles of 32 tokens in turn, with its own
+// running maximum and sums; waves and workgroups are joined at the end.
+//
+// q is scaled to below 2^14 by a power of two per row, exactly but for numbers 2^-28 of the row's largest. The weights with
+// steps are f16, kept near 1 by the exponent `lift` of the largest step in the reference the exponentials are taken from
+// (relative rounding 2^-12 against the 2^-9 of a bf16 result; f16 results add the product with what the rounding left).
+// The weights of the minima are two 16-bit numbers of the cache's type: minimum and step often
+// cancel in a value, so one rounding of each would count several times.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void kv4_attend_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArgs a) {
   constexpr int NG = D / 32, NB = D / 16;
   constexpr int kPad = D + 4;
+  constexpr bool kTwo = __is_same(T, f16_t);
   __shared__ __align__(16) float merge[4][kRows][kPad];
   __shared__ float stats[4][2][kRows];
   __shared__ __align__(16) uint16_t params[4][2][2 * NG][kTok];
@@ -252,111 +269,159 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_kernel(const AttendArg
   const int p0 = n - Q, p1 = n - 1;
   const int W = a.window ? a.window : 0x7fffffff, S = a.sinks;
 
-  // q as B operand, numbers in the codes' order; its sums over the groups
-  frag_t q[NG];
-  float qs[NG];
-  {
-    const uint16_t* row = r < R ? (const uint16_t*)a.q.at(b, kv * G + r / Q, r % Q) : nullptr;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      qs[g] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d0 = D == 128 ? 32 * g + 4 * quad + e : 16 * (2 * g + e / 2) + 4 * quad + 2 * (e & 1);
-        const int d1 = D == 128 ? d0 + 16 : d0 + 1;
-        const uint32_t lo = row ? row[d0] : 0, hi = row ? row[d1] : 0;
-        q[g][e] = lo | (hi << 16);
-        qs[g] += unpack1<T>(lo) + unpack1<T>(hi);
-      }
-      qs[g] += __shfl_xor(qs[g], 16);
-      qs[g] += __shfl_xor(qs[g], 32);
-    }
-  }
-
   const int* table = a.table + b * a.width;
-  const int page_size = a.cache.page;
-  const auto load = [&](int t, int (&page)[2], RawTile<D>& x) {
+  const int last_entry = (int)a.width - 1;
+  // table entries of a tile's two halves (those past the table belong to tokens past the length)
+  const auto entries = [&](int t, int (&entry)[2]) {
 #pragma unroll
     for (int hb = 0; hb < 2; ++hb) {
+      const int at = kTok * t + 16 * hb, i = a.shift >= 0 ? at >> a.shift : at / a.cache.page;
+      entry[hb] = table[min(i, last_entry)];
+    }
+  };
+  const auto load = [&](int t, const int (&entry)[2], RawTile<D>& x, bool (&there)[2]) {
+    int page[2], slots[2];
+#pragma unroll
+    for (int hb = 0; hb < 2; ++hb) {
+      const int e = __builtin_amdgcn_readfirstlane(entry[hb]);
       const int at = kTok * t + 16 * hb;
-      page[hb] = __builtin_amdgcn_readfirstlane(page_of(a.cache, table, a.width, at / page_size));
-      const int pg = max(page[hb], 0), slot = page[hb] < 0 ? 0 : at % page_size;
-      const uint8_t* kc = a.cache.codes + codes_at<D>(a.cache, 0, pg, kv) + (int64_t)slot * (D / 2);
-      const uint8_t* vc = a.cache.codes + codes_at<D>(a.cache, 1, pg, kv) + (int64_t)slot * (D / 2);
+      there[hb] = e >= 0 && e < a.cache.pages;
+      page[hb] = there[hb] ? e : 0;
+      slots[hb] = a.shift >= 0 ? at & (a.cache.page - 1) : at % a.cache.page;
+      const uint8_t* kc = a.cache.codes + codes_at<D>(a.cache, 0, page[hb], kv) + slots[hb] * (D / 2);
+      const uint8_t* vc = a.cache.codes + codes_at<D>(a.cache, 1, page[hb], kv) + slots[hb] * (D / 2);
       if constexpr (D == 128) {
-        const frag_t y = *(const frag_t*)(kc + l * 64 + quad * 16);
+        const frag_t y = *(const frag_t*)(kc + (uint32_t)(l * 64 + quad * 16));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x.k[hb][e] = y[e];
+        for (int e2 = 0; e2 < 4; ++e2) x.k[hb][e2] = y[e2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x.v[4 * hb + e] = *(const uint32_t*)(vc + (4 * quad + e) * 64 + l * 4);
+        for (int e2 = 0; e2 < 4; ++e2) x.v[4 * hb + e2] = *(const uint32_t*)(vc + (uint32_t)(quad * 256 + l * 4) + 64 * e2);
       } else {
-        const u32x2_t y = *(const u32x2_t*)(kc + l * 32 + quad * 8);
+        const u32x2_t y = *(const u32x2_t*)(kc + (uint32_t)(l * 32 + quad * 8));
 #pragma unroll
-        for (int e = 0; e < 2; ++e) x.k[hb][e] = y[e];
+        for (int e2 = 0; e2 < 2; ++e2) x.k[hb][e2] = y[e2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x.v[4 * hb + e] = *(const uint16_t*)(vc + (4 * quad + e) * 32 + l * 2);
+        for (int e2 = 0; e2 < 4; ++e2) x.v[4 * hb + e2] = *(const uint16_t*)(vc + (uint32_t)(quad * 128 + l * 2) + 32 * e2);
       }
     }
     // lane: row lane / 8 of the params, tokens 4 (lane % 8) ..
-    const int row = lane >> 3, tok = 4 * (lane & 7), hb = tok >> 4;
-    const int pg = max(hb ? page[1] : page[0], 0);
-    const int slot = (hb ? page[1] : page[0]) < 0 ? tok & 15 : (kTok * t + tok) % page_size;
-    if (row < 2 * NG) {
+    const int row = min(lane >> 3, 2 * NG - 1), tok = 4 * (lane & 7), hb = tok >> 4;
 #pragma unroll
-      for (int side = 0; side < 2; ++side)
-        x.p[side] = *(const u32x2_t*)(a.cache.params + params_at<D>(a.cache, side, pg, kv) +
-                                      2 * (row * page_size + slot));
+    for (int side = 0; side < 2; ++side) {
+      const int64_t b0 = params_at<D>(a.cache, side, page[0], kv) + 2 * slots[0];
+      const int64_t b1 = params_at<D>(a.cache, side, page[1], kv) + 2 * slots[1];
+      x.p[side] = *(const u32x2_t*)(a.cache.params + (hb ? b1 : b0) + 2 * (row * a.cache.page + (tok & 15)));
     }
   };
 
-  f32x4_t o[NB] = {}, shift[NG] = {}, mins = {};
-  float m = -INFINITY, sum = 0.f;
-  const float c = a.scale * 1.44269504f;
+  // the first tiles are on their way while q is prepared
   RawTile<D> x;
-  int page[2];
-  if (first + wave < last) load(tiles.tile(first + wave), page, x);
+  bool there[2] = {};
+  int entry[2] = {};
+  if (first + wave < last) {
+    entries(tiles.tile(first + wave), entry);
+    load(tiles.tile(first + wave), entry, x, there);
+    entries(tiles.tile(min(first + wave + 4, last - 1)), entry);
+  }
+
+  // q as B operand, f16 numbers in the codes' order, and its sums over the groups in three parts of T
+  frag_t q[NG];
+  frag_t qsum = {0, 0, 0, 0};
+  float c;
+  {
+    const uint8_t* row = (const uint8_t*)a.q.at(b, kv * G + min(r, R - 1) / Q, min(r, R - 1) % Q) + 8 * quad;
+    float f[NG][8];  // [k][e]: number 16 k + 4 quad + e, k = 2 g + e / 4
+    float top = 0.f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const u32x2_t y = *(const u32x2_t*)(row + 32 * (2 * g + u));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f[g][4 * u + e] = r < R ? unpack1<T>(e & 1 ? y[e / 2] >> 16 : y[e / 2] & 0xffffu) : 0.f;
+          top = fmaxf(top, fabsf(f[g][4 * u + e]));
+        }
+      }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const int e2 = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+    c = ldexpf(a.scale * 1.44269504f, e2 + 10);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float sum = 0.f, z[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sum += f[g][e];
+        // codes at odd places are 16 times as large
+        z[e] = ldexpf(f[g][e], 14 - e2 - (D == 128 ? 4 * (g & 1) : 4 * (e / 4)));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        q[g][e] = D == 128 ? pack2<f16_t>(z[e], z[4 + e]) : pack2<f16_t>(z[2 * e], z[2 * e + 1]);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      sum = ldexpf(sum, -10 - e2);
+      const float s0 = round_to<T>(sum), s1 = round_to<T>(sum - s0), s2 = sum - s0 - s1;
+      if (quad == g) qsum = (frag_t){pack2<T>(s0, s1), pack2<T>(s2, 0.f), 0, 0};
+    }
+  }
+
+  f32x4_t o[NB] = {}, mins = {};
+  float m = -INFINITY, ref = 0.f, sum = 0.f;
+  uint32_t most = 0;  // the largest step so far, as its bits
+  int lift = 0;       // its exponent
   for (int it = first + wave; it < last; it += 4) {
     const int j0 = tiles.tile(it) * kTok;
-    const RawTile<D> now = x;
-    const bool there0 = page[0] >= 0, there1 = page[1] >= 0;
-    if (it + 4 < last) load(tiles.tile(it + 4), page, x);
+    RawTile<D> now = x;
+    const bool there0 = there[0], there1 = there[1];
+    if (it + 4 < last) {
+      load(tiles.tile(it + 4), entry, x, there);
+      entries(tiles.tile(min(it + 8, last - 1)), entry);
+    }
+    const bool all = there0 && there1 && p0 >= 0 && j0 + kTok - 1 <= p0 && (p1 - j0 < W || j0 + kTok - 1 < S);
+    if (!all) {  // what the params hold for tokens that no row sees is not used
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = j0 + 4 * (lane & 7) + e;
+        const bool some = ((lane & 7) < 4 ? there0 : there1) && j <= p1 && (p0 - j < W || j < S);
+        const uint32_t keep = some ? 0xffffffffu : e & 1 ? 0xffffu : 0xffff0000u;
+        now.p[0][e / 2] &= keep;
+        now.p[1][e / 2] &= keep;
+      }
+    }
 
     // the tile's params by way of LDS: every lane needs 4 tokens of every row
     uint16_t(*par)[2 * NG][kTok] = params[wave];
-    if ((lane >> 3) < 2 * NG) {
+    if (NG == 4 || lane < 32) {
       *(u32x2_t*)&par[0][lane >> 3][4 * (lane & 7)] = now.p[0];
       *(u32x2_t*)&par[1][lane >> 3][4 * (lane & 7)] = now.p[1];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 
-    // logits of tokens 16 hb + 4 quad + i for row l
+    // logits of tokens 16 hb + 4 quad + i for row l, in units of 1 / c
     float s[8];
 #pragma unroll
     for (int hb = 0; hb < 2; ++hb) {
-      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint32_t low = par[0][NG + quad % NG][16 * hb + l];
+      const uint32_t pair = quad < NG ? low | (low << 16) : 0;
+      f32x4_t y = mfma16<T>((frag_t){pair, pair, 0, 0}, qsum, (f32x4_t){0.f, 0.f, 0.f, 0.f});
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         frag_t f;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          f[e] = D == 128 ? code_pair<T>(now.k[hb][e], g) : code_pair<T>(now.k[hb][e & 1], 2 * g + e / 2);
-        const float z = -16.f * qs[g];
-        const f32x4_t acc = mfma16<T>(f, q[g], (f32x4_t){z, z, z, z});
+          f[e] = D == 128 ? code_pair(now.k[hb][e], g) : code_pair(now.k[hb][e & 1], 2 * g + e / 2);
+        const f32x4_t acc = mfma16<f16_t>(f, q[g], (f32x4_t){0.f, 0.f, 0.f, 0.f});
         const u32x2_t ps = *(const u32x2_t*)&par[0][g][16 * hb + 4 * quad];
-        const u32x2_t pm = *(const u32x2_t*)&par[0][NG + g][16 * hb + 4 * quad];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t bs = i & 1 ? ps[i / 2] >> 16 : ps[i / 2] & 0xffffu;
-          const uint32_t bm = i & 1 ? pm[i / 2] >> 16 : pm[i / 2] & 0xffffu;
-          y[i] = __builtin_fmaf(unpack1<T>(bs), acc[i], y[i]);
-          y[i] = __builtin_fmaf(unpack1<T>(bm), qs[g], y[i]);
-        }
+        for (int i = 0; i < 4; ++i)
+          y[i] = __builtin_fmaf(unpack1<T>(i & 1 ? ps[i / 2] >> 16 : ps[i / 2] & 0xffffu), acc[i], y[i]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * hb + i] = y[i];
     }
-    const bool all = there0 && there1 && p0 >= 0 && j0 + kTok - 1 <= p0 && (p1 - j0 < W || j0 + kTok - 1 < S);
     if (!all) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -370,43 +435,54 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_kernel(const AttendArg
     for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
-    const float mc = (top == -INFINITY ? 0.f : top) * c;
-    if (__any(top > m)) {
-      const float f = exp2_raw(__builtin_fmaf(m, c, -mc));
+    // steps are not negative, so their bits order them
+    const uint32_t b0 = now.p[1][0], b1 = now.p[1][1];
+    const uint32_t steps = lane < 8 * NG ? max(max(b0 & 0xffffu, b0 >> 16), max(b1 & 0xffffu, b1 >> 16)) : 0u;
+    // a new reference where a row's largest logit has grown by more than 4 in log2, or the largest step by a power of two:
+    // until then weights stay below 2^5
+    if (__any((top - m) * c > 4.f || (m == -INFINITY && top > m) || steps > (most | (kTwo ? 0x3ffu : 0x7fu)))) {
+      uint32_t big = steps;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) big = max(big, (uint32_t)__shfl_xor((int)big, d));
+      most = max(most, big);
+      const int lifted = kTwo ? (int)(most >> 10) - 14 : min(max((int)(most >> 7) - 126, -100), 100);
+      const float next = (top == -INFINITY ? 0.f : top * c) + (float)lifted;
+      const float f = m == -INFINITY ? 0.f : exp2_raw(ref - next);
       sum *= f;
 #pragma unroll
       for (int i = 0; i < NB; ++i) o[i] *= f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) shift[g] *= f;
-      mins *= f;
+      mins *= kTwo ? ldexpf(f, lifted - lift) : f;
       m = top;
+      ref = next;
+      lift = lifted;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      s[i] = exp2_raw(__builtin_fmaf(s[i], c, -mc));
+      s[i] = exp2_raw(__builtin_fmaf(s[i], c, -ref));
       sum += s[i];
     }
 
     // sum_t p_t m_t: rows g of the A operand, in the tokens' order of s
     {
-      const int g = l % NG;
-      u32x2_t m0 = *(const u32x2_t*)&par[1][NG + g][4 * quad], m1 = *(const u32x2_t*)&par[1][NG + g][16 + 4 * quad];
-      frag_t fm = {m0[0], m0[1], m1[0], m1[1]};
-      if (!all) {  // what lies in tokens that no row sees is not used
+      const u32x2_t m0 = *(const u32x2_t*)&par[1][NG + l % NG][4 * quad];
+      const u32x2_t m1 = *(const u32x2_t*)&par[1][NG + l % NG][16 + 4 * quad];
+      const frag_t fm = {m0[0], m0[1], m1[0], m1[1]};
+      frag_t fp, fr;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = j0 + 16 * (i >> 2) + 4 * quad + (i & 3);
-          const bool some = (i < 4 ? there0 : there1) && j <= p1 && (p0 - j < W || j < S);
-          fm[i / 2] &= some ? 0xffffffffu : i & 1 ? 0xffffu : 0xffff0000u;
+      for (int e = 0; e < 4; ++e) {
+        uint32_t hi, lo;
+        // f16: without the steps' exponent, which may put weights past its range
+        if constexpr (kTwo) {
+          split_pair<T>(ldexpf(s[2 * e], lift), ldexpf(s[2 * e + 1], lift), &hi, &lo);
+        } else {
+          split_pair<T>(s[2 * e], s[2 * e + 1], &hi, &lo);
         }
+        fp[e] = hi, fr[e] = lo;
       }
-      frag_t fp;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) fp[e] = pack2<T>(s[2 * e], s[2 * e + 1]);
       mins = mfma16<T>(fm, fp, mins);
+      mins = mfma16<T>(fm, fr, mins);
     }
-    // sum_t p_t s_t (16 + c_t): the weights take the steps. They are bf16 for their range; 16-bit floats'
-    // results need more of their digits, a second product with the rest
+    // sum_t p_t s_t c_t
     uint32_t lo[4], hi[4];
     if constexpr (D == 128) {
 #pragma unroll
@@ -425,29 +501,27 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_kernel(const AttendArg
       for (int hb = 0; hb < 2; ++hb) {
         const u32x2_t ps = *(const u32x2_t*)&par[1][g][16 * hb + 4 * quad];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float step = unpack1<T>(i & 1 ? ps[i / 2] >> 16 : ps[i / 2] & 0xffffu);
-          w[4 * hb + i] = s[4 * hb + i] * step;
-          if (!all) w[4 * hb + i] = s[4 * hb + i] == 0.f ? 0.f : w[4 * hb + i];
-        }
+        for (int i = 0; i < 4; ++i)
+          w[4 * hb + i] = s[4 * hb + i] * unpack1<T>(i & 1 ? ps[i / 2] >> 16 : ps[i / 2] & 0xffffu);
       }
       frag_t fw, fr;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        fw[e] = pack2_bf16(w[2 * e], w[2 * e + 1]);
-        fr[e] = pack2_bf16(w[2 * e] - bf16_to_f32(fw[e] & 0xffffu), w[2 * e + 1] - __uint_as_float(fw[e] & 0xffff0000u));
+        if constexpr (kTwo) {
+          uint32_t h2, l2;
+          split_pair<f16_t>(w[2 * e], w[2 * e + 1], &h2, &l2);
+          fw[e] = h2, fr[e] = l2;
+        } else {
+          fw[e] = pack2<f16_t>(w[2 * e], w[2 * e + 1]);
+        }
       }
-      const frag_t bias = {0xc180c180u, 0xc180c180u, 0xc180c180u, 0xc180c180u};  // -16
-      shift[g] = mfma16<bf16_t>(bias, fw, shift[g]);
-      if constexpr (!__is_same(T, bf16_t)) shift[g] = mfma16<bf16_t>(bias, fr, shift[g]);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         frag_t f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          f[e] = D == 128 ? code_pair<bf16_t>(u ? hi[e] : lo[e], g) : code_pair<bf16_t>(lo[e], 2 * g + u);
-        o[2 * g + u] = mfma16<bf16_t>(f, fw, o[2 * g + u]);
-        if constexpr (!__is_same(T, bf16_t)) o[2 * g + u] = mfma16<bf16_t>(f, fr, o[2 * g + u]);
+        for (int e = 0; e < 4; ++e) f[e] = D == 128 ? code_pair(u ? hi[e] : lo[e], g) : code_pair(lo[e], 2 * g + u);
+        o[2 * g + u] = mfma16<f16_t>(f, fw, o[2 * g + u]);
+        if constexpr (kTwo) o[2 * g + u] = mfma16<f16_t>(f, fr, o[2 * g + u]);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -459,24 +533,28 @@ __global__ __launch_bounds__(kThreads, 2) void kv4_attend_kernel(const AttendArg
   sum += __shfl_xor(sum, 32);
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
-    const float add = mins[i / 2 % 4];
-    *(f32x4_t*)&merge[wave][l][16 * i + 4 * quad] = o[i] + shift[i / 2] + (f32x4_t){add, add, add, add};
+    const float add = kTwo ? ldexpf(mins[i / 2], -lift) : mins[i / 2], unit = (D == 128 ? i / 2 : i) & 1 ? kOdd : kEven;
+    f32x4_t y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[i][e], unit, add);
+    *(f32x4_t*)&merge[wave][l][16 * i + 4 * quad] = y;
   }
   if (quad == 0) {
-    stats[wave][0][l] = m * c;
+    stats[wave][0][l] = ref;
     stats[wave][1][l] = sum;
   }
   __syncthreads();
   const int row = tid / 16, d0 = tid % 16 * (D / 16);
   if (r0 + row >= R) return;
-  float top = stats[0][0][row];
+  // waves without a visible token have sum 0 and a reference that is no maximum: they are left out
+  float top = -INFINITY;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) top = fmaxf(top, stats[w][0][row]);
+  for (int w = 0; w < 4; ++w) top = stats[w][1][row] != 0.f ? fmaxf(top, stats[w][0][row]) : top;
   const float base = top == -INFINITY ? 0.f : top;
   float y[D / 16] = {}, total = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const float f = exp2_raw(stats[w][0][row] - base);
+    const float f = stats[w][1][row] != 0.f ? exp2_raw(stats[w][0][row] - base) : 0.f;
     total = __builtin_fmaf(f, stats[w][1][row], total);
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) y[e] = __builtin_fmaf(f, merge[w][row][d0 + e], y[e]);
@@ -720,6 +798,7 @@ extern "C" int pkm_kv4_attend(const void* codes, const void* params, int64_t pag
   const int64_t far = 1 << 30;
   a.window = (int)(window < far ? window : 0), a.sinks = (int)(sinks < far ? sinks : far);
   a.scale = scale;
+  a.shift = (page & (page - 1)) == 0 ? __builtin_ctzll((unsigned long long)page) : -1;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == PKM_DTYPE_BF16) {
     dim == 128 ? launch_attend<bf16_t, 128>(a, st) : launch_attend<bf16_t, 64>(a, st);
