@@ -676,7 +676,7 @@ int pkm_kv4_read(const void* codes, const void* params, int64_t pages, int64_t k
                  const int32_t* counts, int64_t batch, int64_t tokens, const pkm_heads_t* k,
                  const pkm_heads_t* v, void* stream);
 
-/* Workspace bytes pkm_kv4_attend needs (0: none). */
+/* Workspace bytes pkm_kv4_attend needs (0 where it has nothing to do). The workspace is 16-byte aligned. */
 size_t pkm_kv4_attend_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t queries,
                                      int64_t dim, int64_t width, int64_t page, int64_t window, int64_t sinks);
 

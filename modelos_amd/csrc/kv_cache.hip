@@ -180,17 +180,18 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(const StoreArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int kTok = 32;   // tokens of a tile: one wave's step
 constexpr int kRows = 16;  // query rows of a workgroup: the heads that share a key head, times the queries
+constexpr int kGroups = 768;  // workgroups of a large call: 3 on each of 256 CUs run at once
 
 struct AttendArgs {
   Cache cache;
   Heads q, o;
   const int* table;
   const int* lengths;
-  float* part;   // [batch, q_heads, queries, splits, D + 2]: numbers, largest logit, sum
+  float* part;   // [workgroups + segments, 16 rows, D + 2]: numbers, reference, sum
   int64_t width;
   int batch, q_heads, queries;
   int window, sinks;  // window 0: none
-  int per, splits;    // tiles of a workgroup; workgroups of a row block
+  int rows, groups;   // row blocks of a key head; workgroups
   int shift;          // log2 of the page, -1 if it is no power of two
   float scale;
 };
@@ -208,6 +209,82 @@ struct CacheTiles {
   }
   __device__ __forceinline__ int tile(int i) const { return i < sink ? i : i + near; }
 };
+
+// A segment is the tiles of one sequence, key head and row block. How the workgroups share all segments is worked out on the
+// device, where the lengths are:
+//   whole: with many tiles a workgroup, all segments in a row, in that order, are cut into equal shares, so that
+//     ragged lengths cost nothing; a share may reach over several segments. (64 sequences of 4000 to 16000 tokens, 8 key
+//     heads: 180 us; cut segment by segment into pieces of one size, 186 to 215 with the size.)
+//   else each segment is cut on its own, as starting a second segment costs more than the balance gains
+//     (window of 1024, 64 sequences: 26 us against 34).
+// A workgroup's part of a segment goes to a slot of the workspace, or to the output if it is the whole segment.
+struct Shares {
+  bool whole;
+  int per;         // tiles of a workgroup
+  int64_t before;  // tiles (whole) or workgroups of the sequences before b
+  int b, count;    // a sequence and its segments' tiles
+  // of a segment, not whole: workgroups and their tiles
+  __device__ __forceinline__ int pieces() const { return (count + per - 1) / per; }
+  __device__ __forceinline__ int piece() const { return (count + pieces() - 1) / pieces(); }
+};
+
+// Sum over the lanes up to and with the own one.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp_add_u32(uint32_t x) {
+  return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x = dpp_add_u32<0x111>(x);  // row_shr 1, 2, 4, 8
+  x = dpp_add_u32<0x112>(x);
+  x = dpp_add_u32<0x114>(x);
+  x = dpp_add_u32<0x118>(x);
+  x = dpp_add_u32<0x142, 0xa>(x);         // the rows' sums to the rows behind
+  return dpp_add_u32<0x143, 0xc>(x);
+}
+
+// x / y of numbers that are not negative: in 32 bits where x has no more (a 64-bit division takes a microsecond).
+__device__ __forceinline__ int64_t quotient(int64_t x, int y) {
+  return (uint64_t)x >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
+}
+
+// The shares, and the sequence that holds the first tile of workgroup `group` (the batch's size if there is none); or,
+// with group < 0, sequence b. Each wave works them out by itself: 64 sequences at a time.
+__device__ __forceinline__ Shares shares(const AttendArgs& a, int group, int b) {
+  const int lane = threadIdx.x & 63;
+  const int64_t heads = (int64_t)a.cache.heads * a.rows;
+  const auto count = [&](int i) { return i < a.batch ? CacheTiles(a, i).count : 0; };
+  // counts are below 2^25 (the entry point checks the table's width), 64 of them below 2^31
+  const uint32_t mine = count(lane), sums = wave_scan(mine);
+  int64_t total = (uint32_t)__builtin_amdgcn_readlane((int)sums, 63);
+  for (int i = 64; i < a.batch; i += 64)
+    total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(count(i + lane)), 63);
+  total *= heads;
+  Shares r;
+  const int64_t even = quotient(total + a.groups - 1, a.groups);
+  r.whole = even >= 64;
+  r.per = (int)max(even, (int64_t)8);
+  const int64_t first = r.whole ? (int64_t)group * r.per : group;
+  r.b = a.batch;
+  r.before = 0;
+  int64_t passed = 0;  // of the sequences before
+  for (int i0 = 0; i0 < a.batch; i0 += 64) {
+    uint32_t t = i0 ? (uint32_t)count(i0 + lane) : mine;
+    if (!r.whole) t = (t + r.per - 1) / (uint32_t)r.per;
+    const uint32_t upto = i0 || !r.whole ? wave_scan(t) : sums;
+    const int64_t scan = passed + upto * heads, own = t * heads;
+    const uint64_t here = __ballot(group < 0 ? i0 + lane == b : t > 0 && scan - own <= first && first < scan);
+    if (here) {
+      const int at = __builtin_ctzll(here);
+      r.b = i0 + at;
+      r.before = passed + (uint32_t)__builtin_amdgcn_readlane((int)(upto - t), at) * heads;
+      break;
+    }
+    passed += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * heads;
+  }
+  r.b = __builtin_amdgcn_readfirstlane(r.b);
+  r.count = r.b < a.batch ? CacheTiles(a, r.b).count : 0;
+  return r;
+}
 
 // Codes at bits 4 k of both halves of x as f16 numbers c 2^-24 (k even) or c 2^-20 (k odd): subnormal numbers,
 // whose fraction they are. The matrix instructions take them exactly, so there is no conversion and no offset to
@@ -253,15 +330,30 @@ __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArg
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l = lane & 15, quad = lane >> 4;
   const int kv_heads = a.cache.heads, G = a.q_heads / kv_heads, R = G * a.queries;
-  int id = blockIdx.x;
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int kv = id % kv_heads;
-  id /= kv_heads;
-  const int b = id % a.batch, r0 = id / a.batch * kRows;
+  const int group = blockIdx.x;
+  const Shares share = shares(a, group, 0);
+  const int heads = kv_heads * a.rows;
+  int b = share.b;
+  if (b >= a.batch) return;
+  int64_t before = share.before, at, end;  // tiles before the sequence's; the next tile and the share's end
+  int part_head;                           // key head and row block of the segment
+  if (share.whole) {
+    at = (int64_t)group * share.per;
+    end = at + share.per;
+    part_head = (int)quotient(at - before, share.count);
+  } else {
+    const uint32_t piece = (uint32_t)(group - before), pieces = share.pieces();
+    part_head = (int)(piece / pieces);
+    before = 0;
+    at = (int64_t)part_head * share.count + piece % pieces * share.piece();
+    end = min(at + share.piece(), (int64_t)(part_head + 1) * share.count);
+    if (at >= end) return;  // the join does not read it
+  }
+  for (;;) {
   const CacheTiles tiles(a, b);
-  const int first = split * a.per, last = min(first + a.per, tiles.count);
-  if (first >= last && split > 0) return;  // the join does not read it
+  const int64_t start = before + (int64_t)part_head * tiles.count;
+  const int first = (int)(at - start), last = (int)min((int64_t)tiles.count, end - start);
+  const int kv = part_head / a.rows, r0 = part_head % a.rows * kRows;
 
   const int r = r0 + l;  // the lane's row: head kv G + r / queries, query r % queries
   const int Q = a.queries, n = tiles.n;
@@ -279,39 +371,44 @@ __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArg
       entry[hb] = table[min(i, last_entry)];
     }
   };
+  // bytes of a page's codes over all heads; the params of the same tokens take a quarter
+  const int64_t page_bytes = (int64_t)a.cache.heads * a.cache.page * (D / 2);
+  const uint8_t* const kcodes = a.cache.codes + (int64_t)kv * a.cache.page * (D / 2);
+  const uint8_t* const vcodes = kcodes + a.cache.pages * page_bytes;
+  const uint8_t* const kparams = a.cache.params + (int64_t)kv * a.cache.page * (D / 8);
+  const uint8_t* const vparams = kparams + a.cache.pages * page_bytes / 4;
+  // a lane's params: row lane / 8, tokens 4 (lane % 8) ..
+  const uint32_t param_at = 2 * (min(lane >> 3, 2 * NG - 1) * a.cache.page + 4 * (lane & 3));
   const auto load = [&](int t, const int (&entry)[2], RawTile<D>& x, bool (&there)[2]) {
-    int page[2], slots[2];
+    int64_t pofs[2];
 #pragma unroll
     for (int hb = 0; hb < 2; ++hb) {
       const int e = __builtin_amdgcn_readfirstlane(entry[hb]);
       const int at = kTok * t + 16 * hb;
       there[hb] = e >= 0 && e < a.cache.pages;
-      page[hb] = there[hb] ? e : 0;
-      slots[hb] = a.shift >= 0 ? at & (a.cache.page - 1) : at % a.cache.page;
-      const uint8_t* kc = a.cache.codes + codes_at<D>(a.cache, 0, page[hb], kv) + slots[hb] * (D / 2);
-      const uint8_t* vc = a.cache.codes + codes_at<D>(a.cache, 1, page[hb], kv) + slots[hb] * (D / 2);
+      const int slot = a.shift >= 0 ? at & (a.cache.page - 1) : at % a.cache.page;
+      const int64_t page = (there[hb] ? e : 0) * page_bytes;
+      // 16 tokens' codes each, addressed by the lane's place alone
+      const __amdgpu_buffer_rsrc_t kc = row_rsrc(kcodes + (page + slot * (D / 2)), 8 * D);
+      const __amdgpu_buffer_rsrc_t vc = row_rsrc(vcodes + (page + slot * (D / 2)), 8 * D);
+      pofs[hb] = page / 4 + 2 * slot;
       if constexpr (D == 128) {
-        const frag_t y = *(const frag_t*)(kc + (uint32_t)(l * 64 + quad * 16));
+        const frag_t y = __builtin_amdgcn_raw_buffer_load_b128(kc, l * 64 + quad * 16, 0, 0);
 #pragma unroll
         for (int e2 = 0; e2 < 4; ++e2) x.k[hb][e2] = y[e2];
 #pragma unroll
-        for (int e2 = 0; e2 < 4; ++e2) x.v[4 * hb + e2] = *(const uint32_t*)(vc + (uint32_t)(quad * 256 + l * 4) + 64 * e2);
+        for (int e2 = 0; e2 < 4; ++e2) x.v[4 * hb + e2] = __builtin_amdgcn_raw_buffer_load_b32(vc, quad * 256 + l * 4 + 64 * e2, 0, 0);
       } else {
-        const u32x2_t y = *(const u32x2_t*)(kc + (uint32_t)(l * 32 + quad * 8));
+        const u32x2_t y = __builtin_amdgcn_raw_buffer_load_b64(kc, l * 32 + quad * 8, 0, 0);
 #pragma unroll
         for (int e2 = 0; e2 < 2; ++e2) x.k[hb][e2] = y[e2];
 #pragma unroll
-        for (int e2 = 0; e2 < 4; ++e2) x.v[4 * hb + e2] = *(const uint16_t*)(vc + (uint32_t)(quad * 128 + l * 2) + 32 * e2);
+        for (int e2 = 0; e2 < 4; ++e2) x.v[4 * hb + e2] = __builtin_amdgcn_raw_buffer_load_b16(vc, quad * 128 + l * 2 + 32 * e2, 0, 0);
       }
     }
-    // lane: row lane / 8 of the params, tokens 4 (lane % 8) ..
-    const int row = min(lane >> 3, 2 * NG - 1), tok = 4 * (lane & 7), hb = tok >> 4;
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const int64_t b0 = params_at<D>(a.cache, side, page[0], kv) + 2 * slots[0];
-      const int64_t b1 = params_at<D>(a.cache, side, page[1], kv) + 2 * slots[1];
-      x.p[side] = *(const u32x2_t*)(a.cache.params + (hb ? b1 : b0) + 2 * (row * a.cache.page + (tok & 15)));
-    }
+    const int64_t at = (lane & 4 ? pofs[1] : pofs[0]) + param_at;
+    x.p[0] = *(const u32x2_t*)(kparams + at);
+    x.p[1] = *(const u32x2_t*)(vparams + at);
   };
 
   // the first tiles are on their way while q is prepared
@@ -545,7 +642,6 @@ __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArg
   }
   __syncthreads();
   const int row = tid / 16, d0 = tid % 16 * (D / 16);
-  if (r0 + row >= R) return;
   // waves without a visible token have sum 0 and a reference that is no maximum: they are left out
   float top = -INFINITY;
 #pragma unroll
@@ -560,7 +656,8 @@ __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArg
     for (int e = 0; e < D / 16; ++e) y[e] = __builtin_fmaf(f, merge[w][row][d0 + e], y[e]);
   }
   const int head = kv * G + (r0 + row) / Q, query = (r0 + row) % Q;
-  if (a.splits == 1) {
+  if (r0 + row >= R) {
+  } else if (first == 0 && last == tiles.count) {
     const float f = total != 0.f ? 1.f / total : 0.f;
     uint32_t z[D / 32];
 #pragma unroll
@@ -569,61 +666,98 @@ __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArg
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) to[e] = total != 0.f ? z[e] : 0u;
   } else {
-    float* to = a.part + (((int64_t)(b * a.q_heads + head) * Q + query) * a.splits + split) * (D + 2);
+    const int64_t slot = share.whole ? group + (int64_t)b * heads + part_head : group;
+    float* to = a.part + slot * (kRows * (D + 2));
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) to[d0 + e] = y[e];
+    for (int e = 0; e < D / 16; ++e) to[row * D + d0 + e] = y[e];
     if (d0 == 0) {
-      to[D] = top;
-      to[D + 1] = total;
+      to[kRows * D + 2 * row] = top;
+      to[kRows * D + 2 * row + 1] = total;
     }
+  }
+  // the next segment that has tiles
+  at = start + last;
+  if (at >= end) return;
+  if (++part_head == heads) {
+    before = at;
+    part_head = 0;
+    do {
+      if (++b == a.batch) return;
+    } while (CacheTiles(a, b).count == 0);
+  }
+  __syncthreads();
   }
 }
 
-// Joins the parts of one row: 16 groups of 16 lanes take parts in turn.
-template <typename T, int D>
+// Joins the parts of rows, where their segments have several; zeros where they have no tiles. A row is a wave's where there
+// are many, a workgroup's where there are few; 16 lanes take a part at a time.
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(kThreads) void kv4_join_kernel(const AttendArgs a) {
-  __shared__ float numbers[16][D + 4];
-  __shared__ float stats[2][16];
-  const int Q = a.queries, query = blockIdx.x % Q, bh = blockIdx.x / Q;
-  const int b = bh / a.q_heads, head = bh % a.q_heads;
-  const CacheTiles tiles(a, b);
-  const int parts = max(1, (tiles.count + a.per - 1) / a.per);
-  const int g = threadIdx.x / 16, d0 = threadIdx.x % 16 * (D / 16);
-  const float* from = a.part + (int64_t)blockIdx.x * a.splits * (D + 2);
-  float top = -INFINITY;
-  for (int i = g; i < parts; i += 16) top = fmaxf(top, from[(int64_t)i * (D + 2) + D]);
-  float base = top == -INFINITY ? 0.f : top;
-  float y[D / 16] = {}, total = 0.f;
-  for (int i = g; i < parts; i += 16) {
-    const float* p = from + (int64_t)i * (D + 2);
-    const float f = exp2_raw(p[D] - base);
-    total = __builtin_fmaf(f, p[D + 1], total);
+  __shared__ __align__(16) float numbers[16][D];
+  __shared__ float stats[16][2];
+  const int tid = threadIdx.x, wave = tid >> 6, g = tid / 16, d0 = tid % 16 * (D / 16);
+  const int id = WAVES == 4 ? blockIdx.x : 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(wave);
+  const int Q = a.queries, query = id % Q, bh = id / Q;
+  const int b = min(bh / a.q_heads, a.batch - 1), head = bh % a.q_heads, G = a.q_heads / a.cache.heads;
+  const bool there = bh / a.q_heads < a.batch;
+  const int row = head % G * Q + query, part_head = head / G * a.rows + row / kRows;
+  const Shares share = shares(a, -1, b);
+  int parts = 0;
+  int64_t slot = 0;
+  if (share.count == 0) {
+  } else if (share.whole) {
+    const int64_t start = share.before + (int64_t)part_head * share.count, w0 = quotient(start, share.per);
+    parts = (int)(quotient(start + share.count - 1, share.per) - w0) + 1;
+    slot = w0 + (int64_t)b * a.cache.heads * a.rows + part_head;
+  } else {
+    slot = share.before + (int64_t)part_head * share.pieces();
+    parts = (share.count + share.piece() - 1) / share.piece();
+  }
+  if (!there) parts = 1;
+  const float* const from = a.part + slot * (kRows * (D + 2));
+  const int r = row % kRows;
+  float y[D / 16] = {}, top = -INFINITY, total = 0.f;
+  if (parts > 1) {
+#pragma unroll 4
+    for (int i = g % (4 * WAVES); i < parts; i += 4 * WAVES) {
+      const float* p = from + (int64_t)i * (kRows * (D + 2));
+      const float t = p[kRows * D + 2 * r], sum = p[kRows * D + 2 * r + 1];
+      f32x4_t x[D / 64];
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) y[e] = __builtin_fmaf(f, p[d0 + e], y[e]);
+      for (int e = 0; e < D / 64; ++e) x[e] = *(const f32x4_t*)(p + r * D + d0 + 4 * e);
+      const float next = fmaxf(top, t), base = next == -INFINITY ? 0.f : next;
+      const float f0 = exp2_raw(top - base), f1 = exp2_raw(t - base);
+      top = next;
+      total = total * f0 + sum * f1;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) y[e] = y[e] * f0 + x[e / 4][e % 4] * f1;
+    }
   }
 #pragma unroll
   for (int e = 0; e < D / 16; ++e) numbers[g][d0 + e] = y[e];
   if (d0 == 0) {
-    stats[0][g] = top;
-    stats[1][g] = total;
+    stats[g][0] = top;
+    stats[g][1] = total;
   }
   __syncthreads();
-  if ((int)threadIdx.x >= D / 2) return;
-  top = stats[0][0];
+  if (parts == 1) return;  // written by its workgroup, or no row
+  const int lane = WAVES == 4 ? tid : tid & 63, g0 = WAVES == 4 ? 0 : 4 * wave;
+  if (lane >= D / 2) return;
+  top = -INFINITY;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, stats[0][i]);
-  base = top == -INFINITY ? 0.f : top;
+  for (int i = 0; i < 4 * WAVES; ++i) top = fmaxf(top, stats[g0 + i][0]);
+  const float base = top == -INFINITY ? 0.f : top;
   total = 0.f;
   float y0 = 0.f, y1 = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float f = exp2_raw(stats[0][i] - base);
-    total = __builtin_fmaf(f, stats[1][i], total);
-    y0 = __builtin_fmaf(f, numbers[i][2 * threadIdx.x], y0);
-    y1 = __builtin_fmaf(f, numbers[i][2 * threadIdx.x + 1], y1);
+  for (int i = 0; i < 4 * WAVES; ++i) {
+    const float f = exp2_raw(stats[g0 + i][0] - base);
+    total = __builtin_fmaf(f, stats[g0 + i][1], total);
+    y0 = __builtin_fmaf(f, numbers[g0 + i][2 * lane], y0);
+    y1 = __builtin_fmaf(f, numbers[g0 + i][2 * lane + 1], y1);
   }
   const float f = total != 0.f ? 1.f / total : 0.f;
-  ((uint32_t*)a.o.at(b, head, query))[threadIdx.x] = total != 0.f ? pack2<T>(y0 * f, y1 * f) : 0u;
+  ((uint32_t*)a.o.at(b, head, query))[lane] = total != 0.f ? pack2<T>(y0 * f, y1 * f) : 0u;
 }
 
 // ---------------------------------------------------------------------------
@@ -693,33 +827,36 @@ int run_store(const char* what, const StoreArgs& a, int64_t dim, int dtype, void
   return pkm_check_launch(what);
 }
 
-// Tiles of a workgroup and workgroups of a row block, from sizes alone: enough workgroups to fill the card
-// a few times over, tiles enough for 4 waves each.
-void split_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t queries, int64_t width, int64_t page,
-                int64_t window, int64_t sinks, int* per, int* splits) {
+// Shares of a call, from sizes alone: as many workgroups as run at once, none with fewer than 8 tiles. Cut segment by
+// segment, up to one more a segment may be needed; those that are not end at once.
+int attend_groups(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t queries, int64_t width, int64_t page,
+                  int64_t window, int64_t sinks, int64_t* segments) {
   const int64_t rows = (q_heads / kv_heads * queries + kRows - 1) / kRows;
   int64_t most = (width * page + kTok - 1) / kTok;
   if (window > 0) {
     const int64_t seen = (window + queries) / kTok + 2 + (sinks + kTok - 1) / kTok;
     if (seen < most) most = seen;
   }
-  const int64_t blocks = batch * kv_heads * rows;
-  int64_t each = (most * blocks + 2047) / 2048;
-  if (each < 8) each = 8;
-  if (most < 1) most = 1;
-  *per = (int)each;
-  *splits = (int)((most + each - 1) / each);
+  *segments = batch * kv_heads * rows;
+  // (a product of large sizes may not fit; more than kGroups is all that counts)
+  const double tiles = (double)*segments * (double)most;
+  return tiles >= 8.0 * kGroups ? kGroups : (int)(tiles / 8.0) + 1;
 }
 
-int64_t part_bytes(int64_t batch, int64_t q_heads, int64_t queries, int64_t dim, int splits) {
-  return splits == 1 ? 0 : batch * q_heads * queries * splits * (dim + 2) * (int64_t)sizeof(float);
+int64_t part_bytes(int64_t groups, int64_t segments, int64_t dim) {
+  return (groups + segments) * kRows * (dim + 2) * (int64_t)sizeof(float);
 }
 
 template <typename T, int D>
 void launch_attend(const AttendArgs& a, hipStream_t st) {
-  const int rows = (a.q_heads / a.cache.heads * a.queries + kRows - 1) / kRows;
-  kv4_attend_kernel<T, D><<<(unsigned)(a.batch * a.cache.heads * rows * a.splits), kThreads, 0, st>>>(a);
-  if (a.splits > 1) kv4_join_kernel<T, D><<<(unsigned)(a.batch * a.q_heads * a.queries), kThreads, 0, st>>>(a);
+  const unsigned grid = (unsigned)(a.groups + a.batch * a.cache.heads * a.rows);
+  kv4_attend_kernel<T, D><<<grid, kThreads, 0, st>>>(a);
+  const unsigned rows = (unsigned)(a.batch * a.q_heads * a.queries);
+  if (rows >= 512) {
+    kv4_join_kernel<T, D, 1><<<(rows + 3) / 4, kThreads, 0, st>>>(a);
+  } else {
+    kv4_join_kernel<T, D, 4><<<rows, kThreads, 0, st>>>(a);
+  }
 }
 
 }  // namespace
@@ -760,9 +897,9 @@ extern "C" size_t pkm_kv4_attend_workspace_size(int64_t batch, int64_t q_heads, 
                                                 int64_t dim, int64_t width, int64_t page, int64_t window,
                                                 int64_t sinks) {
   if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || queries <= 0 || dim <= 0 || width < 0 || page <= 0) return 0;
-  int per, splits;
-  split_plan(batch, q_heads, kv_heads, queries, width, page, window, sinks, &per, &splits);
-  return (size_t)part_bytes(batch, q_heads, queries, dim, splits);
+  int64_t segments;
+  const int groups = attend_groups(batch, q_heads, kv_heads, queries, width, page, window, sinks, &segments);
+  return (size_t)part_bytes(groups, segments, dim);
 }
 
 extern "C" int pkm_kv4_attend(const void* codes, const void* params, int64_t pages, int64_t kv_heads, int64_t page,
@@ -785,13 +922,15 @@ extern "C" int pkm_kv4_attend(const void* codes, const void* params, int64_t pag
   PKM_REQUIRE(pages > 0, PKM_ERR_UNSUPPORTED, "%s: the cache has no pages", what);
   PKM_REQUIRE(lengths != nullptr && (table != nullptr || width == 0), PKM_ERR_INVALID_ARGUMENT,
               "%s: table and lengths have to be given", what);
-  PKM_REQUIRE(width < (1ll << 31) / page && batch < (1 << 24) && q_heads < (1 << 20) && queries < (1 << 20) &&
+  PKM_REQUIRE(width < (1ll << 30) / page && batch < (1 << 24) && q_heads < (1 << 20) && queries < (1 << 20) &&
                   batch * q_heads * queries < (1ll << 24),
               PKM_ERR_UNSUPPORTED, "%s: too many tokens or rows", what);
-  split_plan(batch, q_heads, kv_heads, queries, width, page, window, sinks, &a.per, &a.splits);
-  PKM_REQUIRE(workspace_bytes >= (size_t)part_bytes(batch, q_heads, queries, dim, a.splits) &&
-                  (a.splits == 1 || workspace != nullptr),
-              PKM_ERR_WORKSPACE, "%s: workspace too small", what);
+  int64_t segments;
+  a.groups = attend_groups(batch, q_heads, kv_heads, queries, width, page, window, sinks, &segments);
+  a.rows = (int)(segments / batch / kv_heads);
+  PKM_REQUIRE(workspace != nullptr && workspace_bytes >= (size_t)part_bytes(a.groups, segments, dim), PKM_ERR_WORKSPACE,
+              "%s: workspace too small", what);
+  PKM_REQUIRE(((uintptr_t)workspace & 15) == 0, PKM_ERR_INVALID_ARGUMENT, "%s: workspace is not 16-byte aligned", what);
   a.q = heads(q), a.o = heads(out);
   a.table = table, a.lengths = lengths, a.part = (float*)workspace, a.width = width;
   a.batch = (int)batch, a.q_heads = (int)q_heads, a.queries = (int)queries;

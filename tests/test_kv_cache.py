@@ -142,4 +142,5 @@ def test_entry_point_statuses(lib):
     assert need > 0
     assert _attend(lib, good, width=4096) == 3
     assert _attend(lib, good, width=4096, ws=P, n=need - 1) == 3
-    assert lib.pkm_kv4_attend_workspace_size(2, 4, 2, 1, 64, 4, 16, 0, 0) == 0
+    assert lib.pkm_kv4_attend_workspace_size(0, 4, 2, 1, 64, 4, 16, 0, 0) == 0
+    assert lib.pkm_kv4_attend_workspace_size(2, 4, 2, 0, 64, 4, 16, 0, 0) == 0
