@@ -10,6 +10,8 @@
 //   codes  [2 (K, V), pages, heads, page, D / 2] bytes
 //   params [2 (K, V), pages, heads, 2 (s, m), D / 32, page] of the cache's type
 // Position t of sequence b lies in page table[b, t / page], slot t % page.
+#include <algorithm>
+
 #include "attn_common.h"
 
 namespace pkm {
@@ -192,6 +194,7 @@ struct AttendArgs {
   int batch, q_heads, queries;
   int window, sinks;  // window 0: none
   int rows, groups;   // row blocks of a key head; workgroups
+  int cut;            // workgroups less what the segments' last pieces waste, where each is cut on its own
   int shift;          // log2 of the page, -1 if it is no power of two
   float scale;
 };
@@ -216,7 +219,7 @@ struct CacheTiles {
 //     ragged lengths cost nothing; a share may reach over several segments. (64 sequences of 4000 to 16000 tokens, 8 key
 //     heads: 180 us; cut segment by segment into pieces of one size, 186 to 215 with the size.)
 //   else each segment is cut on its own, as starting a second segment costs more than the balance gains
-//     (window of 1024, 64 sequences: 26 us against 34).
+//     (window of 1024, 64 sequences: 27 us against 34), into pieces that all run at once (32 us in two rounds).
 // A workgroup's part of a segment goes to a slot of the workspace, or to the output if it is the whole segment.
 struct Shares {
   bool whole;
@@ -262,7 +265,7 @@ __device__ __forceinline__ Shares shares(const AttendArgs& a, int group, int b) 
   Shares r;
   const int64_t even = quotient(total + a.groups - 1, a.groups);
   r.whole = even >= 64;
-  r.per = (int)max(even, (int64_t)8);
+  r.per = (int)(r.whole ? even : max(quotient(total + a.cut - 1, a.cut), (int64_t)8));
   const int64_t first = r.whole ? (int64_t)group * r.per : group;
   r.b = a.batch;
   r.before = 0;
@@ -828,7 +831,8 @@ int run_store(const char* what, const StoreArgs& a, int64_t dim, int dtype, void
 }
 
 // Shares of a call, from sizes alone: as many workgroups as run at once, none with fewer than 8 tiles. Cut segment by
-// segment, up to one more a segment may be needed; those that are not end at once.
+// segment, up to one more a segment may be needed; those that are not end at once. 768: three on each of 256 CUs (512, 1024
+// and 1536 took 183, 209 and 185 us where 768 took 178, and 42, 45 and 48 for one long sequence's 40).
 int attend_groups(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t queries, int64_t width, int64_t page,
                   int64_t window, int64_t sinks, int64_t* segments) {
   const int64_t rows = (q_heads / kv_heads * queries + kRows - 1) / kRows;
@@ -928,6 +932,7 @@ extern "C" int pkm_kv4_attend(const void* codes, const void* params, int64_t pag
   int64_t segments;
   a.groups = attend_groups(batch, q_heads, kv_heads, queries, width, page, window, sinks, &segments);
   a.rows = (int)(segments / batch / kv_heads);
+  a.cut = (int)std::max<int64_t>({1, a.groups / 4, a.groups - segments / 2});
   PKM_REQUIRE(workspace != nullptr && workspace_bytes >= (size_t)part_bytes(a.groups, segments, dim), PKM_ERR_WORKSPACE,
               "%s: workspace too small", what);
   PKM_REQUIRE(((uintptr_t)workspace & 15) == 0, PKM_ERR_INVALID_ARGUMENT, "%s: workspace is not 16-byte aligned", what);
