@@ -51,6 +51,19 @@ struct StoreArgs {
   const int* counts;
   int64_t width;
   int batch, tokens;
+  int shift;  // log2 of the page, -1 if it is no power of two
+};
+
+// Where token t of a vector's sequence lies: its page (-1: nowhere) and slot.
+struct Place {
+  int page, slot;
+  __device__ __forceinline__ Place(const StoreArgs& a, int b, int t) {
+    const int64_t pos = (int64_t)a.starts[b] + t;
+    const uint32_t at = (uint32_t)pos;  // below 2^32
+    const uint32_t index = a.shift >= 0 ? at >> a.shift : at / (uint32_t)a.cache.page;
+    slot = (int)(at - index * (uint32_t)a.cache.page);
+    page = pos < 0 ? -1 : page_of(a.cache, a.table + b * a.width, a.width, index);
+  }
 };
 
 // ---------------------------------------------------------------------------
@@ -68,10 +81,9 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(const StoreArgs a)
   const int head = rest % H, side = (rest / H) & 1, b = rest / H / 2;
   if (b >= a.batch) return;  // the lanes of a vector leave together
   if (t >= min(a.counts[b], a.tokens)) return;
-  const int64_t pos = (int64_t)a.starts[b] + t;
-  const int page = pos < 0 ? -1 : page_of(a.cache, a.table + b * a.width, a.width, pos / a.cache.page);
+  const Place place(a, b, t);
+  const int page = place.page, slot = place.slot;
   if (page < 0) return;
-  const int slot = (int)(pos % a.cache.page);
 
   float x[32];
   const uint8_t* from = (side ? a.v : a.k).at(b, head, t) + 64 * g;
@@ -146,15 +158,14 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(const StoreArgs a) {
   const uint32_t rest = id / T_;
   const int head = rest % H, side = (rest / H) & 1, b = rest / H / 2;
   if (b >= a.batch) return;
-  int page = -1;
-  int64_t pos = 0;
+  int page = -1, slot = 0;
   if (t < a.counts[b]) {
-    pos = (int64_t)a.starts[b] + t;
-    if (pos >= 0) page = page_of(a.cache, a.table + b * a.width, a.width, pos / a.cache.page);
+    const Place place(a, b, t);
+    page = place.page, slot = place.slot;
   }
   uint4 y = make_uint4(0, 0, 0, 0);
   if (page >= 0) {
-    const int slot = (int)(pos % a.cache.page), i = j / 2, g = i / 2;
+    const int i = j / 2, g = i / 2;
     const uint8_t* codes = a.cache.codes + codes_at<D>(a.cache, side, page, head) + (int64_t)slot * (D / 2);
     const uint16_t* p = (const uint16_t*)(a.cache.params + params_at<D>(a.cache, side, page, head)) + slot;
     const float s = unpack1<T>(p[g * a.cache.page]), m = unpack1<T>(p[(NG + g) * a.cache.page]);
@@ -780,6 +791,8 @@ int check_cache(const char* what, Cache* c, void* codes, void* params, int64_t p
   return PKM_OK;
 }
 
+int page_shift(int64_t page) { return (page & (page - 1)) == 0 ? __builtin_ctzll((unsigned long long)page) : -1; }
+
 int check_rows(const char* what, const char* name, const pkm_heads_t* x) {
   PKM_REQUIRE(x != nullptr && x->data != nullptr, PKM_ERR_INVALID_ARGUMENT, "%s: %s is NULL", what, name);
   PKM_REQUIRE(((uintptr_t)x->data & 15) == 0 && x->batch % 8 == 0 && x->head % 8 == 0 && x->token % 8 == 0 &&
@@ -803,6 +816,7 @@ int store_args(const char* what, StoreArgs* a, int64_t dim, int dtype, const pkm
   a->k = heads(k), a->v = heads(v);
   a->table = table, a->starts = starts, a->counts = counts, a->width = width;
   a->batch = (int)batch, a->tokens = (int)tokens;
+  a->shift = page_shift(a->cache.page);
   (void)dim, (void)dtype;
   return PKM_OK;
 }
@@ -942,7 +956,7 @@ extern "C" int pkm_kv4_attend(const void* codes, const void* params, int64_t pag
   const int64_t far = 1 << 30;
   a.window = (int)(window < far ? window : 0), a.sinks = (int)(sinks < far ? sinks : far);
   a.scale = scale;
-  a.shift = (page & (page - 1)) == 0 ? __builtin_ctzll((unsigned long long)page) : -1;
+  a.shift = page_shift(page);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == PKM_DTYPE_BF16) {
     dim == 128 ? launch_attend<bf16_t, 128>(a, st) : launch_attend<bf16_t, 64>(a, st);
