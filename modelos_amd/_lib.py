@@ -464,6 +464,14 @@ def call(name: str, *args) -> None:
         raise PkmError(name, status, msg)
 
 
+def call_on(device: torch.device, name: str, *args) -> None:
+    """call() with `device` current, as launches on its streams need it."""
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
+
+
 def dtype_code(t: torch.Tensor | None) -> int:
     if t is None:
         return DTYPE_NONE

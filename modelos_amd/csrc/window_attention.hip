@@ -187,9 +187,10 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
 #pragma unroll
       for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
       top = fmaxf(top, fmaxf(swap_halves(top), m));
-      const float mc = (top == -INFINITY ? 0.f : top) * c;
-      if (__any(top > m)) {
-        const float f = exp2_raw(__builtin_fmaf(m, c, -mc));
+      // the reference moves only when a row's largest logit has grown by more than 8 in log2 (weights stay below 2^8;
+      // half of the tiles of a long row would otherwise rescale 64 numbers a lane)
+      if (__any((top - m) * c > 8.f)) {
+        const float f = m == -INFINITY ? 0.f : exp2_raw((m - top) * c);
         sum *= f;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
@@ -197,6 +198,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
           for (int i = 0; i < 16; ++i) o[t][i] *= f;
         m = top;
       }
+      const float mc = m == -INFINITY ? 0.f : m * c;
       frag_t pf[4];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
@@ -482,16 +484,35 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(const AttnArgs a) {
   for (int s = 0; s < KS; ++s) v[s] = frag_global<D>(vrow, s, lane);
   const TileLoad<D, kTile, 8> tl(tid);
   const uint32_t qstride = (uint32_t)(2 * a.q.token), gstride = (uint32_t)(2 * a.dO.token);
-  const auto load = [&](int i) {
-    const int head = kv * G + i / count, t0 = (tile0 + i % count) * kTile;
-    lds_u8* buf = lds + i % 3 * STAGE;
-    tl.load(buf, a.q.at(b, head, seq.start + t0), qstride, n - t0, tid);
-    tl.load(buf + TB, a.dO.at(b, head, seq.start + t0), gstride, n - t0, tid);
+  // the next stage to load: its head, first row, place in the ring and addresses
+  int load_head = kv * G, load_t0 = tile0 * kTile, load_at = 0;
+  const uint8_t *qat, *gat;
+  int64_t sat;
+  const auto start_head = [&] {
+    load_t0 = tile0 * kTile;
+    qat = a.q.at(b, load_head, seq.start + load_t0);
+    gat = a.dO.at(b, load_head, seq.start + load_t0);
+    sat = ((int64_t)b * a.q_heads + load_head) * a.tokens + seq.start + load_t0;
+  };
+  const auto load = [&] {
+    const int t0 = load_t0;
+    lds_u8* buf = lds + load_at * STAGE;
+    tl.load(buf, qat, qstride, n - t0, tid);
+    tl.load(buf + TB, gat, gstride, n - t0, tid);
     // 64 rows' lse by wave 0, delta by wave 1; the other waves load lse too, to where nobody reads it, so that
     // every wave has as many loads in flight
-    const float* from = (wave == 1 ? a.delta : a.lse) + ((int64_t)b * a.q_heads + head) * a.tokens + seq.start + t0;
+    const float* from = (wave == 1 ? a.delta : a.lse) + sat;
     const u32x4_t rs = {(uint32_t)(uintptr_t)from, (uint32_t)((uintptr_t)from >> 32), 0x7fffffffu, 0x00020000u};
     load_lds4(rs, buf + 2 * TB + 256 * wave, 4 * (uint32_t)min(lane, n - t0 - 1));
+    load_at = load_at == 2 ? 0 : load_at + 1;
+    load_t0 += kTile;
+    qat += (uint64_t)kTile * qstride;
+    gat += (uint64_t)kTile * gstride;
+    sat += kTile;
+    if (load_t0 == (tile0 + count) * kTile) {
+      ++load_head;
+      start_head();
+    }
   };
 
   f32x16_t dk[DT] = {}, dv[DT] = {};
@@ -500,10 +521,12 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(const AttnArgs a) {
     // rows of the block before the sequence's start or past its end repeat its ends: their columns are dropped
     const TileLoad<D, 128, 8> kl(tid);
     kl.load(keys, a.k.at(b, kv, first), (uint32_t)(2 * a.k.token), seq.start + n - first, tid);
-    load(0);
-    if (total > 1) load(1);
+    start_head();
+    load();
+    if (total > 1) load();
   }
   tile_wait();  // and for v: the compiler does not know of the loads to LDS and would wait for them at its use
+  int pa = tile0 * kTile + kQueries * qw, ring = 0;  // the wave's queries, the stage's place
   for (int it = 0; it < total; ++it) {
     // stage it has come, of every wave's loads; stage it - 1 is read no more
     if (it + 1 < total) {
@@ -513,15 +536,17 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(const AttnArgs a) {
     }
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (it + 2 < total) load(it + 2);
-    const int pa = (tile0 + it % count) * kTile + kQueries * qw;
+    if (it + 2 < total) load();
     if (k0 <= k1 && any_visible(pa, pa + kQueries - 1, k0, k1, W, S)) {
-      const lds_u8* buf = lds + it % 3 * STAGE;
+      const lds_u8* buf = lds + ring * STAGE;
       dkv_step<T, D>(buf + TB / 2 * qw, buf + TB + TB / 2 * qw, buf + 2 * TB + 128 * qw, buf + 2 * TB + 256 + 128 * qw,
                      keys + 32 * kw * (D * 2), v, c,
                      pa + kQueries <= n && all_visible(pa, pa + kQueries - 1, k0, k1, W, S),
                      [&](int i) { return !(pa + i < n && visible(pa + i, key, W, S)); }, dk, dv, lane);
     }
+    ring = ring == 2 ? 0 : ring + 1;
+    pa += kTile;
+    if (pa >= (tile0 + count) * kTile) pa -= count * kTile;
   }
   // the two query halves' sums
   __syncthreads();

@@ -97,9 +97,8 @@ class Int4KVCache:
         self._check_plan("Int4KVCache.append", B, table, starts=starts, counts=counts)
         _require_device(self.params, k, v)
         k, v, table, starts, counts = _rows(k), _rows(v), table.contiguous(), starts.contiguous(), counts.contiguous()
-        with torch.cuda.device(self.device):
-            _lib.call("pkm_kv4_append", *self._sizes(), _lib.heads(k), _lib.heads(v), _lib.ptr(table), table.shape[1],
-                      _lib.ptr(starts), _lib.ptr(counts), B, T, _lib.stream_of(self.device))
+        _lib.call_on(self.device, "pkm_kv4_append", *self._sizes(), _lib.heads(k), _lib.heads(v), _lib.ptr(table), table.shape[1],
+                     _lib.ptr(starts), _lib.ptr(counts), B, T, _lib.stream_of(self.device))
 
     def read(self, table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor,
              tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -111,9 +110,8 @@ class Int4KVCache:
         table, starts, counts = table.contiguous(), starts.contiguous(), counts.contiguous()
         k, v = (torch.empty((B, self.kv_heads, tokens, self.dim), dtype=self.dtype, device=self.device)
                 for _ in range(2))
-        with torch.cuda.device(self.device):
-            _lib.call("pkm_kv4_read", *self._sizes(), _lib.ptr(table), table.shape[1], _lib.ptr(starts),
-                      _lib.ptr(counts), B, tokens, _lib.heads(k), _lib.heads(v), _lib.stream_of(self.device))
+        _lib.call_on(self.device, "pkm_kv4_read", *self._sizes(), _lib.ptr(table), table.shape[1], _lib.ptr(starts),
+                     _lib.ptr(counts), B, tokens, _lib.heads(k), _lib.heads(v), _lib.stream_of(self.device))
         return k, v
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *, window: int | None = None,
@@ -143,7 +141,6 @@ class Int4KVCache:
         ws_bytes = _lib.load().pkm_kv4_attend_workspace_size(B, H, self.kv_heads, Q, D, width, self.page_size, window,
                                                             sinks)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-        with torch.cuda.device(self.device):
-            _lib.call("pkm_kv4_attend", *self._sizes(), _lib.heads(q), _lib.ptr(table), width, _lib.ptr(lengths), B, H,
-                      Q, window, sinks, scale, _lib.heads(out), _lib.ptr(ws), ws_bytes, _lib.stream_of(self.device))
+        _lib.call_on(self.device, "pkm_kv4_attend", *self._sizes(), _lib.heads(q), _lib.ptr(table), width, _lib.ptr(lengths), B, H,
+                     Q, window, sinks, scale, _lib.heads(out), _lib.ptr(ws), ws_bytes, _lib.stream_of(self.device))
         return out

@@ -55,20 +55,23 @@ def _bound(t: torch.Tensor | None) -> torch.Tensor | None:
     return None if t is None else t.contiguous()
 
 
+def _forward(q, k, v, starts, ends, window: int, sinks: int, scale: float, lse):
+    B, H, T, D = q.shape
+    out = _empty_like(q)
+    _lib.call_on(q.device, "pkm_window_attn_fwd", _lib.heads(q), _lib.heads(k), _lib.heads(v), _lib.ptr(starts),
+                 _lib.ptr(ends), B, H, k.shape[1], T, D, _lib.dtype_code(q), window, sinks, scale, _lib.heads(out),
+                 _lib.ptr(lse), _lib.stream_of(q.device))
+    return out
+
+
 class _WindowAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, starts, ends, window: int, sinks: int, scale: float, train: bool):
+    def forward(ctx, q, k, v, starts, ends, window: int, sinks: int, scale: float):
         q, k, v = _readable(q), _readable(k), _readable(v)
-        B, H, T, D = q.shape
-        out = _empty_like(q)
-        lse = torch.empty((B, H, T), dtype=torch.float32, device=q.device) if train else None
-        with torch.cuda.device(q.device):
-            _lib.call("pkm_window_attn_fwd", _lib.heads(q), _lib.heads(k), _lib.heads(v), _lib.ptr(starts),
-                      _lib.ptr(ends), B, H, k.shape[1], T, D, _lib.dtype_code(q), window, sinks, scale,
-                      _lib.heads(out), _lib.ptr(lse), _lib.stream_of(q.device))
-        if train:
-            ctx.save_for_backward(q, k, v, out, lse, starts, ends)
-            ctx.sizes = (window, sinks, scale)
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+        out = _forward(q, k, v, starts, ends, window, sinks, scale, lse)
+        ctx.save_for_backward(q, k, v, out, lse, starts, ends)
+        ctx.sizes = (window, sinks, scale)
         return out
 
     @staticmethod
@@ -80,12 +83,11 @@ class _WindowAttentionFn(torch.autograd.Function):
         dq, dk, dv = _empty_like(q), _empty_like(k), _empty_like(v)
         ws_bytes = _lib.load().pkm_window_attn_bwd_workspace_size(B, H, k.shape[1], T, D, *ctx.sizes[:2])
         ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
-        with torch.cuda.device(q.device):
-            _lib.call("pkm_window_attn_bwd", _lib.heads(q), _lib.heads(k), _lib.heads(v), _lib.heads(out),
-                      _lib.ptr(lse), _lib.heads(grad_out), _lib.ptr(starts), _lib.ptr(ends), B, H, k.shape[1], T, D,
-                      _lib.dtype_code(q), *ctx.sizes, _lib.heads(dq), _lib.heads(dk), _lib.heads(dv), _lib.ptr(ws),
-                      ws_bytes, _lib.stream_of(q.device))
-        return dq, dk, dv, None, None, None, None, None, None
+        _lib.call_on(q.device, "pkm_window_attn_bwd", _lib.heads(q), _lib.heads(k), _lib.heads(v), _lib.heads(out),
+                     _lib.ptr(lse), _lib.heads(grad_out), _lib.ptr(starts), _lib.ptr(ends), B, H, k.shape[1], T, D,
+                     _lib.dtype_code(q), *ctx.sizes, _lib.heads(dq), _lib.heads(dk), _lib.heads(dv), _lib.ptr(ws),
+                     ws_bytes, _lib.stream_of(q.device))
+        return dq, dk, dv, None, None, None, None, None
 
 
 def _check_window(window, sinks) -> tuple[int, int]:
@@ -135,5 +137,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     if T >= _MAX_TOKENS:
         raise NotImplementedError(f"window_attention: {T} tokens are not supported (fewer than {_MAX_TOKENS} are)")
     _require_device(q, k, v, *(t for t in (starts, ends) if t is not None))
-    train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    return _WindowAttentionFn.apply(q, k, v, _bound(starts), _bound(ends), window, sinks, scale, train)
+    starts, ends = _bound(starts), _bound(ends)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _WindowAttentionFn.apply(q, k, v, starts, ends, window, sinks, scale)
+    return _forward(_readable(q), _readable(k), _readable(v), starts, ends, window, sinks, scale, None)
