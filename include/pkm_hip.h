@@ -623,23 +623,27 @@ typedef struct {
  * type (relative to their row's largest so far) for the product with v.
  * lse (float32 [batch, q_heads, tokens], may be NULL): log2 of the rows' sums of
  * exponentials, +inf for rows that see nothing; what the backward reads.
+ * rest (as out, may be NULL): out's error of rounding, rounded itself; with it the
+ * backward's <grad_out, out> is exact to float32.
  */
 int pkm_window_attn_fwd(const pkm_heads_t* q, const pkm_heads_t* k, const pkm_heads_t* v,
                         const int32_t* starts, const int32_t* ends, int64_t batch, int64_t q_heads,
                         int64_t kv_heads, int64_t tokens, int64_t dim, int dtype, int64_t window,
-                        int64_t sinks, float scale, const pkm_heads_t* out, float* lse, void* stream);
+                        int64_t sinks, float scale, const pkm_heads_t* out, const pkm_heads_t* rest, float* lse,
+                        void* stream);
 
 /* Workspace bytes pkm_window_attn_bwd needs. */
 size_t pkm_window_attn_bwd_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
                                           int64_t dim, int64_t window, int64_t sinks);
 
 /*
- * Gradients of pkm_window_attn_fwd, from its inputs, its out and lse, and
+ * Gradients of pkm_window_attn_fwd, from its inputs, its out, rest (or NULL) and lse, and
  * grad_out: dq as q, dk and dv as k and v (summed over the query heads that share
  * a key head), 0 outside [starts, ends). Deterministic. Workspace: 16-byte aligned.
  */
 int pkm_window_attn_bwd(const pkm_heads_t* q, const pkm_heads_t* k, const pkm_heads_t* v,
-                        const pkm_heads_t* out, const float* lse, const pkm_heads_t* grad_out,
+                        const pkm_heads_t* out, const pkm_heads_t* rest, const float* lse,
+                        const pkm_heads_t* grad_out,
                         const int32_t* starts, const int32_t* ends, int64_t batch, int64_t q_heads,
                         int64_t kv_heads, int64_t tokens, int64_t dim, int dtype, int64_t window,
                         int64_t sinks, float scale, const pkm_heads_t* dq, const pkm_heads_t* dk,

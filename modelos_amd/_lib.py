@@ -247,8 +247,10 @@ class Heads(ctypes.Structure):
     _fields_ = [("data", c_void_p), ("batch", c_int64), ("head", c_int64), ("token", c_int64)]
 
 
-def heads(t: torch.Tensor) -> Heads:
+def heads(t: torch.Tensor | None) -> Heads | None:
     """pkm_heads_t of a [batch, heads, tokens, dim] tensor whose last dim is contiguous."""
+    if t is None:
+        return None
     s = t.stride()
     return Heads(t.data_ptr(), s[0], s[1], s[2])
 
@@ -261,14 +263,14 @@ SIGNATURES.update({
             _HEADS, _HEADS, _HEADS, c_void_p, c_void_p,  # q, k, v, starts, ends
             c_int64, c_int64, c_int64, c_int64, c_int64, c_int,  # batch, q_heads, kv_heads, tokens, dim, dtype
             c_int64, c_int64, c_float,  # window, sinks, scale
-            _HEADS, c_void_p, c_void_p,  # out, lse, stream
+            _HEADS, _HEADS, c_void_p, c_void_p,  # out, rest, lse, stream
         ],
     ),
     "pkm_window_attn_bwd_workspace_size": (c_size_t, [c_int64] * 7),
     "pkm_window_attn_bwd": (
         c_int,
         [
-            _HEADS, _HEADS, _HEADS, _HEADS, c_void_p, _HEADS,  # q, k, v, out, lse, grad_out
+            _HEADS, _HEADS, _HEADS, _HEADS, _HEADS, c_void_p, _HEADS,  # q, k, v, out, rest, lse, grad_out
             c_void_p, c_void_p,  # starts, ends
             c_int64, c_int64, c_int64, c_int64, c_int64, c_int,  # batch, q_heads, kv_heads, tokens, dim, dtype
             c_int64, c_int64, c_float,  # window, sinks, scale

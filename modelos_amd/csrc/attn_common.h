@@ -192,17 +192,26 @@ struct Heads {
   }
 };
 
-// Row of a C^T tile set (columns = the lane's row of the tensor, rows = its numbers) times f to memory.
+// Row of a C^T tile set (columns = the lane's row of the tensor, rows = its numbers) times f to memory; with rest, what
+// the rounding left of it there.
 template <typename T, int D>
-__device__ __forceinline__ void store_row(uint8_t* row, const f32x16_t (&acc)[D / 32], float f, int lane) {
+__device__ __forceinline__ void store_row(uint8_t* row, const f32x16_t (&acc)[D / 32], float f, int lane,
+                                          uint8_t* rest = nullptr) {
   const int h = lane >> 5;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      const u32x2_t x = {pack2<T>(acc[t][4 * a] * f, acc[t][4 * a + 1] * f),
-                         pack2<T>(acc[t][4 * a + 2] * f, acc[t][4 * a + 3] * f)};
-      *(u32x2_t*)(row + 2 * (32 * t + 8 * a + 4 * h)) = x;
+      const int at = 2 * (32 * t + 8 * a + 4 * h);
+      u32x2_t x, r;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float y = acc[t][4 * a + 2 * e] * f, z = acc[t][4 * a + 2 * e + 1] * f;
+        x[e] = pack2<T>(y, z);
+        if (rest) r[e] = pack2<T>(y - unpack1<T>(x[e] & 0xffffu), z - unpack1<T>(x[e] >> 16));
+      }
+      *(u32x2_t*)(row + at) = x;
+      if (rest) *(u32x2_t*)(rest + at) = r;
     }
 }
 

@@ -16,6 +16,7 @@ constexpr int kTile = 64;      // rows of an LDS tile
 
 struct AttnArgs {
   Heads q, k, v, o, dO, dq, dk, dv;
+  Heads rest;    // what the rounding left of o, or nothing
   float* lse;    // [batch, q_heads, tokens], in units of log2; +inf where nothing is visible
   float* delta;  // [batch, q_heads, tokens]
   const int* starts;
@@ -229,7 +230,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[t][i] = some ? o[t][i] : 0.f;
-  store_row<T, D>(a.o.at(qb.b, qb.head, row), o, some ? 1.f / sum : 0.f, lane);
+  store_row<T, D>(a.o.at(qb.b, qb.head, row), o, some ? 1.f / sum : 0.f, lane,
+                  a.rest.p ? a.rest.at(qb.b, qb.head, row) : nullptr);
   if (a.lse && h == 0) {
     a.lse[((int64_t)qb.b * a.q_heads + qb.head) * a.tokens + row] =
         some ? m * c + __builtin_amdgcn_logf(sum) : INFINITY;
@@ -239,8 +241,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
 // ---------------------------------------------------------------------------
 // Backward, dQ: as the forward, dS^T = P^T (V dO^T - delta), dQ^T = K^T dS^T.
 //
-// delta comes from the rounded output. What that puts into a row's dS adds up to
-// sum_j dS_j (which is 0), so the sum corrects the delta that dK reads. dS enters its
+// delta comes from the output, with what its rounding left where that was kept. What an error in it puts into a row's dS
+// adds up to sum_j dS_j (which is 0), so the sum corrects the delta that dK reads. dS enters its
 // product as two 16-bit numbers, itself rounded and the rest: keys have a common part,
 // which the exact dS, whose sum is 0, cancels and the roundings of one would not (relative error
 // of dQ 2.7e-3 with one, 2.0e-3 with two in bf16, where the result's own rounding is 1.7e-3).
@@ -276,6 +278,12 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
 #pragma unroll
   for (int s = 0; s < KS; ++s)
     delta = vec_dot<T>(__builtin_bit_cast(uint4, frag_global<D>(orow, s, lane)), __builtin_bit_cast(uint4, g[s]), delta);
+  if (a.rest.p) {
+    const uint8_t* rrow = live ? a.rest.at(qb.b, qb.head, row) : nullptr;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      delta = vec_dot<T>(__builtin_bit_cast(uint4, frag_global<D>(rrow, s, lane)), __builtin_bit_cast(uint4, g[s]), delta);
+  }
   delta += swap_halves(delta);
 
   const uint8_t* kbase = a.k.at(qb.b, qb.kv, seq.start);
@@ -773,16 +781,18 @@ using namespace pkm;
 extern "C" int pkm_window_attn_fwd(const pkm_heads_t* q, const pkm_heads_t* k, const pkm_heads_t* v,
                                    const int32_t* starts, const int32_t* ends, int64_t batch, int64_t q_heads,
                                    int64_t kv_heads, int64_t tokens, int64_t dim, int dtype, int64_t window,
-                                   int64_t sinks, float scale, const pkm_heads_t* out, float* lse, void* stream) {
+                                   int64_t sinks, float scale, const pkm_heads_t* out, const pkm_heads_t* rest, float* lse,
+                                   void* stream) {
   const char* what = "pkm_window_attn_fwd";
   AttnArgs a = {};
   int rc = fill_args(what, &a, batch, q_heads, kv_heads, tokens, dim, dtype, window, sinks, scale);
   if (rc != PKM_OK) return rc;
   if (batch == 0 || tokens == 0) return PKM_OK;
   if ((rc = check_heads(what, "q", q)) || (rc = check_heads(what, "k", k)) || (rc = check_heads(what, "v", v)) ||
-      (rc = check_heads(what, "out", out)))
+      (rc = check_heads(what, "out", out)) || (rest != nullptr && (rc = check_heads(what, "rest", rest))))
     return rc;
   a.q = heads(q), a.k = heads(k), a.v = heads(v), a.o = heads(out);
+  if (rest != nullptr) a.rest = heads(rest);
   a.starts = starts, a.ends = ends, a.lse = lse;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == PKM_DTYPE_BF16) {
@@ -805,7 +815,8 @@ extern "C" size_t pkm_window_attn_bwd_workspace_size(int64_t batch, int64_t q_he
 }
 
 extern "C" int pkm_window_attn_bwd(const pkm_heads_t* q, const pkm_heads_t* k, const pkm_heads_t* v,
-                                   const pkm_heads_t* out, const float* lse, const pkm_heads_t* grad_out,
+                                   const pkm_heads_t* out, const pkm_heads_t* rest, const float* lse,
+                                   const pkm_heads_t* grad_out,
                                    const int32_t* starts, const int32_t* ends, int64_t batch, int64_t q_heads,
                                    int64_t kv_heads, int64_t tokens, int64_t dim, int dtype, int64_t window,
                                    int64_t sinks, float scale, const pkm_heads_t* dq, const pkm_heads_t* dk,
@@ -816,7 +827,8 @@ extern "C" int pkm_window_attn_bwd(const pkm_heads_t* q, const pkm_heads_t* k, c
   if (rc != PKM_OK) return rc;
   if (batch == 0 || tokens == 0) return PKM_OK;
   if ((rc = check_heads(what, "q", q)) || (rc = check_heads(what, "k", k)) || (rc = check_heads(what, "v", v)) ||
-      (rc = check_heads(what, "out", out)) || (rc = check_heads(what, "grad_out", grad_out)) ||
+      (rc = check_heads(what, "out", out)) || (rest != nullptr && (rc = check_heads(what, "rest", rest))) ||
+      (rc = check_heads(what, "grad_out", grad_out)) ||
       (rc = check_heads(what, "dq", dq)) || (rc = check_heads(what, "dk", dk)) || (rc = check_heads(what, "dv", dv)))
     return rc;
   PKM_REQUIRE(lse != nullptr, PKM_ERR_INVALID_ARGUMENT, "%s: lse is NULL", what);
@@ -826,6 +838,7 @@ extern "C" int pkm_window_attn_bwd(const pkm_heads_t* q, const pkm_heads_t* k, c
   PKM_REQUIRE(((uintptr_t)workspace & 15) == 0, PKM_ERR_INVALID_ARGUMENT, "%s: workspace is not 16-byte aligned", what);
   a.q = heads(q), a.k = heads(k), a.v = heads(v), a.o = heads(out), a.dO = heads(grad_out);
   a.dq = heads(dq), a.dk = heads(dk), a.dv = heads(dv);
+  if (rest != nullptr) a.rest = heads(rest);
   a.starts = starts, a.ends = ends, a.lse = const_cast<float*>(lse), a.delta = (float*)workspace;
   a.far = (float*)((uint8_t*)workspace + delta_bytes(a));
   const hipStream_t st = (hipStream_t)stream;

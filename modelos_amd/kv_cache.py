@@ -8,7 +8,7 @@ A head vector is held in groups of 32 numbers: minimum m and step
 s = (max - min) / 15 in the cache's type, codes c = round((x - m) / s); the
 number read back is m + s c, within s / 2 of x up to the rounding of m, s and
 the result. Numbers have to be finite, and far enough from the type's ends that
-max - min and m + 15 s stay inside it. With the parameters a number takes 5
+max - min and m + 15 s stay inside it; attend needs steps between 2^-100 and 2^100. With the parameters a number takes 5
 bits instead of 16.
 
 Pages are the caller's to hand out: `table` [batch, width] (int32, on the
@@ -97,8 +97,8 @@ class Int4KVCache:
         self._check_plan("Int4KVCache.append", B, table, starts=starts, counts=counts)
         _require_device(self.params, k, v)
         k, v, table, starts, counts = _rows(k), _rows(v), table.contiguous(), starts.contiguous(), counts.contiguous()
-        _lib.call_on(self.device, "pkm_kv4_append", *self._sizes(), _lib.heads(k), _lib.heads(v), _lib.ptr(table), table.shape[1],
-                     _lib.ptr(starts), _lib.ptr(counts), B, T, _lib.stream_of(self.device))
+        _lib.call_on(self.device, "pkm_kv4_append", *self._sizes(), _lib.heads(k), _lib.heads(v), _lib.ptr(table),
+                     table.shape[1], _lib.ptr(starts), _lib.ptr(counts), B, T, _lib.stream_of(self.device))
 
     def read(self, table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor,
              tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -141,6 +141,7 @@ class Int4KVCache:
         ws_bytes = _lib.load().pkm_kv4_attend_workspace_size(B, H, self.kv_heads, Q, D, width, self.page_size, window,
                                                             sinks)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-        _lib.call_on(self.device, "pkm_kv4_attend", *self._sizes(), _lib.heads(q), _lib.ptr(table), width, _lib.ptr(lengths), B, H,
-                     Q, window, sinks, scale, _lib.heads(out), _lib.ptr(ws), ws_bytes, _lib.stream_of(self.device))
+        _lib.call_on(self.device, "pkm_kv4_attend", *self._sizes(), _lib.heads(q), _lib.ptr(table), width,
+                     _lib.ptr(lengths), B, H, Q, window, sinks, scale, _lib.heads(out), _lib.ptr(ws), ws_bytes,
+                     _lib.stream_of(self.device))
         return out

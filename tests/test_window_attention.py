@@ -55,7 +55,7 @@ def lib():
 
 
 def _fwd(lib, x, sizes=(1, 4, 2, 8, 64, 1), window=0, sinks=0, scale=0.1):
-    return lib.pkm_window_attn_fwd(x, x, x, None, None, *sizes, window, sinks, scale, x, None, None)
+    return lib.pkm_window_attn_fwd(x, x, x, None, None, *sizes, window, sinks, scale, x, None, None, None)
 
 
 def test_entry_point_statuses(lib):
@@ -93,7 +93,7 @@ def test_backward_workspace(lib):
     assert need >= 4 * 8 * 4
     assert lib.pkm_window_attn_bwd_workspace_size(-1, 4, 2, 8, 64, 0, 0) == 0
     lse = ctypes.c_void_p(1 << 20)
-    run = lambda lse, ws, n: lib.pkm_window_attn_bwd(x, x, x, x, lse, x, None, None, *sizes, 1, 0, 0, 0.1, x, x, x, ws,
+    run = lambda lse, ws, n: lib.pkm_window_attn_bwd(x, x, x, x, None, lse, x, None, None, *sizes, 1, 0, 0, 0.1, x, x, x, ws,
                                                      n, None)
     assert run(None, lse, need) == 1
     assert run(lse, None, need) == 3

@@ -88,6 +88,13 @@ def test_sinks_of_padded_long_sequences(device, dtype, D, window, sinks):
     _check(device, q, k, v, do, window, sinks, starts, ends)
 
 
+@pytest.mark.parametrize("dtype,D", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("window,sinks", [(None, 0), (530, 2)])
+def test_long_windows(device, dtype, D, window, sinks):
+    """Windows that are too long for the output's rounding to be kept."""
+    _check(device, *_inputs(1, 620, 2, 1, D, dtype, seed=18), window, sinks)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
 def test_strides(device, dtype):
     """Heads inside a fused projection, contiguous, expanded, unaligned and sliced: the same numbers every time."""
