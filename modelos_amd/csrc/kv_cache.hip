@@ -819,7 +819,7 @@ int store_args(const char* what, StoreArgs* a, int64_t dim, int dtype, const pkm
   if ((rc = check_rows(what, "k", k)) || (rc = check_rows(what, "v", v))) return rc;
   PKM_REQUIRE(starts != nullptr && counts != nullptr && (table != nullptr || width == 0), PKM_ERR_INVALID_ARGUMENT,
               "%s: table, starts and counts have to be given", what);
-  PKM_REQUIRE(batch < (1ll << 31) && tokens < (1ll << 31) && 2 * batch * tokens < (1ll << 31) / a->cache.heads,
+  PKM_REQUIRE(tokens < (1ll << 30) / a->cache.heads && batch < (1ll << 30) / a->cache.heads / tokens,
               PKM_ERR_UNSUPPORTED, "%s: too many tokens", what);
   a->k = heads(k), a->v = heads(v);
   a->table = table, a->starts = starts, a->counts = counts, a->width = width;
@@ -852,6 +852,13 @@ int run_store(const char* what, const StoreArgs& a, int64_t dim, int dtype, void
   return pkm_check_launch(what);
 }
 
+// Below 2^25 tiles a sequence and 2^24 query rows in all.
+bool attend_sizes_fit(int64_t batch, int64_t q_heads, int64_t queries, int64_t width, int64_t page) {
+  const int64_t most = 1 << 24;
+  return width < (1ll << 30) / page && batch < most && q_heads < most && queries < most && batch * q_heads < most &&
+         batch * q_heads * queries < most;
+}
+
 // Shares of a call, from sizes alone: as many workgroups as run at once, none with fewer than 8 tiles. Cut segment by
 // segment, up to one more a segment may be needed; those that are not end at once. 768: three on each of 256 CUs (512, 1024
 // and 1536 took 183, 209 and 185 us where 768 took 178, and 42, 45 and 48 for one long sequence's 40).
@@ -860,7 +867,8 @@ int attend_groups(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t quer
   const int64_t rows = (q_heads / kv_heads * queries + kRows - 1) / kRows;
   int64_t most = (width * page + kTok - 1) / kTok;
   if (window > 0) {
-    const int64_t seen = (window + queries) / kTok + 2 + (sinks + kTok - 1) / kTok;
+    const int64_t far = 1ll << 40;  // as good as any longer one
+    const int64_t seen = (std::min(window, far) + queries) / kTok + 2 + (std::min(sinks, far) + kTok - 1) / kTok;
     if (seen < most) most = seen;
   }
   *segments = batch * kv_heads * rows;
@@ -922,7 +930,9 @@ extern "C" int pkm_kv4_read(const void* codes, const void* params, int64_t pages
 extern "C" size_t pkm_kv4_attend_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t queries,
                                                 int64_t dim, int64_t width, int64_t page, int64_t window,
                                                 int64_t sinks) {
-  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || queries <= 0 || dim <= 0 || width < 0 || page <= 0) return 0;
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || queries <= 0 || dim <= 0 || dim > 128 || width < 0 || page <= 0 ||
+      window < 0 || sinks < 0 || !attend_sizes_fit(batch, q_heads, queries, width, page))
+    return 0;
   int64_t segments;
   const int groups = attend_groups(batch, q_heads, kv_heads, queries, width, page, window, sinks, &segments);
   return (size_t)part_bytes(groups, segments, dim);
@@ -948,9 +958,8 @@ extern "C" int pkm_kv4_attend(const void* codes, const void* params, int64_t pag
   PKM_REQUIRE(pages > 0, PKM_ERR_UNSUPPORTED, "%s: the cache has no pages", what);
   PKM_REQUIRE(lengths != nullptr && (table != nullptr || width == 0), PKM_ERR_INVALID_ARGUMENT,
               "%s: table and lengths have to be given", what);
-  PKM_REQUIRE(width < (1ll << 30) / page && batch < (1 << 24) && q_heads < (1 << 20) && queries < (1 << 20) &&
-                  batch * q_heads * queries < (1ll << 24),
-              PKM_ERR_UNSUPPORTED, "%s: too many tokens or rows", what);
+  PKM_REQUIRE(attend_sizes_fit(batch, q_heads, queries, width, page), PKM_ERR_UNSUPPORTED,
+              "%s: too many tokens or rows", what);
   int64_t segments;
   a.groups = attend_groups(batch, q_heads, kv_heads, queries, width, page, window, sinks, &segments);
   a.rows = (int)(segments / batch / kv_heads);

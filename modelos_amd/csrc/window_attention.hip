@@ -735,7 +735,8 @@ int fill_args(const char* what, AttnArgs* a, int64_t batch, int64_t q_heads, int
   PKM_REQUIRE(scale > 0.f && scale <= 3.0e38f, PKM_ERR_INVALID_ARGUMENT, "%s: scale has to be positive and finite", what);
   PKM_REQUIRE((dim == 64 || dim == 128) && (dtype == PKM_DTYPE_BF16 || dtype == PKM_DTYPE_F16), PKM_ERR_UNSUPPORTED,
               "%s: head dims 64 and 128 in bf16 and f16 are supported", what);
-  PKM_REQUIRE(tokens < (1 << 24) && batch * q_heads < (1 << 24) && batch * q_heads * ((tokens + 31) / 32) < (1ll << 31),
+  PKM_REQUIRE(tokens < (1 << 24) && batch < (1 << 24) && q_heads < (1 << 24) && batch * q_heads < (1 << 24) &&
+                  batch * q_heads * ((tokens + 31) / 32) < (1ll << 31),
               PKM_ERR_UNSUPPORTED, "%s: too many tokens or heads", what);
   a->batch = (int)batch;
   a->q_heads = (int)q_heads;

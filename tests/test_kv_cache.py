@@ -123,6 +123,8 @@ def test_entry_point_statuses(lib):
     assert _append(lib, good, (4, 2, 16, 96, 1)) == 2
     assert _append(lib, good, (4, 2, 16, 64, 0)) == 2
     assert _append(lib, good, tokens=1 << 31) == 2
+    assert _append(lib, good, batch=(1 << 31) - 1, tokens=(1 << 31) - 1) == 2
+    assert _append(lib, good, batch=1 << 62) == 2
     assert _append(lib, Heads((1 << 20) + 4, 2048, 512, 64)) == 2
     assert _append(lib, good, batch=0) == 0
     assert _append(lib, good, tokens=0) == 0
@@ -134,7 +136,9 @@ def test_entry_point_statuses(lib):
     assert _attend(lib, good, (4, 2, 16, 80, 1)) == 2
     assert _attend(lib, good, (0, 2, 16, 64, 1)) == 2
     assert _attend(lib, good, width=1 << 30) == 2
-    assert _attend(lib, good, queries=1 << 21) == 2
+    assert _attend(lib, good, queries=1 << 24) == 2
+    assert _attend(lib, good, batch=1 << 23, heads=1 << 23, queries=1 << 23) == 2
+    assert lib.pkm_kv4_attend_workspace_size(1 << 23, 1 << 23, 1, 1 << 23, 64, 4, 16, 0, 0) == 0
     assert _attend(lib, Heads(1 << 20, 2044, 512, 64)) == 2
     assert _attend(lib, good, queries=0) == 0
     assert _attend(lib, good, batch=0) == 0

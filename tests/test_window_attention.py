@@ -75,6 +75,7 @@ def test_entry_point_statuses(lib):
     assert _fwd(lib, good, (1, 4, 2, 8, 96, 1)) == 2
     assert _fwd(lib, good, (1, 4, 2, 8, 64, 0)) == 2
     assert _fwd(lib, good, (1, 4, 2, 1 << 24, 64, 1)) == 2
+    assert _fwd(lib, good, (1 << 40, 1 << 40, 1, 8, 64, 1)) == 2
     assert _fwd(lib, Heads((1 << 20) + 8, 2048, 512, 64)) == 2
     assert _fwd(lib, Heads(1 << 20, 2048, 512, 68)) == 2
     assert _fwd(lib, Heads(1 << 20, 2048, 512, 1 << 22)) == 2
