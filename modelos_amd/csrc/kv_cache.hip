@@ -278,7 +278,7 @@ __device__ __forceinline__ Shares shares(const AttendArgs& a, int group, int b) 
   Shares r;
   const int64_t even = quotient(total + a.groups - 1, a.groups);
   r.whole = even >= 64;
-  r.per = (int)(r.whole ? even : max(quotient(total + a.cut - 1, a.cut), (int64_t)8));
+  r.per = (int)(r.whole ? even : max(quotient(total + a.cut - 1, a.cut), (int64_t)4));
   const int64_t first = r.whole ? (int64_t)group * r.per : group;
   r.b = a.batch;
   r.before = 0;
@@ -859,7 +859,8 @@ bool attend_sizes_fit(int64_t batch, int64_t q_heads, int64_t queries, int64_t w
          batch * q_heads * queries < most;
 }
 
-// Shares of a call, from sizes alone: as many workgroups as run at once, none with fewer than 8 tiles. Cut segment by
+// Shares of a call, from sizes alone: as many workgroups as run at once, none with fewer than 4 tiles, one a wave (250
+// tokens: 9.6 us against 12 with two a wave; the same from 1000 on). Cut segment by
 // segment, up to one more a segment may be needed; those that are not end at once. 768: three on each of 256 CUs (512, 1024
 // and 1536 took 183, 209 and 185 us where 768 took 178, and 42, 45 and 48 for one long sequence's 40).
 int attend_groups(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t queries, int64_t width, int64_t page,
@@ -874,7 +875,7 @@ int attend_groups(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t quer
   *segments = batch * kv_heads * rows;
   // (a product of large sizes may not fit; more than kGroups is all that counts)
   const double tiles = (double)*segments * (double)most;
-  return tiles >= 8.0 * kGroups ? kGroups : (int)(tiles / 8.0) + 1;
+  return tiles >= 4.0 * kGroups ? kGroups : (int)(tiles / 4.0) + 1;
 }
 
 int64_t part_bytes(int64_t groups, int64_t segments, int64_t dim) {
