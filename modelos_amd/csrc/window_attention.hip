@@ -574,52 +574,53 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(const AttnArgs a) {
     pa += kTile;
     if (pa >= (tile0 + count) * kTile) pa -= count * kTile;
   }
-  // the two query halves' sums
+  // the two query halves' sums: the waves of the first finish dK, those of the second dV
   __syncthreads();
-  static_assert(4 * 2 * 32 * D * 4 <= KEYS + 3 * STAGE, "four waves' sums fit");
-  float* const sums = (float*)smem + kw * (2 * 32 * D) + lane;
-  if (qw == 1) {
+  static_assert(8 * 32 * D * 4 <= KEYS + 3 * STAGE, "eight waves' sums fit");
+  float* const sums = (float*)smem + lane;
+  const auto give = [&](const f32x16_t(&x)[DT], int slot) {
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        sums[(t * 16 + i) * 64] = dk[t][i];
-        sums[((DT + t) * 16 + i) * 64] = dv[t][i];
+      for (int i = 0; i < 16; ++i) sums[slot * (32 * D) + (t * 16 + i) * 64] = x[t][i];
+  };
+  const auto finish = [&](f32x16_t(&x)[DT], int slot, const Heads& to, float f, int part) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[t][i] += sums[slot * (32 * D) + (t * 16 + i) * 64];
+    if (a.far_chunks && live && key < a.sinks) {  // the far queries' part, in their order
+      const FarPlan far(a, pair, key / 32, n);
+      for (int i = 0; i < far.used; ++i) {
+        const float* from = far.part(a, i) + part + (int64_t)(key % 32) * D + 4 * h;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f32x4_t y = *(const f32x4_t*)(from + 32 * t + 8 * e);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[t][4 * e + r] += y[r];
+          }
       }
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[t][i] = live ? x[t][i] : 0.f;
+    store_row<T, D>(to.at(b, kv, row), x, f, lane);
+  };
+  if (qw == 0) {
+    give(dv, 4 + kw);
+  } else {
+    give(dk, kw);
   }
   __syncthreads();
-  if (qw == 1 || row >= a.tokens) return;
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      dk[t][i] += sums[(t * 16 + i) * 64];
-      dv[t][i] += sums[((DT + t) * 16 + i) * 64];
-    }
-  if (a.far_chunks && live && key < a.sinks) {  // the far queries' part, in their order
-    const FarPlan far(a, pair, key / 32, n);
-    for (int i = 0; i < far.used; ++i) {
-      const float* from = far.part(a, i) + (int64_t)(key % 32) * D + 4 * h;
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            dk[t][4 * e + r] += from[32 * t + 8 * e + r];
-            dv[t][4 * e + r] += from[32 * D + 32 * t + 8 * e + r];
-          }
-    }
+  if (row >= a.tokens) return;
+  if (qw == 0) {
+    finish(dk, kw, a.dk, a.scale, 0);
+  } else {
+    finish(dv, 4 + kw, a.dv, 1.f, 32 * D);
   }
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      dk[t][i] = live ? dk[t][i] : 0.f;
-      dv[t][i] = live ? dv[t][i] : 0.f;
-    }
-  store_row<T, D>(a.dk.at(b, kv, row), dk, a.scale, lane);
-  store_row<T, D>(a.dv.at(b, kv, row), dv, 1.f, lane);
 }
 
 // The sinks' gradients from the queries past their windows: few keys, most queries. A workgroup takes 32 sinks and
