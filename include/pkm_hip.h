@@ -620,7 +620,8 @@ typedef struct {
  * starts, ends: int32 [batch] on the device, clamped to [0, tokens]; NULL: 0, tokens.
  * window 0: no window. dim 64 or 128, bf16 or f16, scale > 0.
  * Logits, softmax and sums are float32; the weights are rounded to the tensors'
- * type (relative to their row's largest so far) for the product with v.
+ * type for the product with v. An infinite or NaN token inside a sequence also reaches
+ * queries that share its tile without seeing it.
  * lse (float32 [batch, q_heads, tokens], may be NULL): log2 of the rows' sums of
  * exponentials, +inf for rows that see nothing; what the backward reads.
  * rest (as out, may be NULL): out's error of rounding, rounded itself; with it the
@@ -690,9 +691,10 @@ size_t pkm_kv4_attend_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_
  * stands at position p = lengths[b] - queries + i and sees the positions j <= p with
  * p - j < window or j < sinks (window 0: no window). q, out: [batch, q_heads, queries,
  * dim] in the cache's type; rows that see nothing (p < 0 among them) are written as 0.
- * Logits, softmax and sums are float32. The weights are rounded to bf16 (f16 caches:
- * to twice its digits) with the values' steps in them, and to the cache's type for
- * the minima. Sums run in a fixed order (deterministic).
+ * Logits, softmax and sums are float32. The weights enter the products with the values'
+ * steps in them as f16 numbers near 1 (f16 caches: two), with the minima as two numbers
+ * of the cache's type. Numbers may be infinite or NaN only in tokens that no query sees;
+ * steps lie between 2^-100 and 2^100. Sums run in a fixed order (deterministic).
  */
 int pkm_kv4_attend(const void* codes, const void* params, int64_t pages, int64_t kv_heads, int64_t page,
                    int64_t dim, int dtype, const pkm_heads_t* q, const int32_t* table, int64_t width,

@@ -670,8 +670,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_far_kernel(const AttnArgs 
     __syncthreads();
     if (u0 + wave < end) {
       const lds_u8* buf = lds + wave * BUF;
-      dkv_step<T, D>(buf, buf + TB, buf + 2 * TB, buf + 2 * TB + 4 * kQueries, keys, v, c, t0 - (32 * block + 31) >= W && 32 * block + 31 < S,
-                     [&](int i) { return t0 + i - key < W || key >= S; }, dk, dv, lane);
+      dkv_step<T, D>(buf, buf + TB, buf + 2 * TB, buf + 2 * TB + 4 * kQueries, keys, v, c,
+                     t0 - (32 * block + 31) >= W && 32 * block + 31 < S, [&](int i) { return t0 + i - key < W || key >= S; }, dk, dv, lane);
     }
     __syncthreads();
   }

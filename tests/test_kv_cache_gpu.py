@@ -1,8 +1,8 @@
 """The 4-bit key / value cache: append and read exactly, attention over it against the formulas in 64 bits.
 
-Bounds of attend: weights with the values' steps in them are rounded to bf16 (u = 2^-8; f16 caches: to a bf16 and
-the rest in bf16, 2^-16), weights of the minima to the cache's type; the result to the cache's type. Codes enter the
-product as 16 + c, and -16 is taken off with the same rounded weights, so the rounding of a weight counts once."""
+Bounds of attend: weights with the values' steps in them may be rounded to bf16 (u = 2^-8; f16 caches: to a bf16 and
+the rest in bf16, 2^-16), weights of the minima to the cache's type, codes may enter the product as 16 + c; the result
+is rounded to the cache's type. The kernel rounds its weights more finely than that."""
 from __future__ import annotations
 
 import pytest
