@@ -47,6 +47,9 @@ __device__ __forceinline__ bool all_visible(int p0, int p1, int j0, int j1, int 
   return j1 <= p0 && (p1 - j0 < W || j1 < S);
 }
 __device__ __forceinline__ bool visible(int p, int j, int W, int S) { return j <= p && (p - j < W || j < S); }
+// The query at position p sees one key alone. Its weight is 1 whatever q and the key are, so their gradients are 0, which
+// dS is only up to rounding: dO V^T and delta are summed in different orders.
+__device__ __forceinline__ bool lone(int p, int W, int S) { return p == 0 || (W == 1 && S == 0); }
 
 // The key tiles that queries [p0, p1] see: tiles [0, sink) hold the sinks, then those of the window follow.
 struct KeyTiles {
@@ -385,7 +388,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dq[t][i] = live ? dq[t][i] : 0.f;
-  store_row<T, D>(a.dq.at(qb.b, qb.head, row), dq, a.scale, lane);
+  store_row<T, D>(a.dq.at(qb.b, qb.head, row), dq, lone(p, W, S) ? 0.f : a.scale, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -409,11 +412,11 @@ struct DkvLds {
 };
 
 // One step: 32 queries, their dO, lse and delta, and the wave's 32 keys in LDS, their values v.
-// masked(i): the row i of the lane's column is not visible; all: none is masked.
+// masked(i): the row i of the lane's column is not visible; all: none is masked. lone0: the step's first query sees one key alone.
 template <typename T, int D, typename F>
 __device__ __forceinline__ void dkv_step(const lds_u8* qtile, const lds_u8* gtile, const lds_u8* lses,
                                          const lds_u8* deltas, const lds_u8* keys, const frag_t (&v)[D / 16], float c,
-                                         bool all, F masked, f32x16_t (&dk)[D / 32], f32x16_t (&dv)[D / 32], int lane) {
+                                         bool all, bool lone0, F masked, f32x16_t (&dk)[D / 32], f32x16_t (&dv)[D / 32], int lane) {
   constexpr int KS = D / 16, DT = D / 32;
   asm volatile("" : "+v"(lane));  // the addresses below are worked out anew in each step: kept over the loop, they spill
   const int h = lane >> 5;
@@ -458,6 +461,7 @@ __device__ __forceinline__ void dkv_step(const lds_u8* qtile, const lds_u8* gtil
       dp[i] = s[i] * (dp[i] - delta[r]);
     }
   }
+  if (lone0) dp[0] = h == 0 ? 0.f * dp[0] : dp[0];
   frag_t pf[2], sf[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -567,7 +571,7 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(const AttnArgs a) {
       const lds_u8* buf = lds + ring * STAGE;
       dkv_step<T, D>(buf + TB / 2 * qw, buf + TB + TB / 2 * qw, buf + 2 * TB + 128 * qw, buf + 2 * TB + 256 + 128 * qw,
                      keys + 32 * kw * (D * 2), v, c,
-                     pa + kQueries <= n && all_visible(pa, pa + kQueries - 1, k0, k1, W, S),
+                     pa + kQueries <= n && all_visible(pa, pa + kQueries - 1, k0, k1, W, S), pa == 0,
                      [&](int i) { return !(pa + i < n && visible(pa + i, key, W, S)); }, dk, dv, lane);
     }
     ring = ring == 2 ? 0 : ring + 1;
@@ -617,7 +621,7 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(const AttnArgs a) {
   __syncthreads();
   if (row >= a.tokens) return;
   if (qw == 0) {
-    finish(dk, kw, a.dk, a.scale, 0);
+    finish(dk, kw, a.dk, W == 1 && a.sinks == 0 ? 0.f : a.scale, 0);
   } else {
     finish(dv, 4 + kw, a.dv, 1.f, 32 * D);
   }
@@ -671,7 +675,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_far_kernel(const AttnArgs 
     if (u0 + wave < end) {
       const lds_u8* buf = lds + wave * BUF;
       dkv_step<T, D>(buf, buf + TB, buf + 2 * TB, buf + 2 * TB + 4 * kQueries, keys, v, c,
-                     t0 - (32 * block + 31) >= W && 32 * block + 31 < S, [&](int i) { return t0 + i - key < W || key >= S; }, dk, dv, lane);
+                     t0 - (32 * block + 31) >= W && 32 * block + 31 < S, false, [&](int i) { return t0 + i - key < W || key >= S; }, dk, dv, lane);
     }
     __syncthreads();
   }

@@ -10,7 +10,9 @@ and out_p = sum_j softmax_j(scale q_p.k_j) v_j over the visible keys. Rows that
 see no key, those of padding among them, are zeros in the output and in the
 gradients; what the inputs hold there is not used (it may be NaN). Key heads
 are shared by consecutive groups of query heads; their gradients are summed
-over the group in a fixed order, so the backward is deterministic.
+over the group in a fixed order, so the backward is deterministic. A row that
+sees one key alone has the weight 1 whatever q and k are: its gradients to both
+are exactly 0.
 
 Logits, softmax statistics and sums are float32. The softmax weights, and in
 the backward their gradients, are rounded to the inputs' type for the matrix
