@@ -30,6 +30,7 @@ from .embedding_bag import _require_device
 from .window_attention import _DIMS, _DTYPES, _check_scale, _check_window
 
 GROUP = 32
+_MAX_POSITIONS = 1 << 30  # of a sequence's table; the entry point takes fewer
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -130,7 +131,7 @@ class Int4KVCache:
             raise ValueError(f"Int4KVCache.attend: q has to be {self.dtype}, got {q.dtype}")
         if torch.is_grad_enabled() and q.requires_grad:
             raise RuntimeError("Int4KVCache.attend has no backward; call it under torch.no_grad() or detach q")
-        window, sinks = _check_window(window, sinks)
+        window, sinks = _check_window(window, sinks, _MAX_POSITIONS)
         scale = _check_scale(scale, self.dim)
         B, H, Q, D = q.shape
         self._check_plan("Int4KVCache.attend", B, table, lengths=lengths)

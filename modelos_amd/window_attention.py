@@ -98,13 +98,13 @@ class _WindowAttentionFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None
 
 
-def _check_window(window, sinks) -> tuple[int, int]:
+def _check_window(window, sinks, most: int) -> tuple[int, int]:
+    """window (0: none) and sinks, cut to `most`, which no sequence reaches: the entry points take 64-bit sizes."""
     if window is not None and (not isinstance(window, int) or isinstance(window, bool) or window < 1):
         raise ValueError(f"window {window!r} has to be a whole number of at least 1, or None")
     if not isinstance(sinks, int) or isinstance(sinks, bool) or sinks < 0:
         raise ValueError(f"sinks {sinks!r} has to be a whole number of at least 0")
-    # longer windows than any sequence are none; the entry points take 64-bit sizes
-    return min(window or 0, _MAX_TOKENS), min(sinks, _MAX_TOKENS)
+    return min(window or 0, most), min(sinks, most)
 
 
 def _check_scale(scale, dim: int) -> float:
@@ -134,7 +134,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     if k.shape[0] != B or k.shape[2] != T or k.shape[3] != D or k.shape[1] == 0 or H == 0 or H % k.shape[1] != 0:
         raise ValueError(f"window_attention: q {tuple(q.shape)} does not match k {tuple(k.shape)} "
                          "(the same batch, tokens and dim, kv_heads dividing q_heads)")
-    window, sinks = _check_window(window, sinks)
+    window, sinks = _check_window(window, sinks, _MAX_TOKENS)
     scale = _check_scale(scale, D)
     for name, t in (("starts", starts), ("ends", ends)):
         if t is not None and (t.dtype != torch.int32 or t.shape != (B,)):
