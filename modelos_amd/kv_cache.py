@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from .embedding_bag import _require_device
-from .window_attention import _DIMS, _DTYPES, _check_scale, _check_window
+from .window_attention import _DIMS, _DTYPES, _check_scale, _check_window, _refuse_tangents
 
 GROUP = 32
 _MAX_POSITIONS = 1 << 30  # of a sequence's table; the entry point takes fewer
@@ -122,7 +122,7 @@ class Int4KVCache:
         lengths: int32 [batch] on the device, tokens of each sequence, the queries' own (already appended)
         among them. Query i stands at p = lengths[b] - queries + i and sees the positions j <= p with
         p - j < window or j < sinks (window None: all). Returns [batch, q_heads, queries, dim]; rows that
-        see nothing are zeros. There is no backward: q that requires a gradient is refused.
+        see nothing are zeros. There are no derivatives: q that requires a gradient or has a tangent is refused.
         """
         if q.dim() != 4 or q.shape[3] != self.dim or q.shape[1] == 0 or q.shape[1] % self.kv_heads != 0:
             raise ValueError(f"Int4KVCache.attend: q {tuple(q.shape)} is not [batch, q_heads, queries, {self.dim}] "
@@ -131,6 +131,7 @@ class Int4KVCache:
             raise ValueError(f"Int4KVCache.attend: q has to be {self.dtype}, got {q.dtype}")
         if torch.is_grad_enabled() and q.requires_grad:
             raise RuntimeError("Int4KVCache.attend has no backward; call it under torch.no_grad() or detach q")
+        _refuse_tangents("Int4KVCache.attend", q)
         window, sinks = _check_window(window, sinks, _MAX_POSITIONS)
         scale = _check_scale(scale, self.dim)
         B, H, Q, D = q.shape

@@ -20,13 +20,15 @@ products they enter, as the inputs are.
 
 Supported: bfloat16 and float16, head dims 64 and 128, on the GPU; anything
 else raises NotImplementedError. There is no CPU path: CPU tensors raise.
-The backward cannot be differentiated again.
+The backward cannot be differentiated again, and there are no forward-mode
+derivatives: dual tensors raise NotImplementedError.
 """
 from __future__ import annotations
 
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .embedding_bag import _require_device
@@ -114,6 +116,12 @@ def _check_scale(scale, dim: int) -> float:
     return scale
 
 
+def _refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
+    """The kernels read the primal numbers alone: a dual tensor's tangent would be lost."""
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int | None = None, sinks: int = 0,
                      starts: torch.Tensor | None = None, ends: torch.Tensor | None = None,
                      scale: float | None = None) -> torch.Tensor:
@@ -144,6 +152,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
                                   "supported (64 or 128 in bfloat16 or float16 are)")
     if T >= _MAX_TOKENS:
         raise NotImplementedError(f"window_attention: {T} tokens are not supported (fewer than {_MAX_TOKENS} are)")
+    _refuse_tangents("window_attention", q, k, v)
     _require_device(q, k, v, *(t for t in (starts, ends) if t is not None))
     starts, ends = _bound(starts), _bound(ends)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
