@@ -16,7 +16,8 @@ are exactly 0.
 
 Logits, softmax statistics and sums are float32. The softmax weights, and in
 the backward their gradients, are rounded to the inputs' type for the matrix
-products they enter, as the inputs are.
+products they enter, as the inputs are; in float16 with a power of two taken out
+of the gradients, so that any size of grad_out keeps its precision.
 
 Supported: bfloat16 and float16, head dims 64 and 128, on the GPU; anything
 else raises NotImplementedError. There is no CPU path: CPU tensors raise.
