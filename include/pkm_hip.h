@@ -624,9 +624,12 @@ typedef struct {
  * queries that share its tile without seeing it.
  * lse (float32 [batch, q_heads, tokens], may be NULL): log2 of the rows' sums of
  * exponentials, +inf for rows that see nothing; what the backward reads.
- * rest (as out, may be NULL): out's error of rounding, rounded itself; with it the
- * backward's <grad_out, out> is exact to float32.
+ * rest (may be NULL): out's error of rounding, rounded itself, for rows that see few
+ * keys: [batch, q_heads, R, dim], its tokens counted from each sequence's start, R = tokens
+ * for windows of up to PKM_ATTN_REST_TOKENS, else min(tokens, PKM_ATTN_REST_TOKENS). The fewer keys
+ * a row sees, the more of its gradient that error is in the backward's <grad_out, out>.
  */
+#define PKM_ATTN_REST_TOKENS 256
 int pkm_window_attn_fwd(const pkm_heads_t* q, const pkm_heads_t* k, const pkm_heads_t* v,
                         const int32_t* starts, const int32_t* ends, int64_t batch, int64_t q_heads,
                         int64_t kv_heads, int64_t tokens, int64_t dim, int dtype, int64_t window,

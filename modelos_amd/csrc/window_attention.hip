@@ -16,13 +16,14 @@ constexpr int kTile = 64;      // rows of an LDS tile
 
 struct AttnArgs {
   Heads q, k, v, o, dO, dq, dk, dv;
-  Heads rest;    // what the rounding left of o, or nothing
+  Heads rest;    // what the rounding left of o at positions [0, rest_rows) of the sequences, or nothing
   float* lse;    // [batch, q_heads, tokens], in units of log2; +inf where nothing is visible
   float* delta;  // [batch, q_heads, tokens]
   const int* starts;
   const int* ends;
   int batch, q_heads, kv_heads, tokens;
   int window, sinks;  // window in [1, tokens] (tokens: no window), sinks in [0, tokens]
+  int rest_rows;
   int pack;           // query heads of one key head that share a workgroup: 1, 2 or 4
   // the backward of the sinks from queries past their windows, when it has workgroups of its own
   float* far;  // [pairs, 32-sink blocks, far_chunks, 2 (dK, dV), 32, dim]
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[t][i] = some ? o[t][i] : 0.f;
   store_row<T, D>(a.o.at(qb.b, qb.head, row), o, some ? 1.f / sum : 0.f, lane,
-                  a.rest.p ? a.rest.at(qb.b, qb.head, row) : nullptr);
+                  a.rest.p && live && p < a.rest_rows ? a.rest.at(qb.b, qb.head, p) : nullptr);
   if (a.lse && h == 0) {
     a.lse[((int64_t)qb.b * a.q_heads + qb.head) * a.tokens + row] =
         some ? m * c + __builtin_amdgcn_logf(sum) : INFINITY;
@@ -277,7 +278,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
 // Backward, dQ: as the forward, dS^T = P^T (V dO^T - delta), dQ^T = K^T dS^T. The 4 x 4096 tokens of a training
 // step (16 / 8 heads of 128, window 1024): 0.25 to 0.27 ms, matrix cores 49 %, vector units 43 % of the cycles.
 //
-// delta comes from the output, with what its rounding left where that was kept. What an error in it puts into a row's dS
+// delta comes from the output, with what its rounding left where that was kept: for rows that see few keys, which are
+// all of a short window's and the first of every sequence. What an error in it puts into a row's dS
 // adds up to sum_j dS_j (which is 0), so the sum corrects the delta that dK reads. dS enters its
 // product as two 16-bit numbers, itself rounded and the rest: keys have a common part,
 // which the exact dS, whose sum is 0, cancels and the roundings of one would not (relative error
@@ -316,8 +318,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
 #pragma unroll
   for (int s = 0; s < KS; ++s)
     delta = vec_dot<T>(__builtin_bit_cast(uint4, frag_global<D>(orow, s, lane)), __builtin_bit_cast(uint4, g[s]), delta);
-  if (a.rest.p) {
-    const uint8_t* rrow = live ? a.rest.at(qb.b, qb.head, row) : nullptr;
+  if (a.rest.p && p0 < a.rest_rows) {
+    const uint8_t* rrow = live && p < a.rest_rows ? a.rest.at(qb.b, qb.head, p) : nullptr;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
       delta = vec_dot<T>(__builtin_bit_cast(uint4, frag_global<D>(rrow, s, lane)), __builtin_bit_cast(uint4, g[s]), delta);
@@ -816,6 +818,7 @@ int fill_args(const char* what, AttnArgs* a, int64_t batch, int64_t q_heads, int
   a->tokens = (int)tokens;
   a->window = (int)(window == 0 || window > tokens ? tokens : window);
   a->sinks = (int)(sinks > tokens ? tokens : sinks);
+  a->rest_rows = a->window <= PKM_ATTN_REST_TOKENS ? (int)tokens : PKM_ATTN_REST_TOKENS;
   a->scale = scale;
   a->dim = (int)dim;
   const int64_t share = q_heads / kv_heads;

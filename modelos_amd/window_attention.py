@@ -38,11 +38,12 @@ _DTYPES = (torch.bfloat16, torch.float16)
 _DIMS = (64, 128)
 _MAX_TOKEN_STRIDE = 1 << 22  # elements; tiles are addressed with 32-bit offsets
 _MAX_TOKENS = 1 << 24
-# Up to this window (or this many tokens) training keeps what the rounding of the output left, a second tensor like it, for
-# the backward's <grad_out, out>. The fewer keys a row sees, the more of its gradient an error there is: without it the
-# error of dq is 2.4 times that of a mere rounding of dq at 2 keys, 1.5 times at 20 and 1.35 at 200 (with it 1.1 to 1.2);
-# at 1024, where it is 1.3, keeping it would cost 1 to 6 % of a training step (4 x 4096 tokens, 16 / 8 heads of 128).
-_REST_WINDOW = 256
+# Training keeps what the rounding of the output left for the backward's <grad_out, out>, for all rows up to this window and
+# else for so many first rows of each sequence (PKM_ATTN_REST_TOKENS). The fewer keys a row sees, the more of its gradient an error
+# there is: without it the error of dq is 2.4 times that of a mere rounding of dq at 2 keys, 1.5 times at 20 and 1.35 at 200
+# (with it 1.1 to 1.2); for all rows at a window of 1024, where it is 1.3, keeping it would cost 1 to 6 % of a training step
+# (4 x 4096 tokens, 16 / 8 heads of 128).
+_REST_TOKENS = 256
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
@@ -79,7 +80,9 @@ class _WindowAttentionFn(torch.autograd.Function):
     def forward(ctx, q, k, v, starts, ends, window: int, sinks: int, scale: float):
         q, k, v = _readable(q), _readable(k), _readable(v)
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-        rest = _empty_like(q) if min(window or q.shape[2], q.shape[2]) <= _REST_WINDOW else None
+        B, H, T, D = q.shape
+        kept = T if 0 < window <= _REST_TOKENS else min(T, _REST_TOKENS)
+        rest = torch.empty((B, H, kept, D), dtype=q.dtype, device=q.device)
         out = _forward(q, k, v, starts, ends, window, sinks, scale, rest, lse)
         ctx.save_for_backward(q, k, v, out, rest, lse, starts, ends)
         ctx.sizes = (window, sinks, scale)
