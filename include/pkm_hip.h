@@ -695,9 +695,10 @@ size_t pkm_kv4_attend_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_
  * p - j < window or j < sinks (window 0: no window). q, out: [batch, q_heads, queries,
  * dim] in the cache's type; rows that see nothing (p < 0 among them) are written as 0.
  * Logits, softmax and sums are float32. The weights enter the products with the values'
- * steps in them as f16 numbers near 1 (f16 caches: two), with the minima as two numbers
- * of the cache's type. Numbers may be infinite or NaN only in tokens that no query sees;
- * steps lie between 2^-100 and 2^100. Sums run in a fixed order (deterministic).
+ * steps in them as f16 numbers (f16 caches: two) of which the largest is near 1 and those
+ * below 2^-14 of it lose bits, with the minima as two numbers of the cache's type. Numbers
+ * may be infinite or NaN only in tokens that no query sees; steps are 0 or lie between 2^-100
+ * and 2^100. Sums run in a fixed order (deterministic).
  */
 int pkm_kv4_attend(const void* codes, const void* params, int64_t pages, int64_t kv_heads, int64_t page,
                    int64_t dim, int dtype, const pkm_heads_t* q, const int32_t* table, int64_t width,

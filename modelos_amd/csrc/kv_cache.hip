@@ -337,10 +337,11 @@ struct RawTile {
 // products that take the 16 off again, 349 us for the first; 128 registers for a fourth workgroup spill, 2 times slower.)
 //
 // q is scaled to below 2^14 by a power of two per row, exactly but for numbers 2^-28 of the row's largest. The weights with
-// steps are f16, kept near 1 by the exponent `lift` of the largest step in the reference the exponentials are taken from
-// (relative rounding 2^-12 against the 2^-9 of a bf16 result; f16 results add the product with what the rounding left).
-// The weights of the minima are two 16-bit numbers of the cache's type: minimum and step often
-// cancel in a value, so one rounding of each would count several times.
+// steps are f16, kept near 1 by 2^-lift, which brings the wave's largest step so far to between 1/2 and 1
+// (rounding 2^-11 of a product against the 2^-8 of a bf16 result, and 2^-25 below 2^-14: products 2^-14 of the
+// largest lose bits; f16 results add the product with what the rounding left). The weights of the minima
+// are two 16-bit numbers of the cache's type: minimum and step often cancel in a value, so one rounding of each would
+// count several times. They do without 2^-lift: minima may be large where all steps are 0.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArgs a) {
   constexpr int NG = D / 32, NB = D / 16;
@@ -489,7 +490,7 @@ __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArg
   f32x4_t o[NB] = {}, mins = {};
   float m = -INFINITY, ref = 0.f, sum = 0.f;
   uint32_t most = 0;  // the largest step so far, as its bits
-  int lift = 0;       // its exponent
+  int lift = 0;       // its exponent; o is in units of 2^lift
   for (int it = first + wave; it < last; it += 4) {
     const int j0 = tiles.tile(it) * kTok;
     RawTile<D> now = x;
@@ -558,19 +559,19 @@ __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArg
     const uint32_t b0 = now.p[1][0], b1 = now.p[1][1];
     const uint32_t steps = lane < 8 * NG ? max(max(b0 & 0xffffu, b0 >> 16), max(b1 & 0xffffu, b1 >> 16)) : 0u;
     // a new reference where a row's largest logit has grown by more than 4 in log2, or the largest step by a power of two:
-    // until then weights stay below 2^5
+    // until then weights stay below 2^4
     if (__any((top - m) * c > 4.f || (m == -INFINITY && top > m) || steps > (most | (kTwo ? 0x3ffu : 0x7fu)))) {
       uint32_t big = steps;
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) big = max(big, (uint32_t)__shfl_xor((int)big, d));
-      most = max(most, big);
+      most = max(most, (uint32_t)__builtin_amdgcn_readfirstlane((int)big));
       const int lifted = kTwo ? (int)(most >> 10) - 14 : min(max((int)(most >> 7) - 126, -100), 100);
-      const float next = (top == -INFINITY ? 0.f : top * c) + (float)lifted;
-      const float f = m == -INFINITY ? 0.f : exp2_raw(ref - next);
+      const float next = top == -INFINITY ? 0.f : top * c;
+      const float f = m == -INFINITY ? 0.f : exp2_raw(ref - next), fo = ldexpf(f, lift - lifted);
       sum *= f;
 #pragma unroll
-      for (int i = 0; i < NB; ++i) o[i] *= f;
-      mins *= kTwo ? ldexpf(f, lifted - lift) : f;
+      for (int i = 0; i < NB; ++i) o[i] *= fo;
+      mins *= f;
       m = top;
       ref = next;
       lift = lifted;
@@ -590,18 +591,16 @@ __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArg
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         uint32_t hi, lo;
-        // f16: without the steps' exponent, which may put weights past its range
-        if constexpr (kTwo) {
-          split_pair<T>(ldexpf(s[2 * e], lift), ldexpf(s[2 * e + 1], lift), &hi, &lo);
-        } else {
-          split_pair<T>(s[2 * e], s[2 * e + 1], &hi, &lo);
-        }
+        split_pair<T>(s[2 * e], s[2 * e + 1], &hi, &lo);
         fp[e] = hi, fr[e] = lo;
       }
       mins = mfma16<T>(fm, fp, mins);
       mins = mfma16<T>(fm, fr, mins);
     }
     // sum_t p_t s_t c_t
+    const float up = ldexpf(1.f, -lift);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] *= up;
     uint32_t lo[4], hi[4];
     if constexpr (D == 128) {
 #pragma unroll
@@ -615,6 +614,8 @@ __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArg
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
+      // f16: group by group, or the groups' pairs of operands together take 50 registers more than there are
+      if constexpr (kTwo) __builtin_amdgcn_sched_barrier(0);
       float w[8];
 #pragma unroll
       for (int hb = 0; hb < 2; ++hb) {
@@ -652,10 +653,10 @@ __global__ __launch_bounds__(kThreads, 3) void kv4_attend_kernel(const AttendArg
   sum += __shfl_xor(sum, 32);
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
-    const float add = kTwo ? ldexpf(mins[i / 2], -lift) : mins[i / 2], unit = (D == 128 ? i / 2 : i) & 1 ? kOdd : kEven;
+    const float unit = ldexpf((D == 128 ? i / 2 : i) & 1 ? kOdd : kEven, lift);
     f32x4_t y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[i][e], unit, add);
+    for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(o[i][e], unit, mins[i / 2]);
     *(f32x4_t*)&merge[wave][l][16 * i + 4 * quad] = y;
   }
   if (quad == 0) {

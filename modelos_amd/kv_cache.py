@@ -8,7 +8,7 @@ A head vector is held in groups of 32 numbers: minimum m and step
 s = (max - min) / 15 in the cache's type, codes c = round((x - m) / s); the
 number read back is m + s c, within s / 2 of x up to the rounding of m, s and
 the result. Numbers have to be finite, and far enough from the type's ends that
-max - min and m + 15 s stay inside it; attend needs steps between 2^-100 and 2^100. With the parameters a number takes 5
+max - min and m + 15 s stay inside it; attend needs steps of 0 or between 2^-100 and 2^100. With the parameters a number takes 5
 bits instead of 16.
 
 Pages are the caller's to hand out: `table` [batch, width] (int32, on the
