@@ -813,20 +813,23 @@ int check_rows(const char* what, const char* name, const pkm_heads_t* x) {
 
 Heads heads(const pkm_heads_t* x) { return {(uint8_t*)x->data, x->batch, x->head, x->token}; }
 
-int store_args(const char* what, StoreArgs* a, int64_t dim, int dtype, const pkm_heads_t* k, const pkm_heads_t* v,
+constexpr int64_t kMaxBlocks = (1ll << 32) / kThreads - 1;  // a launch takes fewer than 2^32 threads
+
+// lanes: that work on one vector
+int store_args(const char* what, StoreArgs* a, int lanes, const pkm_heads_t* k, const pkm_heads_t* v,
                const int32_t* table, int64_t width, const int32_t* starts, const int32_t* counts, int64_t batch,
                int64_t tokens) {
   int rc;
   if ((rc = check_rows(what, "k", k)) || (rc = check_rows(what, "v", v))) return rc;
   PKM_REQUIRE(starts != nullptr && counts != nullptr && (table != nullptr || width == 0), PKM_ERR_INVALID_ARGUMENT,
               "%s: table, starts and counts have to be given", what);
-  PKM_REQUIRE(tokens < (1ll << 30) / a->cache.heads && batch < (1ll << 30) / a->cache.heads / tokens,
+  PKM_REQUIRE(tokens < (1ll << 30) / a->cache.heads && batch < (1ll << 30) / a->cache.heads / tokens &&
+                  2 * batch * tokens * a->cache.heads <= kMaxBlocks * (kThreads / lanes),
               PKM_ERR_UNSUPPORTED, "%s: too many tokens", what);
   a->k = heads(k), a->v = heads(v);
   a->table = table, a->starts = starts, a->counts = counts, a->width = width;
   a->batch = (int)batch, a->tokens = (int)tokens;
   a->shift = page_shift(a->cache.page);
-  (void)dim, (void)dtype;
   return PKM_OK;
 }
 
@@ -853,9 +856,9 @@ int run_store(const char* what, const StoreArgs& a, int64_t dim, int dtype, void
   return pkm_check_launch(what);
 }
 
-// Below 2^25 tiles a sequence and 2^24 query rows in all.
+// Below 2^25 tiles a sequence; query rows, each of which may need a workgroup beside the kGroups, as one launch takes.
 bool attend_sizes_fit(int64_t batch, int64_t q_heads, int64_t queries, int64_t width, int64_t page) {
-  const int64_t most = 1 << 24;
+  const int64_t most = kMaxBlocks - kGroups;
   return width < (1ll << 30) / page && batch < most && q_heads < most && queries < most && batch * q_heads < most &&
          batch * q_heads * queries < most;
 }
@@ -910,7 +913,7 @@ extern "C" int pkm_kv4_append(void* codes, void* params, int64_t pages, int64_t 
   StoreArgs a = {};
   int rc = check_cache(what, &a.cache, codes, params, pages, kv_heads, page, dim, dtype);
   if (rc != PKM_OK) return rc;
-  if ((rc = store_args(what, &a, dim, dtype, k, v, table, width, starts, counts, batch, tokens))) return rc;
+  if ((rc = store_args(what, &a, (int)dim / 32, k, v, table, width, starts, counts, batch, tokens))) return rc;
   return run_store<true>(what, a, dim, dtype, stream);
 }
 
@@ -925,7 +928,7 @@ extern "C" int pkm_kv4_read(const void* codes, const void* params, int64_t pages
   int rc = check_cache(what, &a.cache, const_cast<void*>(codes), const_cast<void*>(params), pages, kv_heads, page, dim,
                        dtype);
   if (rc != PKM_OK) return rc;
-  if ((rc = store_args(what, &a, dim, dtype, k, v, table, width, starts, counts, batch, tokens))) return rc;
+  if ((rc = store_args(what, &a, (int)dim / 8, k, v, table, width, starts, counts, batch, tokens))) return rc;
   return run_store<false>(what, a, dim, dtype, stream);
 }
 
