@@ -6,6 +6,8 @@
 //   o_p = sum_j P_pj v_j,  P_pj = exp(scale q_p.k_j - lse_p),  lse_p = log sum_j exp(scale q_p.k_j)
 //   dV = P^T dO,  dS = P (dO V^T - delta),  delta_p = dO_p.o_p,  dQ = scale dS K,  dK = scale dS^T Q
 // Positions inside the kernels are relative to the sequence's start.
+#include <algorithm>
+
 #include "attn_common.h"
 
 namespace pkm {
@@ -812,6 +814,12 @@ int fill_args(const char* what, AttnArgs* a, int64_t batch, int64_t q_heads, int
   PKM_REQUIRE(tokens < (1 << 24) && batch < (1 << 24) && q_heads < (1 << 24) && batch * q_heads < (1 << 24) &&
                   batch * q_heads * ((tokens + 31) / 32) < (1ll << 31),
               PKM_ERR_UNSUPPORTED, "%s: too many tokens or heads", what);
+  // a launch takes fewer than 2^32 threads: 256 a workgroup, with the far sinks' too, and 512 for dK and dV
+  const int64_t share = q_heads / kv_heads, pack = share % 4 == 0 ? 4 : share % 2 == 0 ? 2 : 1, rows = 128 / pack;
+  PKM_REQUIRE(batch * (q_heads / pack) * ((tokens + rows - 1) / rows) < (1 << 24) &&
+                  batch * kv_heads * ((std::min(sinks, tokens) + 31) / 32) < (1 << 24) &&
+                  batch * kv_heads * ((tokens + 127) / 128) < (1 << 23),
+              PKM_ERR_UNSUPPORTED, "%s: too many tokens or heads", what);
   a->batch = (int)batch;
   a->q_heads = (int)q_heads;
   a->kv_heads = (int)kv_heads;
@@ -821,8 +829,7 @@ int fill_args(const char* what, AttnArgs* a, int64_t batch, int64_t q_heads, int
   a->rest_rows = a->window <= PKM_ATTN_REST_TOKENS ? (int)tokens : PKM_ATTN_REST_TOKENS;
   a->scale = scale;
   a->dim = (int)dim;
-  const int64_t share = q_heads / kv_heads;
-  a->pack = share % 4 == 0 ? 4 : share % 2 == 0 ? 2 : 1;
+  a->pack = (int)pack;
   return PKM_OK;
 }
 

@@ -1,4 +1,4 @@
-"""The largest calls of the 4-bit cache: sizes that one launch does not take are refused as unsupported. CPU only."""
+"""The largest calls of window attention and of the 4-bit cache: sizes that one launch does not take are refused as unsupported. CPU only."""
 from __future__ import annotations
 
 import ctypes
@@ -48,3 +48,17 @@ def test_rows_of_one_launch(lib):
     assert run((1 << 24) - 1024) == 3  # only the workspace is missing
     size = lambda batch: lib.pkm_kv4_attend_workspace_size(batch, 1, 1, 1, 64, 2, 16, 0, 0)
     assert size((1 << 24) - 1) == 0 and size((1 << 24) - 1024) > 0
+
+
+@pytest.mark.parametrize("batch,q_heads,kv_heads,tokens,status", [
+    ((1 << 24) - 1, 1, 1, 1, UNSUPPORTED),  # dK and dV: 512 threads for each
+    (1 << 22, 3, 3, 1, UNSUPPORTED), ((1 << 23) - 1, 1, 1, 1, 3), (1 << 20, 12, 12, 200, UNSUPPORTED),
+    (1 << 10, 16, 4, 1 << 15, 3),  # 2^29 rows: large, but taken
+])
+def test_window_attention_of_one_launch(lib, batch, q_heads, kv_heads, tokens, status):
+    from modelos_amd._lib import Heads
+
+    x = Heads(1 << 20, 0, 0, 0)
+    got = lib.pkm_window_attn_bwd(x, x, x, x, None, P, x, None, None, batch, q_heads, kv_heads, tokens, 64, 1, 0, 0, 0.1, x, x, x,
+                                  None, 0, None)
+    assert got == status  # 3: only the workspace is missing
