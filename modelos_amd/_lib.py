@@ -468,7 +468,7 @@ def call(name: str, *args) -> None:
 
 def call_on(device: torch.device, name: str, *args) -> None:
     """call() with `device` current, as launches on its streams need it."""
-    if device.index is None or device.index == torch._C._cuda_getDevice():
+    if device.index is None or device.index == torch.cuda.current_device():
         return call(name, *args)
     with torch.cuda.device(device):
         return call(name, *args)

@@ -139,8 +139,8 @@ __device__ __forceinline__ void load_lds16(u32x4_t rsrc, lds_u8* to, uint32_t of
 
 // A tile's rows from global memory straight to LDS (no registers in between), by WAVES waves. A wave's load
 // writes 64 chunks of 16 bytes side by side; the permutation is in the addresses that the lanes read. Rows from
-// `last` (>= 1) on repeat row last - 1: what lies outside a sequence is never read. The loads are complete after
-// tile_wait().
+// `last` (>= 1) on repeat row last - 1: what lies behind a sequence is never read. Row 0 is the caller's: a tile that begins before
+// its sequence holds what lies there. The loads are complete after tile_wait().
 template <int D, int ROWS, int WAVES = 4>
 struct TileLoad {
   static constexpr int CH = D / 8, PER = 64 / CH, N = ROWS / PER / WAVES;  // rows of a load, loads of a wave

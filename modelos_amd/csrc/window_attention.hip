@@ -616,7 +616,8 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(const AttnArgs a) {
   float up = kUp;
   const float c = a.scale * 1.44269504f;
   if (total > 0) {
-    // rows of the block before the sequence's start or past its end repeat its ends: their columns are dropped
+    // rows of the block before the sequence's start are read as they are, those past its end repeat its last: whatever they
+    // hold, NaN too, stays in their own columns of the products, which `live` drops
     const TileLoad<D, 128, 8> kl(tid);
     kl.load(keys, a.k.at(b, kv, first), (uint32_t)(2 * a.k.token), seq.start + n - first, tid);
     start_head();
