@@ -91,21 +91,23 @@ struct FarPlan {
 // it is multiplied by a power of two of its column (a query in dQ, a key in dK), the same in both half waves, which
 // starts high and falls when a step's largest number reaches 2^15, to bring that below 2^10. Sums are kept in the same
 // units. 4096 tokens with gradients of 2^-12: errors of dQ and dK 1.01 and 1.03 times those of rounded results (without it
-// 4.6 and 5.7, and NaN where |dS| reaches 2^16), at 4 % of the step's time (4 x 4096 tokens, 16 / 8 heads of 128, window 1024: 0.76 to
-// 0.79 ms). For dK and dV the weights are taken times 2^kWeightLift, for the same reason. bf16 has float32's range.
+// 4.6 and 5.7, and NaN where |dS| reaches 2^16). It costs 2 to 4 % of a step of 4 x 4096 tokens, 16 / 8 heads of 128, window 1024
+// (0.76 to 0.77 and 0.79 ms), and of 3 x 1777 tokens, 12 heads of 64, dQ 48 to 52 us, dK and dV 48 to 53. For dK and dV the weights are taken times 2^kWeightLift, for the same reason. bf16 has float32's range.
 template <typename T>
 constexpr bool kLifts = __is_same(T, f16_t);
 template <typename T>
 constexpr int kWeightLift = kLifts<T> ? 12 : 0;
 
-// The exponent to add to that of the power of two after a step: 0, or less where the column's numbers have grown too large.
-__device__ __forceinline__ int lift_change(const f32x16_t& x) {
+// After a step's numbers: rescale(change) where any of the wave's columns have grown too large, with the exponent to add to that
+// of the lane's power of two: less than 0 there, 0 elsewhere.
+template <typename F>
+__device__ __forceinline__ void lower_lift(const f32x16_t& x, F rescale) {
   float top = fabsf(x[0]);
 #pragma unroll
   for (int i = 1; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
-  if (!__any(top >= 32768.f)) return 0;
+  if (!__any(top >= 32768.f)) return;
   top = fmaxf(top, swap_halves(top));
-  return top >= 32768.f ? min(10 - __builtin_amdgcn_frexp_expf(top), 0) : 0;  // (the exponent of infinity reads as 0)
+  rescale(top >= 32768.f ? min(10 - __builtin_amdgcn_frexp_expf(top), 0) : 0);  // (the exponent of infinity reads as 0)
 }
 
 // A workgroup's share of the queries: 4 waves of 32 rows each, `pack` heads of one key head beside each other.
@@ -137,8 +139,8 @@ struct QueryBlock {
 // the queries' span, and with it the tiles at the window's ends, short.
 //
 // Two workgroups of 4 waves a CU (225 registers; 64 KB of LDS each, two stages). 32768
-// tokens, 32 / 8 heads of 128, window 4096: 1.97 to 2.08 ms, 1000 TFLOP/s of visible pairs, 70 % of a
-// large matrix product's rate. The matrix cores are busy 51 % of the cycles and the vector units 59 %, at
+// tokens, 32 / 8 heads of 128, window 4096: 1.97 to 2.13 ms, 1000 TFLOP/s of visible pairs, 70 % of a
+// large matrix product's rate. The matrix cores are busy 55 % of the cycles and the vector units 55 %, at
 // a clock that the load pulls to 1.9 GHz; each operand fragment read from LDS feeds one
 // product, which is as much as LDS gives (128 bytes a cycle). Measured on the way: tiles through
 // registers 2.43 ms, straight to LDS 2.20, reads issued 2 to 3 products ahead 2.08.
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(const AttnArgs 
 
 // ---------------------------------------------------------------------------
 // Backward, dQ: as the forward, dS^T = P^T (V dO^T - delta), dQ^T = K^T dS^T. The 4 x 4096 tokens of a training
-// step (16 / 8 heads of 128, window 1024): 0.25 to 0.27 ms, matrix cores 49 %, vector units 43 % of the cycles.
+// step (16 / 8 heads of 128, window 1024): 0.25 to 0.28 ms, matrix cores 49 %, vector units 43 % of the cycles.
 //
 // delta comes from the output, with what its rounding left where that was kept: for rows that see few keys, which are
 // all of a short window's and the first of every sequence. What an error in it puts into a row's dS
@@ -387,8 +389,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
           sum += s[i];
         }
         if constexpr (kLifts<T>) {
-          const int change = lift_change(s);
-          if (__any(change != 0)) {
+          lower_lift(s, [&](int change) {
             const float f = ldexpf(1.f, change);
             lift += change;
             lse -= (float)change;
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
             for (int i = 0; i < 16; ++i) s[i] *= f;
 #pragma unroll
             for (int t = 0; t < DT; ++t) dq[t] *= f;
-          }
+          });
         }
         frag_t f[2], r[2];
 #pragma unroll
@@ -439,7 +440,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
 // values in registers: with both in registers a wave needs more than the 256
 // that let two waves share a SIMD. Three stages of tiles, two of them on their way.
 //
-// The same step: 0.33 to 0.36 ms (one wave a SIMD 0.42). Matrix cores 34 %, vector units 31 %: a wave
+// The same step: 0.33 to 0.38 ms (one wave a SIMD 0.42). Matrix cores 34 %, vector units 32 %: a wave
 // issues a third of its time, waits a third for the matrix core and a third for LDS and the barrier.
 // Copies of the kernel without its exponentials, either pair of products, its LDS reads or its loads took
 // 0.30 to 0.33 ms each, so no one of them is the limit; the two halves half a step apart,
@@ -506,15 +507,14 @@ __device__ __forceinline__ void dkv_step(const lds_u8* qtile, const lds_u8* gtil
   }
   if (lone0) dp[0] = h == 0 ? 0.f * dp[0] : dp[0];
   if constexpr (kLifts<T>) {
-    const int change = lift_change(dp);
-    if (__any(change != 0)) {
+    lower_lift(dp, [&](int change) {
       const float f = ldexpf(1.f, change);
       up *= f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] *= f;
 #pragma unroll
       for (int t = 0; t < DT; ++t) dk[t] *= f;
-    }
+    });
   }
   frag_t pf[2], sf[2];
 #pragma unroll
