@@ -332,8 +332,8 @@ struct RawTile {
 // worked on, at three workgroups a CU.
 //
 // Bound by memory where there are many tiles: 64 sequences of 4000 to 16000 tokens, 32 / 8 heads of 128 (828 MB) in
-// 176 to 182 us, 4.5 to 4.7 TB/s of the 4.7 that a large copy reaches; one of 131072 tokens (168 MB) in 40 us, of which 6 are its start and end. 415
-// vector instructions a tile keep the vector units busy 63 % of the cycles. (Codes widened to 16 + c in the query's type, with
+// 176 to 182 us, 4.5 to 4.7 TB/s of the 4.7 that a large copy reaches; one of 131072 tokens (168 MB) in
+// 40 us, of which 6 are its start and end. 415 vector instructions a tile keep the vector units busy 63 % of the cycles. (Codes widened to 16 + c in the query's type, with
 // products that take the 16 off again, 349 us for the first; 128 registers for a fourth workgroup spill, 2 times slower.)
 //
 // q is scaled to below 2^14 by a power of two per row, exactly but for numbers 2^-28 of the row's largest. The weights with

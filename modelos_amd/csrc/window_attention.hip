@@ -92,7 +92,8 @@ struct FarPlan {
 // starts high and falls when a step's largest number reaches 2^15, to bring that below 2^10. Sums are kept in the same
 // units. 4096 tokens with gradients of 2^-12: errors of dQ and dK 1.01 and 1.03 times those of rounded results (without it
 // 4.6 and 5.7, and NaN where |dS| reaches 2^16). It costs 2 to 4 % of a step of 4 x 4096 tokens, 16 / 8 heads of 128, window 1024
-// (0.76 to 0.77 and 0.79 ms), and of 3 x 1777 tokens, 12 heads of 64, dQ 48 to 52 us, dK and dV 48 to 53. For dK and dV the weights are taken times 2^kWeightLift, for the same reason. bf16 has float32's range.
+// (0.76 to 0.77 and 0.79 ms), and of 3 x 1777 tokens, 12 heads of 64, dQ 48 to 52 us, dK and dV 48 to 53. For dK and dV the weights
+// are taken times 2^kWeightLift, for the same reason. bf16 has float32's range.
 template <typename T>
 constexpr bool kLifts = __is_same(T, f16_t);
 template <typename T>
@@ -316,7 +317,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(const AttnArgs a
   const int64_t at = ((int64_t)qb.b * a.q_heads + qb.head) * a.tokens + row;
   float lse = live ? a.lse[at] : INFINITY;
   float delta = 0.f, sum = 0.f;
-  int lift = kLifts<T> ? 80 : 0;  // dS and its sums are in units of 2^-lift, by way of lse: 2^80 times the largest f16 dS fits float32
+  // dS and its sums are in units of 2^-lift, by way of lse; 2^80 times the largest dS of f16 inputs fits float32
+  int lift = kLifts<T> ? 80 : 0;
   lse -= (float)lift;
   const uint8_t* orow = live ? a.o.at(qb.b, qb.head, row) : nullptr;
 #pragma unroll
@@ -746,7 +748,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_far_kernel(const AttnArgs 
     if (u0 + wave < end) {
       const lds_u8* buf = lds + wave * BUF;
       dkv_step<T, D>(buf, buf + TB, buf + 2 * TB, buf + 2 * TB + 4 * kQueries, keys, v, c,
-                     t0 - (32 * block + 31) >= W && 32 * block + 31 < S, false, [&](int i) { return t0 + i - key < W || key >= S; }, dk, dv, up, lane);
+                     t0 - (32 * block + 31) >= W && 32 * block + 31 < S, false,
+                     [&](int i) { return t0 + i - key < W || key >= S; }, dk, dv, up, lane);
     }
     __syncthreads();
   }
