@@ -96,9 +96,10 @@ def draw(rng):
 def _drawn(rng):
     op = rng.choice(["loss", "loss", "embed", "update"])
     if op == "update":
+        dtype = rng.choice(["bf16", "bf16", "f16", "f32"])
         return {"op": op, "vocab": _between(rng, 1, 200000), "hidden": _between(rng, 1, 2048),
                 "layers": rng.choice([0, 1, rng.randint(2, 24)]), "bits": rng.choice([8, 32]),
-                "master": rng.choice([False, True]), "dtype": rng.choice(["bf16", "bf16", "f16", "f32"])}
+                "master": dtype != "f32" and rng.choice([False, True]), "dtype": dtype}
     case = {"op": op, "train": rng.choice([False, True, True]), "tokens": _between(rng, 1, 16384),
             "vocab": _between(rng, 2, 200000)}
     dim = _between(rng, 16, 4096)
