@@ -706,6 +706,65 @@ int pkm_kv4_attend(const void* codes, const void* params, int64_t pages, int64_t
                    int64_t sinks, float scale, const pkm_heads_t* out, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/*
+ * Token embedding: out[t, :] = scale * weight[ids[t], :], rounded once to the table's type.
+ * ids: int32 (ids_bits 32) or int64 (64) on the device; those outside [0, rows) read zeros.
+ * weight: rows row_stride elements apart; out: [tokens, dim].
+ */
+int pkm_embed_fwd(const void* ids, int ids_bits, int64_t tokens, const void* weight, int64_t rows,
+                  int64_t row_stride, int64_t dim, int dtype, float scale, void* out, void* stream);
+
+/* Workspace bytes pkm_embed_bwd needs. */
+size_t pkm_embed_bwd_workspace_size(int64_t tokens, int64_t rows, int64_t dim);
+
+/*
+ * Gradient of pkm_embed_fwd's table: grad_weight[v, :] = scale * the sum of grad_out[t, :]
+ * over the tokens t with ids[t] = v, in the order of the tokens, float32 sums, rounded
+ * once. All [rows, dim] are written. Ids outside [0, rows) and the id `padding` (-1: none)
+ * give no gradient. Deterministic. Workspace: 16-byte aligned.
+ */
+int pkm_embed_bwd(const void* ids, int ids_bits, int64_t tokens, const void* grad_out, int64_t rows,
+                  int64_t dim, int dtype, int64_t padding, float scale, void* grad_weight, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+/*
+ * One tensor of an AdamW step. States of 32 bits: exp_avg and second (of the squared
+ * gradients) are float32 [numel], the scales NULL. States of 8 bits: e4m3 codes [numel]
+ * of m and of r, the root of the second moment, and float32 steps [ceil(numel / 256)].
+ * master: float32 [numel], or NULL for all tensors of a call. step: one float32.
+ */
+typedef struct {
+  void* param;
+  const void* grad; /* of param's type */
+  void* exp_avg;
+  void* second;
+  float* exp_avg_scale;
+  float* second_scale;
+  float* master;
+  float* step;
+  int64_t numel;
+} pkm_adamw_tensor_t;
+
+/* Workspace bytes pkm_adamw_step needs. */
+size_t pkm_adamw_workspace_size(int64_t count);
+
+/*
+ * An AdamW step over `count` tensors of one dtype (`tensors` is read on the host, before the
+ * call returns). step counts on by one, t is its new value; g = grad * *grad_scale (NULL: 1):
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+ *   param = param (1 - lr decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+ * in float32; with a master the update is made to it and param is its rounding. lr_device, if
+ * not NULL, is read on the device in the place of lr.
+ * In 8 bits m and r = sqrt(v) are held in units of their block's step = max / 448: a number
+ * a >= 0, 2^e <= a < 2^(e + 1), e >= -6, becomes floor(a 2^(3 - e) + u) 2^(e - 3), at most
+ * 448, with u = (x >> 12) 2^-20 for m and (x mod 2^20) 2^-20 for r, x = (2654435761 i +
+ * 2246822519 t) mod 2^32 for number i of its tensor; an r above 0 is at least 2^-9. Blocks whose
+ * largest number is below 2^-110 are held as zeros.
+ */
+int pkm_adamw_step(const pkm_adamw_tensor_t* tensors, int64_t count, int dtype, int state_bits, double lr,
+                   const float* lr_device, double beta1, double beta2, double eps, double weight_decay,
+                   const float* grad_scale, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

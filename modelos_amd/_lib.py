@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 import torch  # noqa: F401  (must be imported before the HIP library is opened)
@@ -302,6 +302,42 @@ SIGNATURES.update({
             _HEADS, c_void_p, c_int64, c_void_p,  # q, table, width, lengths
             c_int64, c_int64, c_int64, c_int64, c_int64, c_float,  # batch, q_heads, queries, window, sinks, scale
             _HEADS, c_void_p, c_size_t, c_void_p,  # out, workspace, bytes, stream
+        ],
+    ),
+})
+
+class AdamWTensor(ctypes.Structure):
+    """pkm_adamw_tensor_t: one tensor of an AdamW step."""
+
+    _fields_ = [(name, c_void_p) for name in ("param", "grad", "exp_avg", "second", "exp_avg_scale", "second_scale",
+                                              "master", "step")] + [("numel", c_int64)]
+
+
+SIGNATURES.update({
+    "pkm_embed_fwd": (
+        c_int,
+        [
+            c_void_p, c_int, c_int64,  # ids, bits, tokens
+            c_void_p, c_int64, c_int64, c_int64, c_int, c_float,  # weight, rows, row stride, dim, dtype, scale
+            c_void_p, c_void_p,  # out, stream
+        ],
+    ),
+    "pkm_embed_bwd_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
+    "pkm_embed_bwd": (
+        c_int,
+        [
+            c_void_p, c_int, c_int64, c_void_p,  # ids, bits, tokens, grad_out
+            c_int64, c_int64, c_int, c_int64, c_float,  # rows, dim, dtype, padding, scale
+            c_void_p, c_void_p, c_size_t, c_void_p,  # grad_weight, workspace, bytes, stream
+        ],
+    ),
+    "pkm_adamw_workspace_size": (c_size_t, [c_int64]),
+    "pkm_adamw_step": (
+        c_int,
+        [
+            c_void_p, c_int64, c_int, c_int,  # tensors, count, dtype, state bits
+            c_double, c_void_p, c_double, c_double, c_double, c_double,  # lr, lr on the device, betas, eps, decay
+            c_void_p, c_void_p, c_size_t, c_void_p,  # grad_scale, workspace, bytes, stream
         ],
     ),
 })
