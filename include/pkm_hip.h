@@ -765,6 +765,38 @@ int pkm_adamw_step(const pkm_adamw_tensor_t* tensors, int64_t count, int dtype, 
                    const float* lr_device, double beta1, double beta2, double eps, double weight_decay,
                    const float* grad_scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Softmax cross entropy of a linear layer over a vocabulary, without the logits in memory:
+ *   l_jv = <x_j, weight_v>,  loss_j = log sum_v exp l_jv - l_j,labels_j
+ * x: [tokens, dim], rows x_stride elements apart; weight: [vocab, dim], rows w_stride
+ * apart, 16-byte aligned, w_stride a multiple of 8, what lies between dim and the next
+ * multiple of 8 readable and finite. bf16 or f16 alike. labels: int32 (label_bits 32) or
+ * int64; tokens with the label `ignore` or one outside [0, vocab) do not count: their loss is
+ * 0, what x holds there is not read. reduction 0: loss [tokens]; 1: one number, the mean
+ * over the tokens that count (0 if none does); 2: their sum. float32.
+ * kept: what the backward reads, pkm_linear_ce_kept_size bytes, 16-byte aligned, as the workspace.
+ * Products of the inputs are exact, sums and exponentials float32, in a fixed order
+ * (deterministic).
+ */
+size_t pkm_linear_ce_kept_size(int64_t tokens, int64_t dim);
+size_t pkm_linear_ce_fwd_workspace_size(int64_t tokens, int64_t vocab, int64_t dim);
+int pkm_linear_ce_fwd(const void* x, int64_t x_stride, int64_t tokens, const void* weight, int64_t w_stride,
+                      int64_t vocab, int64_t dim, int dtype, const void* labels, int label_bits,
+                      int64_t ignore, int reduction, float* loss, void* kept, size_t kept_bytes,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of pkm_linear_ce_fwd from what it kept (which is not used up), the same weight
+ * and grad_loss (float32, one number or [tokens] by reduction): dx [tokens, dim], zeros for
+ * tokens that do not count, and dweight [vocab, dim], of the inputs' type, 16-byte aligned;
+ * either may be NULL and is then not computed. The logits' gradients are rounded to the inputs' type for the
+ * products (f16: with a power of two taken out); sums are float32 in a fixed order.
+ */
+size_t pkm_linear_ce_bwd_workspace_size(int64_t tokens, int64_t vocab, int64_t dim);
+int pkm_linear_ce_bwd(void* kept, size_t kept_bytes, int64_t tokens, const void* weight, int64_t w_stride,
+                      int64_t vocab, int64_t dim, int dtype, const float* grad_loss, int reduction,
+                      void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

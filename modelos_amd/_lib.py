@@ -342,6 +342,31 @@ SIGNATURES.update({
     ),
 })
 
+SIGNATURES.update({
+    "pkm_linear_ce_kept_size": (c_size_t, [c_int64, c_int64]),
+    "pkm_linear_ce_fwd_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
+    "pkm_linear_ce_fwd": (
+        c_int,
+        [
+            c_void_p, c_int64, c_int64,  # x, row stride, tokens
+            c_void_p, c_int64, c_int64, c_int64, c_int,  # weight, row stride, vocab, dim, dtype
+            c_void_p, c_int, c_int64, c_int,  # labels, bits, ignore, reduction
+            c_void_p, c_void_p, c_size_t,  # loss, kept, bytes
+            c_void_p, c_size_t, c_void_p,  # workspace, bytes, stream
+        ],
+    ),
+    "pkm_linear_ce_bwd_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
+    "pkm_linear_ce_bwd": (
+        c_int,
+        [
+            c_void_p, c_size_t, c_int64,  # kept, bytes, tokens
+            c_void_p, c_int64, c_int64, c_int64, c_int,  # weight, row stride, vocab, dim, dtype
+            c_void_p, c_int, c_void_p, c_void_p,  # grad_loss, reduction, dx, dweight
+            c_void_p, c_size_t, c_void_p,  # workspace, bytes, stream
+        ],
+    ),
+})
+
 # pkm_score_t
 SCORE_CODES = {"dot": 0, "idw": 1}
 

@@ -1,0 +1,932 @@
+// Softmax cross entropy of a linear layer over a large vocabulary, forward and backward, without the logits in memory,
+// gfx950.
+//
+//   l_jv = <x_j, W_v>    lse_j = log sum_v exp l_jv    loss_j = lse_j - l_j,y_j
+//   d_jv = g_j (exp(l_jv - lse_j) - [v = y_j])    dx_j = sum_v d_jv W_v    dW_v = sum_j d_jv x_j
+//
+// for the tokens whose label lies in [0, vocab) and is not the ignored one: these are copied side by side first ("kept"
+// tokens, padded to whole 128-byte lines), so that nothing is computed for the others and what they hold (NaN) reaches
+// nothing. The number of kept tokens stays on the device.
+//
+// Forward: one product, [vocab, tokens], whose epilogue sums the exponentials of a tile and drops the logits. Backward: for a
+// piece of the vocabulary after the other the same product again, whose epilogue leaves d in 16 bits, and from it the
+// piece's rows of dW, whole, and its part of dx, added up in float32. That is 8 n V D operations where keeping the logits
+// would take 6. What bounds all of it are the matrix cores.
+//
+// The three products are one kernel (ce_product): tiles of 256 x 256 results by 8 waves (2 x 4, each 128 x 64 in 32x32x16
+// products), 64 deep, in two stages of 64 KB of LDS that buffer loads fill without registers. A wave reads the operands of
+// a step of 16 while the matrix cores work on the one before, across tiles and also across results: the grid is one
+// workgroup a CU, and the next result's tiles load while this one's epilogue runs. One barrier a 64.
+//
+// d lies as the epilogue's registers hold it, in blocks of 16 vocabulary entries x 32 tokens (1 KB, 16 bytes a lane): dx's
+// product reads a block as a matrix operand as it is, dW's through the transposing LDS reads.
+#include "attn_common.h"
+
+namespace pkm {
+namespace {
+
+constexpr int kTile = 256, kDepth = 64, kHalf = 32768, kStage = 2 * kHalf;
+constexpr int kThreads = 512;
+constexpr float kLog2e = 1.44269504f;
+
+enum Product { kLoss, kGrads, kDx, kDw };
+
+struct CeArgs {
+  const uint8_t* x;  // kept tokens [npad, dpad]
+  const uint8_t* w;
+  uint8_t* d;  // blocks of a piece [piece / 16][npad / 32][1 KB]
+  int64_t x_stride, w_stride;  // bytes
+  const int32_t* count;  // kept tokens
+  const int32_t* label;  // [npad]
+  const float* ref;      // [npad] the label's logit, the softmax sums' reference
+  const float* lse;      // [npad]
+  const float* weight;   // [npad] of the tokens' gradients
+  float2* sums;          // [2 * vocab tiles][npad] reference and sum of exponentials
+  float* dx;             // [splits][npad][dcols] float32
+  uint8_t* dw;           // [vocab][dim]
+  const float* dw_scale;
+  int64_t vocab, v0;  // v0: the piece's first entry
+  int32_t piece, dim, npad, dcols, splits, add, lg_m, lg_n;
+};
+
+__device__ __forceinline__ int perm16(int k) { return ((k & 3) << 2) | ((k >> 2) & 3); }
+
+// 64 lanes' 16 bytes each from base + their offset to LDS at `to` and on, side by side; vmcnt counts them, the compiler does not.
+// The descriptor may come from a vector instruction (a lane read, a spilled scalar), which a memory instruction has to
+// follow by 5 states: inside the asm only we see to that.
+__device__ __forceinline__ void load16(const uint8_t* base, lds_u8* to, uint32_t offset) {
+  const u32x4_t rs = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uintptr_t)base),
+                      (uint32_t)__builtin_amdgcn_readfirstlane((int)((uintptr_t)base >> 32)), 0x7fffffffu, 0x00020000u};
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"((uint32_t)(uintptr_t)to), "v"(offset), "s"(rs)
+               : "memory");
+}
+
+// The operands' tiles: how a wave loads its four KB of one and reads a matrix operand from it.
+// L = wave + 8 n is the KB that load n fills.
+
+// [256 rows][64 numbers] of a matrix whose rows hold the summed index: 128 bytes a row, chunks permuted by the row. Rows
+// behind the last repeat it; chunks behind the row's end repeat the last one, against zeros of the other operand.
+struct RowsTile {
+  const uint8_t* base;
+  uint32_t off[4];
+  int chunk;
+  __device__ __forceinline__ void at(const uint8_t* p, int64_t stride, int64_t row0, int64_t rows, int wave, int lane) {
+    base = p + row0 * stride;
+    const int64_t last = rows - 1 - row0;
+    chunk = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) off[n] = (uint32_t)(min((int64_t)(8 * wave + 64 * n + (lane >> 3)), last) * stride);
+  }
+  __device__ __forceinline__ void load(lds_u8* to, int step, int chunks, int wave) const {
+    const uint32_t c = (uint32_t)min(step * 8 + chunk, chunks - 1) << 4;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) load16(base, to + (wave + 8 * n) * 1024, off[n] + c);
+  }
+};
+__device__ __forceinline__ uint32_t rows_lane(int lane) {
+  return (lane & 31) * 128 + (((lane >> 5) ^ (lane & 7)) << 4);
+}
+__device__ __forceinline__ frag_t rows_frag(uint32_t at, int t, int s) {
+  return *(const lds_u32x4*)(uintptr_t)((at ^ (uint32_t)(s << 5)) + t * 4096);
+}
+
+// [64 rows][256 columns] of a matrix whose rows are the summed index: 512 bytes a row, chunks permuted by the row.
+struct ColsTile {
+  const uint8_t* base;
+  uint32_t col;
+  __device__ __forceinline__ void at(const uint8_t* p, int col0, int chunks, int wave, int lane) {
+    base = p;
+    col = (uint32_t)min(col0 / 8 + ((lane & 31) ^ perm16(2 * wave + (lane >> 5))), chunks - 1) << 4;
+  }
+  __device__ __forceinline__ void load(lds_u8* to, int step, int64_t stride, int64_t rows, int wave, int lane) const {
+    const uint8_t* const b = base + (int64_t)step * kDepth * stride;
+    const int last = (int)min(rows - 1 - (int64_t)step * kDepth, (int64_t)kDepth);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      load16(b, to + (wave + 8 * n) * 1024, (uint32_t)min(2 * wave + 16 * n + (lane >> 5), last) * (uint32_t)stride + col);
+  }
+};
+__device__ __forceinline__ uint32_t cols_lane(int lane) {
+  const int l = lane & 15, h = lane >> 5, g = (lane >> 4) & 1;
+  return (4 * h + (l >> 2)) * 512 + (((2 * g + ((l & 3) >> 1)) ^ (((l >> 2) << 2) | h)) << 4) + (l & 1) * 8;
+}
+__device__ __forceinline__ frag_t two_tr(uint32_t p, uint32_t q) {
+  const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)p);
+  const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)q);
+  const u32x2_t x = __builtin_bit_cast(u32x2_t, a), y = __builtin_bit_cast(u32x2_t, b);
+  return (frag_t){x[0], x[1], y[0], y[1]};
+}
+// Summed index in the order 4 h + 0..3, 8 + 4 h + 0..3, which is how d's blocks have it.
+__device__ __forceinline__ frag_t cols_frag(uint32_t at, int t, int s) {
+  return two_tr((at ^ (uint32_t)(t << 6)) + s * 8192, (at ^ (uint32_t)((t << 6) | 32)) + s * 8192 + 4096);
+}
+
+// Where a block of d holds lane (h, token)'s 16 bytes: the halves 64 bytes apart in a 128-byte line, for the transposing reads.
+__device__ __forceinline__ int block_lane(int h, int t) { return 32 * h + (t ^ (h << 2)); }
+
+// d as dx's operand: 256 tokens, 64 vocabulary entries. Block (entries n, tokens wave).
+__device__ __forceinline__ void load_tokens(const uint8_t* d, lds_u8* to, int step, int tile, int npad, int wave, int lane) {
+  const uint32_t row = (uint32_t)(npad / 32) * 1024;
+  const uint8_t* const b = d + (int64_t)step * 4 * row + (int64_t)tile * 8192;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) load16(b, to + (wave + 8 * n) * 1024, n * row + wave * 1024 + lane * 16);
+}
+__device__ __forceinline__ uint32_t tokens_lane(int lane) { return block_lane(lane >> 5, lane & 31) * 16; }
+__device__ __forceinline__ frag_t tokens_frag(uint32_t at, int t, int s) {
+  return *(const lds_u32x4*)(uintptr_t)(at + s * 8192 + t * 1024);
+}
+
+// d as dW's operand: 256 vocabulary entries, 64 tokens. Block (entries L / 2, tokens L % 2).
+__device__ __forceinline__ void load_entries(const uint8_t* d, lds_u8* to, int step, int tile, int npad, int wave, int lane) {
+  const uint32_t row = (uint32_t)(npad / 32) * 1024;
+  const uint8_t* const b = d + (int64_t)tile * 16 * row + (int64_t)step * 2048;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int L = wave + 8 * n;
+    load16(b, to + L * 1024, (uint32_t)(L >> 1) * row + (L & 1) * 1024 + lane * 16);
+  }
+}
+__device__ __forceinline__ uint32_t entries_lane(int lane) {
+  const int l = lane & 15, h = lane >> 5, g = (lane >> 4) & 1, p = l & 3;
+  return g * 2048 + block_lane(p & 1, 4 * h + (l >> 2)) * 16 + 8 * (p >> 1);
+}
+__device__ __forceinline__ frag_t entries_frag(uint32_t at, int t, int s) {
+  const uint32_t p = at + t * 4096 + (s >> 1) * 1024 + (s & 1) * 256;
+  return two_tr(p, p + 128);
+}
+
+// Results of a product and their order: blocks of 2^lg_m x 2^lg_n tiles, one XCD's workgroups side by side in it, so that
+// they share the tiles' rows in its L2; blocks run along N first.
+struct Order {
+  int m, n, k, splits, lg_m, lg_n, blocks_n, total, share;
+  __device__ __forceinline__ Order(int m_, int n_, int k_, int splits_, int lg_m_, int lg_n_)
+      : m(m_), n(n_), k(k_), splits(splits_), lg_m(lg_m_), lg_n(lg_n_) {
+    blocks_n = (n + (1 << lg_n) - 1) >> lg_n;
+    total = (((m + (1 << lg_m) - 1) >> lg_m) * blocks_n * splits) << (lg_m + lg_n);
+    share = min(32, (total + 7) / 8);  // results of an XCD at a time
+  }
+};
+struct Result {
+  int i, m, n, split, k0, k1;  // i: the order's place; steps [k0, k1)
+  __device__ __forceinline__ bool next(const Order& o, bool first) {
+    const int b = blockIdx.x, xcd = b & 7, own = b >> 3;
+    if (first) {
+      if (own >= o.share) return false;
+      i = xcd * o.share + own;
+    } else {
+      i += 8 * o.share;
+    }
+    for (; i < o.total; i += 8 * o.share) {
+      const int within = i & ((1 << (o.lg_m + o.lg_n)) - 1), block = i >> (o.lg_m + o.lg_n);
+      const int rest = block / o.splits;
+      split = block - rest * o.splits;
+      m = ((rest / o.blocks_n) << o.lg_m) + (within & ((1 << o.lg_m) - 1));
+      n = ((rest % o.blocks_n) << o.lg_n) + (within >> o.lg_m);
+      if (m >= o.m || n >= o.n) continue;
+      k0 = (int)((int64_t)o.k * split / o.splits);
+      k1 = (int)((int64_t)o.k * (split + 1) / o.splits);
+      if (k1 > k0) return true;
+    }
+    return false;
+  }
+};
+
+// The epilogues. A wave's 128 x 64: acc[t][u][i] is row 32 t + 8 (i / 4) + 4 h + i % 4, column 32 u + lane % 32.
+typedef f32x16_t acc_t[4][2];
+
+__device__ __forceinline__ constexpr int row_of(int t, int i) { return 32 * t + 8 * (i >> 2) + (i & 3); }  // but 4 h
+
+// Nothing moves across: a batch of registers is done with before the next begins.
+__device__ __forceinline__ void batch() { __builtin_amdgcn_sched_barrier(0); }
+
+// Results behind the vocabulary's end, `left` rows from the wave's first: x in their place.
+__device__ __forceinline__ void cut(acc_t& acc, int64_t left, int h, float x) {
+  if (left >= 128) return;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    int most = (int)left - 4 * h;
+    asm volatile("" : "+v"(most));  // compared anew for each half: 64 masks would not fit the scalar registers
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[t][u][i] = row_of(t, i) < most ? acc[t][u][i] : x;
+  }
+}
+
+// The sums of the exponentials of 128 entries for 64 tokens, against the token's reference: the label's logit, which is one of
+// the summands, so that what underflows beside it is nothing. Where one overflows, the 128's own largest takes its place.
+__device__ __forceinline__ void end_loss(const CeArgs& a, acc_t& acc, const Result& r, int wave, int lane) {
+  const int h = lane >> 5, v0 = r.m * kTile + (wave >> 2) * 128;
+  cut(acc, a.vocab - v0, h, -INFINITY);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int j = r.n * kTile + (wave & 3) * 64 + 32 * u + (lane & 31);
+    float ref = a.ref[j];
+    float sum = 0.f;
+    const float c = -ref * kLog2e;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum += exp2_raw(__builtin_fmaf(acc[t][u][i], kLog2e, c));
+      batch();
+    }
+    sum += swap_halves(sum);
+    const bool over = !(sum < 0x1p120f);
+    if (__any(over)) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, acc[t][u][i]);
+      top = fmaxf(top, swap_halves(top));
+      float own = 0.f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) own += exp2_raw((acc[t][u][i] - top) * kLog2e);
+        batch();
+      }
+      own += swap_halves(own);
+      if (over) ref = top, sum = own;
+    }
+    if (h == 0) a.sums[(int64_t)(2 * r.m + (wave >> 2)) * a.npad + j] = make_float2(ref, sum);
+  }
+}
+
+// d of 128 entries for 64 tokens, rounded, in blocks.
+template <typename T>
+__device__ __forceinline__ void end_grads(const CeArgs& a, acc_t& acc, const Result& r, int count, int wave, int lane) {
+  const int h = lane >> 5, v0 = r.m * kTile + (wave >> 2) * 128;
+  cut(acc, a.vocab - a.v0 - v0, h, -INFINITY);
+  const int64_t row = (int64_t)(a.npad / 32) * 1024;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int j = r.n * kTile + (wave & 3) * 64 + 32 * u + (lane & 31);
+    const bool kept = j < count;
+    const float c = kept ? -a.lse[j] * kLog2e : -INFINITY, weight = kept ? a.weight[j] : 0.f;
+    uint8_t* const to = a.d + (int64_t)(v0 / 16) * row + (int64_t)(j >> 5) * 1024;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = exp2_raw(__builtin_fmaf(acc[t][u][8 * s + e], kLog2e, c)) * weight;
+        const u32x4_t x = {pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7])};
+        *(u32x4_t*)(to + (2 * t + s) * row + block_lane(h, lane & 31) * 16) = x;
+      }
+      batch();
+    }
+    // the label's number is exp(l - lse) - 1, rounded once: it takes the place of the one written above
+    const int64_t y = kept ? (int64_t)a.label[j] - a.v0 - v0 : -1;
+    if (__any(y >= 0 && y < 128)) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (y >= 0 && y < 128 && h == 0) {
+        const float x = (exp2_raw(__builtin_fmaf(a.ref[j], kLog2e, c)) - 1.f) * weight;
+        *(uint16_t*)(to + (y >> 4) * row + block_lane((y >> 2) & 1, lane) * 16 + ((y >> 3) & 1) * 8 + (y & 3) * 2) =
+            (uint16_t)pack2<T>(x, x);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void end_dx(const CeArgs& a, acc_t& acc, const Result& r, int wave, int lane) {
+  const int h = lane >> 5;
+  float* const to = a.dx + ((int64_t)r.split * a.npad + r.m * kTile + (wave >> 2) * 128 + 4 * h) * a.dcols + r.n * kTile +
+                    (wave & 3) * 64 + (lane & 31);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (a.add) {
+        float before[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) before[i] = to[(int64_t)row_of(t, i) * a.dcols + 32 * u];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][u][i] += before[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) to[(int64_t)row_of(t, i) * a.dcols + 32 * u] = acc[t][u][i];
+      batch();
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void end_dw(const CeArgs& a, acc_t& acc, const Result& r, int wave, int lane) {
+  const int h = lane >> 5, odd = lane & 1;
+  const float f = *a.dw_scale;
+  // lanes 2 k and 2 k + 1 swap, so that each has two neighbours of one row
+  const int64_t v0 = a.v0 + r.m * kTile + (wave >> 2) * 128 + 4 * h + odd;
+  const int d0 = r.n * kTile + (wave & 3) * 64 + (lane & 31) - odd;
+  const int64_t left = a.vocab - v0;
+  const bool even_rows = (a.dim & 1) == 0;
+  uint8_t* const to = a.dw + 2 * (v0 * a.dim + d0);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float x = acc[t][u][i] * f, y = acc[t][u][i + 1] * f;
+        const float give = odd ? x : y;
+        const float take =
+            __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(give), 0xB1, 0xF, 0xF, false));
+        const uint32_t two = odd ? pack2<T>(take, y) : pack2<T>(x, take);
+        const int d = d0 + 32 * u;
+        if (row_of(t, i) < left && d < a.dim) {
+          uint8_t* const at = to + 2 * ((int64_t)row_of(t, i) * a.dim + 32 * u);
+          if (even_rows) {
+            *(uint32_t*)at = two;
+          } else {
+            *(uint16_t*)at = (uint16_t)two;
+            if (d + 1 < a.dim) *(uint16_t*)(at + 2) = (uint16_t)(two >> 16);
+          }
+        }
+      }
+      batch();
+    }
+}
+
+template <typename T, Product P>
+__global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
+  __shared__ __align__(1024) uint8_t smem[2 * kStage];
+  lds_u8* const lds = (lds_u8*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = __builtin_amdgcn_readfirstlane(*a.count);
+  const int chunks = (a.dim + 7) / 8, dpad = (int)(a.x_stride / 2);
+  const int64_t entries = min((int64_t)a.piece, a.vocab - a.v0);  // of the piece
+  const int token_tiles = (n + kTile - 1) / kTile, entry_tiles = (int)((entries + kTile - 1) / kTile),
+            dim_tiles = a.dcols / kTile;
+  const Order order = P == kLoss || P == kGrads ? Order(entry_tiles, token_tiles, dpad / kDepth, 1, a.lg_m, a.lg_n)
+                      : P == kDx ? Order(token_tiles, dim_tiles, (int)((entries + kDepth - 1) / kDepth), a.splits, a.lg_m, a.lg_n)
+                                 : Order(entry_tiles, dim_tiles, (n + kDepth - 1) / kDepth, 1, a.lg_m, a.lg_n);
+  const uint8_t* const w = a.w + a.v0 * a.w_stride;
+
+  Result run, ahead;  // the result in work, and the one whose tiles are loaded
+  RowsTile ra, rb;
+  ColsTile cb;
+  const auto aim = [&]() {
+    if constexpr (P == kLoss || P == kGrads) {
+      ra.at(w, a.w_stride, (int64_t)ahead.m * kTile, entries, wave, lane);
+      rb.at(a.x, a.x_stride, (int64_t)ahead.n * kTile, n, wave, lane);
+    } else if constexpr (P == kDx) {
+      cb.at(w, ahead.n * kTile, chunks, wave, lane);
+    } else {
+      cb.at(a.x, ahead.n * kTile, dpad / 8, wave, lane);
+    }
+  };
+  const auto load = [&](int stage, int step) {
+    lds_u8* const to = lds + stage * kStage;
+    if constexpr (P == kLoss || P == kGrads) {
+      ra.load(to, step, chunks, wave);
+      rb.load(to + kHalf, step, dpad / 8, wave);
+    } else if constexpr (P == kDx) {
+      load_tokens(a.d, to, step, ahead.m, a.npad, wave, lane);
+      cb.load(to + kHalf, step, a.w_stride, entries, wave, lane);
+    } else {
+      load_entries(a.d, to, step, ahead.m, a.npad, wave, lane);
+      cb.load(to + kHalf, step, a.x_stride, n, wave, lane);
+    }
+  };
+  // the loads run two steps ahead
+  int load_step;
+  bool more = ahead.next(order, true);
+  if (!more) return;
+  run = ahead;
+  aim();
+  load_step = ahead.k0;
+  const auto load_next = [&](int stage) {
+    if (!more) return;
+    load(stage, load_step);
+    if (++load_step == ahead.k1) {
+      more = ahead.next(order, false);
+      if (more) {
+        aim();
+        load_step = ahead.k0;
+      }
+    }
+  };
+
+  // this lane's place in the operands' tiles
+  const uint32_t base = lds_address(lds);
+  const uint32_t at_a = base + (P == kLoss || P == kGrads ? rows_lane(lane) + (wave >> 2) * 16384
+                                : P == kDx                ? tokens_lane(lane) + (wave >> 2) * 4096
+                                                          : entries_lane(lane) + (wave >> 2) * 16384);
+  const uint32_t at_b = base + kHalf + (P == kLoss || P == kGrads ? rows_lane(lane) + (wave & 3) * 8192
+                                                                  : cols_lane(lane) ^ (uint32_t)((wave & 3) * 128));
+  frag_t fa[2][4], fb[2][2];
+  const auto read = [&](int set, int stage, int s) {
+    const uint32_t pa = at_a + stage * kStage, pb = at_b + stage * kStage;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      fb[set][u] = P == kLoss || P == kGrads ? rows_frag(pb, u, s) : cols_frag(pb, u, s);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      fa[set][t] = P == kLoss || P == kGrads ? rows_frag(pa, t, s) : P == kDx ? tokens_frag(pa, t, s) : entries_frag(pa, t, s);
+  };
+  acc_t acc = {};
+  const auto multiply = [&](int set) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) acc[t][u] = mfma32<T>(fa[set][t], fb[set][u], acc[t][u]);
+  };
+
+  load_next(0);
+  const bool two = more;
+  load_next(1);
+  if (two)
+    tile_wait<8>();
+  else
+    tile_wait<0>();
+  __syncthreads();
+  read(0, 0, 0);
+  for (int stage = 0, step = run.k0;; stage ^= 1) {
+#pragma unroll
+    for (int s = 0; s < 3; ++s) {
+      read((s + 1) & 1, stage, s + 1);
+      keep_order();
+      multiply(s & 1);
+      keep_order();
+    }
+    // every wave has read this stage and loaded the next
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const bool ends = ++step == run.k1;
+    Result after = run;
+    const bool last = ends && !after.next(order, false);
+    load_next(stage);
+    if (!last) read(0, stage ^ 1, 0);
+    keep_order();
+    multiply(1);
+    keep_order();
+    if (ends) {
+      if constexpr (P == kLoss) end_loss(a, acc, run, wave, lane);
+      if constexpr (P == kGrads) end_grads<T>(a, acc, run, n, wave, lane);
+      if constexpr (P == kDx) end_dx(a, acc, run, wave, lane);
+      if constexpr (P == kDw) end_dw<T>(a, acc, run, wave, lane);
+      if (last) break;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) acc[t][u] = f32x16_t{};
+      run = after;
+      step = run.k0;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Around the products
+// ---------------------------------------------------------------------------
+constexpr int kPrepareRows = 64;  // tokens of a workgroup of ce_prepare
+constexpr int kJoinTokens = 32, kJoinSlices = 32;
+
+struct Header {
+  int32_t count;   // kept tokens
+  float dw_scale;  // of the results of dW's product
+  float dx_scale;
+};
+
+template <typename L>
+__device__ __forceinline__ int label_of(const void* labels, int64_t i, int64_t ignore, int64_t vocab) {
+  const int64_t y = (int64_t)((const L*)labels)[i];
+  return y == ignore || y < 0 || y >= vocab ? -1 : (int)y;
+}
+
+// The kept tokens side by side: rows, labels, places, and the label's logit as the sums' reference. A workgroup counts
+// the kept tokens before its 64 itself.
+template <typename T, typename L>
+__global__ __launch_bounds__(256) void ce_prepare(const T* __restrict__ x, int64_t x_stride, int64_t tokens,
+                                                  const T* __restrict__ w, int64_t w_stride, int64_t vocab, int dim, int dpad,
+                                                  int wide, const void* labels, int64_t ignore, Header* head, int32_t* place,
+                                                  int32_t* label, float* ref, T* __restrict__ kept, int npad) {
+  __shared__ int32_t before_s[4], places[kPrepareRows], own_s;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int64_t first = (int64_t)blockIdx.x * kPrepareRows;
+  int32_t before = 0;
+  for (int64_t i = tid; i < first; i += 256) before += label_of<L>(labels, i, ignore, vocab) >= 0;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) before += __shfl_xor(before, s);
+  if (lane == 0) before_s[wave] = before;
+  __syncthreads();
+  before = before_s[0] + before_s[1] + before_s[2] + before_s[3];
+  if (wave == 0) {
+    const int64_t i = first + lane;
+    const int y = i < tokens ? label_of<L>(labels, i, ignore, vocab) : -1;
+    const uint64_t live = __ballot(y >= 0);
+    const int at = before + __popcll(live & ((1ull << lane) - 1));
+    places[lane] = y >= 0 ? at : -1;
+    if (y >= 0) label[at] = y;
+    if (i < tokens) place[i] = places[lane];
+    if (lane == 0) own_s = __popcll(live);
+  }
+  __syncthreads();
+  if (blockIdx.x == gridDim.x - 1) {
+    const int count = before + own_s;
+    if (tid == 0) head->count = count;
+    for (int j = count + tid; j < npad; j += 256) {
+      label[j] = -1;
+      ref[j] = 0.f;
+    }
+  }
+  for (int k = wave; k < kPrepareRows; k += 4) {
+    const int at = places[k];
+    if (at < 0) continue;
+    const T* const row = x + (first + k) * x_stride;
+    T* const to = kept + (int64_t)at * dpad;
+    const T* const wy = w + (int64_t)label_of<L>(labels, first + k, ignore, vocab) * w_stride;
+    float dot = 0.f;
+    if (wide) {
+      for (int c = lane; c < dpad / 8; c += 64) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (c < dim / 8) {
+          v = ld16(row + 8 * c);
+          dot = vec_dot<T>(v, ld16(wy + 8 * c), dot);
+        }
+        st16(to + 8 * c, v);
+      }
+    } else {
+      for (int c = lane; c < dpad; c += 64) {
+        uint16_t v = 0;
+        if (c < dim) {
+          v = ((const uint16_t*)row)[c];
+          dot += unpack1<T>(v) * unpack1<T>(((const uint16_t*)wy)[c]);
+        }
+        ((uint16_t*)to)[c] = v;
+      }
+    }
+    dot = group_sum<64>(dot);
+    if (lane == 0) ref[at] = dot;
+  }
+}
+
+// lse and loss of 32 tokens from the tiles' sums.
+__global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(const Header* head, const float2* __restrict__ sums, int parts,
+                                                                    int npad, const float* __restrict__ ref,
+                                                                    float* __restrict__ lse, float* __restrict__ losses,
+                                                                    float* __restrict__ block_sums) {
+  __shared__ float2 s[kJoinSlices][kJoinTokens];
+  const int t = threadIdx.x % kJoinTokens, slice = threadIdx.x / kJoinTokens;
+  const int j = blockIdx.x * kJoinTokens + t, count = head->count;
+  float m = -INFINITY, sum = 0.f;
+  const auto add = [&](float r, float v) {
+    if (r > m) {
+      sum = sum * exp2_raw((m - r) * kLog2e) + v;  // 0 at first
+      m = r;
+    } else {
+      sum += r == m ? v : v * exp2_raw((r - m) * kLog2e);
+    }
+  };
+  if (j < count) {
+#pragma unroll 4
+    for (int p = slice; p < parts; p += kJoinSlices) {
+      const float2 v = sums[(int64_t)p * npad + j];
+      add(v.x, v.y);
+    }
+  }
+  s[slice][t] = make_float2(m, sum);
+  __syncthreads();
+  if (slice != 0) return;
+  float loss = 0.f;
+  if (j < count) {
+    for (int k = 1; k < kJoinSlices; ++k)
+      if (s[k][t].y != 0.f) add(s[k][t].x, s[k][t].y);  // NaN counts as something
+    const float log_sum = __builtin_amdgcn_logf(sum) * 0.693147180559945f;
+    lse[j] = m + log_sum;
+    loss = log_sum + (m - ref[j]);
+    losses[j] = loss;
+  }
+#pragma unroll
+  for (int k = 1; k < kJoinTokens; k <<= 1) loss += __shfl_xor(loss, k);
+  if (t == 0) block_sums[blockIdx.x] = loss;
+}
+
+// The mean or sum of the losses: one workgroup, in a fixed order.
+__global__ __launch_bounds__(1024) void ce_reduce(const Header* head, const float* __restrict__ block_sums, int blocks, int mean,
+                                                  float* out) {
+  __shared__ float s[16];
+  float sum = 0.f;
+  for (int i = threadIdx.x; i < blocks; i += 1024) sum += block_sums[i];
+  sum = group_sum<64>(sum);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  sum = 0.f;
+  for (int k = 0; k < 16; ++k) sum += s[k];
+  out[0] = mean ? sum / (float)max(head->count, 1) : sum;
+}
+
+__global__ __launch_bounds__(256) void ce_scatter(const int32_t* __restrict__ place, const float* __restrict__ losses,
+                                                  int64_t tokens, float* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < tokens) out[i] = place[i] < 0 ? 0.f : losses[place[i]];
+}
+
+// The tokens' gradients as weights of d: g_j over a power of two that the largest is just below, times `lift` (2^14 in f16,
+// whose smallest numbers softmax weights reach; 1 in bf16). The two scales undo it in the results. One gradient for
+// all tokens is a scale alone.
+__global__ __launch_bounds__(1024) void ce_weights(Header* head, const float* __restrict__ grad, int reduction,
+                                                   const int32_t* __restrict__ place, int64_t tokens, float lift,
+                                                   float* __restrict__ weight, int npad) {
+  __shared__ float s[16];
+  const int tid = threadIdx.x;
+  float unit = 1.f;
+  if (reduction == 0) {
+    float top = 0.f;
+    for (int64_t i = tid; i < tokens; i += 1024)
+      if (place[i] >= 0) top = fmaxf(top, fabsf(grad[i]));
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+    if ((tid & 63) == 0) s[tid >> 6] = top;
+    __syncthreads();
+    for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k]);
+    const int e = top > 0.f ? min(max(__builtin_amdgcn_frexp_expf(top), -100), 100) : 0;
+    unit = ldexpf(1.f, e);
+    for (int64_t i = tid; i < tokens; i += 1024)
+      if (place[i] >= 0) weight[place[i]] = grad[i] / unit * lift;
+    for (int j = head->count + tid; j < npad; j += 1024) weight[j] = 0.f;
+  } else {
+    for (int j = tid; j < npad; j += 1024) weight[j] = j < head->count ? lift : 0.f;
+    unit = reduction == 1 ? grad[0] / (float)max(head->count, 1) : grad[0];
+  }
+  if (tid == 0) head->dw_scale = head->dx_scale = unit / lift;
+}
+
+// dx of every token: the splits' sums in order, rounded; zeros for tokens that are not kept. A workgroup a token at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void ce_dx(const Header* head, const int32_t* __restrict__ place, int64_t tokens,
+                                             const float* __restrict__ parts, int splits, int npad, int dcols, int dim,
+                                             T* __restrict__ dx) {
+  const float f = head->dx_scale;
+  for (int64_t i = blockIdx.x; i < tokens; i += gridDim.x) {
+    const int j = place[i];
+    for (int d = threadIdx.x * 4; d < dim; d += 1024) {
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j >= 0)
+        for (int s = 0; s < splits; ++s) {
+          const float4 v = *(const float4*)(parts + ((int64_t)s * npad + j) * dcols + d);
+          sum.x += v.x;
+          sum.y += v.y;
+          sum.z += v.z;
+          sum.w += v.w;
+        }
+      uint16_t* const to = (uint16_t*)(dx + i * dim + d);
+      const uint32_t a = j < 0 ? 0u : pack2<T>(sum.x * f, sum.y * f), b = j < 0 ? 0u : pack2<T>(sum.z * f, sum.w * f);
+      if ((dim & 3) == 0) {
+        *(uint2*)to = make_uint2(a, b);
+      } else {
+        const uint16_t four[4] = {(uint16_t)a, (uint16_t)(a >> 16), (uint16_t)b, (uint16_t)(b >> 16)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (d + k < dim) to[k] = four[k];
+      }
+    }
+  }
+}
+
+// dW without any kept token
+__global__ __launch_bounds__(256) void ce_no_dw(const Header* head, uint16_t* __restrict__ dw, int64_t n) {
+  if (head->count != 0) return;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) dw[i] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// What the forward leaves for the backward, in one buffer.
+struct Kept {
+  int64_t npad, dpad, place, label, ref, lse, x, bytes;
+};
+bool plan_kept(int64_t tokens, int64_t dim, Kept* k) {
+  if (tokens < 0 || dim < 1 || tokens >= (1ll << 22) || dim > 65536) return false;
+  k->npad = up(tokens < 1 ? 1 : tokens, kTile);
+  k->dpad = up(dim, kDepth);
+  k->place = 256;
+  k->label = k->place + k->npad * 4;
+  k->ref = k->label + k->npad * 4;
+  k->lse = k->ref + k->npad * 4;
+  k->x = k->lse + k->npad * 4;
+  k->bytes = k->x + k->npad * k->dpad * 2;
+  return true;
+}
+
+struct Forward {
+  int64_t sums, losses, block_sums, bytes;
+};
+Forward plan_forward(const Kept& k, int64_t vocab) {
+  Forward f;
+  f.sums = 0;
+  f.losses = f.sums + up(vocab, kTile) / 128 * k.npad * 8;
+  f.block_sums = f.losses + k.npad * 4;
+  f.bytes = f.block_sums + k.npad / kJoinTokens * 4;
+  return f;
+}
+
+struct Backward {
+  int64_t piece, splits, dcols, weight, d, dx, bytes;
+};
+Backward plan_backward(const Kept& k, int64_t vocab, int64_t dim) {
+  Backward b;
+  const int64_t all = up(vocab, kTile);
+  // 512 MB of d at a time, and no fewer than 64 tiles of the vocabulary: dW's product has one for each and 256 columns
+  int64_t most = (1ll << 28) / k.npad / kTile * kTile;
+  if (most < 64 * kTile) most = 64 * kTile;
+  const int64_t pieces = (all + most - 1) / most;
+  b.piece = up((all + pieces - 1) / pieces, kTile);
+  b.dcols = up(dim, kTile);
+  // dx's product over few tokens is split along the vocabulary until it fills the CUs, 16 steps at least each
+  const int64_t results = k.npad / kTile * (b.dcols / kTile), steps = b.piece / kDepth;
+  b.splits = 256 / results;
+  if (b.splits > steps / 16) b.splits = steps / 16;
+  if (b.splits < 1) b.splits = 1;
+  b.weight = 0;
+  b.d = b.weight + k.npad * 4;
+  b.dx = b.d + b.piece * k.npad * 2;
+  b.bytes = b.dx + b.splits * k.npad * b.dcols * 4;
+  return b;
+}
+
+// The tiles of an order's block: 2^lg_n of N, of which there are n, and 32 in all.
+void block_of(int64_t n, CeArgs* a) {
+  a->lg_n = n >= 4 ? 2 : n >= 2 ? 1 : 0;
+  a->lg_m = 5 - a->lg_n;
+}
+
+template <typename T, Product P>
+void launch(const CeArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((ce_product<T, P>), dim3(256), dim3(kThreads), 0, st, a);
+}
+
+template <typename T>
+int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, int64_t w_stride, int64_t vocab, int64_t dim,
+                const void* labels, int bits, int64_t ignore, int reduction, float* loss, uint8_t* kept, const Kept& k, uint8_t* ws,
+                const Forward& f, hipStream_t st) {
+  Header* const head = (Header*)kept;
+  int32_t *place = (int32_t*)(kept + k.place), *label = (int32_t*)(kept + k.label);
+  float *ref = (float*)(kept + k.ref), *lse = (float*)(kept + k.lse);
+  const int wide = (((uintptr_t)x | (uintptr_t)w) & 15) == 0 && ((x_stride | w_stride | dim) & 7) == 0;
+  const unsigned blocks = (unsigned)((tokens < 1 ? 1 : tokens) + kPrepareRows - 1) / kPrepareRows;
+  if (bits == 64)
+    hipLaunchKernelGGL((ce_prepare<T, int64_t>), dim3(blocks), dim3(256), 0, st, (const T*)x, x_stride, tokens, (const T*)w,
+                       w_stride, vocab, (int)dim, (int)k.dpad, wide, labels, ignore, head, place, label, ref,
+                       (T*)(kept + k.x), (int)k.npad);
+  else
+    hipLaunchKernelGGL((ce_prepare<T, int32_t>), dim3(blocks), dim3(256), 0, st, (const T*)x, x_stride, tokens, (const T*)w,
+                       w_stride, vocab, (int)dim, (int)k.dpad, wide, labels, ignore, head, place, label, ref,
+                       (T*)(kept + k.x), (int)k.npad);
+  CeArgs a = {};
+  a.x = kept + k.x;
+  a.x_stride = k.dpad * 2;
+  a.w = (const uint8_t*)w;
+  a.w_stride = w_stride * 2;
+  a.count = &head->count;
+  a.label = label;
+  a.ref = ref;
+  a.sums = (float2*)(ws + f.sums);
+  a.vocab = vocab;
+  a.piece = (int32_t)up(vocab, kTile);
+  a.dim = (int32_t)dim;
+  a.npad = (int32_t)k.npad;
+  a.dcols = (int32_t)up(dim, kTile);
+  a.splits = 1;
+  block_of(k.npad / kTile, &a);
+  launch<T, kLoss>(a, st);
+  float *losses = (float*)(ws + f.losses), *block_sums = (float*)(ws + f.block_sums);
+  const int joins = (int)((tokens + kJoinTokens - 1) / kJoinTokens);
+  if (joins > 0)
+    hipLaunchKernelGGL(ce_join, dim3((unsigned)joins), dim3(kJoinTokens * kJoinSlices), 0, st, head, (const float2*)a.sums,
+                     (int)(up(vocab, kTile) / 128), (int)k.npad, ref, lse, losses, block_sums);
+  if (reduction == 0 && tokens > 0)
+    hipLaunchKernelGGL(ce_scatter, dim3((unsigned)((tokens + 255) / 256)), dim3(256), 0, st, place, losses, tokens, loss);
+  if (reduction != 0)
+    hipLaunchKernelGGL(ce_reduce, dim3(1), dim3(1024), 0, st, head, block_sums, joins, reduction == 1, loss);
+  return pkm_check_launch("pkm_linear_ce_fwd");
+}
+
+template <typename T>
+int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, int64_t w_stride, int64_t vocab, int64_t dim,
+                 const float* grad, int reduction, void* dx, void* dw, uint8_t* ws, const Backward& b, hipStream_t st) {
+  Header* const head = (Header*)kept;
+  const int32_t* place = (const int32_t*)(kept + k.place);
+  float* weight = (float*)(ws + b.weight);
+  constexpr float lift = __is_same(T, f16_t) ? 16384.f : 1.f;
+  hipLaunchKernelGGL(ce_weights, dim3(1), dim3(1024), 0, st, head, grad, reduction, place, tokens, lift, weight, (int)k.npad);
+  CeArgs a = {};
+  a.x = kept + k.x;
+  a.x_stride = k.dpad * 2;
+  a.w = (const uint8_t*)w;
+  a.w_stride = w_stride * 2;
+  a.d = ws + b.d;
+  a.count = &head->count;
+  a.label = (const int32_t*)(kept + k.label);
+  a.ref = (const float*)(kept + k.ref);
+  a.lse = (const float*)(kept + k.lse);
+  a.weight = weight;
+  a.dx = (float*)(ws + b.dx);
+  a.dw = (uint8_t*)dw;
+  a.dw_scale = &head->dw_scale;
+  a.vocab = vocab;
+  a.piece = (int32_t)b.piece;
+  a.dim = (int32_t)dim;
+  a.npad = (int32_t)k.npad;
+  a.dcols = (int32_t)b.dcols;
+  for (int64_t v0 = 0; v0 < vocab; v0 += b.piece) {
+    a.v0 = v0;
+    a.splits = 1;
+    block_of(k.npad / kTile, &a);
+    launch<T, kGrads>(a, st);
+    block_of(b.dcols / kTile, &a);
+    if (dw) launch<T, kDw>(a, st);
+    a.splits = (int32_t)b.splits;
+    a.add = v0 > 0;
+    if (dx) launch<T, kDx>(a, st);
+  }
+  if (dx && tokens > 0)
+    hipLaunchKernelGGL(ce_dx<T>, dim3((unsigned)(tokens < 65536 ? tokens : 65536)), dim3(256), 0, st, head, place, tokens, a.dx,
+                       (int)b.splits, (int)k.npad, (int)b.dcols, (int)dim, (T*)dx);
+  if (dw) hipLaunchKernelGGL(ce_no_dw, dim3(1024), dim3(256), 0, st, head, (uint16_t*)dw, vocab * dim);
+  return pkm_check_launch("pkm_linear_ce_bwd");
+}
+
+}  // namespace
+}  // namespace pkm
+
+using namespace pkm;
+
+#define CE_REQUIRE_COMMON(fn)                                                                                               \
+  PKM_REQUIRE(tokens >= 0 && vocab >= 1 && dim >= 1, PKM_ERR_INVALID_ARGUMENT, fn ": %lld tokens, weight [%lld, %lld]",     \
+              (long long)tokens, (long long)vocab, (long long)dim);                                                         \
+  PKM_REQUIRE(dtype == PKM_DTYPE_BF16 || dtype == PKM_DTYPE_F16, PKM_ERR_UNSUPPORTED,                                       \
+              fn ": dtype %d not supported (bfloat16, float16 are)", dtype);                                                \
+  PKM_REQUIRE(tokens < (1ll << 22) && dim <= 65536 && vocab < (1ll << 31), PKM_ERR_UNSUPPORTED,                             \
+              fn ": %lld tokens, weight [%lld, %lld] (fewer than 2^22, 2^31, up to 65536 are supported)", (long long)tokens, \
+              (long long)vocab, (long long)dim);                                                                            \
+  PKM_REQUIRE(reduction >= 0 && reduction <= 2, PKM_ERR_INVALID_ARGUMENT, fn ": reduction %d", reduction);                  \
+  Kept k;                                                                                                                   \
+  plan_kept(tokens, dim, &k);                                                                                               \
+  PKM_REQUIRE((up(vocab, kTile) / kTile + 32) * (k.npad / kTile + 32) < (1ll << 30), PKM_ERR_UNSUPPORTED,                   \
+              fn ": %lld tokens of %lld entries are too many", (long long)tokens, (long long)vocab);                        \
+  PKM_REQUIRE(weight && (((uintptr_t)weight) & 15) == 0 && (w_stride & 7) == 0 && w_stride >= up(dim, 8) &&                 \
+                  w_stride <= (1ll << 22),                                                                                  \
+              PKM_ERR_INVALID_ARGUMENT, fn ": weight has to lie on 16 bytes, its rows a multiple of 8 numbers apart");      \
+  PKM_REQUIRE(kept && (((uintptr_t)kept) & 15) == 0 && kept_bytes >= (size_t)k.bytes, PKM_ERR_WORKSPACE,                    \
+              fn ": kept buffer of %zu bytes, %lld needed", kept_bytes, (long long)k.bytes)
+
+extern "C" size_t pkm_linear_ce_kept_size(int64_t tokens, int64_t dim) {
+  Kept k;
+  return plan_kept(tokens, dim, &k) ? (size_t)k.bytes : 0;
+}
+
+extern "C" size_t pkm_linear_ce_fwd_workspace_size(int64_t tokens, int64_t vocab, int64_t dim) {
+  Kept k;
+  return vocab >= 1 && vocab < (1ll << 31) && plan_kept(tokens, dim, &k) ? (size_t)plan_forward(k, vocab).bytes : 0;
+}
+
+extern "C" size_t pkm_linear_ce_bwd_workspace_size(int64_t tokens, int64_t vocab, int64_t dim) {
+  Kept k;
+  return vocab >= 1 && vocab < (1ll << 31) && plan_kept(tokens, dim, &k) ? (size_t)plan_backward(k, vocab, dim).bytes : 0;
+}
+
+extern "C" int pkm_linear_ce_fwd(const void* x, int64_t x_stride, int64_t tokens, const void* weight, int64_t w_stride,
+                                 int64_t vocab, int64_t dim, int dtype, const void* labels, int label_bits, int64_t ignore,
+                                 int reduction, float* loss, void* kept, size_t kept_bytes, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  CE_REQUIRE_COMMON("pkm_linear_ce_fwd");
+  PKM_REQUIRE(label_bits == 32 || label_bits == 64, PKM_ERR_INVALID_ARGUMENT, "pkm_linear_ce_fwd: labels of %d bits (32 or 64)",
+              label_bits);
+  PKM_REQUIRE(tokens == 0 || (x && labels), PKM_ERR_INVALID_ARGUMENT, "pkm_linear_ce_fwd: null pointer");
+  PKM_REQUIRE(loss || (tokens == 0 && reduction == 0), PKM_ERR_INVALID_ARGUMENT, "pkm_linear_ce_fwd: null pointer");
+  PKM_REQUIRE(x_stride >= 0 && x_stride < (1ll << 40), PKM_ERR_INVALID_ARGUMENT, "pkm_linear_ce_fwd: row stride %lld",
+              (long long)x_stride);
+  const Forward f = plan_forward(k, vocab);
+  PKM_REQUIRE(workspace && (((uintptr_t)workspace) & 15) == 0 && workspace_bytes >= (size_t)f.bytes, PKM_ERR_WORKSPACE,
+              "pkm_linear_ce_fwd: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)f.bytes);
+  return dtype == PKM_DTYPE_BF16
+             ? run_forward<bf16_t>(x, x_stride, tokens, weight, w_stride, vocab, dim, labels, label_bits, ignore, reduction,
+                                   loss, (uint8_t*)kept, k, (uint8_t*)workspace, f, (hipStream_t)stream)
+             : run_forward<f16_t>(x, x_stride, tokens, weight, w_stride, vocab, dim, labels, label_bits, ignore, reduction,
+                                  loss, (uint8_t*)kept, k, (uint8_t*)workspace, f, (hipStream_t)stream);
+}
+
+extern "C" int pkm_linear_ce_bwd(void* kept, size_t kept_bytes, int64_t tokens, const void* weight, int64_t w_stride,
+                                 int64_t vocab, int64_t dim, int dtype, const float* grad_loss, int reduction, void* dx,
+                                 void* dweight, void* workspace, size_t workspace_bytes, void* stream) {
+  CE_REQUIRE_COMMON("pkm_linear_ce_bwd");
+  PKM_REQUIRE(grad_loss || (tokens == 0 && reduction == 0), PKM_ERR_INVALID_ARGUMENT, "pkm_linear_ce_bwd: null pointer");
+  PKM_REQUIRE((((uintptr_t)dx | (uintptr_t)dweight) & 15) == 0, PKM_ERR_INVALID_ARGUMENT,
+              "pkm_linear_ce_bwd: dx and dweight have to lie on 16 bytes");
+  const Backward b = plan_backward(k, vocab, dim);
+  PKM_REQUIRE(workspace && (((uintptr_t)workspace) & 15) == 0 && workspace_bytes >= (size_t)b.bytes, PKM_ERR_WORKSPACE,
+              "pkm_linear_ce_bwd: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)b.bytes);
+  return dtype == PKM_DTYPE_BF16
+             ? run_backward<bf16_t>((uint8_t*)kept, k, tokens, weight, w_stride, vocab, dim, grad_loss, reduction, dx, dweight,
+                                    (uint8_t*)workspace, b, (hipStream_t)stream)
+             : run_backward<f16_t>((uint8_t*)kept, k, tokens, weight, w_stride, vocab, dim, grad_loss, reduction, dx, dweight,
+                                   (uint8_t*)workspace, b, (hipStream_t)stream);
+}

@@ -1,0 +1,228 @@
+"""Cross entropy of a linear layer against the formulas in 64 bits."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from modelos_amd.linear_cross_entropy import linear_cross_entropy
+from oracle import linear_cross_entropy as oracle
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def _inputs(n, V, D, dtype, device, seed=0, lean=12.0, ignored=0.0):
+    """Normed hidden states that lean towards their label's row; labels in [0, V), -100 for the ignored."""
+    gen = torch.Generator().manual_seed(seed)
+    w = torch.randn((V, D), generator=gen) * 0.64 * D**-0.5
+    labels = torch.randint(0, V, (n,), generator=gen)
+    x = torch.randn((n, D), generator=gen)
+    x += lean * torch.rand((n, 1), generator=gen) * w[labels] / w[labels].square().sum(1, keepdim=True).clamp_min(1e-6)
+    labels[torch.rand(n, generator=gen) < ignored] = -100
+    return x.to(dtype).to(device).requires_grad_(), w.to(dtype).to(device).requires_grad_(), labels.to(device), gen
+
+
+def _near(got, want, bound, what):
+    err = (got.detach().cpu().double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {(err / bound.clamp_min(1e-300)).max():.2f} of its bound"
+
+
+def _both(x, w, labels, reduction, gen, size=1.0, **options):
+    loss = linear_cross_entropy(x, w, labels, reduction=reduction, **options)
+    grad = torch.full((), size) if reduction != "none" else size * torch.rand(labels.shape, generator=gen)
+    grads = torch.autograd.grad(loss, (x, w), grad.to(x.device))
+    return loss, grad, grads
+
+
+def _check(x, w, labels, reduction, gen, size=1.0, ignore_index=-100):
+    loss, grad, grads = _both(x, w, labels, reduction, gen, size, ignore_index=ignore_index)
+    assert loss.dtype == torch.float32 and loss.shape == (labels.shape if reduction == "none" else ())
+    assert all(g.shape == t.shape and g.dtype == t.dtype for g, t in zip(grads, (x, w)))
+    D = x.shape[-1]
+    values, bounds = oracle.loss_and_gradients(x.detach().cpu().reshape(-1, D), w.detach().cpu(), labels.cpu().reshape(-1),
+                                               ignore_index, reduction, grad.double().reshape(-1) if reduction == "none" else grad.double())
+    for name, got, want, bound in zip(("loss", "dx", "dW"), (loss, *grads), values, bounds):
+        _near(got.reshape(want.shape), want, bound, f"{name}, {reduction}")
+    return loss, grads
+
+
+SIZES = [
+    # tokens, vocab, dim
+    (1, 1, 8), (1, 2, 1), (3, 7, 5), (64, 300, 64), (255, 257, 72), (257, 130, 200), (256, 256, 256), (300, 1000, 333),
+    (31, 5000, 1000), (1000, 513, 264), (17, 20011, 128), (700, 40, 512),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("n,V,D", SIZES)
+def test_values_and_gradients(n, V, D, reduction, dtype, device):
+    x, w, labels, gen = _inputs(n, V, D, dtype, device, n + V, ignored=0.3 if n > 100 else 0.0)
+    _check(x, w, labels, reduction, gen)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_several_pieces(dtype, device):
+    """More vocabulary than a piece holds (64 tiles of 256), and a last piece that ends inside a tile."""
+    x, w, labels, gen = _inputs(70, 2 * 16384 + 16300, 64, dtype, device)
+    labels[:4] = torch.tensor([16383, 16384, 32768, 2 * 16384 + 16299])
+    _check(x, w, labels, "mean", gen)
+
+
+@pytest.mark.parametrize("dtype,size", [(BF16, 2.0**-40), (BF16, 2.0**20), (F16, 2.0**-10), (F16, 2.0**10)])
+def test_gradients_of_any_size(dtype, size, device):
+    """Softmax weights of 500 entries times 2^-10 lie below f16's smallest numbers: results in its range keep their precision."""
+    x, w, labels, gen = _inputs(200, 500, 64, dtype, device, lean=0.0)
+    _check(x, w, labels, "none", gen, size)
+
+
+def test_large_logits(device):
+    """A label far below the largest logit: the sum of the exponentials leaves float32 against the label's."""
+    x, w, labels, gen = _inputs(100, 700, 64, BF16, device, lean=0.0)
+    with torch.no_grad():
+        x[::3] *= 200
+        x[1::3] *= 20
+    loss, _ = _check(x, w, labels, "none", gen)
+    assert loss.max() > 200
+
+
+def test_rows_that_lean_all_one_way(device):
+    """weight with a common part, which d (whose sum over the vocabulary is 0) cancels."""
+    x, w, labels, gen = _inputs(200, 3000, 128, BF16, device)
+    with torch.no_grad():
+        w += w.std() * 2 * torch.randn(128, generator=gen).to(device)
+    _check(x, w, labels, "mean", gen)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_nothing_counts(reduction, device):
+    x, w, labels, gen = _inputs(70, 90, 40, BF16, device)
+    with torch.no_grad():
+        x.fill_(float("nan"))
+    for some in (torch.full_like(labels, -100), torch.full_like(labels, 90), labels - 1000):
+        loss, _, (dx, dw) = _both(x, w, some, reduction, gen)
+        assert not loss.any() and not dx.any() and not dw.any()
+    x = torch.zeros((0, 40), dtype=BF16, device=device, requires_grad=True)
+    loss, _, (dx, dw) = _both(x, w, labels[:0], reduction, gen)
+    assert not loss.any() and dx.shape == (0, 40) and not dw.any()
+
+
+def test_what_ignored_tokens_hold(device):
+    x, w, labels, gen = _inputs(300, 200, 64, BF16, device, ignored=0.4)
+    labels[7], labels[9] = 200, -1  # outside
+    with torch.no_grad():
+        away = (labels < 0) | (labels >= 200)
+        x[away] = torch.tensor([float("nan"), float("inf")], device=device, dtype=BF16)[torch.arange(int(away.sum())) % 2][:, None]
+    for ignore in (-100, 3):
+        _check(x.detach().requires_grad_(), w, labels.where(labels != -100, ignore), "none", gen, ignore_index=ignore)
+        labels = labels.where(labels != 3, 4)
+
+
+def test_a_token_that_is_not_a_number(device):
+    """Its loss and its gradient are NaN, and dW's rows; the other tokens' losses and gradients are not."""
+    x, w, labels, gen = _inputs(300, 200, 64, BF16, device)
+    with torch.no_grad():
+        x[11, 5] = float("nan")
+    loss, _, (dx, dw) = _both(x, w, labels, "none", gen)
+    assert loss.isnan().nonzero().tolist() == [[11]] and dw.isnan().all()
+    assert dx.isnan().any(1).nonzero().tolist() == [[11]]
+
+
+def test_strides(device):
+    """Rows apart, transposed, not on 16 bytes, one for all; labels of 32 bits and of strides; shapes of several axes."""
+    _, w0, labels, gen = _inputs(120, 150, 64, BF16, device)
+    wide = torch.randn((6, 20, 2, 64), generator=gen).to(BF16).to(device)
+    odd = torch.randn(120 * 64 + 1, generator=gen).to(BF16).to(device)
+    hidden = {"rows apart": wide[:, :, 1], "transposed": wide[:, :, 0].transpose(0, 1), "odd": odd[1:].view(6, 20, 64),
+              "one for all": wide[0, 0, 0].expand(6, 20, 64), "columns apart": wide.flatten()[: 6 * 20 * 128].view(6, 20, 128)[..., ::2]}
+    weights = {"rows apart": torch.cat([w0, w0], 1)[:, :64], "odd": torch.cat([w0.flatten()[:1], w0.flatten()])[1:].view(150, 64),
+               "transposed": w0.T.contiguous().T, "one for all": w0[:1].expand(150, 64), "whole": w0}
+    for name, x in hidden.items():
+        for kind, w in weights.items():
+            y = labels.view(*x.shape[:-1])
+            y = y.int() if kind == "odd" else torch.stack([y, y], -1)[..., 0]
+            _check(x.detach().requires_grad_(), w.detach().requires_grad_(), y, "mean", gen)
+    x = wide[0, 0, 0].detach().requires_grad_()  # a single token without an axis of its own
+    _check(x, w0, labels[0], "mean", gen)
+
+
+def test_one_gradient_alone(device):
+    x, w, labels, gen = _inputs(300, 700, 136, BF16, device)
+    loss, grad, (dx, dw) = _both(x, w, labels, "mean", gen)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, w.detach(), labels), x)[0], dx)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x.detach(), w, labels), w)[0], dw)
+    with torch.no_grad():
+        assert torch.equal(linear_cross_entropy(x, w, labels), loss)
+    loss = linear_cross_entropy(x, w, labels)  # twice through one graph, with the same bits
+    for _ in range(2):
+        again = torch.autograd.grad(loss, (x, w), retain_graph=True)
+        assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
+
+
+def test_against_differences(device):
+    """d loss / d w along one direction, by differences of losses with weights moved along it: exact in bf16, as the step is
+    a power of two of numbers with few digits."""
+    gen = torch.Generator().manual_seed(3)
+    w = (torch.randint(-8, 9, (50, 32), generator=gen) / 16).to(BF16).to(device).requires_grad_()
+    x = (torch.randint(-8, 9, (40, 32), generator=gen) / 8).to(BF16).to(device).requires_grad_()
+    labels = torch.randint(0, 50, (40,), generator=gen).to(device)
+    dx, dw = torch.autograd.grad(linear_cross_entropy(x, w, labels, reduction="sum"), (x, w))
+    h = 2.0**-6
+    for t, grad in ((w, dw), (x, dx)):
+        to = torch.randint(-1, 2, t.shape, generator=gen).to(BF16).to(device)
+        with torch.no_grad():
+            t0 = t.clone()
+            ends = []
+            for s in (h, -h):
+                t.copy_(t0 + s * to)
+                assert torch.equal(t.double(), t0.double() + s * to.double())
+                ends.append(linear_cross_entropy(x, w, labels, reduction="none").double().sum())
+            t.copy_(t0)
+        slope = (ends[0] - ends[1]).item() / (2 * h)
+        exact = (grad.double() * to.double()).sum().item()
+        # third derivative: h^2 / 6 of 40 tokens' softmax moments, logits' slopes up to 32 x 1: (32)^3; measured against
+        # the slopes' own spread |x to| <= 8 typically: 40 h^2 / 6 * 8^3; float32 losses of 4 each, 2^-22 / h; bf16 results
+        bound = 40 * h * h / 6 * 512 + 40 * 4 * 2.0**-22 / h + 2.0**-8 * (grad.double().abs() * to.double().abs()).sum().item()
+        assert abs(slope - exact) <= bound
+
+
+def test_captured(device):
+    """Forward and backward in a graph: hidden states, weights, labels (and how many count) change between replays."""
+    x, w, labels, gen = _inputs(300, 600, 72, BF16, device)
+    grad = torch.ones((), device=device)
+
+    def both():
+        loss = linear_cross_entropy(x, w, labels)
+        return loss.detach(), *torch.autograd.grad(loss, (x, w), grad)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    for k, ignored in enumerate((0.0, 0.9, 1.0, 0.3)):
+        x2, w2, labels2, _ = _inputs(300, 600, 72, BF16, device, seed=k, ignored=ignored)
+        with torch.no_grad():
+            x.copy_(x2)
+            w.copy_(w2)
+        labels.copy_(labels2)
+        grad.fill_(2.0**k)
+        graph.replay()
+        want = both()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+def test_other_stream(device):
+    x, w, labels, gen = _inputs(100, 600, 64, BF16, device)
+    want = _both(x, w, labels, "mean", gen)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = _both(x, w, labels, "mean", gen)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[2], want[2]))
