@@ -31,6 +31,18 @@ constexpr float kLog2e = 1.44269504f;
 
 enum Product { kLoss, kGrads, kDx, kDw };
 
+// What a result of dx's or dW's product is multiplied by.
+struct Scale {
+  const float* value;  // ce_weights'
+  const float* grad;   // or the gradient of the sum or the mean
+  const int32_t* count;
+  float lift;
+  int32_t mean;
+  __device__ __forceinline__ float operator()() const {
+    return grad ? *grad / ((mean ? (float)max(*count, 1) : 1.f) * lift) : *value;
+  }
+};
+
 struct CeArgs {
   const uint8_t* x;  // kept tokens [npad, dpad]
   const uint8_t* w;
@@ -40,11 +52,11 @@ struct CeArgs {
   const int32_t* label;  // [npad]
   const float* ref;      // [npad] the label's logit, the softmax sums' reference
   const float* lse;      // [npad]
-  const float* weight;   // [npad] of the tokens' gradients
+  const float* weight;   // [npad] of the tokens' gradients, or NULL: `lift` for all
   float2* sums;          // [2 * vocab tiles][npad] reference and sum of exponentials
-  float* dx;             // [splits][npad][dcols] float32
+  float* parts;          // [splits][rows][dcols] float32: dx's rows, or dW's where its sum is split
   uint8_t* dw;           // [vocab][dim]
-  const float* dw_scale;
+  Scale scale;
   int64_t vocab, v0;  // v0: the piece's first entry
   int32_t piece, dim, npad, dcols, splits, add, lg_m, lg_n;
 };
@@ -64,7 +76,8 @@ __device__ __forceinline__ void load16(const uint8_t* base, lds_u8* to, uint32_t
 // The operands' tiles: how a wave loads its four KB of one and reads a matrix operand from it.
 // L = wave + 8 n is the KB that load n fills.
 
-// [256 rows][64 numbers] of a matrix whose rows hold the summed index: 128 bytes a row, chunks permuted by the row. Rows
+// [256 rows][64 numbers] of a matrix whose rows hold the summed index: 128 bytes a row, chunks permuted by row / 2, so that
+// 16 rows' chunks fall on all 64 banks. Rows
 // behind the last repeat it; chunks behind the row's end repeat the last one, against zeros of the other operand.
 struct RowsTile {
   const uint8_t* base;
@@ -73,18 +86,17 @@ struct RowsTile {
   __device__ __forceinline__ void at(const uint8_t* p, int64_t stride, int64_t row0, int64_t rows, int wave, int lane) {
     base = p + row0 * stride;
     const int64_t last = rows - 1 - row0;
-    chunk = (lane & 7) ^ (lane >> 3);
+    chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
 #pragma unroll
     for (int n = 0; n < 4; ++n) off[n] = (uint32_t)(min((int64_t)(8 * wave + 64 * n + (lane >> 3)), last) * stride);
   }
-  __device__ __forceinline__ void load(lds_u8* to, int step, int chunks, int wave) const {
+  __device__ __forceinline__ void load(lds_u8* to, int n, int step, int chunks, int wave) const {
     const uint32_t c = (uint32_t)min(step * 8 + chunk, chunks - 1) << 4;
-#pragma unroll
-    for (int n = 0; n < 4; ++n) load16(base, to + (wave + 8 * n) * 1024, off[n] + c);
+    load16(base, to + (wave + 8 * n) * 1024, off[n] + c);
   }
 };
 __device__ __forceinline__ uint32_t rows_lane(int lane) {
-  return (lane & 31) * 128 + (((lane >> 5) ^ (lane & 7)) << 4);
+  return (lane & 31) * 128 + (((lane >> 5) ^ ((lane >> 1) & 7)) << 4);
 }
 __device__ __forceinline__ frag_t rows_frag(uint32_t at, int t, int s) {
   return *(const lds_u32x4*)(uintptr_t)((at ^ (uint32_t)(s << 5)) + t * 4096);
@@ -98,12 +110,10 @@ struct ColsTile {
     base = p;
     col = (uint32_t)min(col0 / 8 + ((lane & 31) ^ perm16(2 * wave + (lane >> 5))), chunks - 1) << 4;
   }
-  __device__ __forceinline__ void load(lds_u8* to, int step, int64_t stride, int64_t rows, int wave, int lane) const {
+  __device__ __forceinline__ void load(lds_u8* to, int n, int step, int64_t stride, int64_t rows, int wave, int lane) const {
     const uint8_t* const b = base + (int64_t)step * kDepth * stride;
     const int last = (int)min(rows - 1 - (int64_t)step * kDepth, (int64_t)kDepth);
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-      load16(b, to + (wave + 8 * n) * 1024, (uint32_t)min(2 * wave + 16 * n + (lane >> 5), last) * (uint32_t)stride + col);
+    load16(b, to + (wave + 8 * n) * 1024, (uint32_t)min(2 * wave + 16 * n + (lane >> 5), last) * (uint32_t)stride + col);
   }
 };
 __device__ __forceinline__ uint32_t cols_lane(int lane) {
@@ -121,38 +131,35 @@ __device__ __forceinline__ frag_t cols_frag(uint32_t at, int t, int s) {
   return two_tr((at ^ (uint32_t)(t << 6)) + s * 8192, (at ^ (uint32_t)((t << 6) | 32)) + s * 8192 + 4096);
 }
 
-// Where a block of d holds lane (h, token)'s 16 bytes: the halves 64 bytes apart in a 128-byte line, for the transposing reads.
-__device__ __forceinline__ int block_lane(int h, int t) { return 32 * h + (t ^ (h << 2)); }
+// Where a block of d, of entries 16 g .. 16 g + 15, holds lane (h, token)'s 16 bytes: the halves 64 bytes apart in a
+// 128-byte line and neighbouring blocks 128 bytes in 256, so that a transposing read falls on all 64 banks.
+__device__ __forceinline__ constexpr int block_lane(int g, int h, int t) { return 32 * h + (t ^ (h << 2) ^ ((g & 1) << 3)); }
 
 // d as dx's operand: 256 tokens, 64 vocabulary entries. Block (entries n, tokens wave).
-__device__ __forceinline__ void load_tokens(const uint8_t* d, lds_u8* to, int step, int tile, int npad, int wave, int lane) {
+__device__ __forceinline__ void load_tokens(const uint8_t* d, lds_u8* to, int n, int step, int tile, int npad, int wave, int lane) {
   const uint32_t row = (uint32_t)(npad / 32) * 1024;
-  const uint8_t* const b = d + (int64_t)step * 4 * row + (int64_t)tile * 8192;
-#pragma unroll
-  for (int n = 0; n < 4; ++n) load16(b, to + (wave + 8 * n) * 1024, n * row + wave * 1024 + lane * 16);
+  const uint8_t* const b = d + ((int64_t)step * 4 + n) * row + (int64_t)tile * 8192 + wave * 1024;
+  load16(b, to + (wave + 8 * n) * 1024, lane * 16);
 }
-__device__ __forceinline__ uint32_t tokens_lane(int lane) { return block_lane(lane >> 5, lane & 31) * 16; }
+__device__ __forceinline__ uint32_t tokens_lane(int lane) { return block_lane(0, lane >> 5, lane & 31) * 16; }
 __device__ __forceinline__ frag_t tokens_frag(uint32_t at, int t, int s) {
-  return *(const lds_u32x4*)(uintptr_t)(at + s * 8192 + t * 1024);
+  return *(const lds_u32x4*)(uintptr_t)((at ^ (uint32_t)((s & 1) << 7)) + s * 8192 + t * 1024);
 }
 
 // d as dW's operand: 256 vocabulary entries, 64 tokens. Block (entries L / 2, tokens L % 2).
-__device__ __forceinline__ void load_entries(const uint8_t* d, lds_u8* to, int step, int tile, int npad, int wave, int lane) {
+__device__ __forceinline__ void load_entries(const uint8_t* d, lds_u8* to, int n, int step, int tile, int npad, int wave, int lane) {
+  const int L = wave + 8 * n;
   const uint32_t row = (uint32_t)(npad / 32) * 1024;
-  const uint8_t* const b = d + (int64_t)tile * 16 * row + (int64_t)step * 2048;
-#pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    const int L = wave + 8 * n;
-    load16(b, to + L * 1024, (uint32_t)(L >> 1) * row + (L & 1) * 1024 + lane * 16);
-  }
+  const uint8_t* const b = d + ((int64_t)tile * 16 + (L >> 1)) * row + (int64_t)step * 2048 + (L & 1) * 1024;
+  load16(b, to + L * 1024, lane * 16);
 }
 __device__ __forceinline__ uint32_t entries_lane(int lane) {
   const int l = lane & 15, h = lane >> 5, g = (lane >> 4) & 1, p = l & 3;
-  return g * 2048 + block_lane(p & 1, 4 * h + (l >> 2)) * 16 + 8 * (p >> 1);
+  return g * 2048 + block_lane(g, p & 1, 4 * h + (l >> 2)) * 16 + 8 * (p >> 1);
 }
 __device__ __forceinline__ frag_t entries_frag(uint32_t at, int t, int s) {
-  const uint32_t p = at + t * 4096 + (s >> 1) * 1024 + (s & 1) * 256;
-  return two_tr(p, p + 128);
+  const int to = t * 4096 + (s >> 1) * 1024 + (s & 1) * 256;
+  return two_tr(at + to, (at ^ 128) + to);
 }
 
 // Results of a product and their order: blocks of 2^lg_m x 2^lg_n tiles, one XCD's workgroups side by side in it, so that
@@ -263,7 +270,7 @@ __device__ __forceinline__ void end_grads(const CeArgs& a, acc_t& acc, const Res
   for (int u = 0; u < 2; ++u) {
     const int j = r.n * kTile + (wave & 3) * 64 + 32 * u + (lane & 31);
     const bool kept = j < count;
-    const float c = kept ? -a.lse[j] * kLog2e : -INFINITY, weight = kept ? a.weight[j] : 0.f;
+    const float c = kept ? -a.lse[j] * kLog2e : -INFINITY, weight = !kept ? 0.f : a.weight ? a.weight[j] : a.scale.lift;
     uint8_t* const to = a.d + (int64_t)(v0 / 16) * row + (int64_t)(j >> 5) * 1024;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -273,7 +280,7 @@ __device__ __forceinline__ void end_grads(const CeArgs& a, acc_t& acc, const Res
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = exp2_raw(__builtin_fmaf(acc[t][u][8 * s + e], kLog2e, c)) * weight;
         const u32x4_t x = {pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7])};
-        *(u32x4_t*)(to + (2 * t + s) * row + block_lane(h, lane & 31) * 16) = x;
+        *(u32x4_t*)(to + (2 * t + s) * row + block_lane(s, h, lane & 31) * 16) = x;
       }
       batch();
     }
@@ -283,16 +290,16 @@ __device__ __forceinline__ void end_grads(const CeArgs& a, acc_t& acc, const Res
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (y >= 0 && y < 128 && h == 0) {
         const float x = (exp2_raw(__builtin_fmaf(a.ref[j], kLog2e, c)) - 1.f) * weight;
-        *(uint16_t*)(to + (y >> 4) * row + block_lane((y >> 2) & 1, lane) * 16 + ((y >> 3) & 1) * 8 + (y & 3) * 2) =
+        *(uint16_t*)(to + (y >> 4) * row + block_lane((y >> 4) & 1, (y >> 2) & 1, lane) * 16 + ((y >> 3) & 1) * 8 + (y & 3) * 2) =
             (uint16_t)pack2<T>(x, x);
       }
     }
   }
 }
 
-__device__ __forceinline__ void end_dx(const CeArgs& a, acc_t& acc, const Result& r, int wave, int lane) {
+__device__ __forceinline__ void end_parts(const CeArgs& a, acc_t& acc, const Result& r, int64_t rows, int wave, int lane) {
   const int h = lane >> 5;
-  float* const to = a.dx + ((int64_t)r.split * a.npad + r.m * kTile + (wave >> 2) * 128 + 4 * h) * a.dcols + r.n * kTile +
+  float* const to = a.parts + (r.split * rows + r.m * kTile + (wave >> 2) * 128 + 4 * h) * a.dcols + r.n * kTile +
                     (wave & 3) * 64 + (lane & 31);
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -314,7 +321,7 @@ __device__ __forceinline__ void end_dx(const CeArgs& a, acc_t& acc, const Result
 template <typename T>
 __device__ __forceinline__ void end_dw(const CeArgs& a, acc_t& acc, const Result& r, int wave, int lane) {
   const int h = lane >> 5, odd = lane & 1;
-  const float f = *a.dw_scale;
+  const float f = a.scale();
   // lanes 2 k and 2 k + 1 swap, so that each has two neighbours of one row
   const int64_t v0 = a.v0 + r.m * kTile + (wave >> 2) * 128 + 4 * h + odd;
   const int d0 = r.n * kTile + (wave & 3) * 64 + (lane & 31) - odd;
@@ -359,7 +366,15 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
             dim_tiles = a.dcols / kTile;
   const Order order = P == kLoss || P == kGrads ? Order(entry_tiles, token_tiles, dpad / kDepth, 1, a.lg_m, a.lg_n)
                       : P == kDx ? Order(token_tiles, dim_tiles, (int)((entries + kDepth - 1) / kDepth), a.splits, a.lg_m, a.lg_n)
-                                 : Order(entry_tiles, dim_tiles, (n + kDepth - 1) / kDepth, 1, a.lg_m, a.lg_n);
+                                 : Order(entry_tiles, dim_tiles, (n + kDepth - 1) / kDepth, a.splits, a.lg_m, a.lg_n);
+  if constexpr (P == kDw) {
+    if (n == 0 && a.splits == 1) {  // no token counts: zeros
+      const int64_t first = a.v0 * a.dim, all = entries * a.dim;
+      for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < all; i += (int64_t)gridDim.x * kThreads)
+        ((uint16_t*)a.dw)[first + i] = 0;
+      return;
+    }
+  }
   const uint8_t* const w = a.w + a.v0 * a.w_stride;
 
   Result run, ahead;  // the result in work, and the one whose tiles are loaded
@@ -375,35 +390,43 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
       cb.at(a.x, ahead.n * kTile, dpad / 8, wave, lane);
     }
   };
-  const auto load = [&](int stage, int step) {
-    lds_u8* const to = lds + stage * kStage;
+  // a wave's eight loads of a step, two steps ahead of the products
+  int load_step;
+  const auto load = [&](int stage, int part) {
+    lds_u8* const to = lds + stage * kStage + (part >> 2) * kHalf;
+    const int q = part & 3;
     if constexpr (P == kLoss || P == kGrads) {
-      ra.load(to, step, chunks, wave);
-      rb.load(to + kHalf, step, dpad / 8, wave);
+      if (part < 4)
+        ra.load(to, q, load_step, chunks, wave);
+      else
+        rb.load(to, q, load_step, dpad / 8, wave);
     } else if constexpr (P == kDx) {
-      load_tokens(a.d, to, step, ahead.m, a.npad, wave, lane);
-      cb.load(to + kHalf, step, a.w_stride, entries, wave, lane);
+      if (part < 4)
+        load_tokens(a.d, to, q, load_step, ahead.m, a.npad, wave, lane);
+      else
+        cb.load(to, q, load_step, a.w_stride, entries, wave, lane);
     } else {
-      load_entries(a.d, to, step, ahead.m, a.npad, wave, lane);
-      cb.load(to + kHalf, step, a.x_stride, n, wave, lane);
+      if (part < 4)
+        load_entries(a.d, to, q, load_step, ahead.m, a.npad, wave, lane);
+      else
+        cb.load(to, q, load_step, a.x_stride, n, wave, lane);
     }
   };
-  // the loads run two steps ahead
-  int load_step;
-  bool more = ahead.next(order, true);
-  if (!more) return;
+  if (!ahead.next(order, true)) return;
   run = ahead;
   aim();
   load_step = ahead.k0;
-  const auto load_next = [&](int stage) {
-    if (!more) return;
-    load(stage, load_step);
-    if (++load_step == ahead.k1) {
-      more = ahead.next(order, false);
-      if (more) {
-        aim();
-        load_step = ahead.k0;
-      }
+  // on to the next step; behind the last one it is loaded again, which nobody reads, so that the loads need no branches
+  const auto loaded = [&]() {
+    if (load_step + 1 < ahead.k1) {
+      ++load_step;
+      return;
+    }
+    Result after = ahead;
+    if (after.next(order, false)) {
+      ahead = after;
+      aim();
+      load_step = ahead.k0;
     }
   };
 
@@ -425,30 +448,37 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
       fa[set][t] = P == kLoss || P == kGrads ? rows_frag(pa, t, s) : P == kDx ? tokens_frag(pa, t, s) : entries_frag(pa, t, s);
   };
   acc_t acc = {};
-  const auto multiply = [&](int set) {
+  // with_each(t): between the products
+  const auto multiply = [&](int set, auto with_each) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) acc[t][u] = mfma32<T>(fa[set][t], fb[set][u], acc[t][u]);
+      keep_order();
+      with_each(t);
+    }
   };
+  const auto nothing = [](int) {};
 
-  load_next(0);
-  const bool two = more;
-  load_next(1);
-  if (two)
-    tile_wait<8>();
-  else
-    tile_wait<0>();
+#pragma unroll
+  for (int part = 0; part < 8; ++part) load(0, part);
+  loaded();
+#pragma unroll
+  for (int part = 0; part < 4; ++part) load(1, part);
+  tile_wait<4>();
   __syncthreads();
   read(0, 0, 0);
   for (int stage = 0, step = run.k0;; stage ^= 1) {
-#pragma unroll
-    for (int s = 0; s < 3; ++s) {
-      read((s + 1) & 1, stage, s + 1);
-      keep_order();
-      multiply(s & 1);
-      keep_order();
-    }
+    read(1, stage, 1);
+    keep_order();
+    multiply(0, [&](int t) { load(stage ^ 1, 4 + t); });
+    loaded();
+    read(0, stage, 2);
+    keep_order();
+    multiply(1, nothing);
+    read(1, stage, 3);
+    keep_order();
+    multiply(0, nothing);
     // every wave has read this stage and loaded the next
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
@@ -458,17 +488,23 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
     const bool ends = ++step == run.k1;
     Result after = run;
     const bool last = ends && !after.next(order, false);
-    load_next(stage);
     if (!last) read(0, stage ^ 1, 0);
     keep_order();
-    multiply(1);
-    keep_order();
+    multiply(1, [&](int t) { load(stage, t); });
     if (ends) {
       if constexpr (P == kLoss) end_loss(a, acc, run, wave, lane);
       if constexpr (P == kGrads) end_grads<T>(a, acc, run, n, wave, lane);
-      if constexpr (P == kDx) end_dx(a, acc, run, wave, lane);
-      if constexpr (P == kDw) end_dw<T>(a, acc, run, wave, lane);
-      if (last) break;
+      if constexpr (P == kDx) end_parts(a, acc, run, a.npad, wave, lane);
+      if constexpr (P == kDw) {
+        if (a.splits > 1)
+          end_parts(a, acc, run, a.piece, wave, lane);
+        else
+          end_dw<T>(a, acc, run, wave, lane);
+      }
+      if (last) {
+        tile_wait<0>();  // no load may outlive the workgroup's LDS
+        break;
+      }
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -482,13 +518,13 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
 // ---------------------------------------------------------------------------
 // Around the products
 // ---------------------------------------------------------------------------
-constexpr int kPrepareRows = 64;  // tokens of a workgroup of ce_prepare
+constexpr int kPrepareRows = 16;  // tokens of a workgroup of ce_prepare, a wave each
 constexpr int kJoinTokens = 32, kJoinSlices = 32;
 
 struct Header {
   int32_t count;   // kept tokens
-  float dw_scale;  // of the results of dW's product
-  float dx_scale;
+  uint32_t ended;  // workgroups of ce_join that are done
+  float scale;     // that undoes the weights of d in the results
 };
 
 template <typename L>
@@ -497,79 +533,93 @@ __device__ __forceinline__ int label_of(const void* labels, int64_t i, int64_t i
   return y == ignore || y < 0 || y >= vocab ? -1 : (int)y;
 }
 
-// The kept tokens side by side: rows, labels, places, and the label's logit as the sums' reference. A workgroup counts
-// the kept tokens before its 64 itself.
+// The kept tokens side by side: rows, labels, places, and the label's logit. A workgroup counts the kept tokens before its 16
+// itself: 16384 tokens' labels are read 512 times in all, 67 MB out of the L2, and no launch is needed to count.
 template <typename T, typename L>
-__global__ __launch_bounds__(256) void ce_prepare(const T* __restrict__ x, int64_t x_stride, int64_t tokens,
-                                                  const T* __restrict__ w, int64_t w_stride, int64_t vocab, int dim, int dpad,
-                                                  int wide, const void* labels, int64_t ignore, Header* head, int32_t* place,
-                                                  int32_t* label, float* ref, T* __restrict__ kept, int npad) {
-  __shared__ int32_t before_s[4], places[kPrepareRows], own_s;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int64_t first = (int64_t)blockIdx.x * kPrepareRows;
+__global__ __launch_bounds__(1024) void ce_prepare(const T* __restrict__ x, int64_t x_stride, int64_t tokens,
+                                                   const T* __restrict__ w, int64_t w_stride, int64_t vocab, int dim, int dpad,
+                                                   int wide, const void* labels, int64_t ignore, Header* head, int32_t* place,
+                                                   int32_t* token, int32_t* label, float* ref, T* __restrict__ kept, int npad,
+                                                   float* losses) {
+  __shared__ int32_t before_s[16], own_s[16];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int64_t first = (int64_t)blockIdx.x * kPrepareRows, i = first + wave;
+  const int y = i < tokens ? label_of<L>(labels, i, ignore, vocab) : -1;
   int32_t before = 0;
-  for (int64_t i = tid; i < first; i += 256) before += label_of<L>(labels, i, ignore, vocab) >= 0;
+  for (int64_t k = tid; k < first; k += 1024) before += label_of<L>(labels, k, ignore, vocab) >= 0;
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) before += __shfl_xor(before, s);
-  if (lane == 0) before_s[wave] = before;
-  __syncthreads();
-  before = before_s[0] + before_s[1] + before_s[2] + before_s[3];
-  if (wave == 0) {
-    const int64_t i = first + lane;
-    const int y = i < tokens ? label_of<L>(labels, i, ignore, vocab) : -1;
-    const uint64_t live = __ballot(y >= 0);
-    const int at = before + __popcll(live & ((1ull << lane) - 1));
-    places[lane] = y >= 0 ? at : -1;
-    if (y >= 0) label[at] = y;
-    if (i < tokens) place[i] = places[lane];
-    if (lane == 0) own_s = __popcll(live);
+  if (lane == 0) {
+    before_s[wave] = before;
+    own_s[wave] = y >= 0;
   }
   __syncthreads();
+  int at = 0, own = 0;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    at += before_s[k];
+    own += own_s[k];
+  }
+  const int count = at + own;  // with this workgroup's
+#pragma unroll
+  for (int k = 0; k < 16; ++k) at += k < wave ? own_s[k] : 0;
   if (blockIdx.x == gridDim.x - 1) {
-    const int count = before + own_s;
-    if (tid == 0) head->count = count;
-    for (int j = count + tid; j < npad; j += 256) {
+    if (tid == 0) {
+      head->count = count;
+      head->ended = 0;
+    }
+    for (int j = count + tid; j < npad; j += 1024) {
       label[j] = -1;
       ref[j] = 0.f;
     }
   }
-  for (int k = wave; k < kPrepareRows; k += 4) {
-    const int at = places[k];
-    if (at < 0) continue;
-    const T* const row = x + (first + k) * x_stride;
-    T* const to = kept + (int64_t)at * dpad;
-    const T* const wy = w + (int64_t)label_of<L>(labels, first + k, ignore, vocab) * w_stride;
-    float dot = 0.f;
-    if (wide) {
-      for (int c = lane; c < dpad / 8; c += 64) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (c < dim / 8) {
-          v = ld16(row + 8 * c);
-          dot = vec_dot<T>(v, ld16(wy + 8 * c), dot);
-        }
-        st16(to + 8 * c, v);
-      }
-    } else {
-      for (int c = lane; c < dpad; c += 64) {
-        uint16_t v = 0;
-        if (c < dim) {
-          v = ((const uint16_t*)row)[c];
-          dot += unpack1<T>(v) * unpack1<T>(((const uint16_t*)wy)[c]);
-        }
-        ((uint16_t*)to)[c] = v;
-      }
+  if (i >= tokens) return;
+  if (lane == 0) {
+    place[i] = y >= 0 ? at : -1;
+    if (y >= 0) {
+      token[at] = (int)i;
+      label[at] = y;
+    } else if (losses) {
+      losses[i] = 0.f;
     }
-    dot = group_sum<64>(dot);
-    if (lane == 0) ref[at] = dot;
   }
+  if (y < 0) return;
+  const T* const row = x + i * x_stride;
+  T* const to = kept + (int64_t)at * dpad;
+  const T* const wy = w + (int64_t)y * w_stride;
+  float dot = 0.f;
+  if (wide) {
+    for (int c = lane; c < dpad / 8; c += 64) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (c < dim / 8) {
+        v = ld16(row + 8 * c);
+        dot = vec_dot<T>(v, ld16(wy + 8 * c), dot);
+      }
+      st16(to + 8 * c, v);
+    }
+  } else {
+    for (int c = lane; c < dpad; c += 64) {
+      uint16_t v = 0;
+      if (c < dim) {
+        v = ((const uint16_t*)row)[c];
+        dot += unpack1<T>(v) * unpack1<T>(((const uint16_t*)wy)[c]);
+      }
+      ((uint16_t*)to)[c] = v;
+    }
+  }
+  dot = group_sum<64>(dot);
+  if (lane == 0) ref[at] = dot;
 }
 
-// lse and loss of 32 tokens from the tiles' sums.
-__global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(const Header* head, const float2* __restrict__ sums, int parts,
+// lse and loss of 32 tokens from the tiles' sums. losses: one for each token. mean: else the workgroup that ends last adds
+// all workgroups' losses, in order.
+__global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(Header* head, const float2* __restrict__ sums, int parts,
                                                                     int npad, const float* __restrict__ ref,
-                                                                    float* __restrict__ lse, float* __restrict__ losses,
-                                                                    float* __restrict__ block_sums) {
+                                                                    const int32_t* __restrict__ token, float* __restrict__ lse,
+                                                                    float* losses, float* block_sums, float* total, int mean) {
   __shared__ float2 s[kJoinSlices][kJoinTokens];
+  __shared__ float sum_s[kJoinSlices / 2];
+  __shared__ bool ends_s;
   const int t = threadIdx.x % kJoinTokens, slice = threadIdx.x / kJoinTokens;
   const int j = blockIdx.x * kJoinTokens + t, count = head->count;
   float m = -INFINITY, sum = 0.f;
@@ -582,99 +632,97 @@ __global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(const Header
     }
   };
   if (j < count) {
-#pragma unroll 4
-    for (int p = slice; p < parts; p += kJoinSlices) {
-      const float2 v = sums[(int64_t)p * npad + j];
-      add(v.x, v.y);
+    constexpr int FLIGHT = 16;
+    for (int p = slice; p < parts; p += kJoinSlices * FLIGHT) {
+      float2 v[FLIGHT];
+#pragma unroll
+      for (int k = 0; k < FLIGHT; ++k) v[k] = sums[(int64_t)min(p + k * kJoinSlices, parts - 1) * npad + j];
+#pragma unroll
+      for (int k = 0; k < FLIGHT; ++k)
+        if (p + k * kJoinSlices < parts) add(v[k].x, v[k].y);
     }
   }
   s[slice][t] = make_float2(m, sum);
   __syncthreads();
-  if (slice != 0) return;
-  float loss = 0.f;
-  if (j < count) {
-    for (int k = 1; k < kJoinSlices; ++k)
-      if (s[k][t].y != 0.f) add(s[k][t].x, s[k][t].y);  // NaN counts as something
-    const float log_sum = __builtin_amdgcn_logf(sum) * 0.693147180559945f;
-    lse[j] = m + log_sum;
-    loss = log_sum + (m - ref[j]);
-    losses[j] = loss;
-  }
+  if (slice == 0) {
+    float loss = 0.f;
+    if (j < count) {
+      for (int k = 1; k < kJoinSlices; ++k)
+        if (s[k][t].y != 0.f) add(s[k][t].x, s[k][t].y);  // NaN counts as something
+      const float log_sum = __builtin_amdgcn_logf(sum) * 0.693147180559945f;
+      lse[j] = m + log_sum;
+      loss = log_sum + (m - ref[j]);
+      if (losses) losses[token[j]] = loss;
+    }
 #pragma unroll
-  for (int k = 1; k < kJoinTokens; k <<= 1) loss += __shfl_xor(loss, k);
-  if (t == 0) block_sums[blockIdx.x] = loss;
-}
-
-// The mean or sum of the losses: one workgroup, in a fixed order.
-__global__ __launch_bounds__(1024) void ce_reduce(const Header* head, const float* __restrict__ block_sums, int blocks, int mean,
-                                                  float* out) {
-  __shared__ float s[16];
-  float sum = 0.f;
-  for (int i = threadIdx.x; i < blocks; i += 1024) sum += block_sums[i];
+    for (int k = 1; k < kJoinTokens; k <<= 1) loss += __shfl_xor(loss, k);
+    if (t == 0 && !losses) {
+      __hip_atomic_store(&block_sums[blockIdx.x], loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      ends_s = __hip_atomic_fetch_add(&head->ended, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
+  }
+  if (losses) return;
+  __syncthreads();
+  if (!ends_s) return;
+  sum = 0.f;
+  for (int k = threadIdx.x; k < (int)gridDim.x; k += kJoinTokens * kJoinSlices)
+    sum += __hip_atomic_load(&block_sums[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   sum = group_sum<64>(sum);
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = sum;
+  if ((threadIdx.x & 63) == 0) sum_s[threadIdx.x >> 6] = sum;
   __syncthreads();
   if (threadIdx.x != 0) return;
   sum = 0.f;
-  for (int k = 0; k < 16; ++k) sum += s[k];
-  out[0] = mean ? sum / (float)max(head->count, 1) : sum;
-}
-
-__global__ __launch_bounds__(256) void ce_scatter(const int32_t* __restrict__ place, const float* __restrict__ losses,
-                                                  int64_t tokens, float* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < tokens) out[i] = place[i] < 0 ? 0.f : losses[place[i]];
+  for (int k = 0; k < kJoinSlices / 2; ++k) sum += sum_s[k];
+  *total = mean ? sum / (float)max(count, 1) : sum;
 }
 
 // The tokens' gradients as weights of d: g_j over a power of two that the largest is just below, times `lift` (2^14 in f16,
-// whose smallest numbers softmax weights reach; 1 in bf16). The two scales undo it in the results. One gradient for
-// all tokens is a scale alone.
-__global__ __launch_bounds__(1024) void ce_weights(Header* head, const float* __restrict__ grad, int reduction,
-                                                   const int32_t* __restrict__ place, int64_t tokens, float lift,
-                                                   float* __restrict__ weight, int npad) {
+// whose smallest numbers softmax weights reach; 1 in bf16); the results' scale undoes it. One gradient for all tokens is
+// a scale alone: nothing is weighted then, and this does not run.
+__global__ __launch_bounds__(1024) void ce_weights(Header* head, const float* __restrict__ grad, const int32_t* __restrict__ place,
+                                                   int64_t tokens, float lift, float* __restrict__ weight) {
   __shared__ float s[16];
   const int tid = threadIdx.x;
-  float unit = 1.f;
-  if (reduction == 0) {
-    float top = 0.f;
-    for (int64_t i = tid; i < tokens; i += 1024)
-      if (place[i] >= 0) top = fmaxf(top, fabsf(grad[i]));
+  float top = 0.f;
+  for (int64_t i = tid; i < tokens; i += 1024)
+    if (place[i] >= 0) top = fmaxf(top, fabsf(grad[i]));
 #pragma unroll
-    for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-    if ((tid & 63) == 0) s[tid >> 6] = top;
-    __syncthreads();
-    for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k]);
-    const int e = top > 0.f ? min(max(__builtin_amdgcn_frexp_expf(top), -100), 100) : 0;
-    unit = ldexpf(1.f, e);
-    for (int64_t i = tid; i < tokens; i += 1024)
-      if (place[i] >= 0) weight[place[i]] = grad[i] / unit * lift;
-    for (int j = head->count + tid; j < npad; j += 1024) weight[j] = 0.f;
-  } else {
-    for (int j = tid; j < npad; j += 1024) weight[j] = j < head->count ? lift : 0.f;
-    unit = reduction == 1 ? grad[0] / (float)max(head->count, 1) : grad[0];
-  }
-  if (tid == 0) head->dw_scale = head->dx_scale = unit / lift;
+  for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+  if ((tid & 63) == 0) s[tid >> 6] = top;
+  __syncthreads();
+  for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k]);
+  const int e = top > 0.f ? min(max(__builtin_amdgcn_frexp_expf(top), -100), 100) : 0;
+  const float unit = ldexpf(1.f, e);
+  for (int64_t i = tid; i < tokens; i += 1024)
+    if (place[i] >= 0) weight[place[i]] = grad[i] / unit * lift;
+  if (tid == 0) head->scale = unit / lift;
 }
 
-// dx of every token: the splits' sums in order, rounded; zeros for tokens that are not kept. A workgroup a token at a time.
+// Rows of results: the splits' sums in order, scaled and rounded. dx: row i from row place[i], zeros if that is negative.
+// dW (place NULL): row i from row i; few kept tokens leave some splits without a step, which wrote nothing. A workgroup a
+// row at a time.
 template <typename T>
-__global__ __launch_bounds__(256) void ce_dx(const Header* head, const int32_t* __restrict__ place, int64_t tokens,
-                                             const float* __restrict__ parts, int splits, int npad, int dcols, int dim,
-                                             T* __restrict__ dx) {
-  const float f = head->dx_scale;
-  for (int64_t i = blockIdx.x; i < tokens; i += gridDim.x) {
-    const int j = place[i];
+__global__ __launch_bounds__(256) void ce_rows(const Scale scale, const int32_t* __restrict__ place, int64_t rows,
+                                               const float* __restrict__ parts, int splits, int64_t rows_pad, int dcols, int dim,
+                                               T* __restrict__ out) {
+  const float f = scale();
+  const int64_t steps = place ? splits : (*scale.count + kDepth - 1) / kDepth;
+  for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
+    const int64_t j = place ? place[i] : i;
     for (int d = threadIdx.x * 4; d < dim; d += 1024) {
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (j >= 0)
+      if (j >= 0) {
+#pragma unroll 8
         for (int s = 0; s < splits; ++s) {
-          const float4 v = *(const float4*)(parts + ((int64_t)s * npad + j) * dcols + d);
+          if (steps * s / splits == steps * (s + 1) / splits) continue;
+          const float4 v = *(const float4*)(parts + (s * rows_pad + j) * dcols + d);
           sum.x += v.x;
           sum.y += v.y;
           sum.z += v.z;
           sum.w += v.w;
         }
-      uint16_t* const to = (uint16_t*)(dx + i * dim + d);
+      }
+      uint16_t* const to = (uint16_t*)(out + i * dim + d);
       const uint32_t a = j < 0 ? 0u : pack2<T>(sum.x * f, sum.y * f), b = j < 0 ? 0u : pack2<T>(sum.z * f, sum.w * f);
       if ((dim & 3) == 0) {
         *(uint2*)to = make_uint2(a, b);
@@ -688,12 +736,6 @@ __global__ __launch_bounds__(256) void ce_dx(const Header* head, const int32_t* 
   }
 }
 
-// dW without any kept token
-__global__ __launch_bounds__(256) void ce_no_dw(const Header* head, uint16_t* __restrict__ dw, int64_t n) {
-  if (head->count != 0) return;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) dw[i] = 0;
-}
-
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
@@ -701,14 +743,15 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // What the forward leaves for the backward, in one buffer.
 struct Kept {
-  int64_t npad, dpad, place, label, ref, lse, x, bytes;
+  int64_t npad, dpad, place, token, label, ref, lse, x, bytes;
 };
 bool plan_kept(int64_t tokens, int64_t dim, Kept* k) {
   if (tokens < 0 || dim < 1 || tokens >= (1ll << 22) || dim > 65536) return false;
   k->npad = up(tokens < 1 ? 1 : tokens, kTile);
   k->dpad = up(dim, kDepth);
   k->place = 256;
-  k->label = k->place + k->npad * 4;
+  k->token = k->place + k->npad * 4;
+  k->label = k->token + k->npad * 4;
   k->ref = k->label + k->npad * 4;
   k->lse = k->ref + k->npad * 4;
   k->x = k->lse + k->npad * 4;
@@ -717,20 +760,26 @@ bool plan_kept(int64_t tokens, int64_t dim, Kept* k) {
 }
 
 struct Forward {
-  int64_t sums, losses, block_sums, bytes;
+  int64_t sums, block_sums, bytes;
 };
 Forward plan_forward(const Kept& k, int64_t vocab) {
   Forward f;
   f.sums = 0;
-  f.losses = f.sums + up(vocab, kTile) / 128 * k.npad * 8;
-  f.block_sums = f.losses + k.npad * 4;
+  f.block_sums = f.sums + up(vocab, kTile) / 128 * k.npad * 8;
   f.bytes = f.block_sums + k.npad / kJoinTokens * 4;
   return f;
 }
 
 struct Backward {
-  int64_t piece, splits, dcols, weight, d, dx, bytes;
+  int64_t piece, dcols, dx_splits, dw_splits, weight, d, dx, dw, bytes;
 };
+// Splits of a product's sum over `steps`, so that few results fill the CUs: 8 steps at least each, which outweigh the partial
+// results' way through memory.
+int64_t splits_of(int64_t results, int64_t steps) {
+  int64_t n = 256 / results;
+  if (n > steps / 8) n = steps / 8;
+  return n < 1 ? 1 : n;
+}
 Backward plan_backward(const Kept& k, int64_t vocab, int64_t dim) {
   Backward b;
   const int64_t all = up(vocab, kTile);
@@ -740,15 +789,14 @@ Backward plan_backward(const Kept& k, int64_t vocab, int64_t dim) {
   const int64_t pieces = (all + most - 1) / most;
   b.piece = up((all + pieces - 1) / pieces, kTile);
   b.dcols = up(dim, kTile);
-  // dx's product over few tokens is split along the vocabulary until it fills the CUs, 16 steps at least each
-  const int64_t results = k.npad / kTile * (b.dcols / kTile), steps = b.piece / kDepth;
-  b.splits = 256 / results;
-  if (b.splits > steps / 16) b.splits = steps / 16;
-  if (b.splits < 1) b.splits = 1;
+  const int64_t cols = b.dcols / kTile;
+  b.dx_splits = splits_of(k.npad / kTile * cols, b.piece / kDepth);
+  b.dw_splits = pieces > 1 ? 1 : splits_of(b.piece / kTile * cols, k.npad / kDepth);
   b.weight = 0;
   b.d = b.weight + k.npad * 4;
   b.dx = b.d + b.piece * k.npad * 2;
-  b.bytes = b.dx + b.splits * k.npad * b.dcols * 4;
+  b.dw = b.dx + b.dx_splits * k.npad * b.dcols * 4;
+  b.bytes = b.dw + (b.dw_splits > 1 ? b.dw_splits * b.piece * b.dcols * 4 : 0);
   return b;
 }
 
@@ -768,18 +816,18 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
                 const void* labels, int bits, int64_t ignore, int reduction, float* loss, uint8_t* kept, const Kept& k, uint8_t* ws,
                 const Forward& f, hipStream_t st) {
   Header* const head = (Header*)kept;
-  int32_t *place = (int32_t*)(kept + k.place), *label = (int32_t*)(kept + k.label);
-  float *ref = (float*)(kept + k.ref), *lse = (float*)(kept + k.lse);
+  int32_t *place = (int32_t*)(kept + k.place), *token = (int32_t*)(kept + k.token), *label = (int32_t*)(kept + k.label);
+  float *ref = (float*)(kept + k.ref), *lse = (float*)(kept + k.lse), *losses = reduction == 0 ? loss : nullptr;
   const int wide = (((uintptr_t)x | (uintptr_t)w) & 15) == 0 && ((x_stride | w_stride | dim) & 7) == 0;
   const unsigned blocks = (unsigned)((tokens < 1 ? 1 : tokens) + kPrepareRows - 1) / kPrepareRows;
   if (bits == 64)
-    hipLaunchKernelGGL((ce_prepare<T, int64_t>), dim3(blocks), dim3(256), 0, st, (const T*)x, x_stride, tokens, (const T*)w,
-                       w_stride, vocab, (int)dim, (int)k.dpad, wide, labels, ignore, head, place, label, ref,
-                       (T*)(kept + k.x), (int)k.npad);
+    hipLaunchKernelGGL((ce_prepare<T, int64_t>), dim3(blocks), dim3(1024), 0, st, (const T*)x, x_stride, tokens, (const T*)w,
+                       w_stride, vocab, (int)dim, (int)k.dpad, wide, labels, ignore, head, place, token, label, ref,
+                       (T*)(kept + k.x), (int)k.npad, losses);
   else
-    hipLaunchKernelGGL((ce_prepare<T, int32_t>), dim3(blocks), dim3(256), 0, st, (const T*)x, x_stride, tokens, (const T*)w,
-                       w_stride, vocab, (int)dim, (int)k.dpad, wide, labels, ignore, head, place, label, ref,
-                       (T*)(kept + k.x), (int)k.npad);
+    hipLaunchKernelGGL((ce_prepare<T, int32_t>), dim3(blocks), dim3(1024), 0, st, (const T*)x, x_stride, tokens, (const T*)w,
+                       w_stride, vocab, (int)dim, (int)k.dpad, wide, labels, ignore, head, place, token, label, ref,
+                       (T*)(kept + k.x), (int)k.npad, losses);
   CeArgs a = {};
   a.x = kept + k.x;
   a.x_stride = k.dpad * 2;
@@ -797,15 +845,11 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
   a.splits = 1;
   block_of(k.npad / kTile, &a);
   launch<T, kLoss>(a, st);
-  float *losses = (float*)(ws + f.losses), *block_sums = (float*)(ws + f.block_sums);
-  const int joins = (int)((tokens + kJoinTokens - 1) / kJoinTokens);
-  if (joins > 0)
-    hipLaunchKernelGGL(ce_join, dim3((unsigned)joins), dim3(kJoinTokens * kJoinSlices), 0, st, head, (const float2*)a.sums,
-                     (int)(up(vocab, kTile) / 128), (int)k.npad, ref, lse, losses, block_sums);
-  if (reduction == 0 && tokens > 0)
-    hipLaunchKernelGGL(ce_scatter, dim3((unsigned)((tokens + 255) / 256)), dim3(256), 0, st, place, losses, tokens, loss);
-  if (reduction != 0)
-    hipLaunchKernelGGL(ce_reduce, dim3(1), dim3(1024), 0, st, head, block_sums, joins, reduction == 1, loss);
+  const int64_t joins = (tokens < 1 ? 1 : tokens) + kJoinTokens - 1;
+  if (reduction == 0 && tokens == 0) return pkm_check_launch("pkm_linear_ce_fwd");  // no loss to write
+  hipLaunchKernelGGL(ce_join, dim3((unsigned)(joins / kJoinTokens)), dim3(kJoinTokens * kJoinSlices), 0, st, head,
+                     (const float2*)a.sums, (int)(up(vocab, kTile) / 128), (int)k.npad, ref, token, lse, losses,
+                     (float*)(ws + f.block_sums), loss, reduction == 1);
   return pkm_check_launch("pkm_linear_ce_fwd");
 }
 
@@ -814,10 +858,13 @@ int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, in
                  const float* grad, int reduction, void* dx, void* dw, uint8_t* ws, const Backward& b, hipStream_t st) {
   Header* const head = (Header*)kept;
   const int32_t* place = (const int32_t*)(kept + k.place);
-  float* weight = (float*)(ws + b.weight);
   constexpr float lift = __is_same(T, f16_t) ? 16384.f : 1.f;
-  hipLaunchKernelGGL(ce_weights, dim3(1), dim3(1024), 0, st, head, grad, reduction, place, tokens, lift, weight, (int)k.npad);
   CeArgs a = {};
+  if (reduction == 0) {
+    float* weight = (float*)(ws + b.weight);
+    a.weight = weight;
+    hipLaunchKernelGGL(ce_weights, dim3(1), dim3(1024), 0, st, head, grad, place, tokens, lift, weight);
+  }
   a.x = kept + k.x;
   a.x_stride = k.dpad * 2;
   a.w = (const uint8_t*)w;
@@ -827,30 +874,39 @@ int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, in
   a.label = (const int32_t*)(kept + k.label);
   a.ref = (const float*)(kept + k.ref);
   a.lse = (const float*)(kept + k.lse);
-  a.weight = weight;
-  a.dx = (float*)(ws + b.dx);
   a.dw = (uint8_t*)dw;
-  a.dw_scale = &head->dw_scale;
+  a.scale = Scale{&head->scale, reduction == 0 ? nullptr : grad, &head->count, lift, reduction == 1};
   a.vocab = vocab;
   a.piece = (int32_t)b.piece;
   a.dim = (int32_t)dim;
   a.npad = (int32_t)k.npad;
   a.dcols = (int32_t)b.dcols;
+  float *dx_parts = (float*)(ws + b.dx), *dw_parts = (float*)(ws + b.dw);
   for (int64_t v0 = 0; v0 < vocab; v0 += b.piece) {
     a.v0 = v0;
     a.splits = 1;
+    a.add = 0;
     block_of(k.npad / kTile, &a);
     launch<T, kGrads>(a, st);
     block_of(b.dcols / kTile, &a);
-    if (dw) launch<T, kDw>(a, st);
-    a.splits = (int32_t)b.splits;
-    a.add = v0 > 0;
-    if (dx) launch<T, kDx>(a, st);
+    if (dw) {
+      a.splits = (int32_t)b.dw_splits;
+      a.parts = dw_parts;
+      launch<T, kDw>(a, st);
+    }
+    if (dx) {
+      a.splits = (int32_t)b.dx_splits;
+      a.parts = dx_parts;
+      a.add = v0 > 0;
+      launch<T, kDx>(a, st);
+    }
   }
-  if (dx && tokens > 0)
-    hipLaunchKernelGGL(ce_dx<T>, dim3((unsigned)(tokens < 65536 ? tokens : 65536)), dim3(256), 0, st, head, place, tokens, a.dx,
-                       (int)b.splits, (int)k.npad, (int)b.dcols, (int)dim, (T*)dx);
-  if (dw) hipLaunchKernelGGL(ce_no_dw, dim3(1024), dim3(256), 0, st, head, (uint16_t*)dw, vocab * dim);
+  const auto rows = [&](const int32_t* from, int64_t n, const float* parts, int64_t splits, int64_t pad, void* out) {
+    hipLaunchKernelGGL(ce_rows<T>, dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, st, a.scale, from, n, parts, (int)splits,
+                       pad, (int)b.dcols, (int)dim, (T*)out);
+  };
+  if (dx && tokens > 0) rows(place, tokens, dx_parts, b.dx_splits, k.npad, dx);
+  if (dw && b.dw_splits > 1) rows(nullptr, vocab, dw_parts, b.dw_splits, b.piece, dw);
   return pkm_check_launch("pkm_linear_ce_bwd");
 }
 

@@ -226,3 +226,12 @@ def test_other_stream(device):
         got = _both(x, w, labels, "mean", gen)
     torch.cuda.current_stream().wait_stream(stream)
     assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[2], want[2]))
+
+
+def test_few_of_many_tokens_count(device):
+    """dW's sum over 3000 tokens is split (one result of 256 x 256); with a handful that count most splits have nothing."""
+    x, w, labels, gen = _inputs(3000, 200, 64, BF16, device)
+    for n in (0, 1, 65, 200, 2999, 3000):
+        some = labels.clone()
+        some[torch.randperm(3000, generator=gen)[: 3000 - n].to(device)] = -100
+        _check(x, w, some, "mean", gen)
