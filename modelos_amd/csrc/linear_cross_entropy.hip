@@ -54,11 +54,11 @@ struct CeArgs {
   const float* lse;      // [npad]
   const float* weight;   // [npad] of the tokens' gradients, or NULL: `lift` for all
   float2* sums;          // [2 * vocab tiles][npad] reference and sum of exponentials
-  float* parts;          // [splits][rows][dcols] float32: dx's rows, or dW's where its sum is split
+  float* parts;          // [splits][whole tiles' rows][dcols] float32: of dx, or of dW where its sum is split
   uint8_t* dw;           // [vocab][dim]
   Scale scale;
   int64_t vocab, v0;  // v0: the piece's first entry
-  int32_t piece, dim, npad, dcols, splits, add, lg_m, lg_n;
+  int32_t piece, dim, npad, dcols, splits, add;
 };
 
 __device__ __forceinline__ int perm16(int k) { return ((k & 3) << 2) | ((k >> 2) & 3); }
@@ -162,14 +162,33 @@ __device__ __forceinline__ frag_t entries_frag(uint32_t at, int t, int s) {
   return two_tr(at + to, (at ^ 128) + to);
 }
 
-// Results of a product and their order: blocks of 2^lg_m x 2^lg_n tiles, one XCD's workgroups side by side in it, so that
-// they share the tiles' rows in its L2; blocks run along N first.
+// Results of a product go in blocks of 2^lg_m x 2^lg_n tiles, 32 at most, to workgroups of one XCD, so that these share the
+// tiles' rows in its L2; blocks run along N first.
+struct Blocks {
+  int lg_m = 0, lg_n, m, n;  // m, n: how many
+  __host__ __device__ Blocks(int64_t tiles_m, int64_t tiles_n) {
+    lg_n = tiles_n >= 4 ? 2 : tiles_n >= 2 ? 1 : 0;
+    while (lg_m < 5 - lg_n && (1 << lg_m) < tiles_m) ++lg_m;
+    m = (int)((tiles_m + (1 << lg_m) - 1) >> lg_m);
+    n = (int)((tiles_n + (1 << lg_n) - 1) >> lg_n);
+  }
+  __host__ __device__ int64_t results() const { return ((int64_t)m * n) << (lg_m + lg_n); }
+};
+
+// Splits of a product's sum over `steps`, so that few results fill the CUs once: 8 steps at least each, which outweigh the
+// partial results' way through memory.
+__host__ __device__ inline int splits_of(int64_t tiles_m, int64_t tiles_n, int64_t steps) {
+  const int64_t results = Blocks(tiles_m, tiles_n).results();
+  int64_t n = results < 1 ? 1 : 256 / results;
+  if (n > steps / 8) n = steps / 8;
+  return n < 1 ? 1 : (int)n;
+}
+
 struct Order {
-  int m, n, k, splits, lg_m, lg_n, blocks_n, total, share;
-  __device__ __forceinline__ Order(int m_, int n_, int k_, int splits_, int lg_m_, int lg_n_)
-      : m(m_), n(n_), k(k_), splits(splits_), lg_m(lg_m_), lg_n(lg_n_) {
-    blocks_n = (n + (1 << lg_n) - 1) >> lg_n;
-    total = (((m + (1 << lg_m) - 1) >> lg_m) * blocks_n * splits) << (lg_m + lg_n);
+  Blocks blocks;
+  int m, n, k, splits, total, share;
+  __device__ __forceinline__ Order(int m_, int n_, int k_, int splits_) : blocks(m_, n_), m(m_), n(n_), k(k_), splits(splits_) {
+    total = (int)blocks.results() * splits;
     share = min(32, (total + 7) / 8);  // results of an XCD at a time
   }
 };
@@ -184,11 +203,11 @@ struct Result {
       i += 8 * o.share;
     }
     for (; i < o.total; i += 8 * o.share) {
-      const int within = i & ((1 << (o.lg_m + o.lg_n)) - 1), block = i >> (o.lg_m + o.lg_n);
-      const int rest = block / o.splits;
+      const int lg_m = o.blocks.lg_m, lg = lg_m + o.blocks.lg_n;
+      const int within = i & ((1 << lg) - 1), block = i >> lg, rest = block / o.splits;
       split = block - rest * o.splits;
-      m = ((rest / o.blocks_n) << o.lg_m) + (within & ((1 << o.lg_m) - 1));
-      n = ((rest % o.blocks_n) << o.lg_n) + (within >> o.lg_m);
+      m = ((rest / o.blocks.n) << lg_m) + (within & ((1 << lg_m) - 1));
+      n = ((rest % o.blocks.n) << o.blocks.lg_n) + (within >> lg_m);
       if (m >= o.m || n >= o.n) continue;
       k0 = (int)((int64_t)o.k * split / o.splits);
       k1 = (int)((int64_t)o.k * (split + 1) / o.splits);
@@ -364,9 +383,10 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
   const int64_t entries = min((int64_t)a.piece, a.vocab - a.v0);  // of the piece
   const int token_tiles = (n + kTile - 1) / kTile, entry_tiles = (int)((entries + kTile - 1) / kTile),
             dim_tiles = a.dcols / kTile;
-  const Order order = P == kLoss || P == kGrads ? Order(entry_tiles, token_tiles, dpad / kDepth, 1, a.lg_m, a.lg_n)
-                      : P == kDx ? Order(token_tiles, dim_tiles, (int)((entries + kDepth - 1) / kDepth), a.splits, a.lg_m, a.lg_n)
-                                 : Order(entry_tiles, dim_tiles, (n + kDepth - 1) / kDepth, a.splits, a.lg_m, a.lg_n);
+  const Order order =
+      P == kLoss || P == kGrads ? Order(entry_tiles, token_tiles, dpad / kDepth, 1)
+      : P == kDx ? Order(token_tiles, dim_tiles, (int)((entries + kDepth - 1) / kDepth), splits_of(token_tiles, dim_tiles, a.piece / kDepth))
+                 : Order(entry_tiles, dim_tiles, (n + kDepth - 1) / kDepth, a.splits);
   if constexpr (P == kDw) {
     if (n == 0 && a.splits == 1) {  // no token counts: zeros
       const int64_t first = a.v0 * a.dim, all = entries * a.dim;
@@ -494,7 +514,7 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
     if (ends) {
       if constexpr (P == kLoss) end_loss(a, acc, run, wave, lane);
       if constexpr (P == kGrads) end_grads<T>(a, acc, run, n, wave, lane);
-      if constexpr (P == kDx) end_parts(a, acc, run, a.npad, wave, lane);
+      if constexpr (P == kDx) end_parts(a, acc, run, token_tiles * kTile, wave, lane);
       if constexpr (P == kDw) {
         if (a.splits > 1)
           end_parts(a, acc, run, a.piece, wave, lane);
@@ -632,7 +652,7 @@ __global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(Header* head
     }
   };
   if (j < count) {
-    constexpr int FLIGHT = 16;
+    constexpr int FLIGHT = 8;
     for (int p = slice; p < parts; p += kJoinSlices * FLIGHT) {
       float2 v[FLIGHT];
 #pragma unroll
@@ -698,29 +718,37 @@ __global__ __launch_bounds__(1024) void ce_weights(Header* head, const float* __
   if (tid == 0) head->scale = unit / lift;
 }
 
-// Rows of results: the splits' sums in order, scaled and rounded. dx: row i from row place[i], zeros if that is negative.
-// dW (place NULL): row i from row i; few kept tokens leave some splits without a step, which wrote nothing. A workgroup a
-// row at a time.
+// Rows of results: the splits' sums in order, scaled and rounded, a workgroup a row at a time. dx: row i from row place[i],
+// zeros if that is negative; `splits` is 0, the kept tokens give it. dW (place NULL): row i from row i; few kept tokens
+// leave some splits without a step, which wrote nothing.
 template <typename T>
 __global__ __launch_bounds__(256) void ce_rows(const Scale scale, const int32_t* __restrict__ place, int64_t rows,
-                                               const float* __restrict__ parts, int splits, int64_t rows_pad, int dcols, int dim,
+                                               const float* __restrict__ parts, int splits, int piece, int dcols, int dim,
                                                T* __restrict__ out) {
   const float f = scale();
-  const int64_t steps = place ? splits : (*scale.count + kDepth - 1) / kDepth;
+  const int n = *scale.count, tiles = (n + kTile - 1) / kTile, steps = (n + kDepth - 1) / kDepth;
+  int64_t pad = piece;
+  if (place) {
+    splits = splits_of(tiles, dcols / kTile, piece / kDepth);
+    pad = tiles * kTile;
+  }
   for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
     const int64_t j = place ? place[i] : i;
     for (int d = threadIdx.x * 4; d < dim; d += 1024) {
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (j >= 0) {
+      const auto add = [&](int s) {
+        const float4 v = *(const float4*)(parts + (s * pad + j) * dcols + d);
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      };
+      if (place && j >= 0) {
 #pragma unroll 8
-        for (int s = 0; s < splits; ++s) {
-          if (steps * s / splits == steps * (s + 1) / splits) continue;
-          const float4 v = *(const float4*)(parts + (s * rows_pad + j) * dcols + d);
-          sum.x += v.x;
-          sum.y += v.y;
-          sum.z += v.z;
-          sum.w += v.w;
-        }
+        for (int s = 0; s < splits; ++s) add(s);
+      } else if (!place) {
+        for (int s = 0; s < splits; ++s)
+          if ((int64_t)steps * s / splits < (int64_t)steps * (s + 1) / splits) add(s);
       }
       uint16_t* const to = (uint16_t*)(out + i * dim + d);
       const uint32_t a = j < 0 ? 0u : pack2<T>(sum.x * f, sum.y * f), b = j < 0 ? 0u : pack2<T>(sum.z * f, sum.w * f);
@@ -771,15 +799,8 @@ Forward plan_forward(const Kept& k, int64_t vocab) {
 }
 
 struct Backward {
-  int64_t piece, dcols, dx_splits, dw_splits, weight, d, dx, dw, bytes;
+  int64_t piece, dcols, dw_splits, weight, d, dx, dw, bytes;
 };
-// Splits of a product's sum over `steps`, so that few results fill the CUs: 8 steps at least each, which outweigh the partial
-// results' way through memory.
-int64_t splits_of(int64_t results, int64_t steps) {
-  int64_t n = 256 / results;
-  if (n > steps / 8) n = steps / 8;
-  return n < 1 ? 1 : n;
-}
 Backward plan_backward(const Kept& k, int64_t vocab, int64_t dim) {
   Backward b;
   const int64_t all = up(vocab, kTile);
@@ -790,20 +811,18 @@ Backward plan_backward(const Kept& k, int64_t vocab, int64_t dim) {
   b.piece = up((all + pieces - 1) / pieces, kTile);
   b.dcols = up(dim, kTile);
   const int64_t cols = b.dcols / kTile;
-  b.dx_splits = splits_of(k.npad / kTile * cols, b.piece / kDepth);
-  b.dw_splits = pieces > 1 ? 1 : splits_of(b.piece / kTile * cols, k.npad / kDepth);
+  b.dw_splits = pieces > 1 ? 1 : splits_of(b.piece / kTile, cols, k.npad / kDepth);
   b.weight = 0;
   b.d = b.weight + k.npad * 4;
   b.dx = b.d + b.piece * k.npad * 2;
-  b.dw = b.dx + b.dx_splits * k.npad * b.dcols * 4;
+  // dx's sum is split by the kept tokens, whose number the device has: splits x tiles of tokens are 256 / cols or fewer where
+  // there are several splits, and no more than the steps allow
+  const int64_t tiles = k.npad / kTile, most_splits = splits_of(1, 1, b.piece / kDepth);
+  int64_t parts = tiles * most_splits < 256 / cols ? tiles * most_splits : 256 / cols;
+  if (parts < tiles) parts = tiles;
+  b.dw = b.dx + parts * kTile * b.dcols * 4;
   b.bytes = b.dw + (b.dw_splits > 1 ? b.dw_splits * b.piece * b.dcols * 4 : 0);
   return b;
-}
-
-// The tiles of an order's block: 2^lg_n of N, of which there are n, and 32 in all.
-void block_of(int64_t n, CeArgs* a) {
-  a->lg_n = n >= 4 ? 2 : n >= 2 ? 1 : 0;
-  a->lg_m = 5 - a->lg_n;
 }
 
 template <typename T, Product P>
@@ -843,7 +862,6 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
   a.npad = (int32_t)k.npad;
   a.dcols = (int32_t)up(dim, kTile);
   a.splits = 1;
-  block_of(k.npad / kTile, &a);
   launch<T, kLoss>(a, st);
   const int64_t joins = (tokens < 1 ? 1 : tokens) + kJoinTokens - 1;
   if (reduction == 0 && tokens == 0) return pkm_check_launch("pkm_linear_ce_fwd");  // no loss to write
@@ -886,27 +904,24 @@ int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, in
     a.v0 = v0;
     a.splits = 1;
     a.add = 0;
-    block_of(k.npad / kTile, &a);
     launch<T, kGrads>(a, st);
-    block_of(b.dcols / kTile, &a);
     if (dw) {
       a.splits = (int32_t)b.dw_splits;
       a.parts = dw_parts;
       launch<T, kDw>(a, st);
     }
     if (dx) {
-      a.splits = (int32_t)b.dx_splits;
       a.parts = dx_parts;
       a.add = v0 > 0;
       launch<T, kDx>(a, st);
     }
   }
-  const auto rows = [&](const int32_t* from, int64_t n, const float* parts, int64_t splits, int64_t pad, void* out) {
+  const auto rows = [&](const int32_t* from, int64_t n, const float* parts, int64_t splits, void* out) {
     hipLaunchKernelGGL(ce_rows<T>, dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, st, a.scale, from, n, parts, (int)splits,
-                       pad, (int)b.dcols, (int)dim, (T*)out);
+                       (int)b.piece, (int)b.dcols, (int)dim, (T*)out);
   };
-  if (dx && tokens > 0) rows(place, tokens, dx_parts, b.dx_splits, k.npad, dx);
-  if (dw && b.dw_splits > 1) rows(nullptr, vocab, dw_parts, b.dw_splits, b.piece, dw);
+  if (dx && tokens > 0) rows(place, tokens, dx_parts, 0, dx);
+  if (dw && b.dw_splits > 1) rows(nullptr, vocab, dw_parts, b.dw_splits, dw);
   return pkm_check_launch("pkm_linear_ce_bwd");
 }
 
