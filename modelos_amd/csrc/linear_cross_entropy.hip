@@ -225,94 +225,115 @@ __device__ __forceinline__ constexpr int row_of(int t, int i) { return 32 * t + 
 // Nothing moves across: a batch of registers is done with before the next begins.
 __device__ __forceinline__ void batch() { __builtin_amdgcn_sched_barrier(0); }
 
-// Results behind the vocabulary's end, `left` rows from the wave's first: x in their place.
-__device__ __forceinline__ void cut(acc_t& acc, int64_t left, int h, float x) {
-  if (left >= 128) return;
+// Results behind the vocabulary's end, `left` rows from the wave's first: -infinity in their place.
+template <int MT, int NU>
+__device__ __forceinline__ void cut(f32x16_t (&acc)[MT][NU], int64_t left, int h) {
+  if (left >= 32 * MT) return;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < NU; ++u) {
     int most = (int)left - 4 * h;
     asm volatile("" : "+v"(most));  // compared anew for each half: 64 masks would not fit the scalar registers
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[t][u][i] = row_of(t, i) < most ? acc[t][u][i] : x;
+      for (int i = 0; i < 16; ++i) acc[t][u][i] = row_of(t, i) < most ? acc[t][u][i] : -INFINITY;
   }
 }
 
-// The sums of the exponentials of 128 entries for 64 tokens, against the token's reference: the label's logit, which is one of
-// the summands, so that what underflows beside it is nothing. Where one overflows, the 128's own largest takes its place.
+// The sum of the exponentials of a wave's entries for the lane's token of column block u, against the token's reference: the
+// label's logit, which is one of the summands, so that what underflows beside it is nothing. Where it overflows, the entries'
+// own largest logit takes the reference's place.
+template <int MT, int NU>
+__device__ __forceinline__ float2 sum_of(const f32x16_t (&acc)[MT][NU], int u, float ref) {
+  float sum = 0.f;
+  const float c = -ref * kLog2e;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += exp2_raw(__builtin_fmaf(acc[t][u][i], kLog2e, c));
+    batch();
+  }
+  sum += swap_halves(sum);
+  const bool over = !(sum < 0x1p120f);
+  if (__any(over)) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, acc[t][u][i]);
+    top = fmaxf(top, swap_halves(top));
+    float own = 0.f;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) own += exp2_raw((acc[t][u][i] - top) * kLog2e);
+      batch();
+    }
+    own += swap_halves(own);
+    if (over) ref = top, sum = own;
+  }
+  return make_float2(ref, sum);
+}
+
+// Two such sums as one.
+__device__ __forceinline__ float2 joined(float2 a, float2 b) {
+  if (b.x > a.x) return make_float2(b.x, a.y * exp2_raw((a.x - b.x) * kLog2e) + b.y);
+  return make_float2(a.x, a.y + (b.x == a.x ? b.y : b.y * exp2_raw((b.x - a.x) * kLog2e)));
+}
+
 __device__ __forceinline__ void end_loss(const CeArgs& a, acc_t& acc, const Result& r, int wave, int lane) {
   const int h = lane >> 5, v0 = r.m * kTile + (wave >> 2) * 128;
-  cut(acc, a.vocab - v0, h, -INFINITY);
+  cut(acc, a.vocab - v0, h);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int j = r.n * kTile + (wave & 3) * 64 + 32 * u + (lane & 31);
-    float ref = a.ref[j];
-    float sum = 0.f;
-    const float c = -ref * kLog2e;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum += exp2_raw(__builtin_fmaf(acc[t][u][i], kLog2e, c));
-      batch();
-    }
-    sum += swap_halves(sum);
-    const bool over = !(sum < 0x1p120f);
-    if (__any(over)) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, acc[t][u][i]);
-      top = fmaxf(top, swap_halves(top));
-      float own = 0.f;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) own += exp2_raw((acc[t][u][i] - top) * kLog2e);
-        batch();
-      }
-      own += swap_halves(own);
-      if (over) ref = top, sum = own;
-    }
-    if (h == 0) a.sums[(int64_t)(2 * r.m + (wave >> 2)) * a.npad + j] = make_float2(ref, sum);
+    const float2 sum = sum_of(acc, u, a.ref[j]);
+    if (h == 0) a.sums[(int64_t)(2 * r.m + (wave >> 2)) * a.npad + j] = sum;
   }
 }
 
-// d of 128 entries for 64 tokens, rounded, in blocks.
+// d of a wave's entries, from v0 of the piece on, for the lane's token j of column block u, rounded, in blocks.
+// c: - lse log2(e), -infinity for a token that is not kept; y: the label's place from v0 on; ref: its logit.
+template <typename T, int MT, int NU>
+__device__ __forceinline__ void grads_of(const CeArgs& a, const f32x16_t (&acc)[MT][NU], int u, int64_t v0, int j, float c,
+                                         float weight, int64_t y, float ref, int lane) {
+  const int h = lane >> 5;
+  const int64_t row = (int64_t)(a.npad / 32) * 1024;
+  uint8_t* const to = a.d + (v0 / 16) * row + (int64_t)(j >> 5) * 1024;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = exp2_raw(__builtin_fmaf(acc[t][u][8 * s + e], kLog2e, c)) * weight;
+      const u32x4_t x = {pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7])};
+      *(u32x4_t*)(to + (2 * t + s) * row + block_lane(s, h, lane & 31) * 16) = x;
+    }
+    batch();
+  }
+  // the label's number is exp(l - lse) - 1, rounded once: it takes the place of the one written above
+  const bool own = y >= 0 && y < 32 * MT;
+  if (__any(own)) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (own && h == 0) {
+      const float x = (exp2_raw(__builtin_fmaf(ref, kLog2e, c)) - 1.f) * weight;
+      *(uint16_t*)(to + (y >> 4) * row + block_lane((y >> 4) & 1, (y >> 2) & 1, lane) * 16 + ((y >> 3) & 1) * 8 + (y & 3) * 2) =
+          (uint16_t)pack2<T>(x, x);
+    }
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void end_grads(const CeArgs& a, acc_t& acc, const Result& r, int count, int wave, int lane) {
-  const int h = lane >> 5, v0 = r.m * kTile + (wave >> 2) * 128;
-  cut(acc, a.vocab - a.v0 - v0, h, -INFINITY);
-  const int64_t row = (int64_t)(a.npad / 32) * 1024;
+  const int64_t v0 = r.m * kTile + (wave >> 2) * 128;
+  cut(acc, a.vocab - a.v0 - v0, lane >> 5);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int j = r.n * kTile + (wave & 3) * 64 + 32 * u + (lane & 31);
     const bool kept = j < count;
     const float c = kept ? -a.lse[j] * kLog2e : -INFINITY, weight = !kept ? 0.f : a.weight ? a.weight[j] : a.scale.lift;
-    uint8_t* const to = a.d + (int64_t)(v0 / 16) * row + (int64_t)(j >> 5) * 1024;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        float f[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = exp2_raw(__builtin_fmaf(acc[t][u][8 * s + e], kLog2e, c)) * weight;
-        const u32x4_t x = {pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7])};
-        *(u32x4_t*)(to + (2 * t + s) * row + block_lane(s, h, lane & 31) * 16) = x;
-      }
-      batch();
-    }
-    // the label's number is exp(l - lse) - 1, rounded once: it takes the place of the one written above
-    const int64_t y = kept ? (int64_t)a.label[j] - a.v0 - v0 : -1;
-    if (__any(y >= 0 && y < 128)) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (y >= 0 && y < 128 && h == 0) {
-        const float x = (exp2_raw(__builtin_fmaf(a.ref[j], kLog2e, c)) - 1.f) * weight;
-        *(uint16_t*)(to + (y >> 4) * row + block_lane((y >> 4) & 1, (y >> 2) & 1, lane) * 16 + ((y >> 3) & 1) * 8 + (y & 3) * 2) =
-            (uint16_t)pack2<T>(x, x);
-      }
-    }
+    grads_of<T>(a, acc, u, v0, j, c, weight, kept ? (int64_t)a.label[j] - a.v0 - v0 : -1, a.ref[j], lane);
   }
 }
 
@@ -536,6 +557,109 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// The same product for few tokens, which reading weight once bounds: tiles of 128 entries x 64 tokens by 8 waves (4 x 2, each
+// 32 x 32), 64 deep, in a ring of five stages of 24 KB, four of which are on their way. What the epilogue reads of the
+// tokens lies in LDS from the start: a load of its own would wait for the whole ring.
+// ---------------------------------------------------------------------------
+constexpr int kFew = 128;  // tokens
+constexpr int kFewM = 128, kFewN = 64, kRing = 5, kFewStage = (kFewM + kFewN) * 128;
+
+template <typename T, Product P>
+__global__ __launch_bounds__(kThreads, 2) void ce_few(const CeArgs a) {
+  static_assert(P == kLoss || P == kGrads, "the products with tokens for columns");
+  __shared__ __align__(1024) uint8_t smem[kRing * kFewStage];
+  __shared__ float ref_s[kFew], lse_s[kFew], weight_s[kFew];
+  __shared__ int32_t label_s[kFew];
+  __shared__ float2 sum_s[kFewM / 32][kFewN];
+  lds_u8* const lds = (lds_u8*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int n = __builtin_amdgcn_readfirstlane(*a.count);
+  const int chunks = (a.dim + 7) / 8, dpad = (int)(a.x_stride / 2);
+  const int64_t entries = min((int64_t)a.piece, a.vocab - a.v0);
+  const Order order((int)((entries + kFewM - 1) / kFewM), (n + kFewN - 1) / kFewN, dpad / kDepth, 1);
+  const uint8_t* const w = a.w + a.v0 * a.w_stride;
+  Result run, ahead;
+  if (!ahead.next(order, true)) return;
+  run = ahead;
+  if (tid < kFew) {
+    const bool kept = tid < n;
+    ref_s[tid] = a.ref[tid];
+    label_s[tid] = a.label[tid];
+    if constexpr (P == kGrads) {
+      lse_s[tid] = kept ? -a.lse[tid] * kLog2e : -INFINITY;
+      weight_s[tid] = !kept ? 0.f : a.weight ? a.weight[tid] : a.scale.lift;
+    }
+  }
+  RowsTile ra, rb;
+  int load_step = ahead.k0;
+  const auto aim = [&]() {
+    ra.at(w, a.w_stride, (int64_t)ahead.m * kFewM, entries, wave, lane);
+    rb.at(a.x, a.x_stride, (int64_t)ahead.n * kFewN, n, wave, lane);
+  };
+  const auto load_next = [&](int stage) {
+    lds_u8* const to = lds + stage * kFewStage;
+    ra.load(to, 0, load_step, chunks, wave);
+    ra.load(to, 1, load_step, chunks, wave);
+    rb.load(to + kFewM * 128, 0, load_step, dpad / 8, wave);
+    if (load_step + 1 < ahead.k1) {
+      ++load_step;
+      return;
+    }
+    Result after = ahead;
+    if (after.next(order, false)) {
+      ahead = after;
+      aim();
+      load_step = ahead.k0;
+    }
+  };
+  aim();
+#pragma unroll
+  for (int k = 0; k < kRing - 1; ++k) load_next(k);
+  const uint32_t at_a = lds_address(lds) + rows_lane(lane) + (wave >> 1) * 4096;
+  const uint32_t at_b = lds_address(lds) + kFewM * 128 + rows_lane(lane) + (wave & 1) * 4096;
+  f32x16_t acc[1][1] = {};
+  for (int stage = 0, step = run.k0;; stage = stage + 1 == kRing ? 0 : stage + 1) {
+    tile_wait<3 * (kRing - 2)>();  // this step's three loads are in
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    load_next(stage == 0 ? kRing - 1 : stage - 1);  // where the step before lay
+    frag_t fa[4], fb[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      fa[s] = rows_frag(at_a + stage * kFewStage, 0, s);
+      fb[s] = rows_frag(at_b + stage * kFewStage, 0, s);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) acc[0][0] = mfma32<T>(fa[s], fb[s], acc[0][0]);
+    if (++step != run.k1) continue;
+    const int64_t v0 = (int64_t)run.m * kFewM + (wave >> 1) * 32;
+    const int column = (wave & 1) * 32 + (lane & 31), j = run.n * kFewN + column;
+    cut(acc, entries - v0, h);
+    if constexpr (P == kLoss) {
+      const float2 sum = sum_of(acc, 0, ref_s[j]);
+      if (h == 0) sum_s[wave >> 1][column] = sum;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (tid < kFewN) {
+        float2 all = sum_s[0][tid];
+#pragma unroll
+        for (int k = 1; k < kFewM / 32; ++k)
+          if (sum_s[k][tid].y != 0.f) all = joined(all, sum_s[k][tid]);
+        a.sums[(int64_t)run.m * a.npad + run.n * kFewN + tid] = all;
+      }
+    } else {
+      grads_of<T>(a, acc, 0, v0, j, lse_s[j], weight_s[j], label_s[j] < 0 ? -1 : label_s[j] - a.v0 - v0, ref_s[j], lane);
+    }
+    acc[0][0] = f32x16_t{};
+    if (!run.next(order, false)) break;
+    step = run.k0;
+  }
+  tile_wait<0>();  // no load may outlive the workgroup's LDS
+}
+
+// ---------------------------------------------------------------------------
 // Around the products
 // ---------------------------------------------------------------------------
 constexpr int kPrepareRows = 16;  // tokens of a workgroup of ce_prepare, a wave each
@@ -644,12 +768,9 @@ __global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(Header* head
   const int j = blockIdx.x * kJoinTokens + t, count = head->count;
   float m = -INFINITY, sum = 0.f;
   const auto add = [&](float r, float v) {
-    if (r > m) {
-      sum = sum * exp2_raw((m - r) * kLog2e) + v;  // 0 at first
-      m = r;
-    } else {
-      sum += r == m ? v : v * exp2_raw((r - m) * kLog2e);
-    }
+    const float2 both = joined(make_float2(m, sum), make_float2(r, v));  // 0 at first
+    m = both.x;
+    sum = both.y;
   };
   if (j < count) {
     constexpr int FLIGHT = 8;
@@ -830,6 +951,14 @@ void launch(const CeArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((ce_product<T, P>), dim3(256), dim3(kThreads), 0, st, a);
 }
 
+template <typename T, Product P>
+void launch_logits(const CeArgs& a, int64_t tokens, hipStream_t st) {
+  if (tokens <= kFew)
+    hipLaunchKernelGGL((ce_few<T, P>), dim3(256), dim3(kThreads), 0, st, a);
+  else
+    launch<T, P>(a, st);
+}
+
 template <typename T>
 int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, int64_t w_stride, int64_t vocab, int64_t dim,
                 const void* labels, int bits, int64_t ignore, int reduction, float* loss, uint8_t* kept, const Kept& k, uint8_t* ws,
@@ -862,11 +991,11 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
   a.npad = (int32_t)k.npad;
   a.dcols = (int32_t)up(dim, kTile);
   a.splits = 1;
-  launch<T, kLoss>(a, st);
+  launch_logits<T, kLoss>(a, tokens, st);
   const int64_t joins = (tokens < 1 ? 1 : tokens) + kJoinTokens - 1;
   if (reduction == 0 && tokens == 0) return pkm_check_launch("pkm_linear_ce_fwd");  // no loss to write
   hipLaunchKernelGGL(ce_join, dim3((unsigned)(joins / kJoinTokens)), dim3(kJoinTokens * kJoinSlices), 0, st, head,
-                     (const float2*)a.sums, (int)(up(vocab, kTile) / 128), (int)k.npad, ref, token, lse, losses,
+                     (const float2*)a.sums, (int)((vocab + 127) / 128), (int)k.npad, ref, token, lse, losses,
                      (float*)(ws + f.block_sums), loss, reduction == 1);
   return pkm_check_launch("pkm_linear_ce_fwd");
 }
@@ -904,7 +1033,7 @@ int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, in
     a.v0 = v0;
     a.splits = 1;
     a.add = 0;
-    launch<T, kGrads>(a, st);
+    launch_logits<T, kGrads>(a, tokens, st);
     if (dw) {
       a.splits = (int32_t)b.dw_splits;
       a.parts = dw_parts;
