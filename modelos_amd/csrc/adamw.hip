@@ -170,16 +170,20 @@ __device__ __forceinline__ float max32(uint32_t x) {
   return __uint_as_float(max(x, (uint32_t)__builtin_amdgcn_ds_swizzle((int)x, 0x401F)));  // lane xor 16
 }
 
-// The code of a >= 0 (units of the step), dither in the low 20 bits of u. A float's bits above bit 20 count e4m3's numbers
-// of the same exponents, so adding the dither below them rounds; under 2^-6, where the spacing stays 2^-9, so do the bits of
-// a + 2^-6. `a` is a product with the step's reciprocal, a few units of its last place off x / step: where the sum comes
-// within 8 of a code's border, `near` falls below 16 and exact_code() decides.
+// The code of a >= 0 (units of the step) in the upper byte, dither in the low 20 bits of u. 2^-120 a has e4m3's exponents
+// as a float32: its bits above bit 20 count e4m3's numbers from 0 on, the smallest ones among them, as float32's own smallest
+// numbers are spaced evenly too. So adding the dither below them rounds. `a` is a product with the step's reciprocal, a few
+// units of its last place off x / step: where the sum comes within 8 of a code's border, `near` falls below 16 << 12 and
+// exact_code() decides. (A code past the largest, 448 and a little, is such a case.)
 __device__ __forceinline__ uint32_t code_of(float a, uint32_t u, uint32_t& near) {
-  const bool small = a < 0x1p-6f;
-  const uint32_t bits = __float_as_uint(small ? a + 0x1p-6f : a) + u;
-  const uint32_t code = (bits >> 20) - (small ? (121u << 3) : (120u << 3));
-  near = min(near, (bits + 8) & 0xfffffu);
-  return code < 0x7eu ? code : 0x7eu;
+  const uint32_t code = (__float_as_uint(a * 0x1p-120f) + u) << 4;
+  near = min(near, (code << 8) + (8u << 12));
+  return code;
+}
+// The upper bytes of four.
+__device__ __forceinline__ uint32_t upper_bytes(const uint32_t* c) {
+  const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0703u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0703u);
+  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
 // The same of x / step, not rounded: x is compared with the border nearest to it, times the step, in one exact sign.
@@ -230,7 +234,7 @@ __device__ __forceinline__ void step8(const Tensor& x, int64_t first, int64_t n,
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int64_t i = first + k * 2048;
-    float m[8], v[8];
+    float m[8], v[8], root[8];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const auto m0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[k][0][w], false),
@@ -246,7 +250,8 @@ __device__ __forceinline__ void step8(const Tensor& x, int64_t first, int64_t n,
       const float ge = g[k][e] * gs, r = v[e] * steps[k][1];
       m[e] = __builtin_fmaf(b.a1, ge, b.b1 * (m[e] * steps[k][0]));
       v[e] = __builtin_fmaf(b.a2, ge * ge, b.b2 * (r * r));
-      p[k][e] = updated(p[k][e], m[e], __builtin_amdgcn_sqrtf(v[e]), c, b.eps);
+      root[e] = __builtin_amdgcn_sqrtf(v[e]);
+      p[k][e] = updated(p[k][e], m[e], root[e], c, b.eps);
       if constexpr (MASTER) asm("" : "+v"(p[k][e]));  // the weight rounds the master, not the operation before it
       top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
       top_v = max(top_v, __float_as_uint(v[e]));
@@ -263,17 +268,21 @@ __device__ __forceinline__ void step8(const Tensor& x, int64_t first, int64_t n,
       x.vs[i / kBlock] = step_r;
     }
     const uint32_t u0 = (uint32_t)i * 2654435761u + (uint32_t)c.t * 2246822519u;
-    uint32_t cm[2] = {}, cr[2] = {}, near = ~0u, u = u0;
+    uint32_t cm[2], cr[2], near = ~0u, u = u0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t a = code_of(fabsf(m[e]) * fm, u >> 12, near);
-      const float r = __builtin_amdgcn_sqrtf(v[e]) * fr;
-      const uint32_t d = max(code_of(r, u & 0xfffffu, near), r > 0.f ? 1u : 0u);
-      cm[e / 4] |= (a | ((__float_as_uint(m[e]) >> 24) & 0x80u)) << (e % 4 * 8);
-      cr[e / 4] |= d << (e % 4 * 8);
-      u += 2654435761u;
+    for (int w = 0; w < 2; ++w) {
+      uint32_t a[4], d[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float r = root[4 * w + e] * fr;
+        a[e] = code_of(fabsf(m[4 * w + e]) * fm, u >> 12, near) | (__float_as_uint(m[4 * w + e]) & 0x80000000u);
+        d[e] = max(code_of(r, u & 0xfffffu, near), min(__float_as_uint(r), 1u) << 24);
+        u += 2654435761u;
+      }
+      cm[w] = upper_bytes(a);
+      cr[w] = upper_bytes(d);
     }
-    if (near < 16) {  // one lane in 4000
+    if (near < (16u << 12)) {  // one lane in 4000
       u = u0;
       cm[0] = cm[1] = cr[0] = cr[1] = 0;
 #pragma unroll
