@@ -170,14 +170,15 @@ __device__ __forceinline__ float max32(uint32_t x) {
   return __uint_as_float(max(x, (uint32_t)__builtin_amdgcn_ds_swizzle((int)x, 0x401F)));  // lane xor 16
 }
 
-// The code of a >= 0 (units of the step) in the upper byte, dither in the low 20 bits of u. 2^-120 a has e4m3's exponents
-// as a float32: its bits above bit 20 count e4m3's numbers from 0 on, the smallest ones among them, as float32's own smallest
-// numbers are spaced evenly too. So adding the dither below them rounds. `a` is a product with the step's reciprocal, a few
-// units of its last place off x / step: where the sum comes within 8 of a code's border, `near` falls below 16 << 12 and
-// exact_code() decides. (A code past the largest, 448 and a little, is such a case.)
+// The code of a >= 0 (units of the step) in the upper byte, from 2^-120 a and the dither in the low 20 bits of u. 2^-120 a
+// has e4m3's exponents as a float32: its bits above bit 20 count e4m3's numbers from 0 on, the smallest ones among them, as
+// float32's own smallest numbers are spaced evenly too. So adding the dither below them rounds. The float32 is a product with
+// the step's reciprocal, a few units of its last place off x / step: where the sum comes within 8 of a code's border, `near`
+// falls below kNear and exact_code() decides. (A code past the largest, 448 and a little, is such a case.)
+constexpr uint32_t kNear = 16u << 12;
 __device__ __forceinline__ uint32_t code_of(float a, uint32_t u, uint32_t& near) {
-  const uint32_t code = (__float_as_uint(a * 0x1p-120f) + u) << 4;
-  near = min(near, (code << 8) + (8u << 12));
+  const uint32_t code = (__float_as_uint(a) + u) << 4;
+  near = min(near, (code << 8) + kNear / 2);
   return code;
 }
 // The upper bytes of four.
@@ -187,20 +188,22 @@ __device__ __forceinline__ uint32_t upper_bytes(const uint32_t* c) {
 }
 
 // The same of x / step, not rounded: x is compared with the border nearest to it, times the step, in one exact sign.
-__device__ __forceinline__ uint32_t exact_code(float x, float step, float f, uint32_t u) {
-  const float a = x * f;
+__device__ __forceinline__ uint32_t exact_code(float x, float step, uint32_t u) {
+  const float a = x / step;
   const bool small = a < 0x1p-6f;
   const uint32_t bits = __float_as_uint(small ? a + 0x1p-6f : a) + u;
   const uint32_t high = (bits + 0x80000u) >> 20;  // the code above the nearest border
   const float at = __uint_as_float((high << 20) - u);
   const float border = small ? at - 0x1p-6f : at;
-  const uint32_t code = high - (__builtin_fmaf(border, step, -x) > 0.f ? 1u : 0u) - (small ? (121u << 3) : (120u << 3));
+  const float up = step < 0x1p-60f ? 0x1p60f : 1.f;  // so that no difference is below float32's smallest numbers
+  const uint32_t code = high - (__builtin_fmaf(border, step * up, -x * up) > 0.f ? 1u : 0u) - (small ? (121u << 3) : (120u << 3));
   return code < 0x7eu ? code : 0x7eu;
 }
 
 // States of 8 bits: twice eight numbers in a row a thread, 2048 apart; the 32 lanes of a block of 256 side by side.
 template <typename T, bool MASTER, typename A>
-__device__ __forceinline__ void step8(const Tensor& x, int64_t first, int64_t n, const Coefs& c, const Betas& b, float gs) {
+__device__ __forceinline__ void step8(const Tensor& x, int64_t first, int64_t n, const Coefs& c, const Betas& b, float gs,
+                                      bool scaled) {
 #pragma clang fp contract(off)  // each operation rounded but for the two written as one: states that do not hang on the build
   float p[2][8], g[2][8], steps[2][2];
   uint32_t codes[2][2][2];  // [numbers][m, r][words]
@@ -244,10 +247,14 @@ __device__ __forceinline__ void step8(const Tensor& x, int64_t first, int64_t n,
       m[4 * w] = m0[0], m[4 * w + 1] = m0[1], m[4 * w + 2] = m1[0], m[4 * w + 3] = m1[1];
       v[4 * w] = v0[0], v[4 * w + 1] = v0[1], v[4 * w + 2] = v1[0], v[4 * w + 3] = v1[1];
     }
+    if (scaled) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[k][e] *= gs;
+    }
     uint32_t top_m = 0, top_v = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float ge = g[k][e] * gs, r = v[e] * steps[k][1];
+      const float ge = g[k][e], r = v[e] * steps[k][1];
       m[e] = __builtin_fmaf(b.a1, ge, b.b1 * (m[e] * steps[k][0]));
       v[e] = __builtin_fmaf(b.a2, ge * ge, b.b2 * (r * r));
       root[e] = __builtin_amdgcn_sqrtf(v[e]);
@@ -261,35 +268,40 @@ __device__ __forceinline__ void step8(const Tensor& x, int64_t first, int64_t n,
     // the root's rounding keeps the order: the largest root is the largest's root
     const float mm = max32(top_m), mr = sqrtf(max32(top_v));
     const bool no_m = mm < kFlush, no_r = mr < kFlush;
-    const float fm = no_m ? 0.f : kTop / mm, fr = no_r ? 0.f : kTop / mr;
+    // 2^-120 / step, as long as that is one of float32's full numbers; exact_code() serves larger blocks
+    const float fm = no_m ? 0.f : kTop * 0x1p-120f * __builtin_amdgcn_rcpf(mm);
+    const float fr = no_r ? 0.f : kTop * 0x1p-120f * __builtin_amdgcn_rcpf(mr);
+    const uint32_t least = no_r ? 0u : 1u << 24;
     const float step_m = no_m ? 0.f : mm * (1.f / kTop), step_r = no_r ? 0.f : mr * (1.f / kTop);
     if ((threadIdx.x & 31) == 0 && i < n) {
       x.ms[i / kBlock] = step_m;
       x.vs[i / kBlock] = step_r;
     }
     const uint32_t u0 = (uint32_t)i * 2654435761u + (uint32_t)c.t * 2246822519u;
-    uint32_t cm[2], cr[2], near = ~0u, u = u0;
+    // v_sqrt_f32 is not exact enough below 2^-126, where the smallest roots of a block of roots up to 2^-43 come from
+    const bool far_off = max(mm, mr) > kTop * 0x1p6f || (mr < 0x1p-43f && !no_r);
+    uint32_t cm[2], cr[2], near = far_off ? 0u : ~0u, u = u0;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       uint32_t a[4], d[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float r = root[4 * w + e] * fr;
         a[e] = code_of(fabsf(m[4 * w + e]) * fm, u >> 12, near) | (__float_as_uint(m[4 * w + e]) & 0x80000000u);
-        d[e] = max(code_of(r, u & 0xfffffu, near), min(__float_as_uint(r), 1u) << 24);
+        // a root above 0 is above 2^-75: `least`, the code 1, or 0
+        d[e] = max(code_of(root[4 * w + e] * fr, u & 0xfffffu, near), min(__float_as_uint(root[4 * w + e]), least));
         u += 2654435761u;
       }
       cm[w] = upper_bytes(a);
       cr[w] = upper_bytes(d);
     }
-    if (near < (16u << 12)) {  // one lane in 4000
+    if (near < kNear) {  // one lane in 4000
       u = u0;
       cm[0] = cm[1] = cr[0] = cr[1] = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint32_t a = no_m ? 0u : exact_code(fabsf(m[e]), step_m, fm, u >> 12);
+        const uint32_t a = no_m ? 0u : exact_code(fabsf(m[e]), step_m, u >> 12);
         const float r = sqrtf(v[e]);
-        const uint32_t d = no_r ? 0u : max(exact_code(r, step_r, fr, u & 0xfffffu), r > 0.f ? 1u : 0u);
+        const uint32_t d = no_r ? 0u : max(exact_code(r, step_r, u & 0xfffffu), r > 0.f ? 1u : 0u);
         cm[e / 4] |= (a | ((__float_as_uint(m[e]) >> 24) & 0x80u)) << (e % 4 * 8);
         cr[e / 4] |= d << (e % 4 * 8);
         u += 2654435761u;
@@ -368,9 +380,9 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table table, Betas b, const 
   } else {
     const int64_t i = first + threadIdx.x * 8;
     if (wide) {
-      step8<T, MASTER, Access<true, NT>>(x, i, n, c, b, gs);
+      step8<T, MASTER, Access<true, NT>>(x, i, n, c, b, gs, grad_scale != nullptr);
     } else {
-      step8<T, MASTER, Access<false, false>>(x, i, n, c, b, gs);
+      step8<T, MASTER, Access<false, false>>(x, i, n, c, b, gs, grad_scale != nullptr);
     }
   }
 }

@@ -289,3 +289,26 @@ def test_other_stream(device):
         AdamW(twins).step()
     torch.cuda.current_stream().wait_stream(stream)
     assert all(torch.equal(p, q) for p, q in zip(params, twins))
+
+
+def test_blocks_of_any_size(device):
+    """Gradients from 1e-25 to 1e15: at the top the codes' scale leaves float32's full numbers, at the bottom the second moments
+    do; another way is taken there."""
+    p = torch.zeros(256 * 41, device=device, requires_grad=True)
+    gen = torch.Generator().manual_seed(11)
+    size = 10.0 ** torch.arange(-25, 16).double()
+    g = (torch.randn((41, 256), generator=gen).double() * size[:, None]).float().flatten()
+    opt = AdamW([p], **HYPER, state_bits=8)
+    for t in (1, 2):
+        before, p0 = ({"exp_avg": torch.zeros(p.shape), "exp_root": torch.zeros(p.shape), "exp_avg_scale": torch.zeros(41),
+                       "exp_root_scale": torch.zeros(41)} if t == 1 else _cpu(opt.state[p])), p.detach().cpu().clone()
+        p.grad = g.to(device)
+        opt.step()
+        after = _cpu(opt.state[p])
+        m0 = oracle.numbers(before["exp_avg"], before["exp_avg_scale"])
+        r0 = oracle.numbers(before["exp_root"], before["exp_root_scale"])
+        m, v = oracle.moments(g, m0, r0 * r0, HYPER["betas"])
+        for name, x, u, least in zip(("exp_avg", "exp_root"), (m, v.double().sqrt().float()), oracle.dither(g.numel(), t), (0.0, 2.0**-9)):
+            held, steps = oracle.hold(x, u, least)
+            assert torch.equal(after[name + "_scale"], steps), name
+            assert torch.equal(after[name].float(), held), name
