@@ -28,7 +28,9 @@ no CPU path: CPU tensors raise.
 """
 from __future__ import annotations
 
+import itertools
 import math
+import operator
 
 import numpy as np
 import torch
@@ -55,7 +57,8 @@ class _Plan:
     def __init__(self, params: list, states: list[dict], bits: int, master: bool):
         self.params, self.states, self.bits = params, states, bits
         self.names = (*_names(bits, master), "step")
-        self.held = [tuple(s[n] for n in self.names) for s in states]
+        self.take = operator.itemgetter(*self.names)
+        self.held = [self.take(s) for s in states]
         self.table = (_lib.AdamWTensor * len(params))()
         self.words = np.frombuffer(self.table, dtype=np.int64).reshape(len(params), _FIELDS)
         self.pointers = [p.data_ptr() for p in params]
@@ -71,9 +74,9 @@ class _Plan:
 
     def stands(self) -> bool:
         """Whether the weights and states are where they were."""
-        names = self.names
-        return all(p.data_ptr() == at for p, at in zip(self.params, self.pointers)) and all(
-            s.get(n) is x for s, held in zip(self.states, self.held) for n, x in zip(names, held))
+        held = itertools.chain.from_iterable(self.held)
+        now = itertools.chain.from_iterable(map(self.take, self.states))
+        return [p.data_ptr() for p in self.params] == self.pointers and all(map(operator.is_, held, now))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -180,26 +183,30 @@ class AdamW(torch.optim.Optimizer):
             bits, master = group["state_bits"], bool(group["master_weights"])
             held = self._plans.get(i)
             if held is None or held[0] != (bits, master) or len(held[1]) != len(params) \
-                    or not all(a is b for a, b in zip(held[1], params)) or not all(plan.stands() for plan in held[2]):
+                    or not all(map(operator.is_, held[1], params)) or not all(plan.stands() for plan in held[2]):
                 held = self._plans[i] = ((bits, master), params, self._plans_of(params, bits, master))
             for plan in held[2]:
                 self._launch(plan, group, grad_scale)
         return loss
 
     def _launch(self, plan: _Plan, group: dict, grad_scale) -> None:
-        grads = []
+        grads, at, dtype = [], [], plan.params[0].dtype
         for p in plan.params:
             g = p.grad
-            if g.layout != torch.strided or g.dtype != p.dtype:
+            if g.dtype is not dtype or g.layout is not torch.strided:
                 raise NotImplementedError(f"AdamW: a gradient of {g.dtype}, {g.layout} for a parameter of {p.dtype} is not "
                                           "supported (dense ones of the parameter's type are)")
-            grads.append(g if g.is_contiguous() else g.contiguous())
+            if not g.is_contiguous():
+                g = g.contiguous()
+                grads.append(g)
+            at.append(g.data_ptr())
         lr = group["lr"]
         lr_device = lr if isinstance(lr, torch.Tensor) and lr.is_cuda else None
-        _require_device(plan.params[0], *grads, *(t for t in (lr_device, grad_scale) if t is not None))
-        plan.words[:, _GRAD] = [g.data_ptr() for g in grads]
+        if lr_device is not None or grad_scale is not None:
+            _require_device(plan.params[0], lr_device, grad_scale)
+        plan.words[:, _GRAD] = at
         ws = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=plan.device)
-        _lib.call_on(plan.device, "pkm_adamw_step", plan.table, len(grads), plan.dtype, plan.bits,
+        _lib.call_on(plan.device, "pkm_adamw_step", plan.table, len(at), plan.dtype, plan.bits,
                      0.0 if lr_device is not None else float(lr), _lib.ptr(lr_device), *group["betas"], group["eps"],
                      group["weight_decay"], _lib.ptr(grad_scale), _lib.ptr(ws), plan.ws_bytes, _lib.stream_of(plan.device))
         torch.autograd.graph.increment_version(plan.params)  # as an update in place does
