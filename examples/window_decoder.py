@@ -2,9 +2,12 @@
 
     python examples/window_decoder.py [--steps 300] [--tokens 24]
 
-The layer attends through a window with sinks (modelos_amd.window_attention),
-reads a product-key memory (modelos_amd.pkm.memory.HashingMemory) in its
-feed-forward slot, and learns sequences in which every token has one successor.
+The layer reads its tokens (modelos_amd.token_embedding), attends through a window
+with sinks (modelos_amd.window_attention), reads a product-key memory
+(modelos_amd.pkm.memory.HashingMemory) in its feed-forward slot, and learns
+sequences in which every token has one successor: the loss comes from the hidden
+states and the tied table without logits (modelos_amd.linear_cross_entropy), the
+update from modelos_amd.adamw.AdamW with float32 masters.
 Then a left-padded batch of prompts goes through the same attention, its keys
 and values into an Int4KVCache, and new tokens are decoded one at a time from
 the cache. The script prints the losses and how many decoded tokens are right.
@@ -21,9 +24,12 @@ import torch.nn.functional as F
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
+from modelos_amd.adamw import AdamW  # noqa: E402
 from modelos_amd.kv_cache import Int4KVCache  # noqa: E402
+from modelos_amd.linear_cross_entropy import linear_cross_entropy  # noqa: E402
 from modelos_amd.pkm.memory import HashingMemory  # noqa: E402
 from modelos_amd.rmsnorm import QueryRMSNorm  # noqa: E402
+from modelos_amd.token_embedding import TokenEmbedding  # noqa: E402
 from modelos_amd.window_attention import window_attention  # noqa: E402
 
 
@@ -58,7 +64,7 @@ class WindowAttention(nn.Module):
 class Decoder(nn.Module):
     def __init__(self, vocab=64, width=256, heads=4, kv_heads=2, dim=64, window=32, sinks=4, positions=512):
         super().__init__()
-        self.embed, self.place = nn.Embedding(vocab, width), nn.Embedding(positions, width)
+        self.embed, self.place = TokenEmbedding(vocab, width), TokenEmbedding(positions, width)
         self.norm1, self.norm2, self.norm3 = (QueryRMSNorm(width) for _ in range(3))
         self.attention = WindowAttention(width, heads, kv_heads, dim, window, sinks)
         self.memory = HashingMemory(input_dim=width, output_dim=width, mem_k_dim=128, mem_heads=2, mem_knn=8,
@@ -70,14 +76,20 @@ class Decoder(nn.Module):
     def inputs(self, tokens, positions):
         return self.embed(tokens) + self.place(positions)
 
+    def hidden(self, x):
+        return self.norm3(x + self.memory(self.norm2(x))[0])
+
     def head(self, x):
-        x = x + self.memory(self.norm2(x))[0]
-        return F.linear(self.norm3(x), self.embed.weight)
+        return F.linear(self.hidden(x), self.embed.weight)
 
     def forward(self, tokens, positions, starts=None):
         x = self.inputs(tokens, positions)
         y, k, v = self.attention(self.norm1(x), starts)
         return self.head(x + y), k, v
+
+    def loss(self, tokens, positions, labels):
+        x = self.inputs(tokens, positions)
+        return linear_cross_entropy(self.hidden(x + self.attention(self.norm1(x))[0]), self.embed.weight, labels)
 
     def decode(self, tokens, cache, table, lengths):
         x = self.inputs(tokens, (lengths - 1)[:, None].long())
@@ -94,13 +106,12 @@ def walks(batch: int, length: int, vocab: int, generator: torch.Generator) -> to
 
 def train(model: Decoder, steps: int, generator: torch.Generator, batch=16, length=129, vocab=64) -> list[float]:
     device = model.embed.weight.device
-    optimizer = torch.optim.AdamW(model.parameters(), lr=2e-3)
+    optimizer = AdamW(model.parameters(), lr=2e-3, master_weights=True)
     positions = torch.arange(length - 1, device=device).expand(batch, -1)
     losses = []
     for _ in range(steps):
         tokens = walks(batch, length, vocab, generator).to(device)
-        logits, _, _ = model(tokens[:, :-1], positions)
-        loss = F.cross_entropy(logits.flatten(0, 1).float(), tokens[:, 1:].flatten())
+        loss = model.loss(tokens[:, :-1], positions, tokens[:, 1:])
         optimizer.zero_grad(set_to_none=True)
         loss.backward()
         optimizer.step()
