@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kTile = 256, kDepth = 64, kHalf = 32768, kStage = 2 * kHalf;
 constexpr int kThreads = 512;
-constexpr float kLog2e = 1.44269504f;
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
 enum Product { kLoss, kGrads, kDx, kDw };
 
@@ -50,7 +50,9 @@ struct CeArgs {
   int64_t x_stride, w_stride;  // bytes
   const int32_t* count;  // kept tokens
   const int32_t* label;  // [npad]
-  const float* ref;      // [npad] the label's logit, the softmax sums' reference
+  const float* ref;      // [npad] the label's logit to a few roundings, the softmax sums' reference
+  float* target;         // [npad] the label's logit as the product gives it
+  const float* loss;     // [npad]
   const float* lse;      // [npad]
   const float* weight;   // [npad] of the tokens' gradients, or NULL: `lift` for all
   float2* sums;          // [2 * vocab tiles][npad] reference and sum of exponentials
@@ -59,6 +61,7 @@ struct CeArgs {
   Scale scale;
   int64_t vocab, v0;  // v0: the piece's first entry
   int32_t piece, dim, npad, dcols, splits, add;
+  int32_t pair;  // few tokens: d as two numbers of 16 bits, the second ones in the token slots behind the first
 };
 
 __device__ __forceinline__ int perm16(int k) { return ((k & 3) << 2) | ((k >> 2) & 3); }
@@ -241,8 +244,9 @@ __device__ __forceinline__ void cut(f32x16_t (&acc)[MT][NU], int64_t left, int h
 }
 
 // The sum of the exponentials of a wave's entries for the lane's token of column block u, against the token's reference: the
-// label's logit, which is one of the summands, so that what underflows beside it is nothing. Where it overflows, the entries'
-// own largest logit takes the reference's place.
+// label's logit, whose own exponential is 1, so that what underflows beside it is nothing. Where it overflows, the entries' own
+// largest logit takes the reference's place. The reference's product with log2(e) is rounded once for all entries; what that
+// adds to all exponents alike comes off the sum.
 template <int MT, int NU>
 __device__ __forceinline__ float2 sum_of(const f32x16_t (&acc)[MT][NU], int u, float ref) {
   float sum = 0.f;
@@ -254,6 +258,7 @@ __device__ __forceinline__ float2 sum_of(const f32x16_t (&acc)[MT][NU], int u, f
     batch();
   }
   sum += swap_halves(sum);
+  sum -= sum * (__builtin_fmaf(ref, kLog2e, c) * kLn2);
   const bool over = !(sum < 0x1p120f);
   if (__any(over)) {
     float top = -INFINITY;
@@ -275,6 +280,27 @@ __device__ __forceinline__ float2 sum_of(const f32x16_t (&acc)[MT][NU], int u, f
   return make_float2(ref, sum);
 }
 
+// The logit of the label, yr rows (less 4 h) below the wave's first, into the token's place, and out of the sum: a loss near 0
+// is the logarithm of 1 + the others' exponentials, which the label's 1 among them would round.
+template <int MT, int NU>
+__device__ __forceinline__ void take_target(f32x16_t (&acc)[MT][NU], int u, int yr, float* to) {
+  const bool own = yr >= 0 && yr < 32 * MT && (yr & 4) == 0;
+  if (!__any(own)) return;
+  asm volatile("" : "+v"(yr));  // as in cut()
+  float z = 0.f;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const bool here = row_of(t, i) == yr;
+      z = here ? acc[t][u][i] : z;
+      acc[t][u][i] = here ? -INFINITY : acc[t][u][i];
+    }
+    batch();
+  }
+  if (own) *to = z;
+}
+
 // Two such sums as one.
 __device__ __forceinline__ float2 joined(float2 a, float2 b) {
   if (b.x > a.x) return make_float2(b.x, a.y * exp2_raw((a.x - b.x) * kLog2e) + b.y);
@@ -287,16 +313,33 @@ __device__ __forceinline__ void end_loss(const CeArgs& a, acc_t& acc, const Resu
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int j = r.n * kTile + (wave & 3) * 64 + 32 * u + (lane & 31);
+    take_target(acc, u, a.label[j] - v0 - 4 * h, a.target + j);
     const float2 sum = sum_of(acc, u, a.ref[j]);
     if (h == 0) a.sums[(int64_t)(2 * r.m + (wave >> 2)) * a.npad + j] = sum;
   }
 }
 
-// d of a wave's entries, from v0 of the piece on, for the lane's token j of column block u, rounded, in blocks.
-// c: - lse log2(e), -infinity for a token that is not kept; y: the label's place from v0 on; ref: its logit.
+// The label's d: exp(l - lse) - 1 = exp(- loss) - 1, with its weight.
+__device__ __forceinline__ float label_d(float loss, float weight) { return expm1f(-loss) * weight; }
+
+// Two numbers of 16 bits for each of f: its rounding and, `low`, the rounding of what that left.
+template <typename T>
+__device__ __forceinline__ u32x4_t rounded(const float (&f)[8], bool low) {
+  u32x4_t x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] = pack2<T>(f[2 * e], f[2 * e + 1]);
+    if (low) x[e] = pack2<T>(f[2 * e] - unpack1<T>(x[e] & 0xffffu), f[2 * e + 1] - unpack1<T>(x[e] >> 16));
+  }
+  return x;
+}
+
+// d of a wave's entries, from v0 of the piece on, for the lane's token j of column block u, rounded, in blocks; with `second`,
+// what the rounding left in the blocks that many bytes further.
+// c: - lse log2(e), -infinity for a token that is not kept; y: the label's place from v0 on.
 template <typename T, int MT, int NU>
 __device__ __forceinline__ void grads_of(const CeArgs& a, const f32x16_t (&acc)[MT][NU], int u, int64_t v0, int j, float c,
-                                         float weight, int64_t y, float ref, int lane) {
+                                         float weight, int64_t y, float loss, int64_t second, int lane) {
   const int h = lane >> 5;
   const int64_t row = (int64_t)(a.npad / 32) * 1024;
   uint8_t* const to = a.d + (v0 / 16) * row + (int64_t)(j >> 5) * 1024;
@@ -307,19 +350,22 @@ __device__ __forceinline__ void grads_of(const CeArgs& a, const f32x16_t (&acc)[
       float f[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = exp2_raw(__builtin_fmaf(acc[t][u][8 * s + e], kLog2e, c)) * weight;
-      const u32x4_t x = {pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7])};
-      *(u32x4_t*)(to + (2 * t + s) * row + block_lane(s, h, lane & 31) * 16) = x;
+      uint8_t* const at = to + (2 * t + s) * row + block_lane(s, h, lane & 31) * 16;
+      *(u32x4_t*)at = rounded<T>(f, false);
+      if (second) *(u32x4_t*)(at + second) = rounded<T>(f, true);
     }
     batch();
   }
-  // the label's number is exp(l - lse) - 1, rounded once: it takes the place of the one written above
+  // the label's number takes the place of the one written above
   const bool own = y >= 0 && y < 32 * MT;
   if (__any(own)) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (own && h == 0) {
-      const float x = (exp2_raw(__builtin_fmaf(ref, kLog2e, c)) - 1.f) * weight;
-      *(uint16_t*)(to + (y >> 4) * row + block_lane((y >> 4) & 1, (y >> 2) & 1, lane) * 16 + ((y >> 3) & 1) * 8 + (y & 3) * 2) =
-          (uint16_t)pack2<T>(x, x);
+      const float x = label_d(loss, weight);
+      uint8_t* const at = to + (y >> 4) * row + block_lane((y >> 4) & 1, (y >> 2) & 1, lane) * 16 + ((y >> 3) & 1) * 8 + (y & 3) * 2;
+      const uint32_t high = pack2<T>(x, x) & 0xffffu;
+      *(uint16_t*)at = (uint16_t)high;
+      if (second) *(uint16_t*)(at + second) = (uint16_t)pack2<T>(x - unpack1<T>(high), 0.f);
     }
   }
 }
@@ -333,7 +379,7 @@ __device__ __forceinline__ void end_grads(const CeArgs& a, acc_t& acc, const Res
     const int j = r.n * kTile + (wave & 3) * 64 + 32 * u + (lane & 31);
     const bool kept = j < count;
     const float c = kept ? -a.lse[j] * kLog2e : -INFINITY, weight = !kept ? 0.f : a.weight ? a.weight[j] : a.scale.lift;
-    grads_of<T>(a, acc, u, v0, j, c, weight, kept ? (int64_t)a.label[j] - a.v0 - v0 : -1, a.ref[j], lane);
+    grads_of<T>(a, acc, u, v0, j, c, weight, kept ? (int64_t)a.label[j] - a.v0 - v0 : -1, a.loss[j], 0, lane);
   }
 }
 
@@ -404,10 +450,11 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
   const int64_t entries = min((int64_t)a.piece, a.vocab - a.v0);  // of the piece
   const int token_tiles = (n + kTile - 1) / kTile, entry_tiles = (int)((entries + kTile - 1) / kTile),
             dim_tiles = a.dcols / kTile;
+  const int token_steps = (n + kDepth - 1) / kDepth;
   const Order order =
       P == kLoss || P == kGrads ? Order(entry_tiles, token_tiles, dpad / kDepth, 1)
       : P == kDx ? Order(token_tiles, dim_tiles, (int)((entries + kDepth - 1) / kDepth), splits_of(token_tiles, dim_tiles, a.piece / kDepth))
-                 : Order(entry_tiles, dim_tiles, (n + kDepth - 1) / kDepth, a.splits);
+                 : Order(entry_tiles, dim_tiles, token_steps * (a.pair ? 2 : 1), a.splits);
   if constexpr (P == kDw) {
     if (n == 0 && a.splits == 1) {  // no token counts: zeros
       const int64_t first = a.v0 * a.dim, all = entries * a.dim;
@@ -450,7 +497,7 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
       if (part < 4)
         load_entries(a.d, to, q, load_step, ahead.m, a.npad, wave, lane);
       else
-        cb.load(to, q, load_step, a.x_stride, n, wave, lane);
+        cb.load(to, q, load_step < token_steps ? load_step : load_step - token_steps, a.x_stride, n, wave, lane);
     }
   };
   if (!ahead.next(order, true)) return;
@@ -568,7 +615,7 @@ template <typename T, Product P>
 __global__ __launch_bounds__(kThreads, 2) void ce_few(const CeArgs a) {
   static_assert(P == kLoss || P == kGrads, "the products with tokens for columns");
   __shared__ __align__(1024) uint8_t smem[kRing * kFewStage];
-  __shared__ float ref_s[kFew], lse_s[kFew], weight_s[kFew];
+  __shared__ float ref_s[kFew], lse_s[kFew], weight_s[kFew];  // kGrads: ref_s is the loss
   __shared__ int32_t label_s[kFew];
   __shared__ float2 sum_s[kFewM / 32][kFewN];
   lds_u8* const lds = (lds_u8*)smem;
@@ -583,7 +630,7 @@ __global__ __launch_bounds__(kThreads, 2) void ce_few(const CeArgs a) {
   run = ahead;
   if (tid < kFew) {
     const bool kept = tid < n;
-    ref_s[tid] = a.ref[tid];
+    ref_s[tid] = P == kLoss ? a.ref[tid] : a.loss[tid];
     label_s[tid] = a.label[tid];
     if constexpr (P == kGrads) {
       lse_s[tid] = kept ? -a.lse[tid] * kLog2e : -INFINITY;
@@ -637,6 +684,7 @@ __global__ __launch_bounds__(kThreads, 2) void ce_few(const CeArgs a) {
     const int column = (wave & 1) * 32 + (lane & 31), j = run.n * kFewN + column;
     cut(acc, entries - v0, h);
     if constexpr (P == kLoss) {
+      take_target(acc, 0, (int)(label_s[j] - v0) - 4 * h, a.target + j);
       const float2 sum = sum_of(acc, 0, ref_s[j]);
       if (h == 0) sum_s[wave >> 1][column] = sum;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -650,7 +698,8 @@ __global__ __launch_bounds__(kThreads, 2) void ce_few(const CeArgs a) {
         a.sums[(int64_t)run.m * a.npad + run.n * kFewN + tid] = all;
       }
     } else {
-      grads_of<T>(a, acc, 0, v0, j, lse_s[j], weight_s[j], label_s[j] < 0 ? -1 : label_s[j] - a.v0 - v0, ref_s[j], lane);
+      grads_of<T>(a, acc, 0, v0, j, lse_s[j], weight_s[j], label_s[j] < 0 ? -1 : label_s[j] - a.v0 - v0, ref_s[j],
+                  (int64_t)order.n * kFewN / 32 * 1024, lane);
     }
     acc[0][0] = f32x16_t{};
     if (!run.next(order, false)) break;
@@ -758,8 +807,8 @@ __global__ __launch_bounds__(1024) void ce_prepare(const T* __restrict__ x, int6
 // lse and loss of 32 tokens from the tiles' sums. losses: one for each token. mean: else the workgroup that ends last adds
 // all workgroups' losses, in order.
 __global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(Header* head, const float2* __restrict__ sums, int parts,
-                                                                    int npad, const float* __restrict__ ref,
-                                                                    const int32_t* __restrict__ token, float* __restrict__ lse,
+                                                                    int npad, const float* __restrict__ target,
+                                                                    const int32_t* __restrict__ token, float* __restrict__ lse, float* __restrict__ own_loss,
                                                                     float* losses, float* block_sums, float* total, int mean) {
   __shared__ float2 s[kJoinSlices][kJoinTokens];
   __shared__ float sum_s[kJoinSlices / 2];
@@ -790,9 +839,12 @@ __global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(Header* head
     if (j < count) {
       for (int k = 1; k < kJoinSlices; ++k)
         if (s[k][t].y != 0.f) add(s[k][t].x, s[k][t].y);  // NaN counts as something
-      const float log_sum = __builtin_amdgcn_logf(sum) * 0.693147180559945f;
-      lse[j] = m + log_sum;
-      loss = log_sum + (m - ref[j]);
+      // log(1 + the others' exponentials against the label's), for exponents of any size
+      const float z = target[j], x = logf(sum) + (m - z);
+      loss = fmaxf(x, 0.f) + log1pf(expf(-fabsf(x)));
+      if (x != x) loss = x;
+      lse[j] = z + loss;
+      own_loss[j] = loss;
       if (losses) losses[token[j]] = loss;
     }
 #pragma unroll
@@ -839,26 +891,35 @@ __global__ __launch_bounds__(1024) void ce_weights(Header* head, const float* __
   if (tid == 0) head->scale = unit / lift;
 }
 
-// Rows of results: the splits' sums in order, scaled and rounded, a workgroup a row at a time. dx: row i from row place[i],
-// zeros if that is negative; `splits` is 0, the kept tokens give it. dW (place NULL): row i from row i; few kept tokens
-// leave some splits without a step, which wrote nothing.
+// What rounding left of the label's d, the one large number among a token's.
 template <typename T>
-__global__ __launch_bounds__(256) void ce_rows(const Scale scale, const int32_t* __restrict__ place, int64_t rows,
-                                               const float* __restrict__ parts, int splits, int piece, int dcols, int dim,
-                                               T* __restrict__ out) {
-  const float f = scale();
-  const int n = *scale.count, tiles = (n + kTile - 1) / kTile, steps = (n + kDepth - 1) / kDepth;
-  int64_t pad = piece;
+__device__ __forceinline__ float label_rest(const CeArgs& a, int64_t j) {
+  const float x = label_d(a.loss[j], a.weight ? a.weight[j] : a.scale.lift);
+  return x - unpack1<T>(pack2<T>(x, x) & 0xffffu);
+}
+
+// Rows of results: the splits' sums in order, scaled and rounded, a workgroup a row at a time. dx (place): row i from row
+// place[i], zeros if that is negative, with what the rounding left of d: of all of it from a row of its own (pair), else of the
+// label's times its row of the weight; `splits` is 0, the kept tokens give it. dW (place NULL): row i from row i; few kept tokens leave some splits without a step, which
+// wrote nothing.
+template <typename T>
+__global__ __launch_bounds__(256) void ce_rows(const CeArgs a, const int32_t* __restrict__ place, int64_t rows,
+                                               const float* __restrict__ parts, int splits, T* __restrict__ out) {
+  const float f = a.scale();
+  const int n = *a.count, tiles = (n + kTile - 1) / kTile, steps = (n + kDepth - 1) / kDepth, dim = a.dim;
+  int64_t pad = a.piece;
   if (place) {
-    splits = splits_of(tiles, dcols / kTile, piece / kDepth);
+    splits = splits_of(tiles, a.dcols / kTile, a.piece / kDepth);
     pad = tiles * kTile;
   }
   for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
     const int64_t j = place ? place[i] : i;
+    const float rest = place && j >= 0 && !a.pair ? label_rest<T>(a, j) : 0.f;
+    const uint8_t* const wy = a.w + (place && j >= 0 ? a.label[j] * a.w_stride : 0);
     for (int d = threadIdx.x * 4; d < dim; d += 1024) {
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      const auto add = [&](int s) {
-        const float4 v = *(const float4*)(parts + (s * pad + j) * dcols + d);
+      const auto add = [&](int s, int64_t row) {
+        const float4 v = *(const float4*)(parts + (s * pad + row) * a.dcols + d);
         sum.x += v.x;
         sum.y += v.y;
         sum.z += v.z;
@@ -866,17 +927,24 @@ __global__ __launch_bounds__(256) void ce_rows(const Scale scale, const int32_t*
       };
       if (place && j >= 0) {
 #pragma unroll 8
-        for (int s = 0; s < splits; ++s) add(s);
+        for (int s = 0; s < splits; ++s) add(s, j);
+        if (a.pair)
+          for (int s = 0; s < splits; ++s) add(s, j + steps * kDepth);
+        const uint2 y = *(const uint2*)(wy + 2 * d);  // rows reach to a multiple of 8
+        sum.x = __builtin_fmaf(rest, unpack1<T>(y.x & 0xffffu), sum.x);
+        sum.y = __builtin_fmaf(rest, unpack1<T>(y.x >> 16), sum.y);
+        sum.z = __builtin_fmaf(rest, unpack1<T>(y.y & 0xffffu), sum.z);
+        sum.w = __builtin_fmaf(rest, unpack1<T>(y.y >> 16), sum.w);
       } else if (!place) {
         for (int s = 0; s < splits; ++s)
-          if ((int64_t)steps * s / splits < (int64_t)steps * (s + 1) / splits) add(s);
+          if ((int64_t)steps * s / splits < (int64_t)steps * (s + 1) / splits) add(s, j);
       }
       uint16_t* const to = (uint16_t*)(out + i * dim + d);
-      const uint32_t a = j < 0 ? 0u : pack2<T>(sum.x * f, sum.y * f), b = j < 0 ? 0u : pack2<T>(sum.z * f, sum.w * f);
+      const uint32_t p = j < 0 ? 0u : pack2<T>(sum.x * f, sum.y * f), q = j < 0 ? 0u : pack2<T>(sum.z * f, sum.w * f);
       if ((dim & 3) == 0) {
-        *(uint2*)to = make_uint2(a, b);
+        *(uint2*)to = make_uint2(p, q);
       } else {
-        const uint16_t four[4] = {(uint16_t)a, (uint16_t)(a >> 16), (uint16_t)b, (uint16_t)(b >> 16)};
+        const uint16_t four[4] = {(uint16_t)p, (uint16_t)(p >> 16), (uint16_t)q, (uint16_t)(q >> 16)};
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (d + k < dim) to[k] = four[k];
@@ -892,7 +960,7 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // What the forward leaves for the backward, in one buffer.
 struct Kept {
-  int64_t npad, dpad, place, token, label, ref, lse, x, bytes;
+  int64_t npad, dpad, place, token, label, ref, target, lse, loss, x, bytes;
 };
 bool plan_kept(int64_t tokens, int64_t dim, Kept* k) {
   if (tokens < 0 || dim < 1 || tokens >= (1ll << 22) || dim > 65536) return false;
@@ -902,8 +970,10 @@ bool plan_kept(int64_t tokens, int64_t dim, Kept* k) {
   k->token = k->place + k->npad * 4;
   k->label = k->token + k->npad * 4;
   k->ref = k->label + k->npad * 4;
-  k->lse = k->ref + k->npad * 4;
-  k->x = k->lse + k->npad * 4;
+  k->target = k->ref + k->npad * 4;
+  k->lse = k->target + k->npad * 4;
+  k->loss = k->lse + k->npad * 4;
+  k->x = k->loss + k->npad * 4;
   k->bytes = k->x + k->npad * k->dpad * 2;
   return true;
 }
@@ -965,7 +1035,7 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
                 const Forward& f, hipStream_t st) {
   Header* const head = (Header*)kept;
   int32_t *place = (int32_t*)(kept + k.place), *token = (int32_t*)(kept + k.token), *label = (int32_t*)(kept + k.label);
-  float *ref = (float*)(kept + k.ref), *lse = (float*)(kept + k.lse), *losses = reduction == 0 ? loss : nullptr;
+  float *ref = (float*)(kept + k.ref), *target = (float*)(kept + k.target), *lse = (float*)(kept + k.lse), *losses = reduction == 0 ? loss : nullptr;
   const int wide = (((uintptr_t)x | (uintptr_t)w) & 15) == 0 && ((x_stride | w_stride | dim) & 7) == 0;
   const unsigned blocks = (unsigned)((tokens < 1 ? 1 : tokens) + kPrepareRows - 1) / kPrepareRows;
   if (bits == 64)
@@ -984,6 +1054,7 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
   a.count = &head->count;
   a.label = label;
   a.ref = ref;
+  a.target = target;
   a.sums = (float2*)(ws + f.sums);
   a.vocab = vocab;
   a.piece = (int32_t)up(vocab, kTile);
@@ -995,7 +1066,7 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
   const int64_t joins = (tokens < 1 ? 1 : tokens) + kJoinTokens - 1;
   if (reduction == 0 && tokens == 0) return pkm_check_launch("pkm_linear_ce_fwd");  // no loss to write
   hipLaunchKernelGGL(ce_join, dim3((unsigned)(joins / kJoinTokens)), dim3(kJoinTokens * kJoinSlices), 0, st, head,
-                     (const float2*)a.sums, (int)((vocab + 127) / 128), (int)k.npad, ref, token, lse, losses,
+                     (const float2*)a.sums, (int)((vocab + 127) / 128), (int)k.npad, target, token, lse, (float*)(kept + k.loss), losses,
                      (float*)(ws + f.block_sums), loss, reduction == 1);
   return pkm_check_launch("pkm_linear_ce_fwd");
 }
@@ -1019,7 +1090,7 @@ int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, in
   a.d = ws + b.d;
   a.count = &head->count;
   a.label = (const int32_t*)(kept + k.label);
-  a.ref = (const float*)(kept + k.ref);
+  a.loss = (const float*)(kept + k.loss);
   a.lse = (const float*)(kept + k.lse);
   a.dw = (uint8_t*)dw;
   a.scale = Scale{&head->scale, reduction == 0 ? nullptr : grad, &head->count, lift, reduction == 1};
@@ -1028,6 +1099,7 @@ int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, in
   a.dim = (int32_t)dim;
   a.npad = (int32_t)k.npad;
   a.dcols = (int32_t)b.dcols;
+  a.pair = tokens <= kFew;
   float *dx_parts = (float*)(ws + b.dx), *dw_parts = (float*)(ws + b.dw);
   for (int64_t v0 = 0; v0 < vocab; v0 += b.piece) {
     a.v0 = v0;
@@ -1046,8 +1118,7 @@ int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, in
     }
   }
   const auto rows = [&](const int32_t* from, int64_t n, const float* parts, int64_t splits, void* out) {
-    hipLaunchKernelGGL(ce_rows<T>, dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, st, a.scale, from, n, parts, (int)splits,
-                       (int)b.piece, (int)b.dcols, (int)dim, (T*)out);
+    hipLaunchKernelGGL(ce_rows<T>, dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, st, a, from, n, parts, (int)splits, (T*)out);
   };
   if (dx && tokens > 0) rows(place, tokens, dx_parts, 0, dx);
   if (dw && b.dw_splits > 1) rows(nullptr, vocab, dw_parts, b.dw_splits, dw);

@@ -235,3 +235,34 @@ def test_few_of_many_tokens_count(device):
         some = labels.clone()
         some[torch.randperm(3000, generator=gen)[: 3000 - n].to(device)] = -100
         _check(x, w, some, "mean", gen)
+
+
+@pytest.mark.parametrize("n", [60, 300])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_losses_near_nothing(n, dtype, device):
+    """Sure tokens: losses of 1e-2 down to 1e-11 and their gradients keep their precision. log(1 + s) of a small s is off
+    by as much of itself as s is, and s by the logits' errors."""
+    x, w, labels, gen = _inputs(n, 400, 64, dtype, device, lean=0.0)
+    with torch.no_grad():
+        far = torch.linspace(10, 40, n)[:, None].to(device) * w[labels].float()
+        x += (far / w[labels].float().square().sum(1, keepdim=True)).to(dtype)
+    loss, grad, (dx, dw) = _both(x, w, labels, "none", gen)
+    xx, ww = x.detach().cpu().double(), w.detach().cpu().double()
+    logits = xx @ ww.T
+    y = labels.cpu()[:, None]
+    others = (logits - logits.gather(1, y)).scatter(1, y, -float("inf"))
+    want = torch.log1p(others.exp().sum(1))
+    assert want.min() < 1e-10 and want.max() > 1e-3  # what the inputs are
+    # two logits of D products each, their difference and its exponential, the sums
+    e = 2.0**-24 * (2 * (64 + 2) * (xx.abs() @ ww.abs().T).max(1).values + 8 * others[others > -1e9].abs().max() + 60)
+    assert ((loss.cpu().double() - want).abs() <= e * want).all()
+    g = grad.double()[:, None]
+    p = others.exp() / (1 + others.exp().sum(1, keepdim=True))
+    d = torch.where(torch.arange(400) == y, torch.expm1(-want)[:, None], p) * g
+    u, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    # f16: the smallest of d, 2^-24 below 2^14 times the largest gradient
+    lost = 2.0**-38 * g.abs().max() if dtype == F16 else 0.0
+    for got, exact, size in ((dx, d @ ww, d.abs() @ ww.abs()), (dw, d.T @ xx, d.T.abs() @ xx.abs())):
+        other = (torch.ones_like(d) @ ww.abs() if got is dx else torch.ones_like(d).T @ xx.abs()) * lost
+        bound = (u + 4 * e.max() + 2.0**-17) * size + other + u * exact.abs() + tiny
+        assert ((got.cpu().double() - exact).abs() <= bound).all()
