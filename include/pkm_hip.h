@@ -793,7 +793,7 @@ int pkm_linear_ce_fwd(const void* x, int64_t x_stride, int64_t tokens, const voi
  * products (f16: with a power of two taken out); sums are float32 in a fixed order.
  */
 size_t pkm_linear_ce_bwd_workspace_size(int64_t tokens, int64_t vocab, int64_t dim);
-int pkm_linear_ce_bwd(void* kept, size_t kept_bytes, int64_t tokens, const void* weight, int64_t w_stride,
+int pkm_linear_ce_bwd(const void* kept, size_t kept_bytes, int64_t tokens, const void* weight, int64_t w_stride,
                       int64_t vocab, int64_t dim, int dtype, const float* grad_loss, int reduction,
                       void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -15,7 +15,8 @@ and the same on every run. Blocks whose largest number is below 2^-110 are held
 as zeros.
 
 16-bit weights lose updates below half their spacing; `master_weights=True` keeps a
-float32 copy ("master") that the update is made to, the weight its rounding.
+float32 copy ("master") that the update is made to, the weight its rounding: who
+changes such a weight otherwise changes its master too, or the next step undoes it.
 
 Steps are counted on the device, one counter a tensor, and nothing synchronises: a
 step can be captured into a graph (after a first one, or a loaded state, has made
@@ -91,6 +92,9 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
+        for group in self.param_groups:  # of an optimizer without these options
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
         self._plans = {}
 
     def add_param_group(self, param_group: dict) -> None:
@@ -174,7 +178,8 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1):
-            raise ValueError(f"AdamW.step: grad_scale has to be one float32 number, got {grad_scale.dtype} {tuple(grad_scale.shape)}")
+            raise ValueError(f"AdamW.step: grad_scale has to be one float32 number, got {grad_scale.dtype} "
+                             f"{tuple(grad_scale.shape)}")
         for i, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:

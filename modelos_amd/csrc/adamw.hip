@@ -8,21 +8,23 @@
 // range: v's exponents are twice r's. A number a >= 0 in units of its step, 2^e <= a < 2^(e + 1), e >= -6, becomes
 // floor(a 2^(3 - e) + u) 2^(e - 3): rounded up or down with a dither u in [0, 1) that runs evenly through all values over
 // the steps, so that what a step adds below a code's spacing is not lost on average. Nearest rounding would lose it every time:
-// with b2 = 0.999 a state falls by 0.05 % a step, a twentieth to an hundredth of half a spacing. r > 0 stays above 0
+// with b2 = 0.999 a root falls by 0.05 % of itself a step, half a spacing is 3 to 6 %. r > 0 stays above 0
 // (2^-9 at least), or m would be divided by nothing.
 //
-// Every number is read once and written once: the step is bound by memory. A workgroup takes 4096 numbers of one tensor;
-// the tensors' pointers travel in the kernel's arguments (48 tensors a launch), so a step copies nothing to the device.
+// Every number is read once and written once: the step is bound by memory. 361 M bf16 numbers with masters in 127 tensors:
+// 1.74 ms (5.8 TB/s); 2^30 bf16 numbers with states in 8 bits 1.78 ms (6.0 TB/s, 50 vector operations a number, which take as
+// long: with 65 it was 1.96). A workgroup takes 4096 numbers of one tensor; the tensors' pointers travel in the kernel's
+// arguments (48 tensors a launch), so a step copies nothing to the device.
 #include "pkm_common.h"
 
 namespace pkm {
 namespace {
 
-constexpr int kTensors = 48;     // of a launch: 72 bytes each of the 4 KB of arguments
-constexpr int kChunk = 4096;         // numbers of a workgroup: 256 threads, 16 each
-constexpr int kSteps = 256;      // step counters of a launch of the first kernel
-constexpr int kBlock = 256;      // numbers that share a step
-constexpr float kTop = 448.f;    // e4m3's largest number
+constexpr int kTensors = 48;  // of a launch: 72 bytes each of the 4 KB of arguments
+constexpr int kChunk = 4096;  // numbers of a workgroup: 256 threads, 16 each
+constexpr int kSteps = 256;   // step counters of a launch of the first kernel
+constexpr int kBlock = 256;   // numbers that share a step
+constexpr float kTop = 448.f; // e4m3's largest number
 constexpr float kFlush = 0x1p-110f;  // a block whose largest number is below is held as zeros: 448 / max stays finite
 
 struct Tensor {
@@ -429,8 +431,8 @@ extern "C" int pkm_adamw_step(const pkm_adamw_tensor_t* tensors, int64_t count, 
   for (int64_t i = 0; i < count; ++i) {
     const pkm_adamw_tensor_t& t = tensors[i];
     PKM_REQUIRE(t.numel >= 0, PKM_ERR_INVALID_ARGUMENT, "pkm_adamw_step: tensor %lld has a negative size", (long long)i);
-    PKM_REQUIRE(t.numel < (1ll << 35), PKM_ERR_UNSUPPORTED, "pkm_adamw_step: tensor %lld has %lld numbers (fewer than 2^35 are supported)",
-                (long long)i, (long long)t.numel);
+    PKM_REQUIRE(t.numel < (1ll << 35), PKM_ERR_UNSUPPORTED,
+                "pkm_adamw_step: tensor %lld has %lld numbers (fewer than 2^35 are supported)", (long long)i, (long long)t.numel);
     PKM_REQUIRE(t.step, PKM_ERR_INVALID_ARGUMENT, "pkm_adamw_step: tensor %lld has no step counter", (long long)i);
     if (t.numel == 0) continue;
     PKM_REQUIRE(t.param && t.grad && t.exp_avg && t.second, PKM_ERR_INVALID_ARGUMENT,

@@ -18,6 +18,12 @@
 // a step of 16 while the matrix cores work on the one before, across tiles and also across results: the grid is one
 // workgroup a CU, and the next result's tiles load while this one's epilogue runs. One barrier a 64.
 //
+// Measured, 16384 tokens, 151936 entries, 1024 wide, bf16: the forward's product 4.2 ms (1210 TFLOP/s), of a piece of 15360
+// entries d 0.495, dW 0.461 and dx 0.428 ms (1040 to 1200); beside them 0.1 ms (copy of the tokens 23 us, join of the tiles'
+// sums 47, dx's rounding 36). The matrix cores are busy 52 to 61 % of the cycles at 1.6 to 2.0 GHz; plain library products of
+// the pieces' shapes take 0.457, 0.668 and 0.444 ms at 1.5 to 1.64 GHz and 50 to 70 %: the clock falls as the load rises, and
+// neither fewer LDS cycles (bank conflicts were half of them) nor loads spread between the products moved the time.
+//
 // d lies as the epilogue's registers hold it, in blocks of 16 vocabulary entries x 32 tokens (1 KB, 16 bytes a lane): dx's
 // product reads a block as a matrix operand as it is, dW's through the transposing LDS reads.
 #include "attn_common.h"
@@ -139,7 +145,8 @@ __device__ __forceinline__ frag_t cols_frag(uint32_t at, int t, int s) {
 __device__ __forceinline__ constexpr int block_lane(int g, int h, int t) { return 32 * h + (t ^ (h << 2) ^ ((g & 1) << 3)); }
 
 // d as dx's operand: 256 tokens, 64 vocabulary entries. Block (entries n, tokens wave).
-__device__ __forceinline__ void load_tokens(const uint8_t* d, lds_u8* to, int n, int step, int tile, int npad, int wave, int lane) {
+__device__ __forceinline__ void load_tokens(const uint8_t* d, lds_u8* to, int n, int step, int tile, int npad, int wave,
+                                            int lane) {
   const uint32_t row = (uint32_t)(npad / 32) * 1024;
   const uint8_t* const b = d + ((int64_t)step * 4 + n) * row + (int64_t)tile * 8192 + wave * 1024;
   load16(b, to + (wave + 8 * n) * 1024, lane * 16);
@@ -150,7 +157,8 @@ __device__ __forceinline__ frag_t tokens_frag(uint32_t at, int t, int s) {
 }
 
 // d as dW's operand: 256 vocabulary entries, 64 tokens. Block (entries L / 2, tokens L % 2).
-__device__ __forceinline__ void load_entries(const uint8_t* d, lds_u8* to, int n, int step, int tile, int npad, int wave, int lane) {
+__device__ __forceinline__ void load_entries(const uint8_t* d, lds_u8* to, int n, int step, int tile, int npad, int wave,
+                                             int lane) {
   const int L = wave + 8 * n;
   const uint32_t row = (uint32_t)(npad / 32) * 1024;
   const uint8_t* const b = d + ((int64_t)tile * 16 + (L >> 1)) * row + (int64_t)step * 2048 + (L & 1) * 1024;
@@ -362,7 +370,8 @@ __device__ __forceinline__ void grads_of(const CeArgs& a, const f32x16_t (&acc)[
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (own && h == 0) {
       const float x = label_d(loss, weight);
-      uint8_t* const at = to + (y >> 4) * row + block_lane((y >> 4) & 1, (y >> 2) & 1, lane) * 16 + ((y >> 3) & 1) * 8 + (y & 3) * 2;
+      uint8_t* const at =
+          to + (y >> 4) * row + block_lane((y >> 4) & 1, (y >> 2) & 1, lane) * 16 + ((y >> 3) & 1) * 8 + (y & 3) * 2;
       const uint32_t high = pack2<T>(x, x) & 0xffffu;
       *(uint16_t*)at = (uint16_t)high;
       if (second) *(uint16_t*)(at + second) = (uint16_t)pack2<T>(x - unpack1<T>(high), 0.f);
@@ -453,7 +462,8 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
   const int token_steps = (n + kDepth - 1) / kDepth;
   const Order order =
       P == kLoss || P == kGrads ? Order(entry_tiles, token_tiles, dpad / kDepth, 1)
-      : P == kDx ? Order(token_tiles, dim_tiles, (int)((entries + kDepth - 1) / kDepth), splits_of(token_tiles, dim_tiles, a.piece / kDepth))
+      : P == kDx ? Order(token_tiles, dim_tiles, (int)((entries + kDepth - 1) / kDepth),
+                         splits_of(token_tiles, dim_tiles, a.piece / kDepth))
                  : Order(entry_tiles, dim_tiles, token_steps * (a.pair ? 2 : 1), a.splits);
   if constexpr (P == kDw) {
     if (n == 0 && a.splits == 1) {  // no token counts: zeros
@@ -604,7 +614,8 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// The same product for few tokens, which reading weight once bounds: tiles of 128 entries x 64 tokens by 8 waves (4 x 2, each
+// The same product for few tokens, which reading weight once bounds (151936 x 1024 bf16, 64 tokens: 60 us, 5.2 TB/s, against
+// 99 with ce_product's tiles; 128 tokens 87 against 99; more go there): tiles of 128 entries x 64 tokens by 8 waves (4 x 2, each
 // 32 x 32), 64 deep, in a ring of five stages of 24 KB, four of which are on their way. What the epilogue reads of the
 // tokens lies in LDS from the start: a load of its own would wait for the whole ring.
 // ---------------------------------------------------------------------------
@@ -717,7 +728,6 @@ constexpr int kJoinTokens = 32, kJoinSlices = 32;
 struct Header {
   int32_t count;   // kept tokens
   uint32_t ended;  // workgroups of ce_join that are done
-  float scale;     // that undoes the weights of d in the results
 };
 
 template <typename L>
@@ -808,7 +818,8 @@ __global__ __launch_bounds__(1024) void ce_prepare(const T* __restrict__ x, int6
 // all workgroups' losses, in order.
 __global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(Header* head, const float2* __restrict__ sums, int parts,
                                                                     int npad, const float* __restrict__ target,
-                                                                    const int32_t* __restrict__ token, float* __restrict__ lse, float* __restrict__ own_loss,
+                                                                    const int32_t* __restrict__ token, float* __restrict__ lse,
+                                                                    float* __restrict__ own_loss,
                                                                     float* losses, float* block_sums, float* total, int mean) {
   __shared__ float2 s[kJoinSlices][kJoinTokens];
   __shared__ float sum_s[kJoinSlices / 2];
@@ -872,7 +883,7 @@ __global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(Header* head
 // The tokens' gradients as weights of d: g_j over a power of two that the largest is just below, times `lift` (2^14 in f16,
 // whose smallest numbers softmax weights reach; 1 in bf16); the results' scale undoes it. One gradient for all tokens is
 // a scale alone: nothing is weighted then, and this does not run.
-__global__ __launch_bounds__(1024) void ce_weights(Header* head, const float* __restrict__ grad, const int32_t* __restrict__ place,
+__global__ __launch_bounds__(1024) void ce_weights(float* scale, const float* __restrict__ grad, const int32_t* __restrict__ place,
                                                    int64_t tokens, float lift, float* __restrict__ weight) {
   __shared__ float s[16];
   const int tid = threadIdx.x;
@@ -888,7 +899,7 @@ __global__ __launch_bounds__(1024) void ce_weights(Header* head, const float* __
   const float unit = ldexpf(1.f, e);
   for (int64_t i = tid; i < tokens; i += 1024)
     if (place[i] >= 0) weight[place[i]] = grad[i] / unit * lift;
-  if (tid == 0) head->scale = unit / lift;
+  if (tid == 0) *scale = unit / lift;
 }
 
 // What rounding left of the label's d, the one large number among a token's.
@@ -899,9 +910,9 @@ __device__ __forceinline__ float label_rest(const CeArgs& a, int64_t j) {
 }
 
 // Rows of results: the splits' sums in order, scaled and rounded, a workgroup a row at a time. dx (place): row i from row
-// place[i], zeros if that is negative, with what the rounding left of d: of all of it from a row of its own (pair), else of the
-// label's times its row of the weight; `splits` is 0, the kept tokens give it. dW (place NULL): row i from row i; few kept tokens leave some splits without a step, which
-// wrote nothing.
+// place[i], zeros if that is negative, with what the rounding left of d: of all of it from a row of its own (pair), else of
+// the label's times its row of the weight; `splits` is 0, the kept tokens give it. dW (place NULL): row i from row i; few kept
+// tokens leave some splits without a step, which wrote nothing.
 template <typename T>
 __global__ __launch_bounds__(256) void ce_rows(const CeArgs a, const int32_t* __restrict__ place, int64_t rows,
                                                const float* __restrict__ parts, int splits, T* __restrict__ out) {
@@ -1003,7 +1014,7 @@ Backward plan_backward(const Kept& k, int64_t vocab, int64_t dim) {
   b.dcols = up(dim, kTile);
   const int64_t cols = b.dcols / kTile;
   b.dw_splits = pieces > 1 ? 1 : splits_of(b.piece / kTile, cols, k.npad / kDepth);
-  b.weight = 0;
+  b.weight = 256;  // behind the results' scale
   b.d = b.weight + k.npad * 4;
   b.dx = b.d + b.piece * k.npad * 2;
   // dx's sum is split by the kept tokens, whose number the device has: splits x tiles of tokens are 256 / cols or fewer where
@@ -1035,7 +1046,8 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
                 const Forward& f, hipStream_t st) {
   Header* const head = (Header*)kept;
   int32_t *place = (int32_t*)(kept + k.place), *token = (int32_t*)(kept + k.token), *label = (int32_t*)(kept + k.label);
-  float *ref = (float*)(kept + k.ref), *target = (float*)(kept + k.target), *lse = (float*)(kept + k.lse), *losses = reduction == 0 ? loss : nullptr;
+  float *ref = (float*)(kept + k.ref), *target = (float*)(kept + k.target), *lse = (float*)(kept + k.lse);
+  float* const losses = reduction == 0 ? loss : nullptr;
   const int wide = (((uintptr_t)x | (uintptr_t)w) & 15) == 0 && ((x_stride | w_stride | dim) & 7) == 0;
   const unsigned blocks = (unsigned)((tokens < 1 ? 1 : tokens) + kPrepareRows - 1) / kPrepareRows;
   if (bits == 64)
@@ -1066,22 +1078,22 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
   const int64_t joins = (tokens < 1 ? 1 : tokens) + kJoinTokens - 1;
   if (reduction == 0 && tokens == 0) return pkm_check_launch("pkm_linear_ce_fwd");  // no loss to write
   hipLaunchKernelGGL(ce_join, dim3((unsigned)(joins / kJoinTokens)), dim3(kJoinTokens * kJoinSlices), 0, st, head,
-                     (const float2*)a.sums, (int)((vocab + 127) / 128), (int)k.npad, target, token, lse, (float*)(kept + k.loss), losses,
-                     (float*)(ws + f.block_sums), loss, reduction == 1);
+                     (const float2*)a.sums, (int)((vocab + 127) / 128), (int)k.npad, target, token, lse,
+                     (float*)(kept + k.loss), losses, (float*)(ws + f.block_sums), loss, reduction == 1);
   return pkm_check_launch("pkm_linear_ce_fwd");
 }
 
 template <typename T>
-int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, int64_t w_stride, int64_t vocab, int64_t dim,
+int run_backward(const uint8_t* kept, const Kept& k, int64_t tokens, const void* w, int64_t w_stride, int64_t vocab, int64_t dim,
                  const float* grad, int reduction, void* dx, void* dw, uint8_t* ws, const Backward& b, hipStream_t st) {
-  Header* const head = (Header*)kept;
+  const Header* const head = (const Header*)kept;
   const int32_t* place = (const int32_t*)(kept + k.place);
   constexpr float lift = __is_same(T, f16_t) ? 16384.f : 1.f;
   CeArgs a = {};
   if (reduction == 0) {
     float* weight = (float*)(ws + b.weight);
     a.weight = weight;
-    hipLaunchKernelGGL(ce_weights, dim3(1), dim3(1024), 0, st, head, grad, place, tokens, lift, weight);
+    hipLaunchKernelGGL(ce_weights, dim3(1), dim3(1024), 0, st, (float*)ws, grad, place, tokens, lift, weight);
   }
   a.x = kept + k.x;
   a.x_stride = k.dpad * 2;
@@ -1093,7 +1105,7 @@ int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, in
   a.loss = (const float*)(kept + k.loss);
   a.lse = (const float*)(kept + k.lse);
   a.dw = (uint8_t*)dw;
-  a.scale = Scale{&head->scale, reduction == 0 ? nullptr : grad, &head->count, lift, reduction == 1};
+  a.scale = Scale{(const float*)ws, reduction == 0 ? nullptr : grad, &head->count, lift, reduction == 1};
   a.vocab = vocab;
   a.piece = (int32_t)b.piece;
   a.dim = (int32_t)dim;
@@ -1118,7 +1130,8 @@ int run_backward(uint8_t* kept, const Kept& k, int64_t tokens, const void* w, in
     }
   }
   const auto rows = [&](const int32_t* from, int64_t n, const float* parts, int64_t splits, void* out) {
-    hipLaunchKernelGGL(ce_rows<T>, dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, st, a, from, n, parts, (int)splits, (T*)out);
+    hipLaunchKernelGGL(ce_rows<T>, dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, st, a, from, n, parts, (int)splits,
+                       (T*)out);
   };
   if (dx && tokens > 0) rows(place, tokens, dx_parts, 0, dx);
   if (dw && b.dw_splits > 1) rows(nullptr, vocab, dw_parts, b.dw_splits, dw);
@@ -1135,8 +1148,8 @@ using namespace pkm;
               (long long)tokens, (long long)vocab, (long long)dim);                                                         \
   PKM_REQUIRE(dtype == PKM_DTYPE_BF16 || dtype == PKM_DTYPE_F16, PKM_ERR_UNSUPPORTED,                                       \
               fn ": dtype %d not supported (bfloat16, float16 are)", dtype);                                                \
-  PKM_REQUIRE(tokens < (1ll << 22) && dim <= 65536 && vocab < (1ll << 31), PKM_ERR_UNSUPPORTED,                             \
-              fn ": %lld tokens, weight [%lld, %lld] (fewer than 2^22, 2^31, up to 65536 are supported)", (long long)tokens, \
+  PKM_REQUIRE(tokens < (1ll << 22) && dim <= 65536 && vocab < (1ll << 30), PKM_ERR_UNSUPPORTED,                             \
+              fn ": %lld tokens, weight [%lld, %lld] (fewer than 2^22, 2^30, up to 65536 are supported)", (long long)tokens, \
               (long long)vocab, (long long)dim);                                                                            \
   PKM_REQUIRE(reduction >= 0 && reduction <= 2, PKM_ERR_INVALID_ARGUMENT, fn ": reduction %d", reduction);                  \
   Kept k;                                                                                                                   \
@@ -1156,12 +1169,12 @@ extern "C" size_t pkm_linear_ce_kept_size(int64_t tokens, int64_t dim) {
 
 extern "C" size_t pkm_linear_ce_fwd_workspace_size(int64_t tokens, int64_t vocab, int64_t dim) {
   Kept k;
-  return vocab >= 1 && vocab < (1ll << 31) && plan_kept(tokens, dim, &k) ? (size_t)plan_forward(k, vocab).bytes : 0;
+  return vocab >= 1 && vocab < (1ll << 30) && plan_kept(tokens, dim, &k) ? (size_t)plan_forward(k, vocab).bytes : 0;
 }
 
 extern "C" size_t pkm_linear_ce_bwd_workspace_size(int64_t tokens, int64_t vocab, int64_t dim) {
   Kept k;
-  return vocab >= 1 && vocab < (1ll << 31) && plan_kept(tokens, dim, &k) ? (size_t)plan_backward(k, vocab, dim).bytes : 0;
+  return vocab >= 1 && vocab < (1ll << 30) && plan_kept(tokens, dim, &k) ? (size_t)plan_backward(k, vocab, dim).bytes : 0;
 }
 
 extern "C" int pkm_linear_ce_fwd(const void* x, int64_t x_stride, int64_t tokens, const void* weight, int64_t w_stride,
@@ -1185,7 +1198,7 @@ extern "C" int pkm_linear_ce_fwd(const void* x, int64_t x_stride, int64_t tokens
                                   loss, (uint8_t*)kept, k, (uint8_t*)workspace, f, (hipStream_t)stream);
 }
 
-extern "C" int pkm_linear_ce_bwd(void* kept, size_t kept_bytes, int64_t tokens, const void* weight, int64_t w_stride,
+extern "C" int pkm_linear_ce_bwd(const void* kept, size_t kept_bytes, int64_t tokens, const void* weight, int64_t w_stride,
                                  int64_t vocab, int64_t dim, int dtype, const float* grad_loss, int reduction, void* dx,
                                  void* dweight, void* workspace, size_t workspace_bytes, void* stream) {
   CE_REQUIRE_COMMON("pkm_linear_ce_bwd");
@@ -1196,8 +1209,8 @@ extern "C" int pkm_linear_ce_bwd(void* kept, size_t kept_bytes, int64_t tokens, 
   PKM_REQUIRE(workspace && (((uintptr_t)workspace) & 15) == 0 && workspace_bytes >= (size_t)b.bytes, PKM_ERR_WORKSPACE,
               "pkm_linear_ce_bwd: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)b.bytes);
   return dtype == PKM_DTYPE_BF16
-             ? run_backward<bf16_t>((uint8_t*)kept, k, tokens, weight, w_stride, vocab, dim, grad_loss, reduction, dx, dweight,
+             ? run_backward<bf16_t>((const uint8_t*)kept, k, tokens, weight, w_stride, vocab, dim, grad_loss, reduction, dx, dweight,
                                     (uint8_t*)workspace, b, (hipStream_t)stream)
-             : run_backward<f16_t>((uint8_t*)kept, k, tokens, weight, w_stride, vocab, dim, grad_loss, reduction, dx, dweight,
+             : run_backward<f16_t>((const uint8_t*)kept, k, tokens, weight, w_stride, vocab, dim, grad_loss, reduction, dx, dweight,
                                    (uint8_t*)workspace, b, (hipStream_t)stream);
 }

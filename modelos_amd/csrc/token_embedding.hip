@@ -16,6 +16,9 @@
 //      chunk, run by run. A run inside its chunk is written; what a run has in a chunk that it crosses goes to the workspace.
 //   3. embed_join_kernel: adds the pieces of the runs that cross chunks, in order.
 // The order of every sum is that of the tokens: the same bits on every run.
+//
+// Measured, 16384 tokens (ids as texts have them) of 151936 x 1024 bf16: forward 15 us, sort beside the zeros 41 to 47 (the sort
+// alone 17; with each workgroup a range of ids, whose first holds half of the tokens, 75), sums 20, join 5.
 #include "pkm_common.h"
 
 namespace pkm {

@@ -8,21 +8,24 @@ and loss are together,
 in pieces of the vocabulary: the forward sums the exponentials of a piece's
 logits and drops them, the backward computes them again, turns them into their
 gradients and those into the piece's rows of weight's gradient and its part of
-hidden's. The largest of it in memory are the gradients of one piece, 512 MB in 16 bits.
+hidden's. The largest of it in memory are the gradients of one piece, about 512 MB in
+16 bits; a training forward keeps a copy of the hidden states that count.
 
 Tokens whose label is ignore_index, or lies outside [0, vocab), do not count:
 their loss is 0, nothing is computed for them, what hidden holds there is not
 used (it may be NaN) and their rows of its gradient are zeros. The mean is over
 the tokens that count, and 0 if none does (where F.cross_entropy's is NaN).
 
-Logits, softmax sums and all other sums are float32, the loss is float32. The
-gradients of the logits are rounded to the inputs' type for the products they
-enter, in float16 with a power of two taken out, so that any size of the loss's gradient
-keeps its precision. Sums run in a fixed order: losses and gradients are
-bitwise deterministic.
+Logits, softmax sums and all other sums are float32, the loss is float32 and keeps
+its precision down to 0. The gradients of the logits are rounded to the inputs'
+type for the products they enter, in float16 with a power of two taken out, so that
+any size of the loss's gradient keeps its precision; up to 128 tokens they enter
+as two such numbers, and what the rounding leaves of the label's is made up for in hidden's
+gradient. Sums run in a fixed order: losses and gradients are bitwise
+deterministic.
 
-Supported: bfloat16 and float16, any vocabulary and up to 65536 numbers a row,
-fewer than 2^22 tokens, on the GPU; anything else raises NotImplementedError.
+Supported: bfloat16 and float16, up to 65536 numbers a row,
+fewer than 2^22 tokens and 2^30 entries, on the GPU; anything else raises NotImplementedError.
 There is no CPU path: CPU tensors raise. The backward cannot be differentiated
 again, and there are no forward-mode derivatives: dual tensors raise
 NotImplementedError.
@@ -39,7 +42,7 @@ from .window_attention import _refuse_tangents
 _DTYPES = (torch.bfloat16, torch.float16)
 _LABELS = {torch.int32: 32, torch.int64: 64}
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
-_MAX_TOKENS, _MAX_DIM, _MAX_STRIDE = 1 << 22, 65536, 1 << 22
+_MAX_TOKENS, _MAX_VOCAB, _MAX_DIM, _MAX_STRIDE = 1 << 22, 1 << 30, 65536, 1 << 22
 
 
 def _buffer(n: int, device) -> torch.Tensor:
@@ -123,7 +126,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     if hidden.dtype not in _DTYPES or weight.dtype != hidden.dtype:
         raise NotImplementedError(f"linear_cross_entropy: {hidden.dtype} with a weight of {weight.dtype} is not supported "
                                   "(bfloat16 and float16 are, both alike)")
-    if labels.numel() >= _MAX_TOKENS or weight.shape[1] > _MAX_DIM or weight.shape[0] >= 1 << 31:
+    if labels.numel() >= _MAX_TOKENS or weight.shape[1] > _MAX_DIM or weight.shape[0] >= _MAX_VOCAB:
         raise NotImplementedError(f"linear_cross_entropy: {labels.numel()} tokens, a weight of {tuple(weight.shape)} are not "
                                   f"supported (fewer than {_MAX_TOKENS} tokens, rows of up to {_MAX_DIM} numbers are)")
     _refuse_tangents("linear_cross_entropy", hidden, weight)

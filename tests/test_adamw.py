@@ -129,3 +129,11 @@ def test_oracle_dither_loses_nothing():
     held = torch.stack([oracle.hold(a, u, 0.0)[0] for u in dithers]).mean(0)
     spacing = torch.tensor([32.0, 2.0**-2, 2.0**-9, 2.0**3]).repeat(64)
     assert ((held - a).abs() <= spacing * off + a * 2.0**-20).all()
+
+
+def test_load_groups_of_another_optimizer():
+    """torch's own AdamW has other options: those that are missing keep their defaults."""
+    p = _param(3)
+    opt = AdamW([p], state_bits=8)
+    opt.load_state_dict(torch.optim.AdamW([_param(3)], lr=0.5).state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5 and opt.param_groups[0]["state_bits"] == 8 and not opt.param_groups[0]["master_weights"]

@@ -63,7 +63,7 @@ def _backward(lib, tokens=10, w=P, w_stride=64, vocab=100, dim=64, dtype=1, grad
 ODD = ctypes.c_void_p((1 << 20) + 8)
 COMMON = [
     (dict(tokens=-1), 1), (dict(vocab=0), 1), (dict(dim=0), 1), (dict(dtype=0), 2), (dict(dtype=9), 2), (dict(tokens=1 << 22), 2),
-    (dict(dim=65537), 2), (dict(vocab=1 << 31), 2), (dict(vocab=(1 << 31) - 1, tokens=1 << 15), 2), (dict(reduction=3), 1),
+    (dict(dim=65537), 2), (dict(vocab=1 << 30), 2), (dict(vocab=(1 << 30) - 1, tokens=1 << 16), 2), (dict(reduction=3), 1),
     (dict(w=None), 1), (dict(w=ODD), 1), (dict(w_stride=63), 1), (dict(w_stride=68), 1), (dict(dim=65, w_stride=64), 1),
     (dict(w_stride=1 << 23), 1), (dict(kept=None), 3), (dict(kept=ODD), 3), (dict(kept_bytes=255), 3), (dict(ws=None), 3),
     (dict(ws=ODD), 3), (dict(ws_bytes=255), 3),
@@ -83,6 +83,6 @@ def test_entry_backward(lib, args, status):
 
 def test_sizes(lib):
     assert lib.pkm_linear_ce_kept_size(1 << 22, 64) == lib.pkm_linear_ce_kept_size(10, 0) == 0
-    assert lib.pkm_linear_ce_fwd_workspace_size(10, 0, 64) == lib.pkm_linear_ce_bwd_workspace_size(10, 1 << 31, 64) == 0
+    assert lib.pkm_linear_ce_fwd_workspace_size(10, 0, 64) == lib.pkm_linear_ce_bwd_workspace_size(10, 1 << 30, 64) == 0
     # 16384 tokens, 151936 entries: no more than 512 MB of the logits' gradients at a time
     assert 16384 * 16384 * 2 * 0.9 < lib.pkm_linear_ce_bwd_workspace_size(16384, 151936, 1024) < 700e6
