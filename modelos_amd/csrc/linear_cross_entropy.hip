@@ -18,9 +18,9 @@
 // a step of 16 while the matrix cores work on the one before, across tiles and also across results: the grid is one
 // workgroup a CU, and the next result's tiles load while this one's epilogue runs. One barrier a 64.
 //
-// Measured, 16384 tokens, 151936 entries, 1024 wide, bf16: the forward's product 4.2 ms (1210 TFLOP/s), of a piece of 15360
+// Measured, 16384 tokens, 151936 entries, 1024 wide, bf16: the forward's product 4.27 ms (1195 TFLOP/s), of a piece of 15360
 // entries d 0.495, dW 0.461 and dx 0.428 ms (1040 to 1200); beside them 0.1 ms (copy of the tokens 23 us, join of the tiles'
-// sums 47, dx's rounding 36). The matrix cores are busy 52 to 61 % of the cycles at 1.6 to 2.0 GHz; plain library products of
+// sums 47, dx's rounding 50). The matrix cores are busy 52 to 61 % of the cycles at 1.6 to 2.0 GHz; plain library products of
 // the pieces' shapes take 0.457, 0.668 and 0.444 ms at 1.5 to 1.64 GHz and 50 to 70 %: the clock falls as the load rises, and
 // neither fewer LDS cycles (bank conflicts were half of them) nor loads spread between the products moved the time.
 //
@@ -251,19 +251,37 @@ __device__ __forceinline__ void cut(f32x16_t (&acc)[MT][NU], int64_t left, int h
   }
 }
 
+// 0 for the label's row, else 1.
+__device__ __forceinline__ float others(int row, float yr) { return fminf((row - yr) * (row - yr), 1.f); }
+
 // The sum of the exponentials of a wave's entries for the lane's token of column block u, against the token's reference: the
 // label's logit, whose own exponential is 1, so that what underflows beside it is nothing. Where it overflows, the entries' own
 // largest logit takes the reference's place. The reference's product with log2(e) is rounded once for all entries; what that
 // adds to all exponents alike comes off the sum.
-template <int MT, int NU>
-__device__ __forceinline__ float2 sum_of(const f32x16_t (&acc)[MT][NU], int u, float ref) {
-  float sum = 0.f;
-  const float c = -ref * kLog2e;
+// OWN: the label may be among the entries, yr rows (less 4 h) below the wave's first: its logit goes to `target`, its exponential
+// is left out. A loss near 0 is the logarithm of 1 + the others' exponentials, which a 1 among them would round. Left out by a
+// factor 0 or 1 (others): the masks of 64 comparisons would not fit the scalar registers.
+template <bool OWN, int MT, int NU>
+__device__ __forceinline__ float2 sum_over(const f32x16_t (&acc)[MT][NU], int u, float ref, int yr, float* target) {
+  float sum = 0.f, z = -INFINITY;
+  const float c = -ref * kLog2e, y = (float)yr;
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += exp2_raw(__builtin_fmaf(acc[t][u][i], kLog2e, c));
+    for (int i = 0; i < 16; ++i) {
+      const float e = exp2_raw(__builtin_fmaf(acc[t][u][i], kLog2e, c));
+      if constexpr (OWN) {
+        const float w = others(row_of(t, i), y);
+        z = fmaxf(z, __builtin_fmaf(w, -3e38f, acc[t][u][i]));
+        sum = __builtin_fmaf(e, w, sum);
+      } else {
+        sum += e;
+      }
+    }
     batch();
+  }
+  if constexpr (OWN) {
+    if (yr >= 0 && yr < 32 * MT && (yr & 4) == 0) *target = z;
   }
   sum += swap_halves(sum);
   sum -= sum * (__builtin_fmaf(ref, kLog2e, c) * kLn2);
@@ -279,7 +297,10 @@ __device__ __forceinline__ float2 sum_of(const f32x16_t (&acc)[MT][NU], int u, f
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) own += exp2_raw((acc[t][u][i] - top) * kLog2e);
+      for (int i = 0; i < 16; ++i) {
+        const float e = exp2_raw((acc[t][u][i] - top) * kLog2e);
+        own = OWN ? __builtin_fmaf(e, others(row_of(t, i), y), own) : own + e;
+      }
       batch();
     }
     own += swap_halves(own);
@@ -287,26 +308,10 @@ __device__ __forceinline__ float2 sum_of(const f32x16_t (&acc)[MT][NU], int u, f
   }
   return make_float2(ref, sum);
 }
-
-// The logit of the label, yr rows (less 4 h) below the wave's first, into the token's place, and out of the sum: a loss near 0
-// is the logarithm of 1 + the others' exponentials, which the label's 1 among them would round.
 template <int MT, int NU>
-__device__ __forceinline__ void take_target(f32x16_t (&acc)[MT][NU], int u, int yr, float* to) {
-  const bool own = yr >= 0 && yr < 32 * MT && (yr & 4) == 0;
-  if (!__any(own)) return;
-  asm volatile("" : "+v"(yr));  // as in cut()
-  float z = 0.f;
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const bool here = row_of(t, i) == yr;
-      z = here ? acc[t][u][i] : z;
-      acc[t][u][i] = here ? -INFINITY : acc[t][u][i];
-    }
-    batch();
-  }
-  if (own) *to = z;
+__device__ __forceinline__ float2 sum_of(const f32x16_t (&acc)[MT][NU], int u, float ref, int yr, float* target) {
+  if (__any(yr >= 0 && yr < 32 * MT)) return sum_over<true>(acc, u, ref, yr, target);
+  return sum_over<false>(acc, u, ref, yr, target);
 }
 
 // Two such sums as one.
@@ -321,8 +326,7 @@ __device__ __forceinline__ void end_loss(const CeArgs& a, acc_t& acc, const Resu
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int j = r.n * kTile + (wave & 3) * 64 + 32 * u + (lane & 31);
-    take_target(acc, u, a.label[j] - v0 - 4 * h, a.target + j);
-    const float2 sum = sum_of(acc, u, a.ref[j]);
+    const float2 sum = sum_of(acc, u, a.ref[j], a.label[j] - v0 - 4 * h, a.target + j);
     if (h == 0) a.sums[(int64_t)(2 * r.m + (wave >> 2)) * a.npad + j] = sum;
   }
 }
@@ -695,8 +699,7 @@ __global__ __launch_bounds__(kThreads, 2) void ce_few(const CeArgs a) {
     const int column = (wave & 1) * 32 + (lane & 31), j = run.n * kFewN + column;
     cut(acc, entries - v0, h);
     if constexpr (P == kLoss) {
-      take_target(acc, 0, (int)(label_s[j] - v0) - 4 * h, a.target + j);
-      const float2 sum = sum_of(acc, 0, ref_s[j]);
+      const float2 sum = sum_of(acc, 0, ref_s[j], (int)(label_s[j] - v0) - 4 * h, a.target + j);
       if (h == 0) sum_s[wave >> 1][column] = sum;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();

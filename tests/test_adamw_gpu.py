@@ -312,3 +312,23 @@ def test_blocks_of_any_size(device):
             held, steps = oracle.hold(x, u, least)
             assert torch.equal(after[name + "_scale"], steps), name
             assert torch.equal(after[name].float(), held), name
+
+
+def test_more_numbers_than_32_bits_count(device):
+    """One tensor of more than 2^32 numbers. A first step moves a weight by lr against its gradient's sign; blocks of 256 end
+    at multiples of 256, so the last 44 are one of their own."""
+    n = (1 << 32) + 300
+    p = torch.zeros(n, dtype=BF16, device=device)
+    at = torch.tensor([0, 5, 1 << 31, (1 << 32) - 1, 1 << 32, n - 1], device=device)
+    p[at] = 1.0
+    p.requires_grad_()
+    p.grad = torch.zeros_like(p)
+    p.grad[at] = torch.tensor([2.0, -2, 2, 2, 2, 2], dtype=BF16, device=device)
+    opt = AdamW([p], lr=0.25, betas=(0.5, 0.5), eps=1e-30, weight_decay=0.0, state_bits=8)
+    opt.step()
+    assert p[at].tolist() == [0.75, 1.25, 0.75, 0.75, 0.75, 0.75]
+    state = opt.state[p]
+    m = oracle.numbers(state["exp_avg"][-300:].cpu(), state["exp_avg_scale"][-2:].cpu())
+    # 448 steps of (max / 448), rounded twice
+    assert ((m[[0, -1]] - 1).abs() <= 2.0**-22).all() and not m[1:-1].any()
+    assert p[(1 << 32) + 1 : n - 1].eq(0).all() and p[6:1000].eq(0).all()

@@ -266,3 +266,28 @@ def test_losses_near_nothing(n, dtype, device):
         other = (torch.ones_like(d) @ ww.abs() if got is dx else torch.ones_like(d).T @ xx.abs()) * lost
         bound = (u + 4 * e.max() + 2.0**-17) * size + other + u * exact.abs() + tiny
         assert ((got.cpu().double() - exact).abs() <= bound).all()
+
+
+def test_offsets_past_32_bits(device):
+    """A weight of more than 2^32 bytes and 2^31 numbers, all zeros but for three rows at its ends and in the middle."""
+    V, D = (1 << 21) + 5, 1032
+    w = torch.zeros((V, D), dtype=BF16, device=device)
+    rows = torch.tensor([0, V // 2, V - 1], device=device)
+    w[rows] = torch.tensor([1.0, 2.0, -1.0], device=device, dtype=BF16)[:, None] / 64
+    w.requires_grad_()
+    x = (torch.eye(3, D, device=device) * 64).to(BF16).requires_grad_()  # the logits of a token: 1, 2 and -1 at the three rows
+    labels = rows[[1, 2, 0]]
+    loss = linear_cross_entropy(x, w, labels, reduction="none")
+    total = torch.tensor([1.0, 2.0, -1.0]).double().exp().sum() + V - 3
+    want = total.log() - torch.tensor([2.0, -1.0, 1.0]).double()
+    assert ((loss.cpu().double() - want).abs() <= 2.0**-20 * want).all()
+    dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+    p = torch.tensor([1.0, 2.0, -1.0]).double().exp() / total
+    for k, v in enumerate(rows.tolist()):  # column t of row v: the d of token t times its 64
+        d = p[k] - (labels.cpu() == v).double()
+        assert ((dw[v, :3].cpu().double() - 64 * d).abs() <= 2.0**-7 * 64 * d.abs()).all()
+        assert not dw[v, 3:].any()
+    other = dw[[1, V // 2 - 1, V // 2 + 1, V - 2], :3].cpu().double()
+    assert ((other - 64 / total).abs() <= 2.0**-7 * 64 / total).all()
+    exact = (p[None] - (labels.cpu()[:, None] == rows.cpu()[None]).double()) @ torch.tensor([1.0, 2.0, -1.0]).double() / 64
+    assert ((dx.cpu().double() - exact[:, None]).abs() <= 2.0**-7 * exact[:, None].abs()).all()
