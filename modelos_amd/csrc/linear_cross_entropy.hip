@@ -1008,15 +1008,30 @@ struct Backward {
 };
 Backward plan_backward(const Kept& k, int64_t vocab, int64_t dim) {
   Backward b;
-  const int64_t all = up(vocab, kTile);
-  // 512 MB of d at a time, and no fewer than 64 tiles of the vocabulary: dW's product has one for each and 256 columns
-  int64_t most = (1ll << 28) / k.npad / kTile * kTile;
-  if (most < 64 * kTile) most = 64 * kTile;
-  const int64_t pieces = (all + most - 1) / most;
-  b.piece = up((all + pieces - 1) / pieces, kTile);
+  const int64_t all = up(vocab, kTile) / kTile, tokens = k.npad / kTile;
+  // 768 MB of d at a time at most, and no fewer than 64 tiles of the vocabulary: dW's product has one for each and 256 columns
+  int64_t most = 3 * (1ll << 27) / k.npad / kTile;
+  if (most < 64) most = 64;
+  // Of the fewest pieces and a few more, those whose products leave the fewest workgroups idle in their last rounds
+  // (2048 tokens, 151936 entries: one piece of 594 tiles 19 + 10 rounds, two of 297 20 + 10; 16384 tokens: ten pieces)
+  const auto rounds = [&](int64_t tiles) {
+    const auto of = [](int64_t m, int64_t n) { return (Blocks(m, n).results() + 255) / 256; };
+    return of(tiles, tokens) * (k.dpad / kDepth + 2) + of(tiles, up(dim, kTile) / kTile) * (k.npad / kDepth + 2);
+  };
+  const int64_t fewest = (all + most - 1) / most;
+  int64_t best = 0, pieces = fewest;
+  for (int64_t n = fewest; n <= fewest + 4 && n <= all; ++n) {
+    const int64_t tiles = (all + n - 1) / n, whole = all / tiles;
+    const int64_t cost = whole * rounds(tiles) + (all > whole * tiles ? rounds(all - whole * tiles) : 0);
+    if (best == 0 || cost < best) {
+      best = cost;
+      pieces = n;
+    }
+  }
+  b.piece = (all + pieces - 1) / pieces * kTile;
   b.dcols = up(dim, kTile);
   const int64_t cols = b.dcols / kTile;
-  b.dw_splits = pieces > 1 ? 1 : splits_of(b.piece / kTile, cols, k.npad / kDepth);
+  b.dw_splits = b.piece < vocab ? 1 : splits_of(b.piece / kTile, cols, k.npad / kDepth);
   b.weight = 256;  // behind the results' scale
   b.d = b.weight + k.npad * 4;
   b.dx = b.d + b.piece * k.npad * 2;

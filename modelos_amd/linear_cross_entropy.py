@@ -8,8 +8,8 @@ and loss are together,
 in pieces of the vocabulary: the forward sums the exponentials of a piece's
 logits and drops them, the backward computes them again, turns them into their
 gradients and those into the piece's rows of weight's gradient and its part of
-hidden's. The largest of it in memory are the gradients of one piece, about 512 MB in
-16 bits; a training forward keeps a copy of the hidden states that count.
+hidden's. The largest of it in memory are the gradients of one piece, up to about 768 MB
+in 16 bits; a training forward keeps a copy of the hidden states that count.
 
 Tokens whose label is ignore_index, or lies outside [0, vocab), do not count:
 their loss is 0, nothing is computed for them, what hidden holds there is not

@@ -4,6 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from modelos_amd import _lib
 from modelos_amd.linear_cross_entropy import linear_cross_entropy
 from oracle import linear_cross_entropy as oracle
 
@@ -65,7 +66,7 @@ def test_values_and_gradients(n, V, D, reduction, dtype, device):
 
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
 def test_several_pieces(dtype, device):
-    """More vocabulary than a piece holds (64 tiles of 256), and a last piece that ends inside a tile."""
+    """Few tokens and much vocabulary, whose last tile is not full."""
     x, w, labels, gen = _inputs(70, 2 * 16384 + 16300, 64, dtype, device)
     labels[:4] = torch.tensor([16383, 16384, 32768, 2 * 16384 + 16299])
     _check(x, w, labels, "mean", gen)
@@ -291,3 +292,18 @@ def test_offsets_past_32_bits(device):
     assert ((other - 64 / total).abs() <= 2.0**-7 * 64 / total).all()
     exact = (p[None] - (labels.cpu()[:, None] == rows.cpu()[None]).double()) @ torch.tensor([1.0, 2.0, -1.0]).double() / 64
     assert ((dx.cpu().double() - exact[:, None]).abs() <= 2.0**-7 * exact[:, None].abs()).all()
+
+
+@pytest.mark.parametrize("ignored", [0.3, 0.999])
+@pytest.mark.parametrize("V", [16384 + 300, 2 * 16384 + 1])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_pieces_of_many_tokens(dtype, V, ignored, device):
+    """24600 tokens: the backward takes 64 tiles of the vocabulary at a time or fewer. The oracle's 64-bit products on the GPU."""
+    n, D = 24600, 24
+    x, w, labels, gen = _inputs(n, V, D, dtype, device, V, ignored=ignored)
+    labels[:6] = torch.tensor([0, 16383, 16384, V // 2 // 256 * 256, V - 2, V - 1])
+    assert _lib.load().pkm_linear_ce_bwd_workspace_size(n, V, D) < 24832 * 2 * V * 0.7  # not all of d
+    loss, grad, grads = _both(x, w, labels, "mean", gen)
+    values, bounds = oracle.loss_and_gradients(x.detach(), w.detach(), labels, -100, "mean", grad.double().to(device))
+    for name, got, want, bound in zip(("loss", "dx", "dW"), (loss, *grads), values, bounds):
+        _near(got, want.cpu(), bound.cpu(), name)
