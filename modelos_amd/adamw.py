@@ -62,7 +62,7 @@ class _Plan:
         self.held = [self.take(s) for s in states]
         self.table = (_lib.AdamWTensor * len(params))()
         self.words = np.frombuffer(self.table, dtype=np.int64).reshape(len(params), _FIELDS)
-        self.pointers = [p.data_ptr() for p in params]
+        self.places = self._places()
         for row, p, s in zip(self.table, params, states):
             row.param, row.exp_avg, row.step, row.numel = p.data_ptr(), s["exp_avg"].data_ptr(), s["step"].data_ptr(), p.numel()
             row.second = s["exp_avg_sq" if bits == 32 else "exp_root"].data_ptr()
@@ -73,11 +73,15 @@ class _Plan:
         self.device, self.dtype = params[0].device, _lib.dtype_code(params[0])
         self.ws_bytes = _lib.load().pkm_adamw_workspace_size(len(params))
 
+    def _places(self) -> list:
+        """Where weights and states lie, which an assignment to their `data` changes too, and the weights' forms."""
+        Tensor, states = torch.Tensor, itertools.chain.from_iterable(map(self.take, self.states))
+        return [*map(Tensor.data_ptr, self.params), *map(Tensor.numel, self.params),
+                *map(Tensor.is_contiguous, self.params), *map(Tensor.data_ptr, states)]
+
     def stands(self) -> bool:
-        """Whether the weights and states are where they were."""
-        held = itertools.chain.from_iterable(self.held)
-        now = itertools.chain.from_iterable(map(self.take, self.states))
-        return [p.data_ptr() for p in self.params] == self.pointers and all(map(operator.is_, held, now))
+        """Whether the weights and states are what and where they were: what is held here keeps its place to itself."""
+        return self._places() == self.places
 
 
 class AdamW(torch.optim.Optimizer):

@@ -332,3 +332,36 @@ def test_more_numbers_than_32_bits_count(device):
     # 448 steps of (max / 448), rounded twice
     assert ((m[[0, -1]] - 1).abs() <= 2.0**-22).all() and not m[1:-1].any()
     assert p[(1 << 32) + 1 : n - 1].eq(0).all() and p[6:1000].eq(0).all()
+
+
+@pytest.mark.parametrize("bits,master", [(8, True), (32, False)])
+def test_data_put_elsewhere(bits, master, device):
+    """A step follows states whose `data` was exchanged, and refuses weights and states that do not fit any more."""
+    gen = torch.Generator().manual_seed(9)
+    (p,) = _params(gen, BF16, device, [(32, 32)])
+    opt = AdamW([p], **HYPER, state_bits=bits, master_weights=master)
+    _grads(gen, [p])
+    opt.step()
+    state, old = opt.state[p], {}
+    for name, x in state.items():
+        old[name] = x.data
+        x.data = x.data.clone()
+    before, p0, kept = _cpu(state), p.detach().cpu().clone(), _cpu(old)
+    opt.step()
+    _check_step(before, _cpu(state), p0, p.detach().cpu(), p.grad.cpu(), 2, bits)
+    assert all(torch.equal(x.cpu().float(), kept[n].float()) for n, x in old.items())
+    whole = p.data
+    p.grad, p.data = None, whole[:8]
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="has to be 1024 contiguous|has to be 256 contiguous|has to be 1 contiguous"):
+        opt.step()
+    p.grad, p.data = None, whole.t()
+    p.grad = torch.ones_like(p)
+    with pytest.raises(NotImplementedError, match="contiguous"):
+        opt.step()
+    p.grad, p.data = None, whole
+    p.grad = torch.ones_like(p)
+    opt.step()
+    state["exp_avg"].data = state["exp_avg"].data.cpu()
+    with pytest.raises(ValueError, match="exp_avg"):
+        opt.step()
