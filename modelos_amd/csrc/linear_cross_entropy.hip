@@ -18,11 +18,12 @@
 // a step of 16 while the matrix cores work on the one before, across tiles and also across results: the grid is one
 // workgroup a CU, and the next result's tiles load while this one's epilogue runs. One barrier a 64.
 //
-// Measured, 16384 tokens, 151936 entries, 1024 wide, bf16: the forward's product 4.27 ms (1195 TFLOP/s), of a piece of 15360
-// entries d 0.495, dW 0.461 and dx 0.428 ms (1040 to 1200); beside them 0.1 ms (copy of the tokens 23 us, join of the tiles'
-// sums 47, dx's rounding 50). The matrix cores are busy 52 to 61 % of the cycles at 1.6 to 2.0 GHz; plain library products of
-// the pieces' shapes take 0.457, 0.668 and 0.444 ms at 1.5 to 1.64 GHz and 50 to 70 %: the clock falls as the load rises, and
-// neither fewer LDS cycles (bank conflicts were half of them) nor loads spread between the products moved the time.
+// Measured, 16384 tokens, 151936 entries, 1024 wide, bf16: the forward's product 4.27 to 4.48 ms (two cards; 1140 to 1195
+// TFLOP/s), of a piece of 15360 entries d 0.50, dW 0.46 and dx 0.43 ms (1040 to 1200); beside them 0.1 ms (copy of the tokens
+// 23 us, join of the tiles' sums 47, dx's rounding 50). The matrix cores are busy 52 to 61 % of the cycles at 1.6 to 2.0 GHz;
+// plain library products of the pieces' shapes take 0.457, 0.668 and 0.444 ms at 1.5 to 1.64 GHz and 50 to 70 %: the clock
+// falls as the load rises, and neither fewer LDS cycles (bank conflicts were half of them) nor loads spread between the
+// products moved the time.
 //
 // d lies as the epilogue's registers hold it, in blocks of 16 vocabulary entries x 32 tokens (1 KB, 16 bytes a lane): dx's
 // product reads a block as a matrix operand as it is, dW's through the transposing LDS reads.
@@ -281,13 +282,13 @@ __device__ __forceinline__ float2 sum_over(const f32x16_t (&acc)[MT][NU], int u,
     batch();
   }
   if constexpr (OWN) {
-    if (yr >= 0 && yr < 32 * MT && (yr & 4) == 0) *target = z;
+    if (yr >= 0 && yr < 32 * MT && (yr & 4) == 0) *target = z < -2e38f ? -INFINITY : z;  // an infinite one, beside the others
   }
   sum += swap_halves(sum);
   sum -= sum * (__builtin_fmaf(ref, kLog2e, c) * kLn2);
   const bool over = !(sum < 0x1p120f);
   if (__any(over)) {
-    float top = -INFINITY;
+    float top = -3e38f;  // finite, for entries that are all -infinity
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -618,7 +619,7 @@ __global__ __launch_bounds__(kThreads, 2) void ce_product(const CeArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// The same product for few tokens, which reading weight once bounds (151936 x 1024 bf16, 64 tokens: 60 us, 5.2 TB/s, against
+// The same product for few tokens, which reading weight once bounds (151936 x 1024 bf16, 64 tokens: 56 us, 5.6 TB/s, against
 // 99 with ce_product's tiles; 128 tokens 87 against 99; more go there): tiles of 128 entries x 64 tokens by 8 waves (4 x 2, each
 // 32 x 32), 64 deep, in a ring of five stages of 24 KB, four of which are on their way. What the epilogue reads of the
 // tokens lies in LDS from the start: a load of its own would wait for the whole ring.
@@ -857,7 +858,7 @@ __global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(Header* head
       const float z = target[j], x = logf(sum) + (m - z);
       loss = fmaxf(x, 0.f) + log1pf(expf(-fabsf(x)));
       if (x != x) loss = x;
-      lse[j] = z + loss;
+      lse[j] = loss < INFINITY ? z + loss : m + logf(sum);
       own_loss[j] = loss;
       if (losses) losses[token[j]] = loss;
     }
@@ -1227,8 +1228,8 @@ extern "C" int pkm_linear_ce_bwd(const void* kept, size_t kept_bytes, int64_t to
   PKM_REQUIRE(workspace && (((uintptr_t)workspace) & 15) == 0 && workspace_bytes >= (size_t)b.bytes, PKM_ERR_WORKSPACE,
               "pkm_linear_ce_bwd: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)b.bytes);
   return dtype == PKM_DTYPE_BF16
-             ? run_backward<bf16_t>((const uint8_t*)kept, k, tokens, weight, w_stride, vocab, dim, grad_loss, reduction, dx, dweight,
-                                    (uint8_t*)workspace, b, (hipStream_t)stream)
+             ? run_backward<bf16_t>((const uint8_t*)kept, k, tokens, weight, w_stride, vocab, dim, grad_loss, reduction, dx,
+                                    dweight, (uint8_t*)workspace, b, (hipStream_t)stream)
              : run_backward<f16_t>((const uint8_t*)kept, k, tokens, weight, w_stride, vocab, dim, grad_loss, reduction, dx, dweight,
                                    (uint8_t*)workspace, b, (hipStream_t)stream);
 }

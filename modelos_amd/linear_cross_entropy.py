@@ -14,7 +14,9 @@ in 16 bits; a training forward keeps a copy of the hidden states that count.
 Tokens whose label is ignore_index, or lies outside [0, vocab), do not count:
 their loss is 0, nothing is computed for them, what hidden holds there is not
 used (it may be NaN) and their rows of its gradient are zeros. The mean is over
-the tokens that count, and 0 if none does (where F.cross_entropy's is NaN).
+the tokens that count, and 0 if none does (where F.cross_entropy's is NaN). An infinite
+weight makes its row's logits infinite or NaN; in the last 8 columns of a weight
+whose rows are no multiple of 64 always NaN.
 
 Logits, softmax sums and all other sums are float32, the loss is float32 and keeps
 its precision down to 0. The gradients of the logits are rounded to the inputs'

@@ -307,3 +307,17 @@ def test_pieces_of_many_tokens(dtype, V, ignored, device):
     values, bounds = oracle.loss_and_gradients(x.detach(), w.detach(), labels, -100, "mean", grad.double().to(device))
     for name, got, want, bound in zip(("loss", "dx", "dW"), (loss, *grads), values, bounds):
         _near(got, want.cpu(), bound.cpu(), name)
+
+
+@pytest.mark.parametrize("n", [3, 200])
+def test_infinite_logits(n, device):
+    """Logits of -infinity: no part of a loss, but of the token whose label has it, whose loss is infinite."""
+    w = torch.zeros((3, 64), dtype=BF16, device=device)
+    w[:, 0] = torch.tensor([-float("inf"), 0.0, 1.0])
+    x = torch.eye(1, 64, dtype=BF16, device=device).expand(n, 64)
+    labels = torch.arange(n, device=device) % 3
+    loss = linear_cross_entropy(x, w, labels, reduction="none").cpu().double()
+    want = torch.nn.functional.cross_entropy((x @ w.T).cpu().double(), labels.cpu(), reduction="none")
+    assert torch.equal(torch.isinf(loss), labels.cpu() == 0) and not loss.isnan().any()
+    fine = labels.cpu() != 0
+    assert ((loss - want)[fine].abs() <= 2.0**-21 * want[fine]).all()
