@@ -7,6 +7,7 @@ from pathlib import Path
 import pytest
 import torch
 import torch.nn.functional as F
+import torch.utils.checkpoint
 
 from modelos_amd.adamw import AdamW
 from modelos_amd.linear_cross_entropy import linear_cross_entropy
@@ -143,3 +144,28 @@ def test_the_example_decoder_trains_through_them(device):
     assert abs(loss.item() - want_loss.item()) <= 2**-8 * 4
     for (name, _), a, b in zip(model.named_parameters(), got, want):
         assert (a.float() - b.float()).norm() <= 8 * 2**-8 * b.float().norm(), name
+
+
+@pytest.mark.parametrize("tokens", [40, 500])
+def test_gradients_twice_and_recomputed(tokens, device):
+    """The same bits from one graph twice, and where a checkpoint runs the forward again."""
+    table, gate = _weights(device)
+    ids, labels = (x[:tokens] for x in _batch(device, 2))
+    loss = _loss(table, gate, ids, labels)
+    first = torch.autograd.grad(loss, (table, gate), retain_graph=True)
+    again = torch.autograd.grad(loss, (table, gate))
+    loss = torch.utils.checkpoint.checkpoint(_loss, table, gate, ids, labels, use_reentrant=False)
+    for a, b, c in zip(first, again, torch.autograd.grad(loss, (table, gate))):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_labels_and_ids_of_one_value(device):
+    """All tokens the same id, all labels the same entry: every sum of the step is one row's."""
+    table, gate = _weights(device)
+    ids, labels = torch.full((TOKENS,), 5, device=device), torch.full((TOKENS,), 5, device=device)
+    got = torch.autograd.grad(_loss(table, gate, ids, labels), (table, gate))
+    t, g = (x.detach().cpu().double().requires_grad_() for x in (table, gate))
+    read = t[ids.cpu()] * 2
+    want = torch.autograd.grad(F.cross_entropy((read * g + read.roll(1, 0)) @ t.T, labels.cpu()), (t, g))
+    for a, b in zip(got, want):  # the roundings of test_gradients_of_a_tied_table; those of equal tokens add up as the values do
+        assert (a.cpu().double() - b).norm() <= 8 * 2**-8 * b.norm()
