@@ -91,6 +91,7 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = False):
         self._plans: dict = {}
+        self._planned: list = []  # the parameters' states when the plans were made
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights))
 
@@ -99,7 +100,7 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:  # of an optimizer without these options
             for name, value in self.defaults.items():
                 group.setdefault(name, value)
-        self._plans = {}
+        self._plans, self._planned = {}, []
 
     def add_param_group(self, param_group: dict) -> None:
         super().add_param_group(param_group)
@@ -184,6 +185,8 @@ class AdamW(torch.optim.Optimizer):
         if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1):
             raise ValueError(f"AdamW.step: grad_scale has to be one float32 number, got {grad_scale.dtype} "
                              f"{tuple(grad_scale.shape)}")
+        if len(self.state) != len(self._planned) or not all(map(operator.is_, self.state.values(), self._planned)):
+            self._plans = {}
         for i, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
@@ -194,6 +197,7 @@ class AdamW(torch.optim.Optimizer):
             if held is None or held[0] != (bits, master) or len(held[1]) != len(params) \
                     or not all(map(operator.is_, held[1], params)) or not all(plan.stands() for plan in held[2]):
                 held = self._plans[i] = ((bits, master), params, self._plans_of(params, bits, master))
+                self._planned = list(self.state.values())
             for plan in held[2]:
                 self._launch(plan, group, grad_scale)
         return loss

@@ -365,3 +365,33 @@ def test_data_put_elsewhere(bits, master, device):
     state["exp_avg"].data = state["exp_avg"].data.cpu()
     with pytest.raises(ValueError, match="exp_avg"):
         opt.step()
+
+
+@pytest.mark.parametrize("how", ["clear", "another", "one", "put back"])
+def test_states_taken_away(how, device):
+    """A step begins anew where a state is gone, and uses the one that is put in its place."""
+    gen = torch.Generator().manual_seed(10)
+    params = _params(gen, F32, device, [(300,), (20,)])
+    opt = AdamW(params, **HYPER)
+    _grads(gen, params)
+    opt.step()
+    held = copy.deepcopy([opt.state[p] for p in params])
+    opt.step()
+    if how == "clear":
+        opt.state.clear()
+    elif how == "another":
+        opt.state = type(opt.state)(dict)
+    elif how == "one":
+        del opt.state[params[1]]
+    else:
+        for p, s in zip(params, held):
+            opt.state[p] = s
+    gone = {"clear": [0, 1], "another": [0, 1], "one": [1], "put back": []}[how]
+    before = [{k: torch.zeros_like(x) for k, x in _cpu(s).items()} if i in gone else
+              _cpu(s if how == "put back" else opt.state[params[i]]) for i, s in enumerate(held)]
+    p0 = [p.detach().cpu().clone() for p in params]
+    opt.step()
+    for i, p in enumerate(params):
+        t = 1 if i in gone else 2 if how == "put back" else 3
+        assert opt.state[p]["step"].item() == t
+        _check_step(before[i], _cpu(opt.state[p]), p0[i], p.detach().cpu(), p.grad.cpu(), t, 32)
