@@ -162,6 +162,8 @@ class AdamW(torch.optim.Optimizer):
             if p.dtype not in _DTYPES or not p.is_contiguous():
                 raise NotImplementedError(f"AdamW: a parameter {tuple(p.shape)} of {p.dtype}, strides {p.stride()} is not "
                                           "supported (contiguous float32, bfloat16 and float16 are)")
+            if p.grad.shape != p.shape:  # of before the weight's data were exchanged
+                raise ValueError(f"AdamW: a gradient {tuple(p.grad.shape)} of a parameter {tuple(p.shape)}")
             _require_device(p)
             # a float32 weight is its own master
             kinds.setdefault((p.device, p.dtype, master and p.dtype != torch.float32), []).append(p)

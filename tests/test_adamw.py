@@ -137,3 +137,10 @@ def test_load_groups_of_another_optimizer():
     opt = AdamW([p], state_bits=8)
     opt.load_state_dict(torch.optim.AdamW([_param(3)], lr=0.5).state_dict())
     assert opt.param_groups[0]["lr"] == 0.5 and opt.param_groups[0]["state_bits"] == 8 and not opt.param_groups[0]["master_weights"]
+
+
+def test_gradient_of_data_that_was_exchanged():
+    p = _param(4)
+    p.data = torch.zeros(9)
+    with pytest.raises(ValueError, match=r"gradient \(4,\) of a parameter \(9,\)"):
+        AdamW([p]).step()
