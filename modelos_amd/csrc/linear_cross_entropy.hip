@@ -256,9 +256,10 @@ __device__ __forceinline__ void cut(f32x16_t (&acc)[MT][NU], int64_t left, int h
 __device__ __forceinline__ float others(int row, float yr) { return fminf((row - yr) * (row - yr), 1.f); }
 
 // The sum of the exponentials of a wave's entries for the lane's token of column block u, against the token's reference: the
-// label's logit, whose own exponential is 1, so that what underflows beside it is nothing. Where it overflows, the entries' own
-// largest logit takes the reference's place. The reference's product with log2(e) is rounded once for all entries; what that
-// adds to all exponents alike comes off the sum.
+// label's logit, whose own exponential is 1, so that what underflows beside it is nothing. Where a sum reaches 2^96, the
+// entries' own largest logit takes the reference's place: up to 2^25 sums of 32 entries or more (fewer than 2^30 in all) are
+// added up against one reference later (joined), and stay below 2^121. The reference's product with log2(e) is rounded once for
+// all entries; what that adds to all exponents alike comes off the sum.
 // OWN: the label may be among the entries, yr rows (less 4 h) below the wave's first: its logit goes to `target`, its exponential
 // is left out. A loss near 0 is the logarithm of 1 + the others' exponentials, which a 1 among them would round. Left out by a
 // factor 0 or 1 (others): the masks of 64 comparisons would not fit the scalar registers.
@@ -286,7 +287,7 @@ __device__ __forceinline__ float2 sum_over(const f32x16_t (&acc)[MT][NU], int u,
   }
   sum += swap_halves(sum);
   sum -= sum * (__builtin_fmaf(ref, kLog2e, c) * kLn2);
-  const bool over = !(sum < 0x1p120f);
+  const bool over = !(sum < 0x1p96f);
   if (__any(over)) {
     float top = -3e38f;  // finite, for entries that are all -infinity
 #pragma unroll

@@ -321,3 +321,36 @@ def test_infinite_logits(n, device):
     assert torch.equal(torch.isinf(loss), labels.cpu() == 0) and not loss.isnan().any()
     fine = labels.cpu() != 0
     assert ((loss - want)[fine].abs() <= 2.0**-21 * want[fine]).all()
+
+
+@pytest.mark.parametrize("n", [64, 300])
+@pytest.mark.parametrize("V", [40000, 151936, 200003])
+def test_a_flat_vocabulary_far_above_the_labels(V, n, device):
+    """Labels 60 to 100 below a vocabulary of equal logits: the sums of the parts of the vocabulary, each against the
+    label's logit, stay in float32 one by one before all of them together do. Every logit is exact: -gap in a label's
+    column 0, zeros elsewhere, a 1 in column 1 of the other rows for dx to see the softmax."""
+    gap = torch.linspace(60, 100, n).to(BF16)
+    labels = torch.randperm(V, generator=torch.Generator().manual_seed(V + n))[:n]
+    w = torch.zeros((V, 8), dtype=BF16)
+    w[:, 1] = 1
+    w[labels, 0], w[labels, 1] = -gap, 0
+    x = torch.eye(1, 8, dtype=BF16).expand(n, 8).contiguous().to(device).requires_grad_()
+    w = w.to(device).requires_grad_()
+    loss = linear_cross_entropy(x, w, labels.to(device), reduction="none")
+    dx, dw = (g.cpu().double() for g in torch.autograd.grad(loss.sum(), (x, w)))
+    gap = gap.double()
+    total = V - n + (-gap).exp().sum()
+    want = total.log() + gap
+    # the exponent's rounding at up to 100 log2(e), the sum of V exponentials, the logarithm's and the sums' roundings
+    bound = 2.0**-24 * (4 * gap + 4 * total.log() + 2 * V**0.5 + 16)
+    _near(loss, want, bound, "loss")
+    # d is rounded, all entries' alike, and the results are; exp(l - lse) is off by what lse is
+    off = 2 * 2.0**-8 + 2.0**-16 + 2 * bound.max()
+    p = 1 / total
+    _near(dx[:, 1], ((V - n) * p).expand(n), off, "dx from the softmax")
+    _near(dx[:, 0], gap, off * gap, "dx from the label")
+    others = torch.ones(V, dtype=torch.bool)
+    others[labels] = False
+    _near(dw[others, 0], (n * p).expand(V - n), off * n * p, "dW of the others")
+    _near(dw[labels, 0], -torch.ones(n), off + 1e-20, "dW of the labels")
+    assert not dw[:, 1:].any()
