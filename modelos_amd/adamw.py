@@ -35,6 +35,7 @@ import operator
 
 import numpy as np
 import torch
+from torch import Tensor
 
 from . import _lib
 from .embedding_bag import _require_device
@@ -44,6 +45,7 @@ _BLOCK = 256
 _CODES = torch.float8_e4m3fn
 _FIELDS = 9  # words of pkm_adamw_tensor_t
 _GRAD = 1  # the gradient's
+_DTYPE = operator.attrgetter("dtype")
 
 
 def _names(bits: int, master: bool) -> tuple[str, ...]:
@@ -74,10 +76,11 @@ class _Plan:
         self.ws_bytes = _lib.load().pkm_adamw_workspace_size(len(params))
 
     def _places(self) -> list:
-        """Where weights and states lie, which an assignment to their `data` changes too, and the weights' forms."""
-        Tensor, states = torch.Tensor, itertools.chain.from_iterable(map(self.take, self.states))
-        return [*map(Tensor.data_ptr, self.params), *map(Tensor.numel, self.params),
-                *map(Tensor.is_contiguous, self.params), *map(Tensor.data_ptr, states)]
+        """Where weights and states lie, which an assignment to their `data` changes too, and what the weights are: another
+        type may have the same memory (a view, or a copy that was put where the weight had been)."""
+        params, states = self.params, itertools.chain.from_iterable(map(self.take, self.states))
+        return [*map(Tensor.data_ptr, params), *map(Tensor.numel, params), *map(Tensor.is_contiguous, params),
+                *map(_DTYPE, params), *map(Tensor.get_device, params), *map(Tensor.data_ptr, states)]
 
     def stands(self) -> bool:
         """Whether the weights and states are what and where they were: what is held here keeps its place to itself."""

@@ -5,11 +5,12 @@ from __future__ import annotations
 import torch
 
 
-def loss_and_gradients(x, w, labels, ignore: int, reduction: str, grad=None):
+def loss_and_gradients(x, w, labels, ignore: int, reduction: str, grad=None, each: bool = False):
     """x [n, D], w [V, D], labels [n]: values (loss, dx, dW) and bounds of the same shapes.
 
     The bounds are those of a kernel that sums in float32, rounds the logits' gradients once to x's type (relative error u)
-    for the products with w and x, and rounds its results once. grad: float64 [] or [n].
+    for the products with w and x, and rounds its results once. grad: float64 [] or [n]. each: f16's logits' gradients are
+    held in units of their own token's gradient, not of the largest.
     """
     n, D = x.shape
     V = w.shape[0]
@@ -40,10 +41,14 @@ def loss_and_gradients(x, w, labels, ignore: int, reduction: str, grad=None):
     d = (p - onehot) * g
     # d: the exponential's error, one float32 rounding more for the label's, the rounding to 16 bits, what f16 cannot hold
     # (2^-24 2^-14 of the largest gradient)
-    e_d = g.abs() * (p * (e_logit + e_lse[:, None]) + f * 4 * (p + onehot)) + u * d.abs() + f * 2.0**-13 * g.abs().max()
+    unit = g.abs() if each else g.abs().max()
+    e_d = g.abs() * (p * (e_logit + e_lse[:, None]) + f * 4 * (p + onehot)) + u * d.abs() + f * 2.0**-13 * unit
     dx, dw = d @ w, d.T @ x
     e_dx = e_d @ w.abs() + f * 64 * (d.abs() @ w.abs())
     e_dw = e_d.T @ x.abs() + f * 64 * (d.abs().T @ x.abs())
+    if each:  # the powers of two between the tokens' go to x: the largest product with its gradient (within a factor of 4) is
+        # 2^15, f16's rounding 2^-25
+        e_dw = e_dw + 2.0**-38 * (g.abs() * x.abs()).max() * (p - onehot).abs().T @ live[:, None].double().expand_as(x)
     # float32 sums of n or V numbers: 64 roundings stand for the blocks of a matrix product and its splits, whose
     # errors add like a random walk
     return ((value, dx, dw),

@@ -395,3 +395,20 @@ def test_states_taken_away(how, device):
         t = 1 if i in gone else 2 if how == "put back" else 3
         assert opt.state[p]["step"].item() == t
         _check_step(before[i], _cpu(opt.state[p]), p0[i], p.detach().cpu(), p.grad.cpu(), t, 32)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_weight_viewed_as_another_type(bits, device):
+    """The same memory as the other type of 16 bits between two steps."""
+    gen = torch.Generator().manual_seed(12)
+    (p,) = _params(gen, BF16, device, [(40, 50)])
+    opt = AdamW([p], **HYPER, state_bits=bits)
+    for _ in range(2):
+        _grads(gen, [p])
+        opt.step()
+    p.grad, p.data = None, p.data.view(F16)
+    _grads(gen, [p])
+    before, p0 = _cpu(opt.state[p]), p.detach().cpu().clone()
+    opt.step()
+    assert p.dtype == F16 and p0.isfinite().all()
+    _check_step(before, _cpu(opt.state[p]), p0, p.detach().cpu(), p.grad.cpu(), 3, bits)
