@@ -73,14 +73,15 @@ class _Plan:
             if master:
                 row.master = s["master"].data_ptr()
         self.device, self.dtype = params[0].device, _lib.dtype_code(params[0])
+        self.grads_are = [*map(Tensor.numel, params), *map(Tensor.get_device, params), *map(_DTYPE, params)]
         self.ws_bytes = _lib.load().pkm_adamw_workspace_size(len(params))
 
     def _places(self) -> list:
-        """Where weights and states lie, which an assignment to their `data` changes too, and what the weights are: another
-        type may have the same memory (a view, or a copy that was put where the weight had been)."""
+        """Where weights and states lie (an address is of one device), which an assignment to their `data` changes too, and
+        what the weights are: another type may have the same memory (a view, or a copy that was put where the weight had been)."""
         params, states = self.params, itertools.chain.from_iterable(map(self.take, self.states))
         return [*map(Tensor.data_ptr, params), *map(Tensor.numel, params), *map(Tensor.is_contiguous, params),
-                *map(_DTYPE, params), *map(Tensor.get_device, params), *map(Tensor.data_ptr, states)]
+                *map(_DTYPE, params), *map(Tensor.data_ptr, states)]
 
     def stands(self) -> bool:
         """Whether the weights and states are what and where they were: what is held here keeps its place to itself."""
@@ -207,24 +208,29 @@ class AdamW(torch.optim.Optimizer):
                 self._launch(plan, group, grad_scale)
         return loss
 
+    @staticmethod
+    def _gradients(plan: _Plan) -> list[torch.Tensor]:
+        """The gradients of a plan's weights, contiguous. Anything may have come to lie in their `data` since the last step."""
+        grads = [p.grad for p in plan.params]
+        whole = all(map(Tensor.is_contiguous, grads))  # which sparse ones are not
+        if not whole or [*map(Tensor.numel, grads), *map(Tensor.get_device, grads), *map(_DTYPE, grads)] != plan.grads_are:
+            for p, g in zip(plan.params, grads):
+                if g.dtype != p.dtype or g.layout is not torch.strided:
+                    raise NotImplementedError(f"AdamW: a gradient of {g.dtype}, {g.layout} for a parameter of {p.dtype} is not "
+                                              "supported (dense ones of the parameter's type are)")
+                if g.shape != p.shape or g.device != p.device:
+                    raise ValueError(f"AdamW: a gradient {tuple(g.shape)} on {g.device} of a parameter {tuple(p.shape)} on {p.device}")
+        return grads if whole else [g.contiguous() for g in grads]
+
     def _launch(self, plan: _Plan, group: dict, grad_scale) -> None:
-        grads, at, dtype = [], [], plan.params[0].dtype
-        for p in plan.params:
-            g = p.grad
-            if g.dtype is not dtype or g.layout is not torch.strided:
-                raise NotImplementedError(f"AdamW: a gradient of {g.dtype}, {g.layout} for a parameter of {p.dtype} is not "
-                                          "supported (dense ones of the parameter's type are)")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                grads.append(g)
-            at.append(g.data_ptr())
+        grads = self._gradients(plan)
         lr = group["lr"]
         lr_device = lr if isinstance(lr, torch.Tensor) and lr.is_cuda else None
         if lr_device is not None or grad_scale is not None:
             _require_device(plan.params[0], lr_device, grad_scale)
-        plan.words[:, _GRAD] = at
+        plan.words[:, _GRAD] = list(map(Tensor.data_ptr, grads))
         ws = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=plan.device)
-        _lib.call_on(plan.device, "pkm_adamw_step", plan.table, len(at), plan.dtype, plan.bits,
+        _lib.call_on(plan.device, "pkm_adamw_step", plan.table, len(grads), plan.dtype, plan.bits,
                      0.0 if lr_device is not None else float(lr), _lib.ptr(lr_device), *group["betas"], group["eps"],
                      group["weight_decay"], _lib.ptr(grad_scale), _lib.ptr(ws), plan.ws_bytes, _lib.stream_of(plan.device))
         torch.autograd.graph.increment_version(plan.params)  # as an update in place does

@@ -412,3 +412,20 @@ def test_a_weight_viewed_as_another_type(bits, device):
     opt.step()
     assert p.dtype == F16 and p0.isfinite().all()
     _check_step(before, _cpu(opt.state[p]), p0, p.detach().cpu(), p.grad.cpu(), 3, bits)
+
+
+def test_a_gradient_moved_to_the_host(device):
+    """torch lets a gradient's data be exchanged for one elsewhere: refused before anything runs."""
+    gen = torch.Generator().manual_seed(13)
+    params = _params(gen, F32, device, [(40,), (7,)])
+    opt = AdamW(params, **HYPER)
+    for _ in range(2):
+        _grads(gen, params)
+        opt.step()
+    _grads(gen, params)
+    params[1].grad.data = params[1].grad.data.cpu()
+    held = copy.deepcopy([p.detach() for p in params]), [_cpu(opt.state[p]) for p in params]
+    with pytest.raises(ValueError, match="on cpu of a parameter"):
+        opt.step()
+    for p, p0, s in zip(params, *held):
+        assert torch.equal(p, p0) and all(torch.equal(x, s[n]) for n, x in _cpu(opt.state[p]).items())

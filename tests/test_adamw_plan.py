@@ -65,3 +65,43 @@ def test_a_weight_of_another_type_in_the_same_place(launches):
     with pytest.raises(ValueError, match="master"):
         opt.step()
     assert not launches
+
+
+@pytest.mark.parametrize("data", [torch.zeros(39), torch.zeros(41), torch.zeros(0)], ids=["shorter", "longer", "none"])
+@pytest.mark.parametrize("which", [0, 2])
+def test_a_gradient_exchanged_for_one_that_does_not_fit(which, data, launches):
+    """Through its `data`, which torch lets pass, between two steps of one plan."""
+    params = [_param(40), _param(3), _param(40)]
+    opt = _steps(params, launches)
+    params[which].grad.data = data
+    with pytest.raises(ValueError, match="gradient"):
+        opt.step()
+    assert not launches
+
+
+def test_gradients_in_other_places_and_orders(launches):
+    """Every step's own gradients are passed on, those of other strides as copies in the weight's order."""
+    params = [_param(4, 6), _param(3), _param(4, 6)]
+    opt = _steps(params, launches)
+    for _ in range(2):
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        params[2].grad = torch.zeros(6, 4).T
+        opt.step()
+        ((_, _, rows),) = launches
+        launches.clear()
+        assert [r["grad"] for r in rows[:2]] == [p.grad.data_ptr() for p in params[:2]]
+        assert rows[2]["grad"] != params[2].grad.data_ptr()
+
+
+@pytest.mark.parametrize("grad", [torch.zeros(4, 6).to_sparse(), torch.zeros(4, 6, dtype=BF16)], ids=["sparse", "bf16"])
+def test_gradients_of_another_kind(grad, launches):
+    p = _param(4, 6)
+    opt = _steps([p], launches)
+    if grad.dtype == p.dtype:
+        p.grad = grad
+    else:
+        p.grad.data = grad
+    with pytest.raises(NotImplementedError, match="gradient"):
+        opt.step()
+    assert not launches
