@@ -25,7 +25,8 @@ device, read when the step runs.
 
 Supported: float32, bfloat16 and float16 parameters on the GPU, contiguous, with
 dense gradients of their type; anything else raises NotImplementedError. There is
-no CPU path: CPU tensors raise.
+no CPU path: CPU tensors raise. The parameters of a group are updated at once: one
+that is there twice, and parameters or states that share memory, raise ValueError.
 """
 from __future__ import annotations
 
@@ -43,8 +44,10 @@ from .embedding_bag import _require_device
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _BLOCK = 256
 _CODES = torch.float8_e4m3fn
+_IN_CODES = ("exp_avg", "exp_root")
 _FIELDS = 9  # words of pkm_adamw_tensor_t
-_GRAD = 1  # the gradient's
+_PARAM, _GRAD, _NUMEL = 0, 1, 8
+_COLUMNS = {"exp_avg": 2, "exp_avg_sq": 3, "exp_root": 3, "exp_avg_scale": 4, "exp_root_scale": 5, "master": 6, "step": 7}
 _DTYPE = operator.attrgetter("dtype")
 
 
@@ -65,16 +68,30 @@ class _Plan:
         self.table = (_lib.AdamWTensor * len(params))()
         self.words = np.frombuffer(self.table, dtype=np.int64).reshape(len(params), _FIELDS)
         self.places = self._places()
-        for row, p, s in zip(self.table, params, states):
-            row.param, row.exp_avg, row.step, row.numel = p.data_ptr(), s["exp_avg"].data_ptr(), s["step"].data_ptr(), p.numel()
-            row.second = s["exp_avg_sq" if bits == 32 else "exp_root"].data_ptr()
-            if bits == 8:
-                row.exp_avg_scale, row.second_scale = s["exp_avg_scale"].data_ptr(), s["exp_root_scale"].data_ptr()
-            if master:
-                row.master = s["master"].data_ptr()
+        columns = (_PARAM, *(_COLUMNS[n] for n in self.names))
+        for column, tensors in zip(columns, zip(*((p, *held) for p, held in zip(params, self.held)))):
+            self.words[:, column] = list(map(Tensor.data_ptr, tensors))
+        self.words[:, _NUMEL] = list(map(Tensor.numel, params))
+        if self._shares_memory(params[0].element_size(), master):
+            raise ValueError(f"AdamW: parameters of one group, or their states, share memory (of {len(params)} of {params[0].dtype}):"
+                             " they would be updated at once")
         self.device, self.dtype = params[0].device, _lib.dtype_code(params[0])
         self.grads_are = [*map(Tensor.numel, params), *map(Tensor.get_device, params), *map(_DTYPE, params)]
         self.ws_bytes = _lib.load().pkm_adamw_workspace_size(len(params))
+
+    def _shares_memory(self, item: int, master: bool) -> bool:
+        """Whether anything that a step writes lies in two places of the table: its rows are worked on at once."""
+        n, held = self.words[:, _NUMEL:], self.bits // 8
+        sizes = n * np.array([item, 0, held, held, 0, 0, 4 * master, 0])
+        if self.bits == 8:
+            sizes[:, 4:6] = -(-n // _BLOCK) * 4
+        sizes[:, 7] = 4
+        begins, sizes = self.words[:, :_NUMEL].flatten(), sizes.ravel()
+        begins[sizes == 0] = 0
+        order = np.argsort(begins)
+        begins = begins[order]
+        ends = begins + sizes[order]
+        return bool((ends[:-1] > begins[1:]).any())
 
     def _places(self) -> list:
         """Where weights and states lie (an address is of one device), which an assignment to their `data` changes too, and
@@ -111,6 +128,8 @@ class AdamW(torch.optim.Optimizer):
         group = self.param_groups[-1]
         try:
             self._check(group)
+            if len(set(map(id, group["params"]))) != len(group["params"]):  # torch warns only
+                raise ValueError("AdamW: a parameter group holds a parameter more than once")
         except Exception:
             self.param_groups.pop()
             raise
@@ -148,17 +167,17 @@ class AdamW(torch.optim.Optimizer):
         return state
 
     @staticmethod
-    def _check_state(state: dict, p: torch.Tensor, bits: int, master: bool) -> None:
-        wide = torch.float32
-        kinds = {"exp_avg": wide if bits == 32 else _CODES, "exp_avg_sq": wide, "exp_root": _CODES, "exp_avg_scale": wide,
-                 "exp_root_scale": wide, "master": wide, "step": wide}
+    def _check_states(states: list[dict], params: list, bits: int, master: bool) -> None:
+        numels, places = list(map(Tensor.numel, params)), list(map(Tensor.get_device, params))
+        blocks = [-(-n // _BLOCK) for n in numels]
         for name in (*_names(bits, master), "step"):
-            x = state.get(name)
-            n = 1 if name == "step" else -(-p.numel() // _BLOCK) if name.endswith("scale") else p.numel()
-            if not isinstance(x, torch.Tensor) or x.dtype != kinds[name] or x.numel() != n or x.device != p.device \
-                    or not x.is_contiguous():
-                raise ValueError(f"AdamW: the state {name!r} of a parameter {tuple(p.shape)} has to be {n} contiguous numbers "
-                                 f"of {kinds[name]} on {p.device}, with state_bits={bits}, master_weights={master}")
+            kind = _CODES if bits == 8 and name in _IN_CODES else torch.float32
+            sizes = [1] * len(params) if name == "step" else blocks if name.endswith("scale") else numels
+            for p, x, n, place in zip(params, (s.get(name) for s in states), sizes, places):
+                if not isinstance(x, Tensor) or x.dtype is not kind or x.numel() != n or not x.is_contiguous() \
+                        or x.get_device() != place:
+                    raise ValueError(f"AdamW: the state {name!r} of a parameter {tuple(p.shape)} has to be {n} contiguous numbers "
+                                     f"of {kind} on {p.device}, with state_bits={bits}, master_weights={master}")
 
     def _plans_of(self, params: list, bits: int, master: bool) -> list[_Plan]:
         kinds: dict = {}
@@ -173,11 +192,12 @@ class AdamW(torch.optim.Optimizer):
             kinds.setdefault((p.device, p.dtype, master and p.dtype != torch.float32), []).append(p)
         plans = []
         for (_, _, with_master), some in kinds.items():
-            for p in some:
-                if not self.state[p]:
-                    self.state[p] = self._new_state(p, bits, with_master)
-                self._check_state(self.state[p], p, bits, with_master)
-            plans.append(_Plan(some, [self.state[p] for p in some], bits, with_master))
+            states = [self.state[p] for p in some]
+            for i, p in enumerate(some):
+                if not states[i]:
+                    states[i] = self.state[p] = self._new_state(p, bits, with_master)
+            self._check_states(states, some, bits, with_master)
+            plans.append(_Plan(some, states, bits, with_master))
         return plans
 
     @torch.no_grad()
@@ -247,7 +267,7 @@ class AdamW(torch.optim.Optimizer):
                 continue
             state = {n: x.to(device=p.device).contiguous() if isinstance(x, torch.Tensor) else x for n, x in saved.items()}
             state["step"] = torch.as_tensor(state["step"], dtype=torch.float32, device=p.device).reshape(())
-            self._check_state(state, p, group["state_bits"], bool(group["master_weights"]) and p.dtype != torch.float32)
+            self._check_states([state], [p], group["state_bits"], bool(group["master_weights"]) and p.dtype != torch.float32)
             self.state[p] = state
 
 

@@ -105,3 +105,42 @@ def test_gradients_of_another_kind(grad, launches):
     with pytest.raises(NotImplementedError, match="gradient"):
         opt.step()
     assert not launches
+
+
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate parameters")
+def test_one_weight_twice(launches):
+    """Two rows of one launch would update the same numbers at once."""
+    p, q = _param(40), _param(3)
+    with pytest.raises(ValueError, match="more than once"):
+        AdamW([p, q, p])
+    opt = AdamW([q])
+    with pytest.raises(ValueError, match="more than once"):
+        opt.add_param_group({"params": [p, p]})
+    assert len(opt.param_groups) == 1
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_weights_that_share_memory(bits, launches):
+    """Of one launch; those that lie side by side in one tensor do not."""
+    flat = torch.zeros(600)
+    a, b, c = (torch.nn.Parameter(flat[i:j]) for i, j in ((0, 300), (300, 600), (299, 301)))
+    for p in (a, b, c):
+        p.grad = torch.zeros_like(p)
+    AdamW([b, a], state_bits=bits).step()
+    assert len(launches) == 1
+    for pair in ([a, c], [c, b], [a, b, c]):
+        with pytest.raises(ValueError, match="share memory"):
+            AdamW(pair, state_bits=bits).step()
+    assert len(launches) == 1
+    AdamW([{"params": [a]}, {"params": [c]}], state_bits=bits).step()  # one after the other
+    assert len(launches) == 3
+
+
+@pytest.mark.parametrize("name", ["exp_avg", "exp_root", "exp_avg_scale", "master", "step"])
+def test_states_that_share_memory(name, launches):
+    params = [_param(300, dtype=BF16), _param(300, dtype=BF16), _param(0, dtype=BF16)]
+    opt = _steps(params, launches, state_bits=8, master_weights=True)
+    opt.state[params[1]][name] = opt.state[params[0]][name]
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
+    assert not launches
