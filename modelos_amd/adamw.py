@@ -67,6 +67,7 @@ class _Plan:
         self.held = [self.take(s) for s in states]
         self.table = (_lib.AdamWTensor * len(params))()
         self.words = np.frombuffer(self.table, dtype=np.int64).reshape(len(params), _FIELDS)
+        self.grads_at = self.words[:, _GRAD]
         self.places = self._places()
         columns = (_PARAM, *(_COLUMNS[n] for n in self.names))
         for column, tensors in zip(columns, zip(*((p, *held) for p, held in zip(params, self.held)))):
@@ -214,9 +215,12 @@ class AdamW(torch.optim.Optimizer):
         if len(self.state) != len(self._planned) or not all(map(operator.is_, self.state.values(), self._planned)):
             self._plans = {}
         for i, group in enumerate(self.param_groups):
-            params = [p for p in group["params"] if p.grad is not None]
+            grads = [p.grad for p in group["params"]]
+            params = [p for p, g in zip(group["params"], grads) if g is not None]
             if not params:
                 continue
+            if len(params) != len(grads):
+                grads = [g for g in grads if g is not None]
             self._check(group)
             bits, master = group["state_bits"], bool(group["master_weights"])
             held = self._plans.get(i)
@@ -225,13 +229,13 @@ class AdamW(torch.optim.Optimizer):
                 held = self._plans[i] = ((bits, master), params, self._plans_of(params, bits, master))
                 self._planned = list(self.state.values())
             for plan in held[2]:
-                self._launch(plan, group, grad_scale)
+                own = grads if len(held[2]) == 1 else [p.grad for p in plan.params]
+                self._launch(plan, group, self._checked(plan, own), grad_scale)
         return loss
 
     @staticmethod
-    def _gradients(plan: _Plan) -> list[torch.Tensor]:
+    def _checked(plan: _Plan, grads: list) -> list[torch.Tensor]:
         """The gradients of a plan's weights, contiguous. Anything may have come to lie in their `data` since the last step."""
-        grads = [p.grad for p in plan.params]
         whole = all(map(Tensor.is_contiguous, grads))  # which sparse ones are not
         if not whole or [*map(Tensor.numel, grads), *map(Tensor.get_device, grads), *map(_DTYPE, grads)] != plan.grads_are:
             for p, g in zip(plan.params, grads):
@@ -242,13 +246,12 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError(f"AdamW: a gradient {tuple(g.shape)} on {g.device} of a parameter {tuple(p.shape)} on {p.device}")
         return grads if whole else [g.contiguous() for g in grads]
 
-    def _launch(self, plan: _Plan, group: dict, grad_scale) -> None:
-        grads = self._gradients(plan)
+    def _launch(self, plan: _Plan, group: dict, grads: list, grad_scale) -> None:
         lr = group["lr"]
         lr_device = lr if isinstance(lr, torch.Tensor) and lr.is_cuda else None
         if lr_device is not None or grad_scale is not None:
             _require_device(plan.params[0], lr_device, grad_scale)
-        plan.words[:, _GRAD] = list(map(Tensor.data_ptr, grads))
+        plan.grads_at[:] = list(map(Tensor.data_ptr, grads))
         ws = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=plan.device)
         _lib.call_on(plan.device, "pkm_adamw_step", plan.table, len(grads), plan.dtype, plan.bits,
                      0.0 if lr_device is not None else float(lr), _lib.ptr(lr_device), *group["betas"], group["eps"],
