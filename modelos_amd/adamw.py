@@ -214,6 +214,7 @@ class AdamW(torch.optim.Optimizer):
                              f"{tuple(grad_scale.shape)}")
         if len(self.state) != len(self._planned) or not all(map(operator.is_, self.state.values(), self._planned)):
             self._plans = {}
+        work = []  # all groups are looked at before the first runs: a step that is refused changes nothing
         for i, group in enumerate(self.param_groups):
             grads = [p.grad for p in group["params"]]
             params = [p for p, g in zip(group["params"], grads) if g is not None]
@@ -230,7 +231,9 @@ class AdamW(torch.optim.Optimizer):
                 self._planned = list(self.state.values())
             for plan in held[2]:
                 own = grads if len(held[2]) == 1 else [p.grad for p in plan.params]
-                self._launch(plan, group, self._checked(plan, own), grad_scale)
+                work.append((plan, group, self._checked(plan, own), self._rate(plan, group, grad_scale)))
+        for plan, group, grads, rate in work:
+            self._launch(plan, group, grads, rate, grad_scale)
         return loss
 
     @staticmethod
@@ -246,16 +249,21 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError(f"AdamW: a gradient {tuple(g.shape)} on {g.device} of a parameter {tuple(p.shape)} on {p.device}")
         return grads if whole else [g.contiguous() for g in grads]
 
-    def _launch(self, plan: _Plan, group: dict, grads: list, grad_scale) -> None:
+    @staticmethod
+    def _rate(plan: _Plan, group: dict, grad_scale) -> tuple:
+        """The rate as a number, and as one on the device."""
         lr = group["lr"]
-        lr_device = lr if isinstance(lr, torch.Tensor) and lr.is_cuda else None
-        if lr_device is not None or grad_scale is not None:
-            _require_device(plan.params[0], lr_device, grad_scale)
+        on_device = lr if isinstance(lr, Tensor) and lr.is_cuda else None
+        if on_device is not None or grad_scale is not None:
+            _require_device(plan.params[0], on_device, grad_scale)
+        return (float(lr), None) if on_device is None else (0.0, on_device)
+
+    def _launch(self, plan: _Plan, group: dict, grads: list, rate: tuple, grad_scale) -> None:
         plan.grads_at[:] = list(map(Tensor.data_ptr, grads))
         ws = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=plan.device)
-        _lib.call_on(plan.device, "pkm_adamw_step", plan.table, len(grads), plan.dtype, plan.bits,
-                     0.0 if lr_device is not None else float(lr), _lib.ptr(lr_device), *group["betas"], group["eps"],
-                     group["weight_decay"], _lib.ptr(grad_scale), _lib.ptr(ws), plan.ws_bytes, _lib.stream_of(plan.device))
+        _lib.call_on(plan.device, "pkm_adamw_step", plan.table, len(grads), plan.dtype, plan.bits, rate[0],
+                     _lib.ptr(rate[1]), *group["betas"], group["eps"], group["weight_decay"], _lib.ptr(grad_scale),
+                     _lib.ptr(ws), plan.ws_bytes, _lib.stream_of(plan.device))
         torch.autograd.graph.increment_version(plan.params)  # as an update in place does
 
     def load_state_dict(self, state_dict: dict) -> None:

@@ -144,3 +144,30 @@ def test_states_that_share_memory(name, launches):
     with pytest.raises(ValueError, match="share memory"):
         opt.step()
     assert not launches
+
+
+@pytest.mark.parametrize("what", ["sparse", "shorter", "rate", "option", "state", "scale"])
+def test_a_refused_step_changes_nothing(what, launches, monkeypatch):
+    """A group that cannot be stepped: neither are the groups before it."""
+    a, b, c = _param(40), _param(40, dtype=BF16), _param(5)
+    opt = _steps([{"params": [a, b]}, {"params": [c]}], launches)
+    if what == "sparse":
+        c.grad = torch.zeros(5).to_sparse()
+    elif what == "shorter":
+        c.grad.data = torch.zeros(4)
+    elif what == "option":
+        opt.param_groups[1]["betas"] = (0.9, 1.0)
+    elif what == "state":
+        opt.state[c]["exp_avg"] = torch.zeros(4)
+    elif what == "rate":
+        opt.param_groups[1]["lr"] = torch.zeros(2)
+
+    def require(*tensors):
+        if any(t is not None and t.dim() == 1 and t.numel() == 1 for t in tensors):
+            raise RuntimeError("elsewhere")
+
+    monkeypatch.setattr(adamw, "_require_device", require)
+    scale = torch.ones(1) if what == "scale" else None
+    with pytest.raises((ValueError, NotImplementedError, RuntimeError)):
+        opt.step(grad_scale=scale)
+    assert not launches
