@@ -30,6 +30,7 @@ that is there twice, and parameters or states that share memory, raise ValueErro
 """
 from __future__ import annotations
 
+import collections
 import itertools
 import math
 import operator
@@ -118,6 +119,8 @@ class AdamW(torch.optim.Optimizer):
                                       master_weights=master_weights))
 
     def __setstate__(self, state):
+        if "_loading" in self.__dict__:
+            state = {**state, "state": self.__dict__.pop("_loading")}
         super().__setstate__(state)
         for group in self.param_groups:  # of an optimizer without these options
             for name, value in self.defaults.items():
@@ -267,19 +270,38 @@ class AdamW(torch.optim.Optimizer):
         torch.autograd.graph.increment_version(plan.params)  # as an update in place does
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As torch's; states keep their types (torch's would take that of the weight)."""
-        super().load_state_dict({**state_dict, "state": {}})
-        self._plans = {}
-        self.state.clear()
-        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        for (group, p), i in zip(((g, p) for g in self.param_groups for p in g["params"]), ids):
-            saved = state_dict["state"].get(i)
-            if not saved:
-                continue
-            state = {n: x.to(device=p.device).contiguous() if isinstance(x, torch.Tensor) else x for n, x in saved.items()}
-            state["step"] = torch.as_tensor(state["step"], dtype=torch.float32, device=p.device).reshape(())
-            self._check_states([state], [p], group["state_bits"], bool(group["master_weights"]) and p.dtype != torch.float32)
-            self.state[p] = state
+        """As torch's; states keep their types (torch's would take that of the weight). One that is refused changes nothing."""
+
+        def take(_, loaded: dict) -> dict:  # the last of the hooks before: what the others have made of it
+            self._loading = self._states_of(loaded)
+            return {**loaded, "state": {}}
+
+        handle = self.register_load_state_dict_pre_hook(take)
+        try:
+            super().load_state_dict(state_dict)  # which hands on to __setstate__
+        finally:
+            handle.remove()
+            self.__dict__.pop("_loading", None)
+
+    def _states_of(self, loaded: dict) -> collections.defaultdict:
+        """What is loaded as the parameters' states, on their devices."""
+        states, names = collections.defaultdict(dict), set()
+        for group, saved in zip(self.param_groups, loaded["param_groups"]):
+            options = {**self.defaults, **saved}
+            self._check(options)
+            for p, i in zip(group["params"], saved["params"]):
+                names.add(i)
+                if not loaded["state"].get(i):
+                    continue
+                state = {n: x.to(device=p.device).contiguous() if isinstance(x, Tensor) else x
+                         for n, x in loaded["state"][i].items()}
+                if "step" in state:  # a counter of its own, which saved ones may share
+                    state["step"] = torch.as_tensor(state["step"], dtype=torch.float32, device=p.device).reshape(()).clone()
+                with_master = bool(options["master_weights"]) and p.dtype != torch.float32
+                self._check_states([state], [p], options["state_bits"], with_master)
+                states[p] = state
+        states.update((i, x) for i, x in loaded["state"].items() if i not in names)  # of no parameter: as torch's
+        return states
 
 
 __all__ = ["AdamW"]

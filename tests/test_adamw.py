@@ -144,3 +144,80 @@ def test_gradient_of_data_that_was_exchanged():
     p.data = torch.zeros(9)
     with pytest.raises(ValueError, match=r"gradient \(4,\) of a parameter \(9,\)"):
         AdamW([p]).step()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_hooks_of_loading_see_the_states(bits):
+    """As with torch's optimizers: a hook before sees, and may change, what is loaded; one behind finds it loaded."""
+    opt = AdamW([_param(300)], state_bits=bits)
+    seen = []
+
+    def before(optimizer, loaded):
+        seen.append((len(optimizer.state), set(loaded["state"][0])))
+        return {**loaded, "state": {0: {**loaded["state"][0], "step": torch.tensor(9.0)}}}
+
+    def behind(optimizer):
+        (state,) = optimizer.state.values()
+        seen.append((state["step"].item(), state["exp_avg"].dtype))
+
+    opt.register_load_state_dict_pre_hook(before)
+    opt.register_load_state_dict_post_hook(behind)
+    state = _state(bits)
+    opt.load_state_dict({"state": {0: state}, "param_groups": opt.state_dict()["param_groups"]})
+    assert seen == [(0, set(state)), (9.0, state["exp_avg"].dtype)]
+
+
+@pytest.mark.parametrize("wrong", ["state", "of another kind", "groups", "sizes", "option"])
+def test_a_refused_load_changes_nothing(wrong):
+    p, q = _param(300), _param(2)
+    opt = AdamW([{"params": [p]}, {"params": [q], "lr": 0.25}], betas=(0.5, 0.5))
+    groups = opt.state_dict()["param_groups"]
+    opt.load_state_dict({"state": {0: _state(), 1: _state(n=2)}, "param_groups": groups})
+    held = {t: dict(s) for t, s in opt.state.items()}
+    new = [{**g, "lr": 0.125} for g in groups]
+    states = {0: _state(step=torch.tensor(8.0)), 1: _state(n=2)}
+    if wrong == "state":
+        states[1] = _state(n=3)
+    elif wrong == "of another kind":
+        new[1]["state_bits"] = 8
+    elif wrong == "groups":
+        new = new[:1]
+    elif wrong == "sizes":
+        new[1] = {**new[1], "params": [1, 2]}
+    else:
+        new[1]["weight_decay"] = -1.0
+    with pytest.raises(ValueError):
+        opt.load_state_dict({"state": states, "param_groups": new})
+    assert [g["lr"] for g in opt.param_groups] == [1e-3, 0.25] and opt.param_groups[1]["state_bits"] == 32
+    assert set(opt.state) == {p, q} and all(opt.state[t][n] is x for t, s in held.items() for n, x in s.items())
+
+
+def test_loaded_options_decide_what_states_are():
+    """Those that are loaded, not those that the optimizer had."""
+    opt = AdamW([_param(300)])
+    saved = AdamW([_param(300)], state_bits=8).state_dict()["param_groups"]
+    opt.load_state_dict({"state": {0: _state(8)}, "param_groups": saved})
+    assert opt.param_groups[0]["state_bits"] == 8 and "exp_root" in opt.state[opt.param_groups[0]["params"][0]]
+
+
+def test_copies():
+    import copy
+
+    opt = AdamW([_param(300, dtype=torch.bfloat16)], state_bits=8)
+    opt.load_state_dict({"state": {0: _state(8)}, "param_groups": opt.state_dict()["param_groups"]})
+    twin = copy.deepcopy(opt)
+    (s,), (t,) = opt.state.values(), twin.state.values()
+    assert set(s) == set(t) and all(x.dtype == t[n].dtype and torch.equal(x.float(), t[n].float()) for n, x in s.items())
+    assert twin.param_groups[0]["state_bits"] == 8
+
+
+def test_loaded_counters_are_their_own():
+    opt = AdamW([_param(300), _param(300)])
+    one = torch.tensor(4.0)
+    opt.load_state_dict({"state": {0: _state(step=one), 1: _state(step=one)}, "param_groups": opt.state_dict()["param_groups"]})
+    a, b = (s["step"] for s in opt.state.values())
+    assert a.item() == b.item() == 4.0 and len({x.data_ptr() for x in (a, b, one)}) == 3
+    without = _state()
+    del without["step"]
+    with pytest.raises(ValueError, match="step"):
+        opt.load_state_dict({"state": {0: without}, "param_groups": opt.state_dict()["param_groups"]})
