@@ -153,6 +153,11 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: {name} {group[name]!r} has to be at least 0")
         if group["state_bits"] not in (8, 32):
             raise ValueError(f"AdamW: state_bits {group['state_bits']!r} has to be 8 or 32")
+        for name in ("amsgrad", "maximize", "differentiable"):  # torch's
+            if group.get(name):
+                raise NotImplementedError(f"AdamW: {name} is not supported")
+        if not group.get("decoupled_weight_decay", True) and group["weight_decay"]:
+            raise NotImplementedError("AdamW: decoupled_weight_decay=False, decay in the gradient, is not supported")
 
     def _new_state(self, p: torch.Tensor, bits: int, master: bool) -> dict:
         if torch.cuda.is_current_stream_capturing():

@@ -221,3 +221,19 @@ def test_loaded_counters_are_their_own():
     del without["step"]
     with pytest.raises(ValueError, match="step"):
         opt.load_state_dict({"state": {0: without}, "param_groups": opt.state_dict()["param_groups"]})
+
+
+@pytest.mark.parametrize("option", [{"amsgrad": True}, {"maximize": True}, {"differentiable": True},
+                                    {"decoupled_weight_decay": False}])
+def test_options_of_torchs_that_are_not_there(option):
+    """Of a group that is given or loaded: not silently left out."""
+    with pytest.raises(NotImplementedError, match=next(iter(option))):
+        AdamW([{"params": [_param(3)], **option}])
+    opt = AdamW([_param(3)])
+    (group,) = opt.state_dict()["param_groups"]
+    with pytest.raises(NotImplementedError, match=next(iter(option))):
+        opt.load_state_dict({"state": {}, "param_groups": [{**group, **option}]})
+    opt.param_groups[0].update(option)
+    with pytest.raises(NotImplementedError, match=next(iter(option))):
+        opt.step()
+    AdamW([{"params": [_param(3)], **option, "weight_decay": 0.0}] if "decoupled_weight_decay" in option else [_param(3)])
