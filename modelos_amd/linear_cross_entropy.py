@@ -28,6 +28,8 @@ deterministic.
 
 Supported: bfloat16 and float16, up to 65536 numbers a row,
 fewer than 2^22 tokens and 2^30 entries, on the GPU; anything else raises NotImplementedError.
+Under torch.autocast hidden and weight are cast to its type first, as a linear layer's
+are, and get gradients of their own type (a float32 table is cast in every call).
 There is no CPU path: CPU tensors raise. The backward cannot be differentiated
 again, and there are no forward-mode derivatives: dual tensors raise
 NotImplementedError.
@@ -42,6 +44,7 @@ from .embedding_bag import _require_device
 from .window_attention import _refuse_tangents
 
 _DTYPES = (torch.bfloat16, torch.float16)
+_CAST = (*_DTYPES, torch.float32)  # what autocast casts
 _LABELS = {torch.int32: 32, torch.int64: 64}
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 _MAX_TOKENS, _MAX_VOCAB, _MAX_DIM, _MAX_STRIDE = 1 << 22, 1 << 30, 65536, 1 << 22
@@ -125,6 +128,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
         raise ValueError(f"linear_cross_entropy: reduction {reduction!r} has to be 'mean', 'sum' or 'none'")
     if not isinstance(ignore_index, int) or isinstance(ignore_index, bool) or not -(1 << 63) <= ignore_index < 1 << 63:
         raise ValueError(f"linear_cross_entropy: ignore_index {ignore_index!r} has to be a whole number of 64 bits")
+    if torch.is_autocast_enabled("cuda"):  # as F.linear there
+        dtype = torch.get_autocast_dtype("cuda")
+        hidden, weight = (t.to(dtype) if t.is_cuda and t.dtype in _CAST else t for t in (hidden, weight))
     if hidden.dtype not in _DTYPES or weight.dtype != hidden.dtype:
         raise NotImplementedError(f"linear_cross_entropy: {hidden.dtype} with a weight of {weight.dtype} is not supported "
                                   "(bfloat16 and float16 are, both alike)")
