@@ -790,7 +790,8 @@ int pkm_linear_ce_fwd(const void* x, int64_t x_stride, int64_t tokens, const voi
  * and grad_loss (float32, one number or [tokens] by reduction): dx [tokens, dim], zeros for
  * tokens that do not count, and dweight [vocab, dim], of the inputs' type, 16-byte aligned;
  * either may be NULL and is then not computed. The logits' gradients are rounded to the inputs' type for the
- * products (f16: with a power of two taken out); sums are float32 in a fixed order.
+ * products (f16: in units of their token's gradient, whose powers of two dweight's product has in a copy of
+ * the hidden states); sums are float32 in a fixed order.
  */
 size_t pkm_linear_ce_bwd_workspace_size(int64_t tokens, int64_t vocab, int64_t dim);
 int pkm_linear_ce_bwd(const void* kept, size_t kept_bytes, int64_t tokens, const void* weight, int64_t w_stride,

@@ -62,6 +62,7 @@ struct CeArgs {
   const float* loss;     // [npad]
   const float* lse;      // [npad]
   const float* weight;   // [npad] of the tokens' gradients, or NULL: `lift` for all
+  const float* unit;     // [npad] what a token's row of dx is multiplied by, or NULL: `scale` for all
   float2* sums;          // [2 * vocab tiles][npad] reference and sum of exponentials
   float* parts;          // [splits][whole tiles' rows][dcols] float32: of dx, or of dW where its sum is split
   uint8_t* dw;           // [vocab][dim]
@@ -741,14 +742,16 @@ __device__ __forceinline__ int label_of(const void* labels, int64_t i, int64_t i
   return y == ignore || y < 0 || y >= vocab ? -1 : (int)y;
 }
 
-// The kept tokens side by side: rows, labels, places, and the label's logit. A workgroup counts the kept tokens before its 16
+constexpr int kNothing = -1000;  // the exponent of a row of zeros
+
+// The kept tokens side by side: rows, labels, places, and the label's logit; in f16 the exponent of a row's largest number. A workgroup counts the kept tokens before its 16
 // itself: 16384 tokens' labels are read 512 times in all, 67 MB out of the L2, and no launch is needed to count.
 template <typename T, typename L>
 __global__ __launch_bounds__(1024) void ce_prepare(const T* __restrict__ x, int64_t x_stride, int64_t tokens,
                                                    const T* __restrict__ w, int64_t w_stride, int64_t vocab, int dim, int dpad,
                                                    int wide, const void* labels, int64_t ignore, Header* head, int32_t* place,
-                                                   int32_t* token, int32_t* label, float* ref, T* __restrict__ kept, int npad,
-                                                   float* losses) {
+                                                   int32_t* token, int32_t* label, float* ref, int32_t* size, T* __restrict__ kept,
+                                                   int npad, float* losses) {
   __shared__ int32_t before_s[16], own_s[16];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int64_t first = (int64_t)blockIdx.x * kPrepareRows, i = first + wave;
@@ -796,12 +799,24 @@ __global__ __launch_bounds__(1024) void ce_prepare(const T* __restrict__ x, int6
   T* const to = kept + (int64_t)at * dpad;
   const T* const wy = w + (int64_t)y * w_stride;
   float dot = 0.f;
+  int top = 0;  // bits of the largest finite number's size, f16
+  const auto measure = [&](uint32_t bits) {
+    const int a = (int)(bits & 0x7fffu);
+    if (a < 0x7c00) top = max(top, a);
+  };
   if (wide) {
     for (int c = lane; c < dpad / 8; c += 64) {
       uint4 v = make_uint4(0, 0, 0, 0);
       if (c < dim / 8) {
         v = ld16(row + 8 * c);
         dot = vec_dot<T>(v, ld16(wy + 8 * c), dot);
+        if constexpr (__is_same(T, f16_t)) {
+#pragma unroll
+          for (const uint32_t two : {v.x, v.y, v.z, v.w}) {
+            measure(two);
+            measure(two >> 16);
+          }
+        }
       }
       st16(to + 8 * c, v);
     }
@@ -811,12 +826,18 @@ __global__ __launch_bounds__(1024) void ce_prepare(const T* __restrict__ x, int6
       if (c < dim) {
         v = ((const uint16_t*)row)[c];
         dot += unpack1<T>(v) * unpack1<T>(((const uint16_t*)wy)[c]);
+        measure(v);
       }
       ((uint16_t*)to)[c] = v;
     }
   }
   dot = group_sum<64>(dot);
   if (lane == 0) ref[at] = dot;
+  if constexpr (__is_same(T, f16_t)) {
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) top = max(top, __shfl_xor(top, s));
+    if (lane == 0) size[at] = top == 0 ? kNothing : __builtin_amdgcn_frexp_expf(unpack1<T>((uint32_t)top));
+  }
 }
 
 // lse and loss of 32 tokens from the tiles' sums. losses: one for each token. mean: else the workgroup that ends last adds
@@ -885,11 +906,10 @@ __global__ __launch_bounds__(kJoinTokens* kJoinSlices) void ce_join(Header* head
   *total = mean ? sum / (float)max(count, 1) : sum;
 }
 
-// The tokens' gradients as weights of d: g_j over a power of two that the largest is just below, times `lift` (2^14 in f16,
-// whose smallest numbers softmax weights reach; 1 in bf16); the results' scale undoes it. One gradient for all tokens is
-// a scale alone: nothing is weighted then, and this does not run.
+// The tokens' gradients as weights of d, in bf16: g_j over a power of two that the largest is just below; the results' scale
+// undoes it. One gradient for all tokens is a scale alone: nothing is weighted then, and neither this nor ce_units runs.
 __global__ __launch_bounds__(1024) void ce_weights(float* scale, const float* __restrict__ grad, const int32_t* __restrict__ place,
-                                                   int64_t tokens, float lift, float* __restrict__ weight) {
+                                                   int64_t tokens, float* __restrict__ weight) {
   __shared__ float s[16];
   const int tid = threadIdx.x;
   float top = 0.f;
@@ -903,8 +923,64 @@ __global__ __launch_bounds__(1024) void ce_weights(float* scale, const float* __
   const int e = top > 0.f ? min(max(__builtin_amdgcn_frexp_expf(top), -100), 100) : 0;
   const float unit = ldexpf(1.f, e);
   for (int64_t i = tid; i < tokens; i += 1024)
-    if (place[i] >= 0) weight[place[i]] = grad[i] / unit * lift;
-  if (tid == 0) *scale = unit / lift;
+    if (place[i] >= 0) weight[place[i]] = grad[i] / unit;
+  if (tid == 0) *scale = unit;
+}
+
+// The same in f16, whose range one power of two does not do for: each token's d is held in units of its own gradient, with
+// its largest numbers near `lift` = 2^14 (its softmax weights reach f16's smallest). dx's rows are scaled one by one (unit). dW
+// sums over tokens: their powers of two go to a copy of the hidden states for that product (ce_scaled), in which the largest
+// product of a gradient and a state is just below 2^15, so that those down to 2^-29 of it keep their precision. (One power
+// for all rounded the d of gradients far below the largest away: 2^-24 of it, a softmax of 32000 entries, were zeros.)
+__global__ __launch_bounds__(1024) void ce_units(float* scale, const float* __restrict__ grad, const int32_t* __restrict__ place,
+                                                 int64_t tokens, float lift, const int32_t* __restrict__ size,
+                                                 float* __restrict__ weight, float* __restrict__ unit, float* __restrict__ factor) {
+  __shared__ int32_t s[16];
+  const int tid = threadIdx.x;
+  const auto exponent = [](float g) { return min(max(__builtin_amdgcn_frexp_expf(g), -100), 100); };
+  int top = kNothing;
+  for (int64_t i = tid; i < tokens; i += 1024) {
+    const int j = place[i];
+    if (j < 0) continue;
+    const float g = grad[i];
+    const bool finite = fabsf(g) < INFINITY;
+    const int e = finite && g != 0.f ? exponent(g) : 0;
+    weight[j] = ldexpf(g, -e) * lift;
+    unit[j] = ldexpf(1.f, e) / lift;
+    if (finite && g != 0.f && size[j] != kNothing) top = max(top, e + size[j]);
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) top = max(top, __shfl_xor(top, k));
+  if ((tid & 63) == 0) s[tid >> 6] = top;
+  __syncthreads();
+  for (int k = 0; k < 16; ++k) top = max(top, s[k]);
+  if (top == kNothing) top = 0;
+  for (int64_t i = tid; i < tokens; i += 1024) {
+    const int j = place[i];
+    if (j < 0) continue;
+    const float g = grad[i];
+    // a gradient of 0 has no part in `top`: its states, which count for nothing, are not to overflow
+    const int e = g == 0.f ? -1000 : fabsf(g) < INFINITY ? exponent(g) : 0;
+    factor[j] = ldexpf(1.f, min(max(e + 15 - top, -126), 126));
+  }
+  if (tid == 0) *scale = ldexpf(1.f, top - 15) / lift;
+}
+
+// The kept tokens' hidden states times their powers of two, f16, a wave a row.
+__global__ __launch_bounds__(256) void ce_scaled(const int32_t* count, const uint8_t* __restrict__ x, const float* __restrict__ factor,
+                                                 int dpad, uint8_t* __restrict__ out) {
+  const int lane = threadIdx.x & 63, n = *count;
+  for (int64_t j = blockIdx.x * 4 + (threadIdx.x >> 6); j < n; j += gridDim.x * 4) {
+    const float by = factor[j];
+    for (int c = lane; c < dpad / 8; c += 64) {
+      const int64_t at = (j * dpad + 8 * c) * 2;
+      float f[8];
+      VecTraits<f16_t>::unpack(ld16(x + at), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= by;
+      st16(out + at, VecTraits<f16_t>::pack(f));
+    }
+  }
 }
 
 // What rounding left of the label's d, the one large number among a token's.
@@ -921,7 +997,7 @@ __device__ __forceinline__ float label_rest(const CeArgs& a, int64_t j) {
 template <typename T>
 __global__ __launch_bounds__(256) void ce_rows(const CeArgs a, const int32_t* __restrict__ place, int64_t rows,
                                                const float* __restrict__ parts, int splits, T* __restrict__ out) {
-  const float f = a.scale();
+  const float all = a.scale();
   const int n = *a.count, tiles = (n + kTile - 1) / kTile, steps = (n + kDepth - 1) / kDepth, dim = a.dim;
   int64_t pad = a.piece;
   if (place) {
@@ -931,6 +1007,7 @@ __global__ __launch_bounds__(256) void ce_rows(const CeArgs a, const int32_t* __
   for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
     const int64_t j = place ? place[i] : i;
     const float rest = place && j >= 0 && !a.pair ? label_rest<T>(a, j) : 0.f;
+    const float f = place && j >= 0 && a.unit ? a.unit[j] : all;
     const uint8_t* const wy = a.w + (place && j >= 0 ? a.label[j] * a.w_stride : 0);
     for (int d = threadIdx.x * 4; d < dim; d += 1024) {
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -976,7 +1053,7 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // What the forward leaves for the backward, in one buffer.
 struct Kept {
-  int64_t npad, dpad, place, token, label, ref, target, lse, loss, x, bytes;
+  int64_t npad, dpad, place, token, label, ref, target, lse, loss, size, x, bytes;
 };
 bool plan_kept(int64_t tokens, int64_t dim, Kept* k) {
   if (tokens < 0 || dim < 1 || tokens >= (1ll << 22) || dim > 65536) return false;
@@ -989,7 +1066,8 @@ bool plan_kept(int64_t tokens, int64_t dim, Kept* k) {
   k->target = k->ref + k->npad * 4;
   k->lse = k->target + k->npad * 4;
   k->loss = k->lse + k->npad * 4;
-  k->x = k->loss + k->npad * 4;
+  k->size = k->loss + k->npad * 4;
+  k->x = k->size + k->npad * 4;
   k->bytes = k->x + k->npad * k->dpad * 2;
   return true;
 }
@@ -1006,7 +1084,7 @@ Forward plan_forward(const Kept& k, int64_t vocab) {
 }
 
 struct Backward {
-  int64_t piece, dcols, dw_splits, weight, d, dx, dw, bytes;
+  int64_t piece, dcols, dw_splits, weight, unit, factor, scaled, d, dx, dw, bytes;
 };
 Backward plan_backward(const Kept& k, int64_t vocab, int64_t dim) {
   Backward b;
@@ -1035,7 +1113,10 @@ Backward plan_backward(const Kept& k, int64_t vocab, int64_t dim) {
   const int64_t cols = b.dcols / kTile;
   b.dw_splits = b.piece < vocab ? 1 : splits_of(b.piece / kTile, cols, k.npad / kDepth);
   b.weight = 256;  // behind the results' scale
-  b.d = b.weight + k.npad * 4;
+  b.unit = b.weight + k.npad * 4;
+  b.factor = b.unit + k.npad * 4;
+  b.scaled = b.factor + k.npad * 4;
+  b.d = b.scaled + k.npad * k.dpad * 2;
   b.dx = b.d + b.piece * k.npad * 2;
   // dx's sum is split by the kept tokens, whose number the device has: splits x tiles of tokens are 256 / cols or fewer where
   // there are several splits, and no more than the steps allow
@@ -1073,11 +1154,11 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
   if (bits == 64)
     hipLaunchKernelGGL((ce_prepare<T, int64_t>), dim3(blocks), dim3(1024), 0, st, (const T*)x, x_stride, tokens, (const T*)w,
                        w_stride, vocab, (int)dim, (int)k.dpad, wide, labels, ignore, head, place, token, label, ref,
-                       (T*)(kept + k.x), (int)k.npad, losses);
+                       (int32_t*)(kept + k.size), (T*)(kept + k.x), (int)k.npad, losses);
   else
     hipLaunchKernelGGL((ce_prepare<T, int32_t>), dim3(blocks), dim3(1024), 0, st, (const T*)x, x_stride, tokens, (const T*)w,
                        w_stride, vocab, (int)dim, (int)k.dpad, wide, labels, ignore, head, place, token, label, ref,
-                       (T*)(kept + k.x), (int)k.npad, losses);
+                       (int32_t*)(kept + k.size), (T*)(kept + k.x), (int)k.npad, losses);
   CeArgs a = {};
   a.x = kept + k.x;
   a.x_stride = k.dpad * 2;
@@ -1108,14 +1189,29 @@ int run_backward(const uint8_t* kept, const Kept& k, int64_t tokens, const void*
                  const float* grad, int reduction, void* dx, void* dw, uint8_t* ws, const Backward& b, hipStream_t st) {
   const Header* const head = (const Header*)kept;
   const int32_t* place = (const int32_t*)(kept + k.place);
-  constexpr float lift = __is_same(T, f16_t) ? 16384.f : 1.f;
+  constexpr bool half = __is_same(T, f16_t);
+  constexpr float lift = half ? 16384.f : 1.f;
   CeArgs a = {};
+  const uint8_t* dw_x = kept + k.x;
   if (reduction == 0) {
     float* weight = (float*)(ws + b.weight);
     a.weight = weight;
-    hipLaunchKernelGGL(ce_weights, dim3(1), dim3(1024), 0, st, (float*)ws, grad, place, tokens, lift, weight);
+    if constexpr (half) {
+      float *unit = (float*)(ws + b.unit), *factor = (float*)(ws + b.factor);
+      a.unit = unit;
+      hipLaunchKernelGGL(ce_units, dim3(1), dim3(1024), 0, st, (float*)ws, grad, place, tokens, lift,
+                         (const int32_t*)(kept + k.size), weight, unit, factor);
+      if (dw) {
+        dw_x = ws + b.scaled;
+        const int64_t blocks = (tokens + 3) / 4;
+        if (blocks > 0)
+          hipLaunchKernelGGL(ce_scaled, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, &head->count,
+                             kept + k.x, factor, (int)k.dpad, ws + b.scaled);
+      }
+    } else {
+      hipLaunchKernelGGL(ce_weights, dim3(1), dim3(1024), 0, st, (float*)ws, grad, place, tokens, weight);
+    }
   }
-  a.x = kept + k.x;
   a.x_stride = k.dpad * 2;
   a.w = (const uint8_t*)w;
   a.w_stride = w_stride * 2;
@@ -1135,10 +1231,12 @@ int run_backward(const uint8_t* kept, const Kept& k, int64_t tokens, const void*
   float *dx_parts = (float*)(ws + b.dx), *dw_parts = (float*)(ws + b.dw);
   for (int64_t v0 = 0; v0 < vocab; v0 += b.piece) {
     a.v0 = v0;
+    a.x = kept + k.x;
     a.splits = 1;
     a.add = 0;
     launch_logits<T, kGrads>(a, tokens, st);
     if (dw) {
+      a.x = dw_x;
       a.splits = (int32_t)b.dw_splits;
       a.parts = dw_parts;
       launch<T, kDw>(a, st);

@@ -20,8 +20,10 @@ whose rows are no multiple of 64 always NaN.
 
 Logits, softmax sums and all other sums are float32, the loss is float32 and keeps
 its precision down to 0. The gradients of the logits are rounded to the inputs'
-type for the products they enter, in float16 with a power of two taken out, so that
-any size of the loss's gradient keeps its precision; up to 128 tokens they enter
+type for the products they enter, in float16 in units of their token's own gradient,
+so that gradients of any size, also of tokens far apart, keep their precision (in
+weight's gradient, which sums over tokens, those whose product with the hidden state
+is no smaller than 2^-29 of the call's largest); up to 128 tokens they enter
 as two such numbers, and what the rounding leaves of the label's is made up for in hidden's
 gradient. Sums run in a fixed order: losses and gradients are bitwise
 deterministic.
