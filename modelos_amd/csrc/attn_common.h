@@ -131,9 +131,10 @@ __device__ __forceinline__ frag_t frag_global(const void* row, int s, int lane) 
 
 // 64 lanes' 16 bytes each from a buffer at the lanes' offsets to LDS at `to` (uniform) and on, side by side. In asm,
 // so that the compiler does not wait for it at the next transposing read of another tile; there is no register
-// for it to lose, and tile_wait() before the barrier is the wait. The s_nop: m0 is read one state after its write.
+// for it to lose, and tile_wait() before the barrier is the wait. The s_nop: m0 is read one state after its write, a
+// descriptor that a vector instruction wrote (a lane read, a spilled scalar) five; the compiler does not see to it in here.
 __device__ __forceinline__ void load_lds16(u32x4_t rsrc, lds_u8* to, uint32_t offset) {
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"((uint32_t)(uintptr_t)to), "v"(offset), "s"(rsrc)
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"((uint32_t)(uintptr_t)to), "v"(offset), "s"(rsrc)
                : "memory");
 }
 
@@ -164,7 +165,7 @@ struct TileLoad {
 };
 // 64 lanes' float each, as load_lds16.
 __device__ __forceinline__ void load_lds4(u32x4_t rsrc, lds_u8* to, uint32_t offset) {
-  asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"{m0}"((uint32_t)(uintptr_t)to), "v"(offset), "s"(rsrc)
+  asm volatile("s_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"{m0}"((uint32_t)(uintptr_t)to), "v"(offset), "s"(rsrc)
                : "memory");
 }
 
