@@ -1339,13 +1339,15 @@ __device__ __forceinline__ void append_pair(uint32_t p, uint32_t key, uint32_t* 
 // (which turns its lgkmcnt waits into lgkmcnt(0)); the caller waits with
 // s_waitcnt vmcnt(0) before the barrier that publishes the data.
 // The LDS offset of dst is the low word of its flat address; M0 (reserved to
-// the compiler) is restored after the load has read it.
+// the compiler) is read by the load one state after its write (the s_nop) and
+// restored after the load has read it.
 __device__ __forceinline__ void dma16(const void* src, unsigned char* dst) {
   const uint32_t m0v = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)dst);
   uint32_t saved;
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
       "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
       "global_load_lds_dwordx4 %1, off\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)

@@ -45,3 +45,12 @@ def test_scalar_operands_are_waited_for(where, lines, operands):
     scalars = {str(i) for i, c in enumerate(re.findall(r"\"(=?&?\{?\w+\}?)\"\s*\(", operands)) if c == "s"}
     if read & scalars:
         assert states(lines[:at]) >= 5, lines
+
+
+@pytest.mark.parametrize("where,lines,operands", [pytest.param(*s, id=s[0]) for s in statements()
+                                                  if any("lds" in x.split() or "_lds_" in x for x in s[1])])
+def test_m0_is_waited_for(where, lines, operands):
+    at = next(i for i, x in enumerate(lines) if "lds" in x.split() or "_lds_" in x)
+    writes = [i for i, x in enumerate(lines[:at]) if re.match(r"s_\w+ m0,", x)]
+    begin = writes[-1] + 1 if writes else 0  # else the compiler writes it right before
+    assert states(lines[begin:at]) >= 1, lines
