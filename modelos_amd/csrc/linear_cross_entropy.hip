@@ -729,6 +729,10 @@ __global__ __launch_bounds__(kThreads, 2) void ce_few(const CeArgs a) {
 // Around the products
 // ---------------------------------------------------------------------------
 constexpr int kPrepareRows = 16;  // tokens of a workgroup of ce_prepare, a wave each
+constexpr int kCounted = 1024;    // of one of ce_count
+// Tokens up to which ce_prepare counts alone: all of the forward with 256 entries, 64 wide, 28 us so and 28 to 30 with ce_count at 8192
+// tokens, 39 and 37 at 16384; 152 and 91 at 65536, 18700 and 1250 at 2^20.
+constexpr int64_t kFewToCount = 12288;
 constexpr int kJoinTokens = 32, kJoinSlices = 32;
 
 struct Header {
@@ -742,22 +746,34 @@ __device__ __forceinline__ int label_of(const void* labels, int64_t i, int64_t i
   return y == ignore || y < 0 || y >= vocab ? -1 : (int)y;
 }
 
+// Kept tokens of 1024 each: what ce_prepare counts from where a count of all labels before would be too long.
+template <typename L>
+__global__ __launch_bounds__(kCounted) void ce_count(const void* labels, int64_t tokens, int64_t ignore, int64_t vocab,
+                                                     int32_t* counts) {
+  const int64_t i = (int64_t)blockIdx.x * kCounted + threadIdx.x;
+  const int n = __syncthreads_count(i < tokens && label_of<L>(labels, i, ignore, vocab) >= 0);
+  if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+
 constexpr int kNothing = -1000;  // the exponent of a row of zeros
 
-// The kept tokens side by side: rows, labels, places, and the label's logit; in f16 the exponent of a row's largest number. A workgroup counts the kept tokens before its 16
-// itself: 16384 tokens' labels are read 512 times in all, 67 MB out of the L2, and no launch is needed to count.
+// The kept tokens side by side: rows, labels, places, and the label's logit; in f16 the exponent of a row's largest number. A
+// workgroup counts the kept tokens before its 16 itself: 16384 tokens' labels are read 512 times in all, 67 MB out of the L2,
+// and no launch is needed to count. For more tokens, whose square that grows with, from ce_count's sums of 1024.
 template <typename T, typename L>
 __global__ __launch_bounds__(1024) void ce_prepare(const T* __restrict__ x, int64_t x_stride, int64_t tokens,
                                                    const T* __restrict__ w, int64_t w_stride, int64_t vocab, int dim, int dpad,
                                                    int wide, const void* labels, int64_t ignore, Header* head, int32_t* place,
                                                    int32_t* token, int32_t* label, float* ref, int32_t* size, T* __restrict__ kept,
-                                                   int npad, float* losses) {
+                                                   int npad, float* losses, const int32_t* __restrict__ counts) {
   __shared__ int32_t before_s[16], own_s[16];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int64_t first = (int64_t)blockIdx.x * kPrepareRows, i = first + wave;
   const int y = i < tokens ? label_of<L>(labels, i, ignore, vocab) : -1;
   int32_t before = 0;
-  for (int64_t k = tid; k < first; k += 1024) before += label_of<L>(labels, k, ignore, vocab) >= 0;
+  const int64_t whole = counts ? first / kCounted : 0;
+  for (int64_t k = tid; k < whole; k += 1024) before += counts[k];
+  for (int64_t k = whole * kCounted + tid; k < first; k += 1024) before += label_of<L>(labels, k, ignore, vocab) >= 0;
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) before += __shfl_xor(before, s);
   if (lane == 0) {
@@ -1073,13 +1089,14 @@ bool plan_kept(int64_t tokens, int64_t dim, Kept* k) {
 }
 
 struct Forward {
-  int64_t sums, block_sums, bytes;
+  int64_t sums, block_sums, counts, bytes;
 };
 Forward plan_forward(const Kept& k, int64_t vocab) {
   Forward f;
   f.sums = 0;
   f.block_sums = f.sums + up(vocab, kTile) / 128 * k.npad * 8;
-  f.bytes = f.block_sums + k.npad / kJoinTokens * 4;
+  f.counts = f.block_sums + k.npad / kJoinTokens * 4;
+  f.bytes = f.counts + up(k.npad, kCounted) / kCounted * 4;
   return f;
 }
 
@@ -1151,14 +1168,20 @@ int run_forward(const void* x, int64_t x_stride, int64_t tokens, const void* w, 
   float* const losses = reduction == 0 ? loss : nullptr;
   const int wide = (((uintptr_t)x | (uintptr_t)w) & 15) == 0 && ((x_stride | w_stride | dim) & 7) == 0;
   const unsigned blocks = (unsigned)((tokens < 1 ? 1 : tokens) + kPrepareRows - 1) / kPrepareRows;
+  int32_t* const counts = tokens > kFewToCount ? (int32_t*)(ws + f.counts) : nullptr;
+  const dim3 counted((unsigned)((tokens + kCounted - 1) / kCounted));
+  if (counts && bits == 64)
+    hipLaunchKernelGGL((ce_count<int64_t>), counted, dim3(kCounted), 0, st, labels, tokens, ignore, vocab, counts);
+  else if (counts)
+    hipLaunchKernelGGL((ce_count<int32_t>), counted, dim3(kCounted), 0, st, labels, tokens, ignore, vocab, counts);
   if (bits == 64)
     hipLaunchKernelGGL((ce_prepare<T, int64_t>), dim3(blocks), dim3(1024), 0, st, (const T*)x, x_stride, tokens, (const T*)w,
                        w_stride, vocab, (int)dim, (int)k.dpad, wide, labels, ignore, head, place, token, label, ref,
-                       (int32_t*)(kept + k.size), (T*)(kept + k.x), (int)k.npad, losses);
+                       (int32_t*)(kept + k.size), (T*)(kept + k.x), (int)k.npad, losses, counts);
   else
     hipLaunchKernelGGL((ce_prepare<T, int32_t>), dim3(blocks), dim3(1024), 0, st, (const T*)x, x_stride, tokens, (const T*)w,
                        w_stride, vocab, (int)dim, (int)k.dpad, wide, labels, ignore, head, place, token, label, ref,
-                       (int32_t*)(kept + k.size), (T*)(kept + k.x), (int)k.npad, losses);
+                       (int32_t*)(kept + k.size), (T*)(kept + k.x), (int)k.npad, losses, counts);
   CeArgs a = {};
   a.x = kept + k.x;
   a.x_stride = k.dpad * 2;

@@ -354,3 +354,19 @@ def test_a_flat_vocabulary_far_above_the_labels(V, n, device):
     _near(dw[others, 0], (n * p).expand(V - n), off * n * p, "dW of the others")
     _near(dw[labels, 0], -torch.ones(n), off + 1e-20, "dW of the labels")
     assert not dw[:, 1:].any()
+
+
+@pytest.mark.parametrize("n", [12288, 12289, 70001, (1 << 20) + 5])
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64], ids=["i32", "i64"])
+@pytest.mark.parametrize("ignored", [0.0, 0.4, 0.9999])
+def test_long_batches(ignored, kind, n, device):
+    """From 12289 tokens on the kept ones are counted by a launch of its own. The oracle's 64-bit products on the GPU."""
+    x, w, labels, gen = _inputs(n, 40, 16, BF16, device, n, lean=4.0, ignored=ignored)
+    labels[n - 1] = 7
+    loss, grad, grads = _both(x, w, labels.to(kind), "none", gen)
+    values, bounds = oracle.loss_and_gradients(x.detach(), w.detach(), labels, -100, "none", grad.double().to(device))
+    for name, got, want, bound in zip(("loss", "dx", "dW"), (loss, *grads), values, bounds):
+        _near(got, want.cpu(), bound.cpu(), name)
+    mean = linear_cross_entropy(x, w, labels.to(kind))
+    count = max(1, int((labels >= 0).sum()))
+    assert abs(mean.item() - values[0].sum().item() / count) <= (bounds[0].sum().item() + 2.0**-24 * 40 * values[0].sum().item()) / count
