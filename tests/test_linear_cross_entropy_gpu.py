@@ -370,3 +370,16 @@ def test_long_batches(ignored, kind, n, device):
     mean = linear_cross_entropy(x, w, labels.to(kind))
     count = max(1, int((labels >= 0).sum()))
     assert abs(mean.item() - values[0].sum().item() / count) <= (bounds[0].sum().item() + 2.0**-24 * 40 * values[0].sum().item()) / count
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("n", [60, 300])
+def test_other_gradients_through_one_graph(n, dtype, device):
+    """What the forward keeps is not changed by a backward: one with other gradients gives what a graph of its own does."""
+    x, w, labels, gen = _inputs(n, 300, 64, dtype, device)
+    ways = [size * torch.randn(n, generator=gen).to(device) for size in (1.0, 2.0**8, 2.0**-8)]
+    loss = linear_cross_entropy(x, w, labels, reduction="none")
+    for grad in ways:
+        one = torch.autograd.grad(loss, (x, w), grad, retain_graph=True)
+        own = torch.autograd.grad(linear_cross_entropy(x, w, labels, reduction="none"), (x, w), grad)
+        assert all(torch.equal(a, b) for a, b in zip(one, own))
