@@ -759,7 +759,9 @@ size_t pkm_adamw_workspace_size(int64_t count);
  * a >= 0, 2^e <= a < 2^(e + 1), e >= -6, becomes floor(a 2^(3 - e) + u) 2^(e - 3), at most
  * 448, with u = (x >> 12) 2^-20 for m and (x mod 2^20) 2^-20 for r, x = (2654435761 i +
  * 2246822519 t) mod 2^32 for number i of its tensor; an r above 0 is at least 2^-9. Blocks whose
- * largest number is below 2^-110 are held as zeros.
+ * largest number is below 2^-110 are held as zeros; one with an infinite or NaN gradient has a
+ * step that is none, which makes all its weights NaN in the next call. No two tensors of a call, nor their
+ * states, may share memory: all are updated at once.
  */
 int pkm_adamw_step(const pkm_adamw_tensor_t* tensors, int64_t count, int dtype, int state_bits, double lr,
                    const float* lr_device, double beta1, double beta2, double eps, double weight_decay,

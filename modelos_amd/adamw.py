@@ -12,7 +12,10 @@ float32 step for each 256 numbers in a row of the tensor ("exp_avg_scale",
 "exp_root_scale": the block's largest / 448): 2 bytes a number instead of 8. The
 rounding is dithered over the steps, so that small changes are kept on average,
 and the same on every run. Blocks whose largest number is below 2^-110 are held
-as zeros.
+as zeros. A gradient that is infinite or NaN makes its block's step so: all 256
+weights of the block are NaN from the next step on (with 32 bits only its own).
+Nothing on the device leaves such a step out: whoever scales a loss looks at its
+gradients before the step, and does not capture that step into a graph.
 
 16-bit weights lose updates below half their spacing; `master_weights=True` keeps a
 float32 copy ("master") that the update is made to, the weight its rounding: who

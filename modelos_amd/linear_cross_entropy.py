@@ -8,8 +8,12 @@ and loss are together,
 in pieces of the vocabulary: the forward sums the exponentials of a piece's
 logits and drops them, the backward computes them again, turns them into their
 gradients and those into the piece's rows of weight's gradient and its part of
-hidden's. The largest of it in memory are the gradients of one piece, up to about 768 MB
-in 16 bits; a training forward keeps a copy of the hidden states that count.
+hidden's. The largest of it in memory are the gradients of one piece in 16 bits: up to
+about 768 MB, and for more than 24576 tokens, whose pieces get no smaller than 16384
+entries, 32 KB a token (2 GiB at 65536); beside them 4 bytes a number of hidden for its
+gradient's sums and 2 for a scaled copy. The forward needs 8 bytes a token for every 128
+entries. A training forward keeps a copy of the hidden states that count, and of a weight
+that it had to copy for its rows (below), until its backward.
 
 Tokens whose label is ignore_index, or lies outside [0, vocab), do not count:
 their loss is 0, nothing is computed for them, what hidden holds there is not
@@ -116,7 +120,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
 
     hidden: [..., dim]; weight: [vocab, dim] of hidden's type; labels: int32 or int64 of hidden's shape without the last.
     ignore_index: the label of tokens that do not count. reduction: "mean" over the tokens that count, "sum", or "none"
-    (a loss for each label). Any strides; rows of weight that are not whole, aligned 16-byte vectors cost a copy of it.
+    (a loss for each label). Any strides; rows of weight that are not whole, aligned 16-byte vectors (a dim that is no
+    multiple of 8 among them) cost a copy of it in every call.
     Returns float32.
     """
     if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:

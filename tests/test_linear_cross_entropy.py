@@ -86,3 +86,19 @@ def test_sizes(lib):
     assert lib.pkm_linear_ce_fwd_workspace_size(10, 0, 64) == lib.pkm_linear_ce_bwd_workspace_size(10, 1 << 30, 64) == 0
     # 16384 tokens, 151936 entries: no more than 768 MB of the logits' gradients at a time, and 67 MB of dx's sums
     assert 16384 * 16384 < lib.pkm_linear_ce_bwd_workspace_size(16384, 151936, 1024) < (768 << 20) + 70e6
+
+
+@pytest.mark.parametrize("dim", [64, 1000, 4096])
+@pytest.mark.parametrize("vocab", [300, 151936])
+@pytest.mark.parametrize("tokens", [100, 16384, 24576, 65536, 1 << 18, 1 << 20])
+def test_sizes_of_long_batches(lib, tokens, vocab, dim):
+    """What the documentation says a call needs: one piece's gradients, 768 MB or 32 KB a token, hidden's sums and copy; sums of
+    128 entries each in the forward. Tokens and widths count in whole tiles of 256, widths of a copy in 64; the sums of few
+    tokens are split, up to 256 tiles."""
+    up = lambda n, to: -(-n // to) * to
+    n, few = up(tokens, 256), 256 * 256 * 256 * 4
+    pieces = min(max(768 << 20, 32768 * n), 2 * n * up(vocab, 256))
+    rest = n * (4 * up(dim, 256) + 2 * up(dim, 64) + 16) + 256
+    split = 256 * 256 * 256 * 4 if vocab == 300 else 0  # dW's sums, where the vocabulary is one piece
+    assert lib.pkm_linear_ce_bwd_workspace_size(tokens, vocab, dim) <= pieces + rest + few + split
+    assert lib.pkm_linear_ce_fwd_workspace_size(tokens, vocab, dim) <= n * (8 * up(vocab, 256) // 128 + 1) + 4096
