@@ -18,9 +18,9 @@
 // a step of 16 while the matrix cores work on the one before, across tiles and also across results: the grid is one
 // workgroup a CU, and the next result's tiles load while this one's epilogue runs. One barrier a 64.
 //
-// Measured, 16384 tokens, 151936 entries, 1024 wide, bf16: the forward's product 4.27 to 4.48 ms (two cards; 1140 to 1195
-// TFLOP/s), of a piece of 15360 entries d 0.50, dW 0.46 and dx 0.43 ms (1040 to 1200); beside them 0.1 ms (copy of the tokens
-// 23 us, join of the tiles' sums 47, dx's rounding 50). The matrix cores are busy 52 to 61 % of the cycles at 1.6 to 2.0 GHz;
+// Measured, 16384 tokens, 151936 entries, 1024 wide, bf16: the forward's product 4.16 to 4.48 ms (several cards; 1140 to 1225
+// TFLOP/s), of a piece of 15360 entries d 0.49, dW 0.44 and dx 0.42 ms (1040 to 1200); beside them 0.1 ms (count and copy of the
+// tokens 23 us, join of the tiles' sums 47, dx's rounding 50). The matrix cores are busy 52 to 61 % of the cycles at 1.6 to 2.0 GHz;
 // plain library products of the pieces' shapes take 0.457, 0.668 and 0.444 ms at 1.5 to 1.64 GHz and 50 to 70 %: the clock
 // falls as the load rises, and neither fewer LDS cycles (bank conflicts were half of them) nor loads spread between the
 // products moved the time.
